@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import c_double, c_float, c_int, c_int64, c_void_p, c_char_p
 
 import torch
@@ -99,6 +100,10 @@ _SIGNATURES = {
     "cf_conv_mfma_choice": [_P, _P],
     "cf_conv_halo_pair_args": [_P],
     "cf_conv_args_sizes": [_P],
+    # argument blocks packed by the *_ARGS below
+    "cf_decay_attention": [_P],
+    "cf_decay_attention_step": [_P],
+    "cf_rotary": [_P],
 }
 
 _D = c_double
@@ -132,6 +137,14 @@ class ConvMfmaArgs(ctypes.Structure):
 
 class ConvHaloPairArgs(ctypes.Structure):
     _fields_ = _CONV_HALO_PAIR_FIELDS
+
+
+# The argument blocks of the sequence operators (include/catfuse_amd.h:
+# CfDecayAttentionArgs, CfDecayStepArgs, CfRotaryArgs), packed as bytes by one
+# call: Q a pointer, q an int64, d a double, every field 8 bytes.
+DECAY_ATTENTION_ARGS = struct.Struct("=8Q21qdQ")
+DECAY_STEP_ARGS = struct.Struct("=7Q17qdQ")
+ROTARY_ARGS = struct.Struct("=8Q33qdQ")
 _RESTYPES = {"cf_error_string": c_char_p}
 
 _lib = None

@@ -11,7 +11,13 @@ standalone tails in catfuse/kernels/*.py).
   add_lif(x1, x2, v_carry=None, ...), add_bn_lif(a, x, scale, bias, ...),
   avgpool_lif(x, v_carry=None, ...), linear_lif(x, w, bias=None, ...)
 
-Each call starts from the initial membrane state (v = v_reset), like the
+Operators of ordered tokens (catfuse_amd.sequence):
+  decay_attention(q, k, v, log_decay, ...), decay_attention_step(q, k, v,
+                  log_decay, state, ...), qk_norm_rotary(q, k, positions,
+                  freqs, ...), rotary(x, positions, freqs, ...),
+                  rotary_freqs(pairs, ...)
+
+Each LIF call starts from the initial membrane state (v = v_reset), like the
 reference's single-block (K = T) launchers, unless a carry tensor is given;
 the `*_lif` tails return (spikes, v_final).  Packed weights are cached by
 tensor identity and version.
@@ -21,6 +27,8 @@ from __future__ import annotations
 import torch
 
 from catfuse_amd.runtime import ID_ADD_Z, ConvLIFRunner, avgpool2x2_lif, lif_multistep
+from catfuse_amd.sequence import (decay_attention, decay_attention_step, qk_norm_rotary, rotary,
+                                  rotary_freqs)
 
 _RUNNERS: dict = {}
 
@@ -126,4 +134,5 @@ def linear_lif(x, w, bias=None, v_carry=None, tau=2.0, v_th=1.0, v_reset=0.0, de
 
 __all__ = ["partial_fusion_conv_lif", "partial_fusion_conv_bn_lif",
            "partial_fusion_conv_bn_add_lif", "add_lif", "add_bn_lif", "bn_lif", "avgpool_lif",
-           "linear_lif"]
+           "linear_lif", "decay_attention", "decay_attention_step", "qk_norm_rotary", "rotary",
+           "rotary_freqs"]

@@ -780,6 +780,97 @@ int cf_conv_sparse_noalloc(const void* x, int64_t Cin, const void* w_packed, con
                            int epilogue, double tau, double v_th, double v_reset, int hard_reset,
                            int decay_input, void* stream);
 
+/* ---- Sequence operators -------------------------------------------------
+ * Softmax-free causal attention with a decay for each head, its single-token
+ * form, and the norms and position rotation of its heads.  No counterpart in
+ * the reference.  Arguments come in one block, every field 8 bytes in this
+ * order; strides are in elements, the last dimension of every tensor is
+ * contiguous; dtype: 0 fp32, 1 fp16, 2 bf16 (of q, k, v and out). */
+#define CF_SEQ_MAX_HEADS 4096
+#define CF_DECAY_MAX_DK 256
+#define CF_DECAY_MAX_DV 1024
+#define CF_DECAY_MAX_SEQS 65535
+#define CF_ROTARY_MAX_DIM 512
+#define CF_ROTARY_MAX_AXES 3
+
+/* out_t = scale q_t S_t, S_t = w S_{t-1} + k_t v_t^T, w = exp(log_decay[h]),
+ * for every sequence and head, from S = state_in[seq][h] (nullable: zeros);
+ * the last S goes to state_out (nullable).  States fp32 [seqs][heads][dk][dv].
+ * Query head h reads key and value head h / (heads / kv_heads).
+ * cu_seqlens null: `seqs` sequences of `tokens` rows, the strides *_batch
+ * apart.  Else int32 (cu_wide 0) or int64 offsets [seqs + 1] in device memory:
+ * sequence b is rows cu[b] .. cu[b + 1] - 1 of `tokens` rows; offsets are
+ * clamped to 0 .. tokens and a decreasing one gives an empty sequence; rows of
+ * no sequence are zeroed (zero_rest) or left as they were.  out must not
+ * overlap the inputs. */
+typedef struct CfDecayAttentionArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const float* log_decay;
+  const float* state_in;
+  float* state_out;
+  void* out;
+  const void* cu_seqlens;
+  int64_t cu_wide, zero_rest, dtype, seqs, tokens, heads, kv_heads, dk, dv;
+  int64_t q_batch, q_token, q_head, k_batch, k_token, k_head;
+  int64_t v_batch, v_token, v_head, out_batch, out_token, out_head;
+  double scale;
+  void* stream;
+} CfDecayAttentionArgs;
+int cf_decay_attention(const CfDecayAttentionArgs* args);
+
+/* One token for each of `rows` sequences: S = state + slot * state_slot,
+ * [heads][dk][dv], updated in place (S <- w S + k v^T, out = scale q S).
+ * slot = slots[row] (int32, or int64 with slots_wide; null: row).  Slots
+ * outside 0 .. pool - 1 give zeros and touch no state; rows of one slot are
+ * consecutive tokens, in the order of the rows. */
+typedef struct CfDecayStepArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const float* log_decay;
+  float* state;
+  void* out;
+  const void* slots;
+  int64_t slots_wide, dtype, rows, heads, kv_heads, dk, dv, pool, state_slot;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+  double scale;
+  void* stream;
+} CfDecayStepArgs;
+int cf_decay_attention_step(const CfDecayStepArgs* args);
+
+/* Rotation of the heads x [outer][inner][x_heads][d] and, with k_heads > 0, k
+ * (same tokens and d) by the angle position * freqs[pair], pairs (i, i +
+ * pairs) or (2 i, 2 i + 1) interleaved, channels past 2 * pairs passed on;
+ * inverse turns back.  Pair i takes axis 0 below section1, axis 1 below
+ * section2, else axis 2 (axes 1: always axis 0; axes 2: section2 unused).
+ * positions int32 (pos_kind 0), int64 (1) or fp32 (2), strides pos_axis,
+ * pos_outer, pos_inner; freqs fp64 [pairs], radians a position.  norm: each
+ * head is first divided by sqrt(mean(x^2) + eps) and multiplied by its
+ * weights (nullable; fp32 or of dtype; *_weight_head: 0, or the elements from
+ * one head's weights to the next).  An output may be its own input, with the
+ * same strides; it must not overlap inputs otherwise. */
+typedef struct CfRotaryArgs {
+  const void* x;
+  void* x_out;
+  const void* x_weight;
+  const void* k;
+  void* k_out;
+  const void* k_weight;
+  const void* positions;
+  const double* freqs;
+  int64_t x_weight_f32, x_weight_head, k_weight_f32, k_weight_head, pos_kind, dtype;
+  int64_t outer, inner, x_heads, k_heads, d, pairs, axes, section1, section2;
+  int64_t interleaved, norm, inverse;
+  int64_t pos_axis, pos_outer, pos_inner;
+  int64_t x_outer, x_inner, x_head, x_out_outer, x_out_inner, x_out_head;
+  int64_t k_outer, k_inner, k_head, k_out_outer, k_out_inner, k_out_head;
+  double eps;
+  void* stream;
+} CfRotaryArgs;
+int cf_rotary(const CfRotaryArgs* args);
+
 /* Diagnostic: one wave computes D(32x32 fp32) = A(32x16 fp16) * B(16x32
  * fp16) through the matrix-core lane mapping cf_conv_mfma relies on.
  * No reference counterpart (layout self-test). */
