@@ -142,7 +142,7 @@ class ConvHaloPairArgs(ctypes.Structure):
 # The argument blocks of the sequence operators (include/catfuse_amd.h:
 # CfDecayAttentionArgs, CfDecayStepArgs, CfRotaryArgs), packed as bytes by one
 # call: Q a pointer, q an int64, d a double, every field 8 bytes.
-DECAY_ATTENTION_ARGS = struct.Struct("=8Q21qdQ")
+DECAY_ATTENTION_ARGS = struct.Struct("=8Q21qQ2qdQ")
 DECAY_STEP_ARGS = struct.Struct("=7Q17qdQ")
 ROTARY_ARGS = struct.Struct("=8Q33qdQ")
 _RESTYPES = {"cf_error_string": c_char_p}

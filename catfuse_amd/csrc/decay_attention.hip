@@ -4,6 +4,24 @@
 // per sequence and head, S a dk x dv matrix in fp32.  Query head h reads key
 // and value head h / (heads / kv_heads).
 //
+// By chunks of C tokens (i, j the places in a chunk, S the state before it):
+//   o_i = scale (w^(i+1) q_i S + sum_{j <= i} w^(i-j) (q_i . k_j) v_j)
+//   S  <- w^C S + sum_j w^(C-1-j) k_j v_j^T
+// which is four products for the matrix cores.  Every power of w has an
+// exponent of at least zero, so none leaves the range of fp32 where w <= 1.
+//
+// Precision.  The matrix cores multiply bf16 and add fp32.  A number that is
+// not a bf16 one enters a product as a sum of two or three of them, its first,
+// second and third eight bits: fp16 inputs as two and fp32 inputs as three
+// (both exact), the weighted values of the state's update as three (exact up
+// to their own rounding), the state and the scores on their way to the output
+// as two for 16-bit outputs (2^-16 of each term, an eighth of a bit of fp16)
+// and as three for fp32 ones.  Products of parts below 2^-24 of the whole
+// (2^-16 on the way to a 16-bit output) are left out.
+//
+// A value that is not finite must not reach the tokens before it, where the
+// product has a zero for it (0 * inf is NaN): see below at `clean`.
+//
 // No counterpart in the reference; the causal, ordered relative of the
 // spiking attention core in attention.hip.
 #include "cf_seq.h"
@@ -19,95 +37,648 @@ struct DecayArgs {
   float* state_out;
   void* out;
   const void* cu;
+  float* ws;                 // states of segments [segment][heads][dk][dv]
   int cu_wide, zero_rest;
   int64_t seqs, tokens;      // tokens: rows in all (packed) or of each sequence
-  int heads, group, dk, dv;
+  int64_t segment, segments; // tokens a segment; segments in all at most
+  int heads, group, dk, dv, slices;
   int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, ob, ot, oh;
+  int vec_q, vec_k, vec_v, vec_o;   // 16-byte accesses are aligned and whole
   float scale;
 };
 
-// One token after another: a workgroup holds 64 columns of one sequence and
-// head's state in registers, wave g the rows g R .. g R + R - 1.
-template <typename T, int R>
-__global__ __launch_bounds__(256) void decay_recurrent_kernel(DecayArgs a) {
-  constexpr int TOK = 16, DKP = 4 * R;
-  __shared__ float qs[TOK][DKP], ks[TOK][DKP];
-  __shared__ float part[TOK][4][64];
-  const int tid = threadIdx.x, col = tid & 63, g = tid >> 6;
-  const int c = blockIdx.x * 64 + col, h = blockIdx.y;
-  const int64_t b = blockIdx.z;
-  int64_t begin = 0, len = a.tokens;
-  if (a.cu != nullptr) {
-    begin = seq_offset(a.cu, a.cu_wide, b, a.tokens);
-    const int64_t end = seq_offset(a.cu, a.cu_wide, b + 1, a.tokens);
-    len = end > begin ? end - begin : 0;
-  }
-  const int64_t row0 = a.cu != nullptr ? 0 : b;
-  const T* q = (const T*)a.q + row0 * a.qb + begin * a.qt + h * a.qh;
-  const T* k = (const T*)a.k + row0 * a.kb + begin * a.kt + (h / a.group) * a.kh;
-  const T* v = (const T*)a.v + row0 * a.vb + begin * a.vt + (h / a.group) * a.vh;
-  T* o = (T*)a.out + row0 * a.ob + begin * a.ot + h * a.oh;
-  const bool mine = c < a.dv;
-  const float w = (float)exp((double)a.log_decay[h]);
-  float s[R];
-  const int64_t sbase = ((b * a.heads + h) * a.dk) * (int64_t)a.dv + c;
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t OOB = 0x80000000u;      // an offset beyond every range used here
+
+// Parts of eight bits that an input's number has.
+template <typename T> constexpr int parts_of() { return sizeof(T) == 4 ? 3 : 2; }
+template <> constexpr int parts_of<bf16_t>() { return 1; }
+
+__device__ __forceinline__ float high_part(float x) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) & 0xffff0000u);
+}
+__device__ __forceinline__ uint32_t pack_high(float lo, float hi) {
+  return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo),
+                               0x07060302u);
+}
+__device__ __forceinline__ uint32_t pack_rounded(float lo, float hi) {
+  const f2 x = {lo, hi};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf2));
+}
+
+// x as N parts, most significant first: leading ones cut off (the rest is
+// exact), the last of fewer than three rounded (cutting it off would shrink
+// every number).
+template <int N>
+__device__ __forceinline__ void split8(const float* x, u32x4* out) {
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int d = g * R + r;
-    s[r] = a.state_in != nullptr && mine && d < a.dk ? a.state_in[sbase + (int64_t)d * a.dv] : 0.0f;
-  }
-  for (int64_t t0 = 0; t0 < len; t0 += TOK) {
-    const int n = (int)(len - t0 < TOK ? len - t0 : TOK);
-    __syncthreads();
-    for (int i = tid; i < TOK * DKP; i += 256) {
-      const int t = i / DKP, d = i % DKP;
-      const bool in = t < n && d < a.dk;
-      qs[t][d] = in ? to_f(q[(t0 + t) * a.qt + d]) : 0.0f;
-      ks[t][d] = in ? to_f(k[(t0 + t) * a.kt + d]) : 0.0f;
-    }
-    __syncthreads();
-    for (int t = 0; t < n; ++t) {
-      const float x = mine ? to_f(v[(t0 + t) * a.vt + c]) : 0.0f;
-      float p = 0.0f;
+  for (int p = 0; p < 4; ++p) {
+    float a = x[2 * p], b = x[2 * p + 1];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        s[r] = __builtin_fmaf(s[r], w, ks[t][g * R + r] * x);
-        p = __builtin_fmaf(qs[t][g * R + r], s[r], p);
+    for (int n = 0; n < N; ++n) {
+      if (n == N - 1 && N < 3) {
+        out[n][p] = pack_rounded(a, b);
+      } else {
+        out[n][p] = pack_high(a, b);
+        a -= high_part(a);
+        b -= high_part(b);
       }
-      part[t][g][col] = p;
+    }
+  }
+}
+
+__device__ __forceinline__ f16v mfma(u32x4 a, u32x4 b, f16v c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a),
+                                                 __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes,
+                                           0x00020000);
+}
+
+// LDS images of a chunk: [part][C rows][D channels] bf16, unpadded, the
+// 16-byte pieces of a row exchanged by row so that both kinds of reads spread
+// over all banks: 16 bytes of 16 rows on end (operands whose product runs over
+// the channels), and 8 bytes of 4 rows on end, 32 channels wide (the
+// transposing reads of operands whose product runs over the tokens).
+template <int D>
+__device__ __forceinline__ int swizzle(int row) {
+  constexpr int SH = D >= 128 ? 0 : (D == 64 ? 1 : 2);
+  return ((row >> 2) & 3) | (((row & 3) >> SH) << 2);
+}
+template <int C, int D>
+__device__ __forceinline__ int image_at(int part, int row, int piece) {   // in bytes
+  return ((part * C + row) * (D / 8) + (piece ^ swizzle<D>(row))) * 16;
+}
+
+// One unit of a chunk: 8 channels of a row, as loaded.
+template <typename T>
+struct Unit { u32x4 w[sizeof(T) / 2]; };
+
+template <typename T>
+__device__ __forceinline__ Unit<T> load_unit(const T* base, __amdgpu_buffer_rsrc_t rsrc, int row,
+                                             int piece, int n, int64_t stride, int d, int vec) {
+  Unit<T> u;
+  constexpr int PER = 16 / sizeof(T);
+  if (vec) {
+#pragma unroll
+    for (int p = 0; p < (int)(sizeof(T) / 2); ++p) {
+      const int c = piece * 8 + p * PER;
+      const uint32_t off = (uint32_t)((row * (int)stride + c) * (int)sizeof(T));
+      u.w[p] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, row < n && c < d ? off : OOB, 0, 0);
+    }
+  } else {
+    Vec<T, 8> x{};
+    if (row < n) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = piece * 8 + i;
+        if (c < d) x.v[i] = base[(int64_t)row * stride + c];
+      }
+    }
+    u = __builtin_bit_cast(Unit<T>, x);
+  }
+  return u;
+}
+
+template <typename T, int C, int D>
+__device__ __forceinline__ void store_unit(char* image, const Unit<T>& u, int row, int piece) {
+  if constexpr (parts_of<T>() == 1) {
+    *reinterpret_cast<u32x4*>(image + image_at<C, D>(0, row, piece)) = u.w[0];
+  } else {
+    typedef Vec<T, 8> V8;
+    const V8 x = __builtin_bit_cast(V8, u);
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = to_f(x.v[i]);
+    u32x4 parts[parts_of<T>()];
+    split8<parts_of<T>()>(f, parts);
+#pragma unroll
+    for (int n = 0; n < parts_of<T>(); ++n)
+      *reinterpret_cast<u32x4*>(image + image_at<C, D>(n, row, piece)) = parts[n];
+  }
+}
+
+// An operand of a product over the channels: lane l holds row 32 tile + l % 32,
+// channels 16 s + 8 (l / 32) .. + 7.
+template <int C, int D>
+__device__ __forceinline__ u32x4 row_operand(const char* image, int part, int tile, int s, int lane) {
+  return *reinterpret_cast<const u32x4*>(
+      image + image_at<C, D>(part, 32 * tile + (lane & 31), 2 * s + (lane >> 5)));
+}
+
+// An operand of a product over the tokens: lane l holds a channel, and of the
+// tokens 16 s .. 16 s + 15 those that a 32 x 32 accumulator's registers 8 s' ..
+// 8 s' + 7 are rows of: 16 s + 4 (l / 32) + 0 .. 3 and the same plus 8.  Each of
+// the two reads turns a block of 4 tokens x 16 channels: lane l % 16 passes the
+// address of token (l % 16) / 4, channels 4 (l % 4) .. + 3 and gets channel
+// l % 16 of the four tokens.  `turned`: the channels in the order in which the
+// rows of an accumulator are contiguous for the lanes (below at S).
+template <int C, int D>
+__device__ __forceinline__ u32x4 token_operand(const char* image, int part, int tile, int s,
+                                               int lane, bool turned) {
+  const int four = lane & 3, block = turned ? ((four & 1) << 1) | (four >> 1) : four;
+  const int c = 32 * tile + ((lane >> 4) & 1) * 16 + 4 * block;
+  u32x4 r;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int row = 16 * s + 8 * e + 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const char* p = image + image_at<C, D>(part, row, c >> 3) + (c & 4) * 2;
+    const u32x2 t = __builtin_bit_cast(
+        u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p));
+    r[2 * e] = t[0];
+    r[2 * e + 1] = t[1];
+  }
+  return r;
+}
+
+// Which (sequence, segment) a segment number is.  Packed sequences: every
+// wave scans the offsets, 64 a time, each offset at least its predecessor.
+struct Span { int64_t seq, part, parts, begin, len; };   // of the sequence; seq < 0: none
+
+__device__ __forceinline__ Span find_span(const DecayArgs& a, int64_t w) {
+  Span s;
+  if (a.cu == nullptr) {
+    s.parts = a.tokens > 0 ? (a.tokens + a.segment - 1) / a.segment : 1;
+    s.seq = w / s.parts;
+    s.part = w % s.parts;
+    s.begin = 0;
+    s.len = a.tokens;
+    if (s.seq >= a.seqs) s.seq = -1;
+    return s;
+  }
+  const int lane = threadIdx.x & 63;
+  int64_t before = 0, top = 0;               // segments and the largest offset so far
+  for (int64_t b0 = 0; b0 < a.seqs; b0 += 64) {
+    const int64_t b = b0 + lane;
+    const bool in = b < a.seqs;
+    int64_t x = in ? seq_offset(a.cu, a.cu_wide, b, a.tokens) : 0;
+    int64_t y = in ? seq_offset(a.cu, a.cu_wide, b + 1, a.tokens) : 0;
+    if (x < top) x = top;
+    if (y < x) y = x;
+    int64_t m = y;                           // running maximum over the lanes
+    for (int d = 1; d < 64; d *= 2) {
+      const int64_t o = __shfl_up(m, d, 64);
+      if (lane >= d && o > m) m = o;
+    }
+    const int64_t prev = __shfl_up(m, 1, 64);
+    const int64_t begin = lane > 0 && prev > x ? prev : x, end = m;
+    const int64_t len = end > begin ? end - begin : 0;
+    const int64_t parts = !in ? 0 : (len > 0 ? (len + a.segment - 1) / a.segment : 1);
+    int64_t sum = parts;
+    for (int d = 1; d < 64; d *= 2) {
+      const int64_t o = __shfl_up(sum, d, 64);
+      if (lane >= d) sum += o;
+    }
+    const int64_t first = before + sum - parts;
+    const uint64_t hit = __ballot(in && w >= first && w < first + parts);
+    if (hit != 0) {
+      const int l = __ffsll((unsigned long long)hit) - 1;
+      s.seq = b0 + l;
+      s.part = w - __shfl(first, l, 64);
+      s.parts = __shfl(parts, l, 64);
+      s.begin = __shfl(begin, l, 64);
+      s.len = __shfl(len, l, 64);
+      return s;
+    }
+    before += __shfl(sum, 63, 64);
+    const int64_t t = __shfl(m, 63, 64);
+    if (t > top) top = t;
+  }
+  s.seq = -1;
+  s.part = s.parts = s.begin = s.len = 0;
+  return s;
+}
+
+// A workgroup takes a segment of a sequence, one head, 32 NW columns of the
+// values; wave w the columns 32 w .. + 31 with their part of S (all DKP rows,
+// in accumulators) throughout.  OUT: the outputs of the segment, from the state
+// that the segments before it left in the workspace (Horner's rule over them);
+// else the segment's own contribution to the state, for the others.
+//
+// S as accumulators: tile t, register r of a lane is row (channel of k)
+// 32 t + 16 (r / 8) + 8 (lane / 32) + r % 8, column lane % 32: the rows of K's
+// operand are taken in that order, so that eight registers on end are an
+// operand of the next chunk's q S as they lie.
+template <typename T, int DKP, int NW, int C, bool OUT>
+__global__ __launch_bounds__(64 * NW) void decay_chunk_kernel(DecayArgs a) {
+  constexpr int NL = parts_of<T>(), NP = NL == 3 ? 3 : 2, NT = 64 * NW;
+  constexpr int KT = DKP / 32, KS = DKP / 16, CT = C / 32, CS = C / 16, DVW = 32 * NW;
+  constexpr int QK_BYTES = NL * C * DKP * 2, V_BYTES = NL * C * DVW * 2;
+  constexpr int TILES = CT * (CT + 1) / 2;                     // score tiles that are not masked
+  constexpr int P_BYTES = CT > 1 && OUT ? TILES * 2 * NP * 1024 : 16;
+  __shared__ __attribute__((aligned(16))) char ksh[QK_BYTES];
+  __shared__ __attribute__((aligned(16))) char vsh[V_BYTES];
+  __shared__ __attribute__((aligned(16))) char qsh[OUT ? QK_BYTES : 16];
+  __shared__ __attribute__((aligned(16))) char psh[P_BYTES];
+  __shared__ float pow_sh[C + 1];            // w^n
+  __shared__ float end_sh[2 * C];            // w^(C - 1 - j), then zeros
+
+  const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  // Query heads of one key head and the slices of their values read the same
+  // rows: consecutive workgroups of one XCD (workgroup number mod 8).
+  const int shared = a.group * a.slices, kv_heads = a.heads / a.group;
+  const int64_t slot = blockIdx.x >> 3;
+  const int64_t super = slot / shared * 8 + (blockIdx.x & 7);
+  const int inner = (int)(slot % shared);
+  const int64_t w = super / kv_heads;
+  if (w >= a.segments) return;
+  const int hk = (int)(super % kv_heads), h = hk * a.group + inner / a.slices;
+  const int dv0 = inner % a.slices * DVW;
+
+  const Span sp = find_span(a, w);
+  if (sp.seq < 0) return;
+  const bool last = sp.part == sp.parts - 1;
+  if (!OUT && last) return;                  // no segment reads it
+  const int64_t tok0 = sp.part * a.segment;
+  const int64_t len = sp.len - tok0 < a.segment ? sp.len - tok0 : a.segment;
+  const int64_t row0 = a.cu != nullptr ? 0 : sp.seq, begin = sp.begin + tok0;
+  const T* q = (const T*)a.q + row0 * a.qb + begin * a.qt + h * a.qh;
+  const T* k = (const T*)a.k + row0 * a.kb + begin * a.kt + hk * a.kh;
+  const T* v = (const T*)a.v + row0 * a.vb + begin * a.vt + hk * a.vh + dv0;
+  T* o = (T*)a.out + row0 * a.ob + begin * a.ot + h * a.oh + dv0;
+  const int dvs = a.dv - dv0 < DVW ? a.dv - dv0 : DVW;         // columns of this slice
+
+  const double ld = (double)a.log_decay[h];
+  for (int n = tid; n <= C; n += NT) {
+    const float p = n == 0 ? 1.0f : (float)exp(n * ld);
+    pow_sh[n] = p;
+    if (n < C) {
+      end_sh[C - 1 - n] = p;
+      end_sh[C + n] = 0.0f;
+    }
+  }
+  // w^C as a sum of two floats: its rounding would add up over the chunks
+  const double wc = exp(C * ld);
+  const float wch = (float)wc, wcl = wc < 1e300 ? (float)(wc - (double)wch) : 0.0f;
+
+  f16v S[KT];
+#pragma unroll
+  for (int t = 0; t < KT; ++t) S[t] = f16v{};
+  const int sc = 32 * wave + col;            // this lane's column of the slice
+  auto state_row = [&](int t, int r) { return 32 * t + 16 * (r >> 3) + 8 * hi + (r & 7); };
+  if (OUT) {
+    if (a.state_in != nullptr) {
+      const float* p = a.state_in + (sp.seq * a.heads + h) * (int64_t)a.dk * a.dv + dv0 + sc;
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int d = state_row(t, r);
+          if (d < a.dk && sc < dvs) S[t][r] = p[(int64_t)d * a.dv];
+        }
+    }
+    if (sp.part > 0) {
+      const double ws = exp((double)a.segment * ld);
+      const float wsh = (float)ws, wsl = ws < 1e300 ? (float)(ws - (double)wsh) : 0.0f;
+      for (int64_t m = w - sp.part; m < w; ++m) {
+        const float* p = a.ws + (m * a.heads + h) * (int64_t)a.dk * a.dv + dv0 + sc;
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int d = state_row(t, r);
+            const float x = d < a.dk && sc < dvs ? p[(int64_t)d * a.dv] : 0.0f;
+            S[t][r] = __builtin_fmaf(S[t][r], wsh, __builtin_fmaf(S[t][r], wsl, x));
+          }
+      }
+    }
+  }
+
+  // units of a thread: piece u % (D / 8) of row u / (D / 8)
+  constexpr int UK = C * (DKP / 8) / NT, UV = C * (DVW / 8) / NT;
+  static_assert(UK * NT == C * (DKP / 8) && UV * NT == C * (DVW / 8), "whole units");
+  Unit<T> ku[UK], vu[UV], qu[OUT ? UK : 1];
+  auto load_chunk = [&](int64_t t0) {
+    const int n = (int)(len - t0 < C ? len - t0 : C);
+    const T* kc = k + t0 * a.kt;
+    const T* vc = v + t0 * a.vt;
+    const T* qc = q + t0 * a.qt;
+    auto bytes = [&](int64_t st, int d) { return (uint32_t)(((n - 1) * st + d) * (int64_t)sizeof(T)); };
+    const __amdgpu_buffer_rsrc_t rk = rows_rsrc(kc, bytes(a.kt, a.dk));
+    const __amdgpu_buffer_rsrc_t rv = rows_rsrc(vc, bytes(a.vt, dvs));
+#pragma unroll
+    for (int i = 0; i < UK; ++i) {
+      const int u = tid + NT * i, row = u / (DKP / 8), piece = u % (DKP / 8);
+      ku[i] = load_unit<T>(kc, rk, row, piece, n, a.kt, a.dk, a.vec_k);
+    }
+#pragma unroll
+    for (int i = 0; i < UV; ++i) {
+      const int u = tid + NT * i, row = u / (DVW / 8), piece = u % (DVW / 8);
+      vu[i] = load_unit<T>(vc, rv, row, piece, n, a.vt, dvs, a.vec_v);
+    }
+    if constexpr (OUT) {
+      const __amdgpu_buffer_rsrc_t rq = rows_rsrc(qc, bytes(a.qt, a.dk));
+#pragma unroll
+      for (int i = 0; i < UK; ++i) {
+        const int u = tid + NT * i, row = u / (DKP / 8), piece = u % (DKP / 8);
+        qu[i] = load_unit<T>(qc, rq, row, piece, n, a.qt, a.dk, a.vec_q);
+      }
+    }
+  };
+
+  if (len > 0) load_chunk(0);
+  for (int64_t t0 = 0; t0 < len; t0 += C) {
+    const int n = (int)(len - t0 < C ? len - t0 : C);
+    __syncthreads();                         // the last chunk's images are read
+#pragma unroll
+    for (int i = 0; i < UK; ++i) {
+      const int u = tid + NT * i, row = u / (DKP / 8), piece = u % (DKP / 8);
+      store_unit<T, C, DKP>(ksh, ku[i], row, piece);
+      if constexpr (OUT) store_unit<T, C, DKP>(qsh, qu[i], row, piece);
+    }
+#pragma unroll
+    for (int i = 0; i < UV; ++i) {
+      const int u = tid + NT * i, row = u / (DVW / 8), piece = u % (DVW / 8);
+      store_unit<T, C, DVW>(vsh, vu[i], row, piece);
     }
     __syncthreads();
-    for (int t = g; t < n; t += 4)
-      if (mine)
-        o[(t0 + t) * a.ot + c] = from_f<T>(
-            ((part[t][0][col] + part[t][1][col]) + (part[t][2][col] + part[t][3][col])) * a.scale);
-  }
-  if (a.state_out != nullptr) {
+    if (t0 + C < len) load_chunk(t0 + C);
+
+    u32x4 vop[CS][NL];                       // lane: column sc, tokens as token_operand
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int d = g * R + r;
-      if (mine && d < a.dk) a.state_out[sbase + (int64_t)d * a.dv] = s[r];
+    for (int s = 0; s < CS; ++s)
+#pragma unroll
+      for (int p = 0; p < NL; ++p) vop[s][p] = token_operand<C, DVW>(vsh, p, wave, s, lane, false);
+
+    if constexpr (OUT) {
+      // Scores K Q^T of 32 keys (rows) x 32 queries (columns): eight registers
+      // on end are an operand of V^T P^T as they lie.  One tile: every wave
+      // for itself; three: a tile a wave, exchanged in LDS.
+      u32x4 pop[CT > 1 ? 1 : 2][NP];
+      auto score_tile = [&](int kt, int qt, u32x4 (*ops)[NP]) {
+        f16v acc = {};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          u32x4 ak[NL], bq[NL];
+#pragma unroll
+          for (int p = 0; p < NL; ++p) {
+            ak[p] = row_operand<C, DKP>(ksh, p, kt, s, lane);
+            bq[p] = row_operand<C, DKP>(qsh, p, qt, s, lane);
+          }
+#pragma unroll
+          for (int x = 0; x < NL; ++x)
+#pragma unroll
+            for (int y = 0; y < NL; ++y)
+              if (x + y < (NL == 1 ? 1 : NP)) acc = mfma(ak[x], bq[y], acc);
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          float x[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int key = 16 * s + 8 * (j >> 2) + 4 * hi + (j & 3);
+            const int gap = 32 * (qt - kt) + col - key;
+            x[j] = gap >= 0 ? acc[8 * s + j] * pow_sh[gap >= 0 ? gap : 0] : 0.0f;
+          }
+          split8<NP>(x, ops[s]);
+        }
+      };
+      if constexpr (CT > 1) {
+        for (int tile = wave; tile < TILES; tile += NW) {
+          const int qt = tile == 0 ? 0 : 1, kt = tile == 2 ? 1 : 0;    // (0,0) (0,1) (1,1)
+          u32x4 ops[2][NP];
+          score_tile(kt, qt, ops);
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+              *reinterpret_cast<u32x4*>(psh + (((tile * 2 + s) * NP + p) * 64 + lane) * 16) =
+                  ops[s][p];
+        }
+      } else {
+        score_tile(0, 0, pop);
+      }
+      if constexpr (CT > 1) __syncthreads();
+
+      // O^T = w^(i+1) S^T Q^T + V^T P^T: rows columns of the values, columns
+      // queries.  A value that is not finite gives NaN wherever it meets a
+      // masked score's zero; then the product is taken again without such
+      // values (clean), and the queries from each one's token on become NaN.
+      f16v acc[CT];
+      int bad_from = C;                      // of this lane's column: first such token
+      for (bool clean = false;;) {
+#pragma unroll
+        for (int qt = 0; qt < CT; ++qt) acc[qt] = f16v{};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          float x[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = S[s / 2][8 * (s & 1) + j];
+          u32x4 as[NP];
+          split8<NP>(x, as);
+#pragma unroll
+          for (int qt = 0; qt < CT; ++qt) {
+#pragma unroll
+            for (int y = 0; y < NL; ++y) {
+              const u32x4 bq = row_operand<C, DKP>(qsh, y, qt, s, lane);
+#pragma unroll
+              for (int x2 = 0; x2 < NP; ++x2)
+                if (x2 + y < NP) acc[qt] = mfma(as[x2], bq, acc[qt]);
+            }
+          }
+        }
+#pragma unroll
+        for (int qt = 0; qt < CT; ++qt) {
+          const float f = pow_sh[32 * qt + col + 1];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[qt][r] *= f;
+        }
+#pragma unroll
+        for (int kt = 0; kt < CT; ++kt)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            u32x4 av[NL];
+#pragma unroll
+            for (int p = 0; p < NL; ++p) av[p] = vop[2 * kt + s][p];
+            if (clean) {
+#pragma unroll
+              for (int j = 7; j >= 0; --j) {
+                float x = 0.0f;
+#pragma unroll
+                for (int p = 0; p < NL; ++p) {
+                  const uint32_t word = av[p][j >> 1];
+                  x += __builtin_bit_cast(float, (j & 1) ? word & 0xffff0000u : word << 16);
+                }
+                if (!(__builtin_fabsf(x) < __builtin_inff())) {
+                  const int tok = 32 * kt + 16 * s + 8 * (j >> 2) + 4 * hi + (j & 3);
+                  if (tok < bad_from) bad_from = tok;
+#pragma unroll
+                  for (int p = 0; p < NL; ++p) av[p][j >> 1] &= (j & 1) ? 0xffffu : 0xffff0000u;
+                }
+              }
+            }
+#pragma unroll
+            for (int qt = kt; qt < CT; ++qt)
+#pragma unroll
+              for (int y = 0; y < NP; ++y) {
+                const u32x4 bp = CT > 1 ? *reinterpret_cast<const u32x4*>(
+                                              psh + ((((kt + qt) * 2 + s) * NP + y) * 64 + lane) * 16)
+                                        : pop[CT > 1 ? 0 : s][y];
+#pragma unroll
+                for (int p = 0; p < NL; ++p)
+                  if (p + y < NP) acc[qt] = mfma(av[p], bp, acc[qt]);
+              }
+          }
+        if (clean) break;
+        bool nan = false;
+#pragma unroll
+        for (int qt = 0; qt < CT; ++qt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) nan |= acc[qt][r] != acc[qt][r];
+        if (__ballot(nan) == 0) break;
+        clean = true;
+      }
+      if (__ballot(bad_from < C) != 0) {
+        const int other = __shfl_xor(bad_from, 32, 64);
+        if (other < bad_from) bad_from = other;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int from = __shfl(bad_from, 8 * (r >> 2) + 4 * hi + (r & 3), 64);
+#pragma unroll
+          for (int qt = 0; qt < CT; ++qt)
+            if (32 * qt + col >= from) acc[qt][r] = __builtin_nanf("");
+        }
+      }
+#pragma unroll
+      for (int qt = 0; qt < CT; ++qt) {
+        const int i = 32 * qt + col;
+        T* const orow = o + (t0 + i) * a.ot + 32 * wave;
+        if (a.vec_o) {
+          if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int c = 8 * g + 4 * hi;
+              Vec<T, 4> y;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) y.v[j] = acc[qt][4 * g + j] * a.scale;
+              if (i < n && 32 * wave + c < dvs) *reinterpret_cast<Vec<T, 4>*>(orow + c) = y;
+            }
+          } else {
+            // both halves of the wave exchange quads: eight columns a lane
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              uint32_t x[2], y[2];
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                Vec<T, 2> lo, up;
+                lo.v[0] = from_f<T>(acc[qt][8 * g + 2 * j] * a.scale);
+                lo.v[1] = from_f<T>(acc[qt][8 * g + 2 * j + 1] * a.scale);
+                up.v[0] = from_f<T>(acc[qt][8 * g + 4 + 2 * j] * a.scale);
+                up.v[1] = from_f<T>(acc[qt][8 * g + 4 + 2 * j + 1] * a.scale);
+                const auto sw = __builtin_amdgcn_permlane32_swap(
+                    __builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, up), false, false);
+                x[j] = sw[0];
+                y[j] = sw[1];
+              }
+              const int c = 16 * g + 8 * hi;
+              const u32x4 out = {x[0], x[1], y[0], y[1]};
+              if (i < n && 32 * wave + c < dvs) *reinterpret_cast<u32x4*>(orow + c) = out;
+            }
+          }
+        } else if (i < n) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int c = 8 * (r >> 2) + 4 * hi + (r & 3);
+            if (32 * wave + c < dvs) orow[c] = from_f<T>(acc[qt][r] * a.scale);
+          }
+        }
+      }
+    }
+
+    // S <- w^n S + K^T (w^(n-1-j) V)
+    const float fh = n == C ? wch : pow_sh[n], fl = n == C ? wcl : 0.0f;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[t][r] = __builtin_fmaf(S[t][r], fh, S[t][r] * fl);
+#pragma unroll
+    for (int s = 0; s < CS; ++s) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int tok = 16 * s + 8 * (j >> 2) + 4 * hi + (j & 3);
+        float y = 0.0f;
+#pragma unroll
+        for (int p = 0; p < NL; ++p) {
+          const uint32_t word = vop[s][p][j >> 1];
+          y += __builtin_bit_cast(float, (j & 1) ? word & 0xffff0000u : word << 16);
+        }
+        x[j] = y * end_sh[tok + C - n];
+      }
+      u32x4 bv[3];
+      split8<3>(x, bv);
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+#pragma unroll
+        for (int y = 0; y < NL; ++y) {
+          const u32x4 ak = token_operand<C, DKP>(ksh, y, t, s, lane, true);
+#pragma unroll
+          for (int p = 0; p < 3; ++p)
+            if (p + y < 3) S[t] = mfma(ak, bv[p], S[t]);
+        }
+      }
     }
   }
-  if (a.cu != nullptr && a.zero_rest) {   // rows of no sequence
-    T* all = (T*)a.out + h * a.oh;
-    if (b == 0)
-      for (int64_t t = g; t < begin; t += 4)
-        if (mine) all[t * a.ot + c] = from_f<T>(0.0f);
-    if (b == a.seqs - 1)
-      for (int64_t t = begin + len + g; t < a.tokens; t += 4)
-        if (mine) all[t * a.ot + c] = from_f<T>(0.0f);
+
+  float* const left = OUT ? (last ? a.state_out : nullptr) : a.ws;
+  if (left != nullptr) {
+    const int64_t at = OUT ? sp.seq : w;
+    float* p = left + (at * a.heads + h) * (int64_t)a.dk * a.dv + dv0 + sc;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int d = state_row(t, r);
+        if (d < a.dk && sc < dvs) p[(int64_t)d * a.dv] = S[t][r];
+      }
   }
+  if (OUT && a.cu != nullptr && a.zero_rest) {   // rows of no sequence
+    T* const all = (T*)a.out + h * a.oh + dv0;
+    auto clear = [&](int64_t from, int64_t to) {
+      for (int64_t t = from + tid / DVW; t < to; t += NT / DVW)
+        if (tid % DVW < dvs) all[t * a.ot + tid % DVW] = from_f<T>(0.0f);
+    };
+    if (sp.seq == 0 && sp.part == 0) clear(0, sp.begin);
+    if (sp.seq == a.seqs - 1 && last) clear(sp.begin + sp.len, a.tokens);
+  }
+}
+
+template <typename T, int DKP, int NW, int C>
+hipError_t launch_chunks(DecayArgs a, hipStream_t st) {
+  a.slices = (a.dv + 32 * NW - 1) / (32 * NW);
+  const int64_t shared = (int64_t)a.group * a.slices, kv_heads = a.heads / a.group;
+  const int64_t supers = a.segments * kv_heads;
+  const int64_t grid = (supers + 7) / 8 * 8 * shared;
+  if (grid * 64 * NW > 0xffffffffll) return hipErrorInvalidValue;
+  if (a.ws != nullptr) {
+    hipLaunchKernelGGL((decay_chunk_kernel<T, DKP, NW, C, false>), dim3((unsigned)grid),
+                       dim3(64 * NW), 0, st, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL((decay_chunk_kernel<T, DKP, NW, C, true>), dim3((unsigned)grid),
+                     dim3(64 * NW), 0, st, a);
+  return hipGetLastError();
 }
 
 template <typename T>
 hipError_t launch_decay(const DecayArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)((a.dv + 63) / 64), (unsigned)a.heads, (unsigned)a.seqs);
-  if (a.dk <= 32) hipLaunchKernelGGL((decay_recurrent_kernel<T, 8>), grid, dim3(256), 0, st, a);
-  else if (a.dk <= 64) hipLaunchKernelGGL((decay_recurrent_kernel<T, 16>), grid, dim3(256), 0, st, a);
-  else if (a.dk <= 128) hipLaunchKernelGGL((decay_recurrent_kernel<T, 32>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((decay_recurrent_kernel<T, 64>), grid, dim3(256), 0, st, a);
-  return hipGetLastError();
+  constexpr int C = sizeof(T) == 2 && parts_of<T>() == 1 ? 64 : 32;
+  if (a.dk <= 32) return launch_chunks<T, 32, 1, C>(a, st);
+  if (a.dk <= 64) return launch_chunks<T, 64, 2, C>(a, st);
+  if (a.dk <= 128) return launch_chunks<T, 128, 4, C>(a, st);
+  return launch_chunks<T, 256, 4, 32>(a, st);
 }
 
 }  // namespace
@@ -117,8 +688,11 @@ CF_API int cf_decay_attention(const CfDecayAttentionArgs* p) {
   const CfDecayAttentionArgs& x = *p;
   if (x.seqs < 0 || x.tokens < 0 || x.heads < 1 || x.kv_heads < 1 || x.heads % x.kv_heads != 0 ||
       x.heads > CF_SEQ_MAX_HEADS || x.dk < 1 || x.dk > CF_DECAY_MAX_DK || x.dv < 1 ||
-      x.dv > CF_DECAY_MAX_DV || x.dtype < 0 || x.dtype > 2 || x.seqs > CF_DECAY_MAX_SEQS)
+      x.dv > CF_DECAY_MAX_DV || x.dtype < 0 || x.dtype > 2 || x.seqs > CF_DECAY_MAX_SEQS ||
+      x.segment < 0 || x.segment % CF_DECAY_CHUNK != 0 || x.workspace_bytes < 0)
     return (int)hipErrorInvalidValue;
+  for (int64_t s : {x.q_token, x.k_token, x.v_token, x.out_token})
+    if (s < 0 || s > CF_DECAY_MAX_TOKEN_STRIDE) return (int)hipErrorInvalidValue;
   if (x.seqs == 0) return 0;
   if (!x.log_decay || (x.tokens > 0 && (!x.q || !x.k || !x.v || !x.out)))
     return (int)hipErrorInvalidValue;
@@ -132,10 +706,30 @@ CF_API int cf_decay_attention(const CfDecayAttentionArgs* p) {
   a.seqs = x.seqs; a.tokens = x.tokens;
   a.heads = (int)x.heads; a.group = (int)(x.heads / x.kv_heads);
   a.dk = (int)x.dk; a.dv = (int)x.dv;
+  a.ws = nullptr;
+  a.segment = x.tokens > 0 ? x.tokens : 1;
+  a.segments = x.seqs;
+  if (x.segment > 0 && x.segment < x.tokens) {
+    a.segment = x.segment;
+    a.segments = x.cu_seqlens ? x.tokens / x.segment + x.seqs
+                              : x.seqs * ((x.tokens + x.segment - 1) / x.segment);
+    if (!x.workspace || x.workspace_bytes / 4 / x.heads / x.dk / x.dv < a.segments)
+      return (int)hipErrorInvalidValue;
+    a.ws = (float*)x.workspace;
+  }
   a.qb = x.q_batch; a.qt = x.q_token; a.qh = x.q_head;
   a.kb = x.k_batch; a.kt = x.k_token; a.kh = x.k_head;
   a.vb = x.v_batch; a.vt = x.v_token; a.vh = x.v_head;
   a.ob = x.out_batch; a.ot = x.out_token; a.oh = x.out_head;
+  const int size = x.dtype == SEQ_F32 ? 4 : 2, per = 16 / size;
+  auto vec = [&](const void* base, int64_t b, int64_t t, int64_t h, int64_t d, int64_t whole) {
+    return (uintptr_t)base % 16 == 0 && b % per == 0 && t % per == 0 && h % per == 0 &&
+           d % whole == 0;
+  };
+  a.vec_q = vec(x.q, a.qb, a.qt, a.qh, x.dk, per);
+  a.vec_k = vec(x.k, a.kb, a.kt, a.kh, x.dk, per);
+  a.vec_v = vec(x.v, a.vb, a.vt, a.vh, x.dv, per);
+  a.vec_o = vec(x.out, a.ob, a.ot, a.oh, x.dv, per);
   a.scale = (float)x.scale;
   hipStream_t st = (hipStream_t)x.stream;
   hipError_t e;

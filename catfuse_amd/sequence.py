@@ -32,6 +32,8 @@ MAX_HEADS = 4096            # CF_SEQ_MAX_HEADS
 MAX_KEY_DIM = 256           # CF_DECAY_MAX_DK
 MAX_VALUE_DIM = 1024        # CF_DECAY_MAX_DV
 MAX_SEQUENCES = 65535       # CF_DECAY_MAX_SEQS
+CHUNK = 64                  # CF_DECAY_CHUNK
+MAX_TOKEN_STRIDE = 8000000  # CF_DECAY_MAX_TOKEN_STRIDE
 MAX_ROTARY_DIM = 512        # CF_ROTARY_MAX_DIM
 MAX_AXES = 3                # CF_ROTARY_MAX_AXES
 
@@ -167,6 +169,18 @@ def _call(fn, what: str, dev, args) -> None:
 # attention with a decay for each head
 # ---------------------------------------------------------------------------
 
+def _segment(seqs: int, tokens: int, packed: bool, heads: int, dk: int, dv: int):
+    """(tokens a segment, segments in all); (0, 0): whole sequences."""
+    width = 32 if dk <= 32 else 64 if dk <= 64 else 128
+    columns = heads * -(-dv // width)          # workgroups of one segment
+    total = tokens if packed else seqs * tokens
+    wanted = -(-1024 // columns)
+    segment = max(256, -(-total // (wanted * CHUNK)) * CHUNK)
+    if segment >= tokens or (not packed and seqs * columns >= 512):
+        return 0, 0
+    return segment, tokens // segment + seqs if packed else seqs * -(-tokens // segment)
+
+
 def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, *,
                     scale: Optional[float] = None, state: Optional[torch.Tensor] = None,
                     cu_seqlens: Optional[torch.Tensor] = None,
@@ -188,7 +202,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     state: fp32 [sequences, H, dk, dv], S before the first token (None: zeros).
     cu_seqlens: int32 or int64 [sequences + 1], in device memory and therefore
     not checked: offsets are clamped to 0 .. tokens, one below its predecessor
-    gives an empty sequence.  Rows of no sequence are zero in a new output and
+    counts as that.  Rows of no sequence are zero in a new output and
     stay as they are in one given as `out`.
     out: a tensor for the output, apart from the inputs.
 
@@ -213,6 +227,10 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
         _require(state, "state", (torch.float32,), dev)
         if state.shape != (B, H, dk, dv) or not state.is_contiguous():
             raise ValueError(f"state must be contiguous [{B}, {H}, {dk}, {dv}]")
+    for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
+        if t is not None and t.stride(-3) > MAX_TOKEN_STRIDE and t.shape[-3] > 1:
+            raise ValueError(f"tokens of {name} lie {t.stride(-3)} elements apart (at most "
+                             f"{MAX_TOKEN_STRIDE})")
     zero_rest = out is None
     out = _output(out, "out", q.shape[:-1] + (dv,), q,
                   (q, k, v, log_decay, state, cu_seqlens))
@@ -222,6 +240,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
         if zero_rest:
             out.zero_()
         return (out, left) if return_state else out
+    segment, segments = _segment(B, N, cu_seqlens is not None, H, dk, dv)
+    ws = torch.empty((segments, H, dk, dv), dtype=torch.float32, device=dev) if segments else None
     ev = _t0()
     args = _hip.DECAY_ATTENTION_ARGS.pack(
         ptr(q), ptr(k), ptr(v), ptr(log_decay), ptr(state) or 0, ptr(left) or 0, ptr(out),
@@ -229,6 +249,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
         zero_rest, _DTYPES[q.dtype], B, N, H, k.shape[-2], dk, dv, qb, q.stride(-3), q.stride(-2),
         kb, k.stride(-3), k.stride(-2), vb, v.stride(-3), v.stride(-2),
         out.stride(0) if cu_seqlens is None else 0, out.stride(-3), out.stride(-2),
+        ptr(ws) or 0, segment, 0 if ws is None else 4 * ws.numel(),
         float(dk ** -0.5 if scale is None else scale), _hip.stream(dev))
     _call(_hip.lib().cf_decay_attention, "cf_decay_attention", dev, args)
     if ev is not None:

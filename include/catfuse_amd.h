@@ -790,6 +790,8 @@ int cf_conv_sparse_noalloc(const void* x, int64_t Cin, const void* w_packed, con
 #define CF_DECAY_MAX_DK 256
 #define CF_DECAY_MAX_DV 1024
 #define CF_DECAY_MAX_SEQS 65535
+#define CF_DECAY_CHUNK 64
+#define CF_DECAY_MAX_TOKEN_STRIDE 8000000
 #define CF_ROTARY_MAX_DIM 512
 #define CF_ROTARY_MAX_AXES 3
 
@@ -800,9 +802,15 @@ int cf_conv_sparse_noalloc(const void* x, int64_t Cin, const void* w_packed, con
  * cu_seqlens null: `seqs` sequences of `tokens` rows, the strides *_batch
  * apart.  Else int32 (cu_wide 0) or int64 offsets [seqs + 1] in device memory:
  * sequence b is rows cu[b] .. cu[b + 1] - 1 of `tokens` rows; offsets are
- * clamped to 0 .. tokens and a decreasing one gives an empty sequence; rows of
+ * clamped to 0 .. tokens and one below its predecessor counts as that; rows of
  * no sequence are zeroed (zero_rest) or left as they were.  out must not
- * overlap the inputs. */
+ * overlap the inputs.
+ * segment (0, or a multiple of CF_DECAY_CHUNK): sequences are split into
+ * segments of so many tokens that run side by side, with the segments' states
+ * in the workspace: fp32 [n][heads][dk][dv], n = tokens / segment + seqs of
+ * packed sequences, seqs * ceil(tokens / segment) of equal ones; unused where
+ * segment is 0 or not below tokens.  Token strides are 0 ..
+ * CF_DECAY_MAX_TOKEN_STRIDE. */
 typedef struct CfDecayAttentionArgs {
   const void* q;
   const void* k;
@@ -815,6 +823,8 @@ typedef struct CfDecayAttentionArgs {
   int64_t cu_wide, zero_rest, dtype, seqs, tokens, heads, kv_heads, dk, dv;
   int64_t q_batch, q_token, q_head, k_batch, k_token, k_head;
   int64_t v_batch, v_token, v_head, out_batch, out_token, out_head;
+  void* workspace;
+  int64_t segment, workspace_bytes;
   double scale;
   void* stream;
 } CfDecayAttentionArgs;

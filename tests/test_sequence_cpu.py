@@ -41,6 +41,8 @@ def test_limits_mirror_the_header():
     assert sequence.MAX_VALUE_DIM == limit("CF_DECAY_MAX_DV")
     assert sequence.MAX_SEQUENCES == limit("CF_DECAY_MAX_SEQS")
     assert sequence.MAX_ROTARY_DIM == limit("CF_ROTARY_MAX_DIM")
+    assert sequence.CHUNK == limit("CF_DECAY_CHUNK")
+    assert sequence.MAX_TOKEN_STRIDE == limit("CF_DECAY_MAX_TOKEN_STRIDE")
     assert sequence.MAX_AXES == limit("CF_ROTARY_MAX_AXES")
 
 
@@ -69,9 +71,12 @@ def test_c_entries_refuse():
     for bad in (dict(seqs=-1), dict(seqs=65536), dict(tokens=-1), dict(heads=0), dict(kv_heads=0),
                 dict(heads=3, kv_heads=2), dict(heads=4097), dict(dk=0), dict(dk=257), dict(dv=0),
                 dict(dv=1025), dict(dtype=3), dict(dtype=-1), dict(q=0), dict(v=0), dict(out=0),
-                dict(log_decay=0)):
-        assert attention(**bad) == INVALID, bad
-    assert attention(seqs=0) == 0          # nothing to do, nothing launched
+                dict(log_decay=0), dict(segment=100), dict(segment=-64), dict(q_token=-1),
+                dict(out_token=8000001), dict(segment=64, tokens=65, workspace=0),
+                # 65 tokens of a packed sequence in segments of 64: up to two states of 1 x 1
+                dict(segment=64, tokens=65, workspace_bytes=4)):
+        assert attention(**dict(dict(segment=0), **bad)) == INVALID, bad
+    assert attention(seqs=0, segment=0) == 0          # nothing to do, nothing launched
 
     def step(**f):
         return L.cf_decay_attention_step(_block("CfDecayStepArgs", _hip.DECAY_STEP_ARGS, **f))
@@ -126,6 +131,12 @@ def _attn(**change):
 def test_attention_refuses(error, match, change):
     with pytest.raises(error, match=match):
         _attn(**change)
+
+
+def test_attention_refuses_far_tokens():
+    q = torch.empty(8000009).as_strided((1, 2, 1, 8), (0, 8000001, 8, 1))
+    with pytest.raises(ValueError, match="elements apart"):
+        _attn(q=q, k=torch.zeros(1, 2, 1, 8), v=torch.zeros(1, 2, 1, 6), log_decay=torch.zeros(1))
 
 
 def test_attention_refuses_packed():
