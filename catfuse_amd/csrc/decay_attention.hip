@@ -20,7 +20,7 @@
 // (2^-16 on the way to a 16-bit output) are left out.
 //
 // A value that is not finite must not reach the tokens before it, where the
-// product has a zero for it (0 * inf is NaN): see below at `clean`.
+// product has a zero for it (0 * inf is NaN): see below at `bad_from`.
 //
 // No counterpart in the reference; the causal, ordered relative of the
 // spiking attention core in attention.hip.
@@ -43,7 +43,7 @@ struct DecayArgs {
   int64_t segment, segments; // tokens a segment; segments in all at most
   int heads, group, dk, dv, slices;
   int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, ob, ot, oh;
-  int vec_q, vec_k, vec_v, vec_o;   // 16-byte accesses are aligned and whole
+  int vec;                   // 16-byte accesses are aligned and whole
   float scale;
 };
 
@@ -123,30 +123,39 @@ __device__ __forceinline__ int image_at(int part, int row, int piece) {   // in 
 template <typename T>
 struct Unit { u32x4 w[sizeof(T) / 2]; };
 
-template <typename T>
-__device__ __forceinline__ Unit<T> load_unit(const T* base, __amdgpu_buffer_rsrc_t rsrc, int row,
-                                             int piece, int n, int64_t stride, int d, int vec) {
-  Unit<T> u;
-  constexpr int PER = 16 / sizeof(T);
-  if (vec) {
+// This thread's units of a chunk's image: piece tid % (D / 8) of the rows
+// tid / (D / 8) + i NT / (D / 8).  Rows from n on and channels from d on are
+// zeros: out of the buffer's range (VEC: 16-byte loads, from aligned rows of
+// whole 16-byte pieces) or not read.
+template <typename T, int U, int D, int NT, bool VEC>
+__device__ __forceinline__ void load_units(Unit<T>* u, const T* base, int n, int64_t stride, int d) {
+  constexpr int PER = 16 / sizeof(T), ROWS = NT / (D / 8);
+  const int row = threadIdx.x / (D / 8), c0 = threadIdx.x % (D / 8) * 8;
+  if constexpr (VEC) {
+    const int st = (int)stride * (int)sizeof(T);
+    const __amdgpu_buffer_rsrc_t rsrc =
+        rows_rsrc(base, (uint32_t)((n - 1) * st + d * (int)sizeof(T)));
+    const uint32_t at = (uint32_t)(row * st + c0 * (int)sizeof(T));
 #pragma unroll
-    for (int p = 0; p < (int)(sizeof(T) / 2); ++p) {
-      const int c = piece * 8 + p * PER;
-      const uint32_t off = (uint32_t)((row * (int)stride + c) * (int)sizeof(T));
-      u.w[p] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, row < n && c < d ? off : OOB, 0, 0);
-    }
-  } else {
-    Vec<T, 8> x{};
-    if (row < n) {
+    for (int i = 0; i < U; ++i)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int c = piece * 8 + i;
-        if (c < d) x.v[i] = base[(int64_t)row * stride + c];
+      for (int p = 0; p < (int)(sizeof(T) / 2); ++p) {
+        const uint32_t off = at + (uint32_t)(i * ROWS * st + 16 * p);
+        u[i].w[p] = __builtin_amdgcn_raw_buffer_load_b128(
+            rsrc, row + i * ROWS < n && c0 + p * PER < d ? off : OOB, 0, 0);
       }
+  } else {
+    typedef Vec<T, 8> V8;
+#pragma unroll 1
+    for (int i = 0; i < U; ++i) {
+      V8 x{};
+      const int r = row + i * ROWS;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (r < n && c0 + j < d) x.v[j] = base[(int64_t)r * stride + c0 + j];
+      u[i] = __builtin_bit_cast(Unit<T>, x);
     }
-    u = __builtin_bit_cast(Unit<T>, x);
   }
-  return u;
 }
 
 template <typename T, int C, int D>
@@ -204,6 +213,13 @@ __device__ __forceinline__ u32x4 token_operand(const char* image, int part, int 
 // wave scans the offsets, 64 a time, each offset at least its predecessor.
 struct Span { int64_t seq, part, parts, begin, len; };   // of the sequence; seq < 0: none
 
+// The same value in every lane, kept in scalar registers.
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)x);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)x >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+
 __device__ __forceinline__ Span find_span(const DecayArgs& a, int64_t w) {
   Span s;
   if (a.cu == nullptr) {
@@ -243,14 +259,14 @@ __device__ __forceinline__ Span find_span(const DecayArgs& a, int64_t w) {
     if (hit != 0) {
       const int l = __ffsll((unsigned long long)hit) - 1;
       s.seq = b0 + l;
-      s.part = w - __shfl(first, l, 64);
-      s.parts = __shfl(parts, l, 64);
-      s.begin = __shfl(begin, l, 64);
-      s.len = __shfl(len, l, 64);
+      s.part = uniform(w - __shfl(first, l, 64));
+      s.parts = uniform(__shfl(parts, l, 64));
+      s.begin = uniform(__shfl(begin, l, 64));
+      s.len = uniform(__shfl(len, l, 64));
       return s;
     }
-    before += __shfl(sum, 63, 64);
-    const int64_t t = __shfl(m, 63, 64);
+    before += uniform(__shfl(sum, 63, 64));
+    const int64_t t = uniform(__shfl(m, 63, 64));
     if (t > top) top = t;
   }
   s.seq = -1;
@@ -268,8 +284,9 @@ __device__ __forceinline__ Span find_span(const DecayArgs& a, int64_t w) {
 // 32 t + 16 (r / 8) + 8 (lane / 32) + r % 8, column lane % 32: the rows of K's
 // operand are taken in that order, so that eight registers on end are an
 // operand of the next chunk's q S as they lie.
-template <typename T, int DKP, int NW, int C, bool OUT>
-__global__ __launch_bounds__(64 * NW) void decay_chunk_kernel(DecayArgs a) {
+template <typename T, int DKP, int NW, int C, bool OUT, bool VEC>
+__global__ __launch_bounds__(64 * NW, DKP <= 128 && sizeof(T) == 2 ? 2 : 1)
+void decay_chunk_kernel(DecayArgs a) {
   constexpr int NL = parts_of<T>(), NP = NL == 3 ? 3 : 2, NT = 64 * NW;
   constexpr int KT = DKP / 32, KS = DKP / 16, CT = C / 32, CS = C / 16, DVW = 32 * NW;
   constexpr int QK_BYTES = NL * C * DKP * 2, V_BYTES = NL * C * DVW * 2;
@@ -279,7 +296,7 @@ __global__ __launch_bounds__(64 * NW) void decay_chunk_kernel(DecayArgs a) {
   __shared__ __attribute__((aligned(16))) char vsh[V_BYTES];
   __shared__ __attribute__((aligned(16))) char qsh[OUT ? QK_BYTES : 16];
   __shared__ __attribute__((aligned(16))) char psh[P_BYTES];
-  __shared__ float pow_sh[C + 1];            // w^n
+  __shared__ float pow_sh[C + 1];            // scale w^n
   __shared__ float end_sh[2 * C];            // w^(C - 1 - j), then zeros
 
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, col = lane & 31;
@@ -287,34 +304,38 @@ __global__ __launch_bounds__(64 * NW) void decay_chunk_kernel(DecayArgs a) {
 
   // Query heads of one key head and the slices of their values read the same
   // rows: consecutive workgroups of one XCD (workgroup number mod 8).
-  const int shared = a.group * a.slices, kv_heads = a.heads / a.group;
-  const int64_t slot = blockIdx.x >> 3;
-  const int64_t super = slot / shared * 8 + (blockIdx.x & 7);
-  const int inner = (int)(slot % shared);
+  const unsigned shared = (unsigned)(a.group * a.slices), kv_heads = (unsigned)(a.heads / a.group);
+  const unsigned slot = blockIdx.x >> 3;
+  const unsigned super = slot / shared * 8 + (blockIdx.x & 7), inner = slot % shared;
   const int64_t w = super / kv_heads;
   if (w >= a.segments) return;
-  const int hk = (int)(super % kv_heads), h = hk * a.group + inner / a.slices;
-  const int dv0 = inner % a.slices * DVW;
+  const int hk = (int)(super % kv_heads), h = hk * a.group + (int)(inner / (unsigned)a.slices);
+  const int dv0 = (int)(inner % (unsigned)a.slices) * DVW;
 
   const Span sp = find_span(a, w);
   if (sp.seq < 0) return;
   const bool last = sp.part == sp.parts - 1;
   if (!OUT && last) return;                  // no segment reads it
-  const int64_t tok0 = sp.part * a.segment;
-  const int64_t len = sp.len - tok0 < a.segment ? sp.len - tok0 : a.segment;
-  const int64_t row0 = a.cu != nullptr ? 0 : sp.seq, begin = sp.begin + tok0;
-  const T* q = (const T*)a.q + row0 * a.qb + begin * a.qt + h * a.qh;
-  const T* k = (const T*)a.k + row0 * a.kb + begin * a.kt + hk * a.kh;
-  const T* v = (const T*)a.v + row0 * a.vb + begin * a.vt + hk * a.vh + dv0;
-  T* o = (T*)a.out + row0 * a.ob + begin * a.ot + h * a.oh + dv0;
   const int dvs = a.dv - dv0 < DVW ? a.dv - dv0 : DVW;         // columns of this slice
+  const T *kp, *vp, *qp;
+  T* op;
+  int left;                                  // tokens from here to the segment's end
+  {
+    const int64_t tok0 = sp.part * a.segment, row0 = a.cu != nullptr ? 0 : sp.seq;
+    const int64_t begin = sp.begin + tok0;
+    left = (int)(sp.len - tok0 < a.segment ? sp.len - tok0 : a.segment);
+    qp = (const T*)a.q + row0 * a.qb + begin * a.qt + h * a.qh;
+    kp = (const T*)a.k + row0 * a.kb + begin * a.kt + hk * a.kh;
+    vp = (const T*)a.v + row0 * a.vb + begin * a.vt + hk * a.vh + dv0;
+    op = (T*)a.out + row0 * a.ob + begin * a.ot + h * a.oh + dv0;
+  }
 
   const double ld = (double)a.log_decay[h];
   for (int n = tid; n <= C; n += NT) {
-    const float p = n == 0 ? 1.0f : (float)exp(n * ld);
-    pow_sh[n] = p;
+    const double p = n == 0 ? 1.0 : exp(n * ld);
+    pow_sh[n] = (float)(p * (double)a.scale);
     if (n < C) {
-      end_sh[C - 1 - n] = p;
+      end_sh[C - 1 - n] = (float)p;
       end_sh[C + n] = 0.0f;
     }
   }
@@ -326,70 +347,55 @@ __global__ __launch_bounds__(64 * NW) void decay_chunk_kernel(DecayArgs a) {
 #pragma unroll
   for (int t = 0; t < KT; ++t) S[t] = f16v{};
   const int sc = 32 * wave + col;            // this lane's column of the slice
-  auto state_row = [&](int t, int r) { return 32 * t + 16 * (r >> 3) + 8 * hi + (r & 7); };
+  // this lane's place in a state: of its first row; the others are dv apart,
+  // rows from dk on and columns from dvs on out of the buffer's range
+  const uint32_t s_at = sc < dvs ? 4u * (uint32_t)(8 * hi * a.dv + dv0 + sc) : OOB;
+  auto s_off = [&](int t, int r) {
+    return s_at + 4u * (uint32_t)((32 * t + 16 * (r >> 3) + (r & 7)) * a.dv);
+  };
+  auto state_of = [&](const float* base, int64_t i) {
+    return rows_rsrc(base + (i * a.heads + h) * (int64_t)a.dk * a.dv, 4u * a.dk * a.dv);
+  };
   if (OUT) {
     if (a.state_in != nullptr) {
-      const float* p = a.state_in + (sp.seq * a.heads + h) * (int64_t)a.dk * a.dv + dv0 + sc;
+      const __amdgpu_buffer_rsrc_t rs = state_of(a.state_in, sp.seq);
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int d = state_row(t, r);
-          if (d < a.dk && sc < dvs) S[t][r] = p[(int64_t)d * a.dv];
-        }
+        for (int r = 0; r < 16; ++r)
+          S[t][r] = __builtin_bit_cast(
+              float, __builtin_amdgcn_raw_buffer_load_b32(rs, s_off(t, r), 0, 0));
     }
     if (sp.part > 0) {
       const double ws = exp((double)a.segment * ld);
       const float wsh = (float)ws, wsl = ws < 1e300 ? (float)(ws - (double)wsh) : 0.0f;
       for (int64_t m = w - sp.part; m < w; ++m) {
-        const float* p = a.ws + (m * a.heads + h) * (int64_t)a.dk * a.dv + dv0 + sc;
+        const __amdgpu_buffer_rsrc_t rs = state_of(a.ws, m);
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int d = state_row(t, r);
-            const float x = d < a.dk && sc < dvs ? p[(int64_t)d * a.dv] : 0.0f;
+            const float x = __builtin_bit_cast(
+                float, __builtin_amdgcn_raw_buffer_load_b32(rs, s_off(t, r), 0, 0));
             S[t][r] = __builtin_fmaf(S[t][r], wsh, __builtin_fmaf(S[t][r], wsl, x));
           }
       }
     }
   }
 
-  // units of a thread: piece u % (D / 8) of row u / (D / 8)
-  constexpr int UK = C * (DKP / 8) / NT, UV = C * (DVW / 8) / NT;
+  constexpr int UK = C * (DKP / 8) / NT, UV = C * (DVW / 8) / NT;   // units of a thread
   static_assert(UK * NT == C * (DKP / 8) && UV * NT == C * (DVW / 8), "whole units");
   Unit<T> ku[UK], vu[UV], qu[OUT ? UK : 1];
-  auto load_chunk = [&](int64_t t0) {
-    const int n = (int)(len - t0 < C ? len - t0 : C);
-    const T* kc = k + t0 * a.kt;
-    const T* vc = v + t0 * a.vt;
-    const T* qc = q + t0 * a.qt;
-    auto bytes = [&](int64_t st, int d) { return (uint32_t)(((n - 1) * st + d) * (int64_t)sizeof(T)); };
-    const __amdgpu_buffer_rsrc_t rk = rows_rsrc(kc, bytes(a.kt, a.dk));
-    const __amdgpu_buffer_rsrc_t rv = rows_rsrc(vc, bytes(a.vt, dvs));
-#pragma unroll
-    for (int i = 0; i < UK; ++i) {
-      const int u = tid + NT * i, row = u / (DKP / 8), piece = u % (DKP / 8);
-      ku[i] = load_unit<T>(kc, rk, row, piece, n, a.kt, a.dk, a.vec_k);
-    }
-#pragma unroll
-    for (int i = 0; i < UV; ++i) {
-      const int u = tid + NT * i, row = u / (DVW / 8), piece = u % (DVW / 8);
-      vu[i] = load_unit<T>(vc, rv, row, piece, n, a.vt, dvs, a.vec_v);
-    }
-    if constexpr (OUT) {
-      const __amdgpu_buffer_rsrc_t rq = rows_rsrc(qc, bytes(a.qt, a.dk));
-#pragma unroll
-      for (int i = 0; i < UK; ++i) {
-        const int u = tid + NT * i, row = u / (DKP / 8), piece = u % (DKP / 8);
-        qu[i] = load_unit<T>(qc, rq, row, piece, n, a.qt, a.dk, a.vec_q);
-      }
-    }
+  auto load_chunk = [&]() {
+    const int n = left < C ? left : C;
+    load_units<T, UK, DKP, NT, VEC>(ku, kp, n, a.kt, a.dk);
+    load_units<T, UV, DVW, NT, VEC>(vu, vp, n, a.vt, dvs);
+    if constexpr (OUT) load_units<T, UK, DKP, NT, VEC>(qu, qp, n, a.qt, a.dk);
   };
 
-  if (len > 0) load_chunk(0);
-  for (int64_t t0 = 0; t0 < len; t0 += C) {
-    const int n = (int)(len - t0 < C ? len - t0 : C);
+  if (left > 0) load_chunk();
+  while (left > 0) {
+    const int n = left < C ? left : C;
     __syncthreads();                         // the last chunk's images are read
 #pragma unroll
     for (int i = 0; i < UK; ++i) {
@@ -403,13 +409,46 @@ __global__ __launch_bounds__(64 * NW) void decay_chunk_kernel(DecayArgs a) {
       store_unit<T, C, DVW>(vsh, vu[i], row, piece);
     }
     __syncthreads();
-    if (t0 + C < len) load_chunk(t0 + C);
+    left -= n;
+    kp += C * a.kt;
+    vp += C * a.vt;
+    qp += C * a.qt;
+    if (left > 0) load_chunk();
 
     u32x4 vop[CS][NL];                       // lane: column sc, tokens as token_operand
 #pragma unroll
     for (int s = 0; s < CS; ++s)
 #pragma unroll
       for (int p = 0; p < NL; ++p) vop[s][p] = token_operand<C, DVW>(vsh, p, wave, s, lane, false);
+
+    // A value that is not finite would give NaN wherever it meets a masked
+    // score's zero: it is taken out, and what depends on it set to NaN below
+    // (this lane's column: the queries from its token on, and the state).
+    int bad_from = C;
+    {
+      uint32_t any = 0u;                     // exponents of all ones, of the leading parts
+#pragma unroll
+      for (int s = 0; s < CS; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) any |= (vop[s][0][i] & 0x7f807f80u) + 0x00800080u;
+      if (__ballot((any & 0x80008000u) != 0u) != 0) {
+#pragma unroll
+        for (int s = 0; s < CS; ++s)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t m = (j & 1) ? 0x7f800000u : 0x00007f80u;
+            if ((vop[s][0][j >> 1] & m) == m) {
+              const int tok = 16 * s + 8 * (j >> 2) + 4 * hi + (j & 3);
+              if (tok < bad_from) bad_from = tok;
+#pragma unroll
+              for (int p = 0; p < NL; ++p) vop[s][p][j >> 1] &= (j & 1) ? 0xffffu : 0xffff0000u;
+            }
+          }
+        const int other = __shfl_xor(bad_from, 32, 64);
+        if (other < bad_from) bad_from = other;
+      }
+    }
+    const bool any_bad = __ballot(bad_from < C) != 0;
 
     if constexpr (OUT) {
       // Scores K Q^T of 32 keys (rows) x 32 queries (columns): eight registers
@@ -459,89 +498,53 @@ __global__ __launch_bounds__(64 * NW) void decay_chunk_kernel(DecayArgs a) {
       } else {
         score_tile(0, 0, pop);
       }
-      if constexpr (CT > 1) __syncthreads();
 
-      // O^T = w^(i+1) S^T Q^T + V^T P^T: rows columns of the values, columns
-      // queries.  A value that is not finite gives NaN wherever it meets a
-      // masked score's zero; then the product is taken again without such
-      // values (clean), and the queries from each one's token on become NaN.
+      // O^T = scale w^(i+1) S^T Q^T + V^T P^T: rows columns of the values,
+      // columns queries (P holds the scale).
       f16v acc[CT];
-      int bad_from = C;                      // of this lane's column: first such token
-      for (bool clean = false;;) {
 #pragma unroll
-        for (int qt = 0; qt < CT; ++qt) acc[qt] = f16v{};
+      for (int qt = 0; qt < CT; ++qt) acc[qt] = f16v{};
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          float x[8];
+      for (int s = 0; s < KS; ++s) {
+        float x[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = S[s / 2][8 * (s & 1) + j];
-          u32x4 as[NP];
-          split8<NP>(x, as);
-#pragma unroll
-          for (int qt = 0; qt < CT; ++qt) {
-#pragma unroll
-            for (int y = 0; y < NL; ++y) {
-              const u32x4 bq = row_operand<C, DKP>(qsh, y, qt, s, lane);
-#pragma unroll
-              for (int x2 = 0; x2 < NP; ++x2)
-                if (x2 + y < NP) acc[qt] = mfma(as[x2], bq, acc[qt]);
-            }
-          }
-        }
+        for (int j = 0; j < 8; ++j) x[j] = S[s / 2][8 * (s & 1) + j];
+        u32x4 as[NP];
+        split8<NP>(x, as);
 #pragma unroll
         for (int qt = 0; qt < CT; ++qt) {
-          const float f = pow_sh[32 * qt + col + 1];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) acc[qt][r] *= f;
-        }
+          for (int y = 0; y < NL; ++y) {
+            const u32x4 bq = row_operand<C, DKP>(qsh, y, qt, s, lane);
 #pragma unroll
-        for (int kt = 0; kt < CT; ++kt)
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            u32x4 av[NL];
-#pragma unroll
-            for (int p = 0; p < NL; ++p) av[p] = vop[2 * kt + s][p];
-            if (clean) {
-#pragma unroll
-              for (int j = 7; j >= 0; --j) {
-                float x = 0.0f;
-#pragma unroll
-                for (int p = 0; p < NL; ++p) {
-                  const uint32_t word = av[p][j >> 1];
-                  x += __builtin_bit_cast(float, (j & 1) ? word & 0xffff0000u : word << 16);
-                }
-                if (!(__builtin_fabsf(x) < __builtin_inff())) {
-                  const int tok = 32 * kt + 16 * s + 8 * (j >> 2) + 4 * hi + (j & 3);
-                  if (tok < bad_from) bad_from = tok;
-#pragma unroll
-                  for (int p = 0; p < NL; ++p) av[p][j >> 1] &= (j & 1) ? 0xffffu : 0xffff0000u;
-                }
-              }
-            }
-#pragma unroll
-            for (int qt = kt; qt < CT; ++qt)
-#pragma unroll
-              for (int y = 0; y < NP; ++y) {
-                const u32x4 bp = CT > 1 ? *reinterpret_cast<const u32x4*>(
-                                              psh + ((((kt + qt) * 2 + s) * NP + y) * 64 + lane) * 16)
-                                        : pop[CT > 1 ? 0 : s][y];
-#pragma unroll
-                for (int p = 0; p < NL; ++p)
-                  if (p + y < NP) acc[qt] = mfma(av[p], bp, acc[qt]);
-              }
+            for (int x2 = 0; x2 < NP; ++x2)
+              if (x2 + y < NP) acc[qt] = mfma(as[x2], bq, acc[qt]);
           }
-        if (clean) break;
-        bool nan = false;
-#pragma unroll
-        for (int qt = 0; qt < CT; ++qt)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) nan |= acc[qt][r] != acc[qt][r];
-        if (__ballot(nan) == 0) break;
-        clean = true;
+        }
       }
-      if (__ballot(bad_from < C) != 0) {
-        const int other = __shfl_xor(bad_from, 32, 64);
-        if (other < bad_from) bad_from = other;
+#pragma unroll
+      for (int qt = 0; qt < CT; ++qt) {
+        const float f = pow_sh[32 * qt + col + 1];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[qt][r] *= f;
+      }
+      if constexpr (CT > 1) __syncthreads();
+#pragma unroll
+      for (int kt = 0; kt < CT; ++kt)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int qt = kt; qt < CT; ++qt)
+#pragma unroll
+            for (int y = 0; y < NP; ++y) {
+              const u32x4 bp = CT > 1 ? *reinterpret_cast<const u32x4*>(
+                                            psh + ((((kt + qt) * 2 + s) * NP + y) * 64 + lane) * 16)
+                                      : pop[CT > 1 ? 0 : s][y];
+#pragma unroll
+              for (int p = 0; p < NL; ++p)
+                if (p + y < NP) acc[qt] = mfma(vop[2 * kt + s][p], bp, acc[qt]);
+            }
+      if (any_bad) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int from = __shfl(bad_from, 8 * (r >> 2) + 4 * hi + (r & 3), 64);
@@ -550,19 +553,25 @@ __global__ __launch_bounds__(64 * NW) void decay_chunk_kernel(DecayArgs a) {
             if (32 * qt + col >= from) acc[qt][r] = __builtin_nanf("");
         }
       }
+      if constexpr (VEC) {
+        // rows from n on and columns from dvs on: out of the buffer's range
+        const int st = (int)a.ot * (int)sizeof(T);
+        const __amdgpu_buffer_rsrc_t ro =
+            rows_rsrc(op, (uint32_t)((n - 1) * st + dvs * (int)sizeof(T)));
+        auto at = [&](int i, int c) {
+          return i < n && c < dvs ? (uint32_t)(i * st + c * (int)sizeof(T)) : OOB;
+        };
 #pragma unroll
-      for (int qt = 0; qt < CT; ++qt) {
-        const int i = 32 * qt + col;
-        T* const orow = o + (t0 + i) * a.ot + 32 * wave;
-        if (a.vec_o) {
+        for (int qt = 0; qt < CT; ++qt) {
+          const int i = 32 * qt + col;
           if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-              const int c = 8 * g + 4 * hi;
               Vec<T, 4> y;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) y.v[j] = acc[qt][4 * g + j] * a.scale;
-              if (i < n && 32 * wave + c < dvs) *reinterpret_cast<Vec<T, 4>*>(orow + c) = y;
+              for (int j = 0; j < 4; ++j) y.v[j] = acc[qt][4 * g + j];
+              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), ro,
+                                                     at(i, 32 * wave + 8 * g + 4 * hi), 0, 0);
             }
           } else {
             // both halves of the wave exchange quads: eight columns a lane
@@ -572,32 +581,40 @@ __global__ __launch_bounds__(64 * NW) void decay_chunk_kernel(DecayArgs a) {
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
                 Vec<T, 2> lo, up;
-                lo.v[0] = from_f<T>(acc[qt][8 * g + 2 * j] * a.scale);
-                lo.v[1] = from_f<T>(acc[qt][8 * g + 2 * j + 1] * a.scale);
-                up.v[0] = from_f<T>(acc[qt][8 * g + 4 + 2 * j] * a.scale);
-                up.v[1] = from_f<T>(acc[qt][8 * g + 4 + 2 * j + 1] * a.scale);
+                lo.v[0] = from_f<T>(acc[qt][8 * g + 2 * j]);
+                lo.v[1] = from_f<T>(acc[qt][8 * g + 2 * j + 1]);
+                up.v[0] = from_f<T>(acc[qt][8 * g + 4 + 2 * j]);
+                up.v[1] = from_f<T>(acc[qt][8 * g + 4 + 2 * j + 1]);
                 const auto sw = __builtin_amdgcn_permlane32_swap(
                     __builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, up), false, false);
                 x[j] = sw[0];
                 y[j] = sw[1];
               }
-              const int c = 16 * g + 8 * hi;
               const u32x4 out = {x[0], x[1], y[0], y[1]};
-              if (i < n && 32 * wave + c < dvs) *reinterpret_cast<u32x4*>(orow + c) = out;
+              __builtin_amdgcn_raw_buffer_store_b128(out, ro, at(i, 32 * wave + 16 * g + 8 * hi), 0,
+                                                     0);
             }
           }
-        } else if (i < n) {
+        }
+      } else {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int c = 8 * (r >> 2) + 4 * hi + (r & 3);
-            if (32 * wave + c < dvs) orow[c] = from_f<T>(acc[qt][r] * a.scale);
+        for (int qt = 0; qt < CT; ++qt) {
+          const int i = 32 * qt + col;
+          T* const orow = op + i * a.ot + 32 * wave;
+          if (i < n) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int c = 8 * (r >> 2) + 4 * hi + (r & 3);
+              if (32 * wave + c < dvs) orow[c] = from_f<T>(acc[qt][r]);
+            }
           }
         }
       }
+      op += C * a.ot;
     }
 
     // S <- w^n S + K^T (w^(n-1-j) V)
-    const float fh = n == C ? wch : pow_sh[n], fl = n == C ? wcl : 0.0f;
+    const float fh = n == C ? wch : end_sh[C - 1 - n], fl = n == C ? wcl : 0.0f;
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -612,7 +629,8 @@ __global__ __launch_bounds__(64 * NW) void decay_chunk_kernel(DecayArgs a) {
 #pragma unroll
         for (int p = 0; p < NL; ++p) {
           const uint32_t word = vop[s][p][j >> 1];
-          y += __builtin_bit_cast(float, (j & 1) ? word & 0xffff0000u : word << 16);
+          const float z = __builtin_bit_cast(float, (j & 1) ? word & 0xffff0000u : word << 16);
+          y = p == 0 ? z : y + z;
         }
         x[j] = y * end_sh[tok + C - n];
       }
@@ -629,19 +647,23 @@ __global__ __launch_bounds__(64 * NW) void decay_chunk_kernel(DecayArgs a) {
         }
       }
     }
+    if (any_bad && bad_from < C) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[t][r] = __builtin_nanf("");
+    }
   }
 
-  float* const left = OUT ? (last ? a.state_out : nullptr) : a.ws;
-  if (left != nullptr) {
-    const int64_t at = OUT ? sp.seq : w;
-    float* p = left + (at * a.heads + h) * (int64_t)a.dk * a.dv + dv0 + sc;
+  float* const to = OUT ? (last ? a.state_out : nullptr) : a.ws;
+  if (to != nullptr) {
+    const __amdgpu_buffer_rsrc_t rs = state_of(to, OUT ? sp.seq : w);
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int d = state_row(t, r);
-        if (d < a.dk && sc < dvs) p[(int64_t)d * a.dv] = S[t][r];
-      }
+      for (int r = 0; r < 16; ++r)
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, (float)S[t][r]), rs,
+                                              s_off(t, r), 0, 0);
   }
   if (OUT && a.cu != nullptr && a.zero_rest) {   // rows of no sequence
     T* const all = (T*)a.out + h * a.oh + dv0;
@@ -654,31 +676,35 @@ __global__ __launch_bounds__(64 * NW) void decay_chunk_kernel(DecayArgs a) {
   }
 }
 
-template <typename T, int DKP, int NW, int C>
+template <typename T, int DKP, int NW, int C, bool VEC>
 hipError_t launch_chunks(DecayArgs a, hipStream_t st) {
   a.slices = (a.dv + 32 * NW - 1) / (32 * NW);
   const int64_t shared = (int64_t)a.group * a.slices, kv_heads = a.heads / a.group;
-  const int64_t supers = a.segments * kv_heads;
-  const int64_t grid = (supers + 7) / 8 * 8 * shared;
+  const int64_t grid = (a.segments * kv_heads + 7) / 8 * 8 * shared;
   if (grid * 64 * NW > 0xffffffffll) return hipErrorInvalidValue;
   if (a.ws != nullptr) {
-    hipLaunchKernelGGL((decay_chunk_kernel<T, DKP, NW, C, false>), dim3((unsigned)grid),
+    hipLaunchKernelGGL((decay_chunk_kernel<T, DKP, NW, C, false, VEC>), dim3((unsigned)grid),
                        dim3(64 * NW), 0, st, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((decay_chunk_kernel<T, DKP, NW, C, true>), dim3((unsigned)grid),
+  hipLaunchKernelGGL((decay_chunk_kernel<T, DKP, NW, C, true, VEC>), dim3((unsigned)grid),
                      dim3(64 * NW), 0, st, a);
   return hipGetLastError();
 }
 
+template <typename T, bool VEC>
+hipError_t launch_decay_v(const DecayArgs& a, hipStream_t st) {
+  constexpr int C = sizeof(T) == 2 && parts_of<T>() == 1 ? 64 : 32;
+  if (a.dk <= 32) return launch_chunks<T, 32, 1, C, VEC>(a, st);
+  if (a.dk <= 64) return launch_chunks<T, 64, 2, C, VEC>(a, st);
+  if (a.dk <= 128) return launch_chunks<T, 128, 4, C, VEC>(a, st);
+  return launch_chunks<T, 256, 4, 32, VEC>(a, st);
+}
+
 template <typename T>
 hipError_t launch_decay(const DecayArgs& a, hipStream_t st) {
-  constexpr int C = sizeof(T) == 2 && parts_of<T>() == 1 ? 64 : 32;
-  if (a.dk <= 32) return launch_chunks<T, 32, 1, C>(a, st);
-  if (a.dk <= 64) return launch_chunks<T, 64, 2, C>(a, st);
-  if (a.dk <= 128) return launch_chunks<T, 128, 4, C>(a, st);
-  return launch_chunks<T, 256, 4, 32>(a, st);
+  return a.vec ? launch_decay_v<T, true>(a, st) : launch_decay_v<T, false>(a, st);
 }
 
 }  // namespace
@@ -689,7 +715,7 @@ CF_API int cf_decay_attention(const CfDecayAttentionArgs* p) {
   if (x.seqs < 0 || x.tokens < 0 || x.heads < 1 || x.kv_heads < 1 || x.heads % x.kv_heads != 0 ||
       x.heads > CF_SEQ_MAX_HEADS || x.dk < 1 || x.dk > CF_DECAY_MAX_DK || x.dv < 1 ||
       x.dv > CF_DECAY_MAX_DV || x.dtype < 0 || x.dtype > 2 || x.seqs > CF_DECAY_MAX_SEQS ||
-      x.segment < 0 || x.segment % CF_DECAY_CHUNK != 0 || x.workspace_bytes < 0)
+      x.tokens > CF_DECAY_MAX_TOKENS || x.segment < 0 || x.segment % CF_DECAY_CHUNK != 0 || x.workspace_bytes < 0)
     return (int)hipErrorInvalidValue;
   for (int64_t s : {x.q_token, x.k_token, x.v_token, x.out_token})
     if (s < 0 || s > CF_DECAY_MAX_TOKEN_STRIDE) return (int)hipErrorInvalidValue;
@@ -722,14 +748,12 @@ CF_API int cf_decay_attention(const CfDecayAttentionArgs* p) {
   a.vb = x.v_batch; a.vt = x.v_token; a.vh = x.v_head;
   a.ob = x.out_batch; a.ot = x.out_token; a.oh = x.out_head;
   const int size = x.dtype == SEQ_F32 ? 4 : 2, per = 16 / size;
-  auto vec = [&](const void* base, int64_t b, int64_t t, int64_t h, int64_t d, int64_t whole) {
+  auto vec = [&](const void* base, int64_t b, int64_t t, int64_t h, int64_t d) {
     return (uintptr_t)base % 16 == 0 && b % per == 0 && t % per == 0 && h % per == 0 &&
-           d % whole == 0;
+           d % per == 0;
   };
-  a.vec_q = vec(x.q, a.qb, a.qt, a.qh, x.dk, per);
-  a.vec_k = vec(x.k, a.kb, a.kt, a.kh, x.dk, per);
-  a.vec_v = vec(x.v, a.vb, a.vt, a.vh, x.dv, per);
-  a.vec_o = vec(x.out, a.ob, a.ot, a.oh, x.dv, per);
+  a.vec = vec(x.q, a.qb, a.qt, a.qh, x.dk) && vec(x.k, a.kb, a.kt, a.kh, x.dk) &&
+          vec(x.v, a.vb, a.vt, a.vh, x.dv) && vec(x.out, a.ob, a.ot, a.oh, x.dv);
   a.scale = (float)x.scale;
   hipStream_t st = (hipStream_t)x.stream;
   hipError_t e;

@@ -790,6 +790,7 @@ int cf_conv_sparse_noalloc(const void* x, int64_t Cin, const void* w_packed, con
 #define CF_DECAY_MAX_DK 256
 #define CF_DECAY_MAX_DV 1024
 #define CF_DECAY_MAX_SEQS 65535
+#define CF_DECAY_MAX_TOKENS 2000000000
 #define CF_DECAY_CHUNK 64
 #define CF_DECAY_MAX_TOKEN_STRIDE 8000000
 #define CF_ROTARY_MAX_DIM 512
