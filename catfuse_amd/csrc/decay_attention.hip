@@ -37,7 +37,8 @@ struct DecayArgs {
   float* state_out;
   void* out;
   const void* cu;
-  float* ws;                 // states of segments [segment][heads][dk][dv]
+  float* ws;                 // states of segments [segment][heads][dk][dv], or null
+  void* spans;               // which sequence's they are: Span [segment]
   int cu_wide, zero_rest;
   int64_t seqs, tokens;      // tokens: rows in all (packed) or of each sequence
   int64_t segment, segments; // tokens a segment; segments in all at most
@@ -77,21 +78,22 @@ __device__ __forceinline__ uint32_t pack_rounded(float lo, float hi) {
 // exact), the last of fewer than three rounded (cutting it off would shrink
 // every number).
 template <int N>
-__device__ __forceinline__ void split8(const float* x, u32x4* out) {
+__device__ __forceinline__ void split2(float a, float b, u32x4* out, int p) {
 #pragma unroll
-  for (int p = 0; p < 4; ++p) {
-    float a = x[2 * p], b = x[2 * p + 1];
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      if (n == N - 1 && N < 3) {
-        out[n][p] = pack_rounded(a, b);
-      } else {
-        out[n][p] = pack_high(a, b);
-        a -= high_part(a);
-        b -= high_part(b);
-      }
+  for (int n = 0; n < N; ++n) {
+    if (n == N - 1 && N < 3) {
+      out[n][p] = pack_rounded(a, b);
+    } else {
+      out[n][p] = pack_high(a, b);
+      a -= high_part(a);
+      b -= high_part(b);
     }
   }
+}
+template <int N>
+__device__ __forceinline__ void split8(const float* x, u32x4* out) {
+#pragma unroll
+  for (int p = 0; p < 4; ++p) split2<N>(x[2 * p], x[2 * p + 1], out, p);
 }
 
 __device__ __forceinline__ f16v mfma(u32x4 a, u32x4 b, f16v c) {
@@ -158,6 +160,44 @@ __device__ __forceinline__ void load_units(Unit<T>* u, const T* base, int n, int
   }
 }
 
+// The same for bf16, straight into the image: lane l of a wave's i-th copy fills
+// the 16 bytes l of its 1 KB.  Not known to the compiler, which would wait for
+// these copies at every read of LDS; the kernel waits (wait_copies) before the
+// barrier that hands an image over.
+typedef int v4i __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void copy16(v4i rsrc, uint32_t off, uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %0, %1, 0 offen lds"
+      :
+      : "v"(off), "s"(rsrc), "s"(lds)
+      : "memory", "m0");
+}
+template <int LATER>   // all but the LATER accesses of memory issued last
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LATER) : "memory");
+}
+template <int U, int D, int NW>
+__device__ __forceinline__ void copy_units(char* image, const bf16_t* base, int n, int64_t stride,
+                                           int d, int wave, int lane) {
+  const int st = (int)stride * 2;
+  const uint64_t p = (uint64_t)(uintptr_t)base;
+  v4i rsrc;
+  rsrc[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)p);
+  rsrc[1] = __builtin_amdgcn_readfirstlane((int)((uint32_t)(p >> 32) & 0xffffu));
+  rsrc[2] = __builtin_amdgcn_readfirstlane((n - 1) * st + d * 2);
+  rsrc[3] = 0x00020000;
+  const uint32_t to = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)image;
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const int u = (i * NW + wave) * 64 + lane, row = u / (D / 8);
+    const int c = ((u % (D / 8)) ^ swizzle<D>(row)) * 8;
+    copy16(rsrc, row < n && c < d ? (uint32_t)(row * st + c * 2) : OOB,
+           __builtin_amdgcn_readfirstlane(to + (uint32_t)((i * NW + wave) * 1024)));
+  }
+}
+
 template <typename T, int C, int D>
 __device__ __forceinline__ void store_unit(char* image, const Unit<T>& u, int row, int piece) {
   if constexpr (parts_of<T>() == 1) {
@@ -177,11 +217,17 @@ __device__ __forceinline__ void store_unit(char* image, const Unit<T>& u, int ro
 }
 
 // An operand of a product over the channels: lane l holds row 32 tile + l % 32,
-// channels 16 s + 8 (l / 32) .. + 7.
+// channels 16 s + 8 (l / 32) .. + 7.  `at`: row_base plus the image's offset (a
+// multiple of a row's bytes, so that the pieces' bits can be exchanged in it).
+template <int D>
+__device__ __forceinline__ uint32_t row_base(int lane) {
+  const int row = lane & 31;
+  return (uint32_t)(row * D * 2 + (((lane >> 5) ^ swizzle<D>(row)) << 4));
+}
 template <int C, int D>
-__device__ __forceinline__ u32x4 row_operand(const char* image, int part, int tile, int s, int lane) {
-  return *reinterpret_cast<const u32x4*>(
-      image + image_at<C, D>(part, 32 * tile + (lane & 31), 2 * s + (lane >> 5)));
+__device__ __forceinline__ u32x4 row_operand(const char* lds, uint32_t at, int part, int tile, int s) {
+  return *reinterpret_cast<const u32x4*>(lds + (at ^ (uint32_t)(s << 5)) +
+                                         (part * C + 32 * tile) * D * 2);
 }
 
 // An operand of a product over the tokens: lane l holds a channel, and of the
@@ -191,16 +237,19 @@ __device__ __forceinline__ u32x4 row_operand(const char* image, int part, int ti
 // address of token (l % 16) / 4, channels 4 (l % 4) .. + 3 and gets channel
 // l % 16 of the four tokens.  `turned`: the channels in the order in which the
 // rows of an accumulator are contiguous for the lanes (below at S).
-template <int C, int D>
-__device__ __forceinline__ u32x4 token_operand(const char* image, int part, int tile, int s,
-                                               int lane, bool turned) {
+template <int D>
+__device__ __forceinline__ uint32_t token_base(int lane, bool turned) {
   const int four = lane & 3, block = turned ? ((four & 1) << 1) | (four >> 1) : four;
-  const int c = 32 * tile + ((lane >> 4) & 1) * 16 + 4 * block;
+  const int row = 4 * (lane >> 5) + ((lane & 15) >> 2), piece = 2 * ((lane >> 4) & 1) + (block >> 1);
+  return (uint32_t)(row * D * 2 + ((piece ^ swizzle<D>(row)) << 4) + (block & 1) * 8);
+}
+template <int C, int D>
+__device__ __forceinline__ u32x4 token_operand(const char* lds, uint32_t at, int part, int tile, int s) {
   u32x4 r;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    const int row = 16 * s + 8 * e + 4 * (lane >> 5) + ((lane & 15) >> 2);
-    const char* p = image + image_at<C, D>(part, row, c >> 3) + (c & 4) * 2;
+    // swizzle(row + 8) = swizzle(row) ^ 2; of 16 rows on it is the same
+    const char* p = lds + (at ^ (uint32_t)((tile << 6) | (e << 5))) + (part * C + 16 * s + 8 * e) * D * 2;
     const u32x2 t = __builtin_bit_cast(
         u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p));
     r[2 * e] = t[0];
@@ -211,7 +260,8 @@ __device__ __forceinline__ u32x4 token_operand(const char* image, int part, int 
 
 // Which (sequence, segment) a segment number is.  Packed sequences: every
 // wave scans the offsets, 64 a time, each offset at least its predecessor.
-struct Span { int64_t seq, part, parts, begin, len; };   // of the sequence; seq < 0: none
+struct alignas(16) Span { int64_t seq, part, parts, begin, len; };   // seq < 0: none
+static_assert(sizeof(Span) == CF_DECAY_SPAN_BYTES, "the workspace has one a segment");
 
 // The same value in every lane, kept in scalar registers.
 __device__ __forceinline__ int64_t uniform(int64_t x) {
@@ -274,29 +324,37 @@ __device__ __forceinline__ Span find_span(const DecayArgs& a, int64_t w) {
   return s;
 }
 
+// The same, as the launch of the segments' own states noted it.
+__device__ __forceinline__ Span read_span(const DecayArgs& a, int64_t w) {
+  const Span s = reinterpret_cast<const Span*>(a.spans)[w];
+  return {uniform(s.seq), uniform(s.part), uniform(s.parts), uniform(s.begin), uniform(s.len)};
+}
+
 // A workgroup takes a segment of a sequence, one head, 32 NW columns of the
 // values; wave w the columns 32 w .. + 31 with their part of S (all DKP rows,
 // in accumulators) throughout.  OUT: the outputs of the segment, from the state
-// that the segments before it left in the workspace (Horner's rule over them);
-// else the segment's own contribution to the state, for the others.
+// before it in the workspace; else the segment's own contribution to the
+// state, to the workspace (decay_join_kernel makes the one of the other).
 //
 // S as accumulators: tile t, register r of a lane is row (channel of k)
 // 32 t + 16 (r / 8) + 8 (lane / 32) + r % 8, column lane % 32: the rows of K's
 // operand are taken in that order, so that eight registers on end are an
 // operand of the next chunk's q S as they lie.
 template <typename T, int DKP, int NW, int C, bool OUT, bool VEC>
-__global__ __launch_bounds__(64 * NW, DKP <= 128 && sizeof(T) == 2 ? 2 : 1)
+__global__ __launch_bounds__(64 * NW, DKP > 128 || sizeof(T) == 4 ? 1 : (VEC && parts_of<T>() == 1 ? 3 : 2))
 void decay_chunk_kernel(DecayArgs a) {
   constexpr int NL = parts_of<T>(), NP = NL == 3 ? 3 : 2, NT = 64 * NW;
   constexpr int KT = DKP / 32, KS = DKP / 16, CT = C / 32, CS = C / 16, DVW = 32 * NW;
   constexpr int QK_BYTES = NL * C * DKP * 2, V_BYTES = NL * C * DVW * 2;
   constexpr int TILES = CT * (CT + 1) / 2;                     // score tiles that are not masked
   constexpr int P_BYTES = CT > 1 && OUT ? TILES * 2 * NP * 1024 : 16;
-  __shared__ __attribute__((aligned(16))) char ksh[QK_BYTES];
-  __shared__ __attribute__((aligned(16))) char vsh[V_BYTES];
-  __shared__ __attribute__((aligned(16))) char qsh[OUT ? QK_BYTES : 16];
+  constexpr bool ASYNC = VEC && NL == 1;     // copied straight to LDS, two images by turns
+  constexpr int IMAGES = ASYNC ? 2 : 1;
+  constexpr int Q_AT = QK_BYTES, V_AT = Q_AT + (OUT ? QK_BYTES : 0), IMAGE = V_AT + V_BYTES;
+  __shared__ __attribute__((aligned(512))) char lds[IMAGES * IMAGE];   // of K, Q and V
   __shared__ __attribute__((aligned(16))) char psh[P_BYTES];
-  __shared__ float pow_sh[C + 1];            // scale w^n
+  __shared__ float pow_all[32 + C + 1];      // 32 zeros, then scale w^n
+  float* const pow_sh = pow_all + 32;
   __shared__ float end_sh[2 * C];            // w^(C - 1 - j), then zeros
 
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, col = lane & 31;
@@ -312,7 +370,8 @@ void decay_chunk_kernel(DecayArgs a) {
   const int hk = (int)(super % kv_heads), h = hk * a.group + (int)(inner / (unsigned)a.slices);
   const int dv0 = (int)(inner % (unsigned)a.slices) * DVW;
 
-  const Span sp = find_span(a, w);
+  const Span sp = OUT && a.ws != nullptr ? read_span(a, w) : find_span(a, w);
+  if (!OUT && hk == 0 && inner == 0 && tid == 0) reinterpret_cast<Span*>(a.spans)[w] = sp;
   if (sp.seq < 0) return;
   const bool last = sp.part == sp.parts - 1;
   if (!OUT && last) return;                  // no segment reads it
@@ -331,6 +390,7 @@ void decay_chunk_kernel(DecayArgs a) {
   }
 
   const double ld = (double)a.log_decay[h];
+  if (tid < 32) pow_all[tid] = 0.0f;
   for (int n = tid; n <= C; n += NT) {
     const double p = n == 0 ? 1.0 : exp(n * ld);
     pow_sh[n] = (float)(p * (double)a.scale);
@@ -339,9 +399,12 @@ void decay_chunk_kernel(DecayArgs a) {
       end_sh[C + n] = 0.0f;
     }
   }
-  // w^C as a sum of two floats: its rounding would add up over the chunks
+  // The rounding of w^C would add up over the chunks: every eighth makes up
+  // for eight of them.
   const double wc = exp(C * ld);
-  const float wch = (float)wc, wcl = wc < 1e300 ? (float)(wc - (double)wch) : 0.0f;
+  const float wch = (float)wc;
+  const float wc8 = wc > 1e-30 && wc < 1e30 ? (float)(8.0 * (wc - (double)wch) / wc) : 0.0f;
+  int chunk = 0;
 
   f16v S[KT];
 #pragma unroll
@@ -357,8 +420,9 @@ void decay_chunk_kernel(DecayArgs a) {
     return rows_rsrc(base + (i * a.heads + h) * (int64_t)a.dk * a.dv, 4u * a.dk * a.dv);
   };
   if (OUT) {
-    if (a.state_in != nullptr) {
-      const __amdgpu_buffer_rsrc_t rs = state_of(a.state_in, sp.seq);
+    const float* const from = sp.part > 0 ? a.ws : a.state_in;
+    if (from != nullptr) {
+      const __amdgpu_buffer_rsrc_t rs = state_of(from, sp.part > 0 ? w : sp.seq);
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -366,49 +430,53 @@ void decay_chunk_kernel(DecayArgs a) {
           S[t][r] = __builtin_bit_cast(
               float, __builtin_amdgcn_raw_buffer_load_b32(rs, s_off(t, r), 0, 0));
     }
-    if (sp.part > 0) {
-      const double ws = exp((double)a.segment * ld);
-      const float wsh = (float)ws, wsl = ws < 1e300 ? (float)(ws - (double)wsh) : 0.0f;
-      for (int64_t m = w - sp.part; m < w; ++m) {
-        const __amdgpu_buffer_rsrc_t rs = state_of(a.ws, m);
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float x = __builtin_bit_cast(
-                float, __builtin_amdgcn_raw_buffer_load_b32(rs, s_off(t, r), 0, 0));
-            S[t][r] = __builtin_fmaf(S[t][r], wsh, __builtin_fmaf(S[t][r], wsl, x));
-          }
-      }
-    }
   }
 
   constexpr int UK = C * (DKP / 8) / NT, UV = C * (DVW / 8) / NT;   // units of a thread
   static_assert(UK * NT == C * (DKP / 8) && UV * NT == C * (DVW / 8), "whole units");
   Unit<T> ku[UK], vu[UV], qu[OUT ? UK : 1];
+  int image = 0;                             // where the next chunk's lies
   auto load_chunk = [&]() {
     const int n = left < C ? left : C;
-    load_units<T, UK, DKP, NT, VEC>(ku, kp, n, a.kt, a.dk);
-    load_units<T, UV, DVW, NT, VEC>(vu, vp, n, a.vt, dvs);
-    if constexpr (OUT) load_units<T, UK, DKP, NT, VEC>(qu, qp, n, a.qt, a.dk);
+    if constexpr (ASYNC) {
+      copy_units<UK, DKP, NW>(lds + image, kp, n, a.kt, a.dk, wave, lane);
+      if constexpr (OUT) copy_units<UK, DKP, NW>(lds + image + Q_AT, qp, n, a.qt, a.dk, wave, lane);
+      copy_units<UV, DVW, NW>(lds + image + V_AT, vp, n, a.vt, dvs, wave, lane);
+    } else {
+      load_units<T, UK, DKP, NT, VEC>(ku, kp, n, a.kt, a.dk);
+      load_units<T, UV, DVW, NT, VEC>(vu, vp, n, a.vt, dvs);
+      if constexpr (OUT) load_units<T, UK, DKP, NT, VEC>(qu, qp, n, a.qt, a.dk);
+    }
   };
 
   if (left > 0) load_chunk();
+  if constexpr (ASYNC) wait_copies<0>();
   while (left > 0) {
     const int n = left < C ? left : C;
-    __syncthreads();                         // the last chunk's images are read
+    const uint32_t at_row = row_base<DKP>(lane) + (ASYNC ? image : 0);
+    const uint32_t at_key = token_base<DKP>(lane, true) + (ASYNC ? image : 0);
+    const uint32_t at_value = (token_base<DVW>(lane, false) ^ (uint32_t)(wave << 6)) +
+                              (ASYNC ? image : 0);
+    if constexpr (ASYNC) {
+      // this chunk's copies are older than the last one's stores (2 CT)
+      wait_copies<OUT ? 2 * CT : 0>();
+      __syncthreads();                       // ... and the other image is read
+      image = IMAGE - image;
+    } else {
+      __syncthreads();                       // the last chunk's images are read
 #pragma unroll
-    for (int i = 0; i < UK; ++i) {
-      const int u = tid + NT * i, row = u / (DKP / 8), piece = u % (DKP / 8);
-      store_unit<T, C, DKP>(ksh, ku[i], row, piece);
-      if constexpr (OUT) store_unit<T, C, DKP>(qsh, qu[i], row, piece);
-    }
+      for (int i = 0; i < UK; ++i) {
+        const int u = tid + NT * i, row = u / (DKP / 8), piece = u % (DKP / 8);
+        store_unit<T, C, DKP>(lds, ku[i], row, piece);
+        if constexpr (OUT) store_unit<T, C, DKP>(lds + Q_AT, qu[i], row, piece);
+      }
 #pragma unroll
-    for (int i = 0; i < UV; ++i) {
-      const int u = tid + NT * i, row = u / (DVW / 8), piece = u % (DVW / 8);
-      store_unit<T, C, DVW>(vsh, vu[i], row, piece);
+      for (int i = 0; i < UV; ++i) {
+        const int u = tid + NT * i, row = u / (DVW / 8), piece = u % (DVW / 8);
+        store_unit<T, C, DVW>(lds + V_AT, vu[i], row, piece);
+      }
+      __syncthreads();
     }
-    __syncthreads();
     left -= n;
     kp += C * a.kt;
     vp += C * a.vt;
@@ -419,7 +487,7 @@ void decay_chunk_kernel(DecayArgs a) {
 #pragma unroll
     for (int s = 0; s < CS; ++s)
 #pragma unroll
-      for (int p = 0; p < NL; ++p) vop[s][p] = token_operand<C, DVW>(vsh, p, wave, s, lane, false);
+      for (int p = 0; p < NL; ++p) vop[s][p] = token_operand<C, DVW>(lds + V_AT, at_value, p, 0, s);
 
     // A value that is not finite would give NaN wherever it meets a masked
     // score's zero: it is taken out, and what depends on it set to NaN below
@@ -450,6 +518,31 @@ void decay_chunk_kernel(DecayArgs a) {
     }
     const bool any_bad = __ballot(bad_from < C) != 0;
 
+    const float fade = n == C ? wch : end_sh[C - 1 - n];
+    if ((++chunk & 7) == 0 && n == C) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[t][r] = __builtin_fmaf(S[t][r], wc8, S[t][r]);
+    }
+
+    // two tokens (2 p, 2 p + 1 of a lane's eight) of the operand w^(n-1-j) v_j of
+    // S's update
+    auto weigh = [&](int s, int p, u32x4* to) {
+      float y[2];
+#pragma unroll
+      for (int l = 0; l < NL; ++l) {
+        const uint32_t word = vop[s][l][p];
+        const float a = __builtin_bit_cast(float, word << 16);
+        const float b = __builtin_bit_cast(float, word & 0xffff0000u);
+        y[0] = l == 0 ? a : y[0] + a;
+        y[1] = l == 0 ? b : y[1] + b;
+      }
+      const int tok = 16 * s + 8 * (p >> 1) + 4 * hi + 2 * (p & 1);
+      split2<3>(y[0] * end_sh[tok + C - n], y[1] * end_sh[tok + 1 + C - n], to, p);
+    };
+    f16v acc[CT];
+
     if constexpr (OUT) {
       // Scores K Q^T of 32 keys (rows) x 32 queries (columns): eight registers
       // on end are an operand of V^T P^T as they lie.  One tile: every wave
@@ -462,8 +555,8 @@ void decay_chunk_kernel(DecayArgs a) {
           u32x4 ak[NL], bq[NL];
 #pragma unroll
           for (int p = 0; p < NL; ++p) {
-            ak[p] = row_operand<C, DKP>(ksh, p, kt, s, lane);
-            bq[p] = row_operand<C, DKP>(qsh, p, qt, s, lane);
+            ak[p] = row_operand<C, DKP>(lds, at_row, p, kt, s);
+            bq[p] = row_operand<C, DKP>(lds + Q_AT, at_row, p, qt, s);
           }
 #pragma unroll
           for (int x = 0; x < NL; ++x)
@@ -471,14 +564,19 @@ void decay_chunk_kernel(DecayArgs a) {
             for (int y = 0; y < NL; ++y)
               if (x + y < (NL == 1 ? 1 : NP)) acc = mfma(ak[x], bq[y], acc);
         }
+        // query minus key, less a constant of the register; opaque: 16 powers and
+        // masks kept over the chunks cost more registers than there are
+        int gap0 = 32 * (qt - kt) + col - 4 * hi;
+        asm volatile("" : "+v"(gap0));
+        const float* const powers = pow_sh + gap0;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           float x[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const int key = 16 * s + 8 * (j >> 2) + 4 * hi + (j & 3);
-            const int gap = 32 * (qt - kt) + col - key;
-            x[j] = gap >= 0 ? acc[8 * s + j] * pow_sh[gap >= 0 ? gap : 0] : 0.0f;
+            const int key = 16 * s + 8 * (j >> 2) + (j & 3);
+            const float y = acc[8 * s + j] * powers[-key];
+            x[j] = gap0 >= key ? y : 0.0f;
           }
           split8<NP>(x, ops[s]);
         }
@@ -501,7 +599,6 @@ void decay_chunk_kernel(DecayArgs a) {
 
       // O^T = scale w^(i+1) S^T Q^T + V^T P^T: rows columns of the values,
       // columns queries (P holds the scale).
-      f16v acc[CT];
 #pragma unroll
       for (int qt = 0; qt < CT; ++qt) acc[qt] = f16v{};
 #pragma unroll
@@ -512,10 +609,12 @@ void decay_chunk_kernel(DecayArgs a) {
         u32x4 as[NP];
         split8<NP>(x, as);
 #pragma unroll
+        for (int j = 0; j < 8; ++j) S[s / 2][8 * (s & 1) + j] = x[j] * fade;
+#pragma unroll
         for (int qt = 0; qt < CT; ++qt) {
 #pragma unroll
           for (int y = 0; y < NL; ++y) {
-            const u32x4 bq = row_operand<C, DKP>(qsh, y, qt, s, lane);
+            const u32x4 bq = row_operand<C, DKP>(lds + Q_AT, at_row, y, qt, s);
 #pragma unroll
             for (int x2 = 0; x2 < NP; ++x2)
               if (x2 + y < NP) acc[qt] = mfma(as[x2], bq, acc[qt]);
@@ -532,7 +631,7 @@ void decay_chunk_kernel(DecayArgs a) {
 #pragma unroll
       for (int kt = 0; kt < CT; ++kt)
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < 2; ++s) {
 #pragma unroll
           for (int qt = kt; qt < CT; ++qt)
 #pragma unroll
@@ -544,6 +643,15 @@ void decay_chunk_kernel(DecayArgs a) {
               for (int p = 0; p < NL; ++p)
                 if (p + y < NP) acc[qt] = mfma(vop[2 * kt + s][p], bp, acc[qt]);
             }
+        }
+    } else {
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[t][r] *= fade;
+    }
+
+    if constexpr (OUT) {
       if (any_bad) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -612,40 +720,21 @@ void decay_chunk_kernel(DecayArgs a) {
       }
       op += C * a.ot;
     }
-
-    // S <- w^n S + K^T (w^(n-1-j) V)
-    const float fh = n == C ? wch : end_sh[C - 1 - n], fl = n == C ? wcl : 0.0f;
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) S[t][r] = __builtin_fmaf(S[t][r], fh, S[t][r] * fl);
+    // S <- w^n S (above) + K^T (w^(n-1-j) V)
 #pragma unroll
     for (int s = 0; s < CS; ++s) {
-      float x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int tok = 16 * s + 8 * (j >> 2) + 4 * hi + (j & 3);
-        float y = 0.0f;
-#pragma unroll
-        for (int p = 0; p < NL; ++p) {
-          const uint32_t word = vop[s][p][j >> 1];
-          const float z = __builtin_bit_cast(float, (j & 1) ? word & 0xffff0000u : word << 16);
-          y = p == 0 ? z : y + z;
-        }
-        x[j] = y * end_sh[tok + C - n];
-      }
       u32x4 bv[3];
-      split8<3>(x, bv);
 #pragma unroll
-      for (int t = 0; t < KT; ++t) {
+      for (int p = 0; p < 4; ++p) weigh(s, p, bv);
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int y = 0; y < NL; ++y) {
-          const u32x4 ak = token_operand<C, DKP>(ksh, y, t, s, lane, true);
+          const u32x4 ak = token_operand<C, DKP>(lds, at_key, y, t, s);
 #pragma unroll
           for (int p = 0; p < 3; ++p)
             if (p + y < 3) S[t] = mfma(ak, bv[p], S[t]);
         }
-      }
     }
     if (any_bad && bad_from < C) {
 #pragma unroll
@@ -676,16 +765,69 @@ void decay_chunk_kernel(DecayArgs a) {
   }
 }
 
+// The states before the segments of a sequence from the segments' own: an
+// element of the state a thread, over the segments in their order, in place.
+// Reads and writes the workspace once, JOIN_AHEAD segments in flight (a sum over
+// all earlier segments in every workgroup of the outputs' kernel instead took
+// as long as the outputs from 32 segments on).
+constexpr int JOIN_AHEAD = 8;
+template <int N>
+__global__ __launch_bounds__(256) void decay_join_kernel(DecayArgs a) {
+  typedef Vec<float, N> V;
+  const int64_t w = blockIdx.y;
+  const Span sp = read_span(a, w);
+  if (sp.seq < 0 || sp.part != 0 || sp.parts < 2) return;
+  const int h = blockIdx.z;
+  const int64_t size = (int64_t)a.dk * a.dv, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N;
+  if (i >= size) return;
+  // w^segment as a sum of two floats: its rounding would add up
+  const double f = exp((double)a.segment * (double)a.log_decay[h]);
+  const float fh = (float)f, fl = f < 1e300 ? (float)(f - (double)fh) : 0.0f;
+  float* const p = a.ws + (w * a.heads + h) * size + i;
+  const int64_t step = a.heads * size, n = sp.parts - 1;      // the last one has none of its own
+  V s{};
+  if (a.state_in != nullptr)
+    s = *reinterpret_cast<const V*>(a.state_in + (sp.seq * a.heads + h) * size + i);
+  for (int64_t m0 = 0; m0 < n; m0 += JOIN_AHEAD) {
+    V x[JOIN_AHEAD];
+#pragma unroll
+    for (int j = 0; j < JOIN_AHEAD; ++j)
+      if (m0 + j < n) x[j] = *reinterpret_cast<const V*>(p + (m0 + j) * step);
+#pragma unroll
+    for (int j = 0; j < JOIN_AHEAD; ++j) {
+      if (m0 + j >= n) break;
+      *reinterpret_cast<V*>(p + (m0 + j) * step) = s;
+#pragma unroll
+      for (int c = 0; c < N; ++c)
+        s.v[c] = __builtin_fmaf(s.v[c], fh, __builtin_fmaf(s.v[c], fl, x[j].v[c]));
+    }
+  }
+  *reinterpret_cast<V*>(p + n * step) = s;
+}
+
+hipError_t launch_join(const DecayArgs& a, hipStream_t st) {
+  const int64_t size = (int64_t)a.dk * a.dv;
+  const bool wide = size % 4 == 0 && (uintptr_t)a.ws % 16 == 0 && (uintptr_t)a.state_in % 16 == 0;
+  const dim3 grid((unsigned)((size / (wide ? 4 : 1) + 255) / 256), (unsigned)a.segments,
+                  (unsigned)a.heads);
+  if (wide) hipLaunchKernelGGL(decay_join_kernel<4>, grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(decay_join_kernel<1>, grid, dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
 template <typename T, int DKP, int NW, int C, bool VEC>
 hipError_t launch_chunks(DecayArgs a, hipStream_t st) {
   a.slices = (a.dv + 32 * NW - 1) / (32 * NW);
   const int64_t shared = (int64_t)a.group * a.slices, kv_heads = a.heads / a.group;
   const int64_t grid = (a.segments * kv_heads + 7) / 8 * 8 * shared;
-  if (grid * 64 * NW > 0xffffffffll) return hipErrorInvalidValue;
+  if (grid * 64 * NW > 0xffffffffll || (a.ws != nullptr && a.segments > 65535))
+    return hipErrorInvalidValue;
   if (a.ws != nullptr) {
     hipLaunchKernelGGL((decay_chunk_kernel<T, DKP, NW, C, false, VEC>), dim3((unsigned)grid),
                        dim3(64 * NW), 0, st, a);
-    const hipError_t e = hipGetLastError();
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    e = launch_join(a, st);
     if (e != hipSuccess) return e;
   }
   hipLaunchKernelGGL((decay_chunk_kernel<T, DKP, NW, C, true, VEC>), dim3((unsigned)grid),
@@ -695,7 +837,7 @@ hipError_t launch_chunks(DecayArgs a, hipStream_t st) {
 
 template <typename T, bool VEC>
 hipError_t launch_decay_v(const DecayArgs& a, hipStream_t st) {
-  constexpr int C = sizeof(T) == 2 && parts_of<T>() == 1 ? 64 : 32;
+  constexpr int C = 32;
   if (a.dk <= 32) return launch_chunks<T, 32, 1, C, VEC>(a, st);
   if (a.dk <= 64) return launch_chunks<T, 64, 2, C, VEC>(a, st);
   if (a.dk <= 128) return launch_chunks<T, 128, 4, C, VEC>(a, st);
@@ -733,15 +875,18 @@ CF_API int cf_decay_attention(const CfDecayAttentionArgs* p) {
   a.heads = (int)x.heads; a.group = (int)(x.heads / x.kv_heads);
   a.dk = (int)x.dk; a.dv = (int)x.dv;
   a.ws = nullptr;
+  a.spans = nullptr;
   a.segment = x.tokens > 0 ? x.tokens : 1;
   a.segments = x.seqs;
   if (x.segment > 0 && x.segment < x.tokens) {
     a.segment = x.segment;
     a.segments = x.cu_seqlens ? x.tokens / x.segment + x.seqs
                               : x.seqs * ((x.tokens + x.segment - 1) / x.segment);
-    if (!x.workspace || x.workspace_bytes / 4 / x.heads / x.dk / x.dv < a.segments)
+    const int64_t state = 4 * x.heads * x.dk * x.dv;
+    if (!x.workspace || x.workspace_bytes / (state + CF_DECAY_SPAN_BYTES) < a.segments)
       return (int)hipErrorInvalidValue;
-    a.ws = (float*)x.workspace;
+    a.spans = x.workspace;
+    a.ws = (float*)((char*)x.workspace + a.segments * CF_DECAY_SPAN_BYTES);
   }
   a.qb = x.q_batch; a.qt = x.q_token; a.qh = x.q_head;
   a.kb = x.k_batch; a.kt = x.k_token; a.kh = x.k_head;

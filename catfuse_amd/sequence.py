@@ -33,6 +33,7 @@ MAX_KEY_DIM = 256           # CF_DECAY_MAX_DK
 MAX_VALUE_DIM = 1024        # CF_DECAY_MAX_DV
 MAX_SEQUENCES = 65535       # CF_DECAY_MAX_SEQS
 CHUNK = 64                  # CF_DECAY_CHUNK
+SPAN_BYTES = 48             # CF_DECAY_SPAN_BYTES
 MAX_TOKEN_STRIDE = 8000000  # CF_DECAY_MAX_TOKEN_STRIDE
 MAX_ROTARY_DIM = 512        # CF_ROTARY_MAX_DIM
 MAX_AXES = 3                # CF_ROTARY_MAX_AXES
@@ -174,7 +175,7 @@ def _segment(seqs: int, tokens: int, packed: bool, heads: int, dk: int, dv: int)
     width = 32 if dk <= 32 else 64 if dk <= 64 else 128
     columns = heads * -(-dv // width)          # workgroups of one segment
     total = tokens if packed else seqs * tokens
-    wanted = -(-1024 // columns)
+    wanted = -(-512 // columns)
     segment = max(256, -(-total // (wanted * CHUNK)) * CHUNK)
     if segment >= tokens or (not packed and seqs * columns >= 512):
         return 0, 0
@@ -241,7 +242,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
             out.zero_()
         return (out, left) if return_state else out
     segment, segments = _segment(B, N, cu_seqlens is not None, H, dk, dv)
-    ws = torch.empty((segments, H, dk, dv), dtype=torch.float32, device=dev) if segments else None
+    ws_bytes = segments * (4 * H * dk * dv + SPAN_BYTES)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if segments else None
     ev = _t0()
     args = _hip.DECAY_ATTENTION_ARGS.pack(
         ptr(q), ptr(k), ptr(v), ptr(log_decay), ptr(state) or 0, ptr(left) or 0, ptr(out),
@@ -249,7 +251,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
         zero_rest, _DTYPES[q.dtype], B, N, H, k.shape[-2], dk, dv, qb, q.stride(-3), q.stride(-2),
         kb, k.stride(-3), k.stride(-2), vb, v.stride(-3), v.stride(-2),
         out.stride(0) if cu_seqlens is None else 0, out.stride(-3), out.stride(-2),
-        ptr(ws) or 0, segment, 0 if ws is None else 4 * ws.numel(),
+        ptr(ws) or 0, segment, ws_bytes,
         float(dk ** -0.5 if scale is None else scale), _hip.stream(dev))
     _call(_hip.lib().cf_decay_attention, "cf_decay_attention", dev, args)
     if ev is not None:

@@ -792,6 +792,7 @@ int cf_conv_sparse_noalloc(const void* x, int64_t Cin, const void* w_packed, con
 #define CF_DECAY_MAX_SEQS 65535
 #define CF_DECAY_MAX_TOKENS 2000000000
 #define CF_DECAY_CHUNK 64
+#define CF_DECAY_SPAN_BYTES 48
 #define CF_DECAY_MAX_TOKEN_STRIDE 8000000
 #define CF_ROTARY_MAX_DIM 512
 #define CF_ROTARY_MAX_AXES 3
@@ -807,10 +808,11 @@ int cf_conv_sparse_noalloc(const void* x, int64_t Cin, const void* w_packed, con
  * no sequence are zeroed (zero_rest) or left as they were.  out must not
  * overlap the inputs.
  * segment (0, or a multiple of CF_DECAY_CHUNK): sequences are split into
- * segments of so many tokens that run side by side, with the segments' states
- * in the workspace: fp32 [n][heads][dk][dv], n = tokens / segment + seqs of
- * packed sequences, seqs * ceil(tokens / segment) of equal ones; unused where
- * segment is 0 or not below tokens.  Token strides are 0 ..
+ * segments of so many tokens that run side by side, with CF_DECAY_SPAN_BYTES
+ * and a state [heads][dk][dv] a segment in the workspace (16-byte aligned, as
+ * hipMalloc gives it), n of both: n = tokens / segment + seqs of packed
+ * sequences, seqs * ceil(tokens / segment) of equal ones; unused where segment
+ * is 0 or not below tokens.  Token strides are 0 ..
  * CF_DECAY_MAX_TOKEN_STRIDE. */
 typedef struct CfDecayAttentionArgs {
   const void* q;

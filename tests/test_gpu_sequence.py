@@ -218,10 +218,11 @@ def test_attention_keeps_later_values_from_earlier_tokens(cuda, dtype, bad, whic
 def test_attention_decay_ends(cuda, dtype):
     """log_decay -inf (only the token itself), 0 (everything), above 0 (the
     past grows) and one so low that its powers vanish."""
-    q, k, v = _inputs((1, 100, 4, 32), (1, 100, 4, 32), 32, dtype, 8)
-    f = torch.tensor([-math.inf, 0.0, 0.02, -50.0])
-    state = torch.randn(1, 4, 32, 32, generator=torch.Generator().manual_seed(4))
-    _check_attention(cuda, q, k, v, f, None, state, None, dtype)
+    for N, growth in ((100, 0.02), (900, 0.002)):
+        q, k, v = _inputs((1, N, 4, 32), (1, N, 4, 32), 32, dtype, 8)
+        f = torch.tensor([-math.inf, 0.0, growth, -50.0])
+        state = torch.randn(1, 4, 32, 32, generator=torch.Generator().manual_seed(4))
+        _check_attention(cuda, q, k, v, f, None, state, None, dtype)
 
 
 def test_attention_large_values(cuda):

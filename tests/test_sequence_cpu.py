@@ -41,6 +41,7 @@ def test_limits_mirror_the_header():
     assert sequence.MAX_VALUE_DIM == limit("CF_DECAY_MAX_DV")
     assert sequence.MAX_SEQUENCES == limit("CF_DECAY_MAX_SEQS")
     assert sequence.MAX_ROTARY_DIM == limit("CF_ROTARY_MAX_DIM")
+    assert sequence.SPAN_BYTES == limit("CF_DECAY_SPAN_BYTES")
     assert sequence.CHUNK == limit("CF_DECAY_CHUNK")
     assert sequence.MAX_TOKEN_STRIDE == limit("CF_DECAY_MAX_TOKEN_STRIDE")
     assert sequence.MAX_AXES == limit("CF_ROTARY_MAX_AXES")
@@ -74,7 +75,7 @@ def test_c_entries_refuse():
                 dict(log_decay=0), dict(segment=100), dict(segment=-64), dict(q_token=-1),
                 dict(out_token=8000001), dict(segment=64, tokens=65, workspace=0),
                 # 65 tokens of a packed sequence in segments of 64: up to two states of 1 x 1
-                dict(segment=64, tokens=65, workspace_bytes=4)):
+                dict(segment=64, tokens=65, workspace_bytes=2 * 52 - 1)):
         assert attention(**dict(dict(segment=0), **bad)) == INVALID, bad
     assert attention(seqs=0, segment=0) == 0          # nothing to do, nothing launched
 
