@@ -74,15 +74,15 @@ __device__ __forceinline__ uint32_t pack_rounded(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf2));
 }
 
-// x as N parts, most significant first: leading ones cut off (the rest is
-// exact), the last of fewer than three rounded (cutting it off would shrink
-// every number).
+// Two numbers as N parts, most significant first, in word p of the N operands:
+// leading parts cut off (the rest is exact), the last of fewer than three
+// rounded (cutting it off would shrink every number).
 template <int N>
 __device__ __forceinline__ void split2(float a, float b, u32x4* out, int p) {
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    if (n == N - 1 && N < 3) {
-      out[n][p] = pack_rounded(a, b);
+    if (n == N - 1) {
+      out[n][p] = N < 3 ? pack_rounded(a, b) : pack_high(a, b);
     } else {
       out[n][p] = pack_high(a, b);
       a -= high_part(a);
@@ -160,44 +160,6 @@ __device__ __forceinline__ void load_units(Unit<T>* u, const T* base, int n, int
   }
 }
 
-// The same for bf16, straight into the image: lane l of a wave's i-th copy fills
-// the 16 bytes l of its 1 KB.  Not known to the compiler, which would wait for
-// these copies at every read of LDS; the kernel waits (wait_copies) before the
-// barrier that hands an image over.
-typedef int v4i __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ void copy16(v4i rsrc, uint32_t off, uint32_t lds) {
-  asm volatile(
-      "s_mov_b32 m0, %2\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %0, %1, 0 offen lds"
-      :
-      : "v"(off), "s"(rsrc), "s"(lds)
-      : "memory", "m0");
-}
-template <int LATER>   // all but the LATER accesses of memory issued last
-__device__ __forceinline__ void wait_copies() {
-  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LATER) : "memory");
-}
-template <int U, int D, int NW>
-__device__ __forceinline__ void copy_units(char* image, const bf16_t* base, int n, int64_t stride,
-                                           int d, int wave, int lane) {
-  const int st = (int)stride * 2;
-  const uint64_t p = (uint64_t)(uintptr_t)base;
-  v4i rsrc;
-  rsrc[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)p);
-  rsrc[1] = __builtin_amdgcn_readfirstlane((int)((uint32_t)(p >> 32) & 0xffffu));
-  rsrc[2] = __builtin_amdgcn_readfirstlane((n - 1) * st + d * 2);
-  rsrc[3] = 0x00020000;
-  const uint32_t to = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)image;
-#pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const int u = (i * NW + wave) * 64 + lane, row = u / (D / 8);
-    const int c = ((u % (D / 8)) ^ swizzle<D>(row)) * 8;
-    copy16(rsrc, row < n && c < d ? (uint32_t)(row * st + c * 2) : OOB,
-           __builtin_amdgcn_readfirstlane(to + (uint32_t)((i * NW + wave) * 1024)));
-  }
-}
-
 template <typename T, int C, int D>
 __device__ __forceinline__ void store_unit(char* image, const Unit<T>& u, int row, int piece) {
   if constexpr (parts_of<T>() == 1) {
@@ -257,6 +219,9 @@ __device__ __forceinline__ u32x4 token_operand(const char* lds, uint32_t at, int
   }
   return r;
 }
+
+// The compiler moves nothing across.
+__device__ __forceinline__ void step() { __builtin_amdgcn_sched_barrier(0); }
 
 // Which (sequence, segment) a segment number is.  Packed sequences: every
 // wave scans the offsets, 64 a time, each offset at least its predecessor.
@@ -341,21 +306,20 @@ __device__ __forceinline__ Span read_span(const DecayArgs& a, int64_t w) {
 // operand are taken in that order, so that eight registers on end are an
 // operand of the next chunk's q S as they lie.
 template <typename T, int DKP, int NW, int C, bool OUT, bool VEC>
-__global__ __launch_bounds__(64 * NW, DKP > 128 || sizeof(T) == 4 ? 1 : (VEC && parts_of<T>() == 1 ? 3 : 2))
+__global__ __launch_bounds__(64 * NW, DKP <= 128 && sizeof(T) == 2 ? 2 : 1)
 void decay_chunk_kernel(DecayArgs a) {
   constexpr int NL = parts_of<T>(), NP = NL == 3 ? 3 : 2, NT = 64 * NW;
   constexpr int KT = DKP / 32, KS = DKP / 16, CT = C / 32, CS = C / 16, DVW = 32 * NW;
   constexpr int QK_BYTES = NL * C * DKP * 2, V_BYTES = NL * C * DVW * 2;
   constexpr int TILES = CT * (CT + 1) / 2;                     // score tiles that are not masked
   constexpr int P_BYTES = CT > 1 && OUT ? TILES * 2 * NP * 1024 : 16;
-  constexpr bool ASYNC = VEC && NL == 1;     // copied straight to LDS, two images by turns
-  constexpr int IMAGES = ASYNC ? 2 : 1;
   constexpr int Q_AT = QK_BYTES, V_AT = Q_AT + (OUT ? QK_BYTES : 0), IMAGE = V_AT + V_BYTES;
-  __shared__ __attribute__((aligned(512))) char lds[IMAGES * IMAGE];   // of K, Q and V
+  __shared__ __attribute__((aligned(512))) char lds[IMAGE];     // of K, Q and V
   __shared__ __attribute__((aligned(16))) char psh[P_BYTES];
   __shared__ float pow_all[32 + C + 1];      // 32 zeros, then scale w^n
   float* const pow_sh = pow_all + 32;
-  __shared__ float end_sh[2 * C];            // w^(C - 1 - j), then zeros
+  __shared__ float plain_sh[C];              // w^n
+  __shared__ __attribute__((aligned(16))) float end_sh[C];   // w^(n - 1 - j) of a chunk of n tokens
 
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -394,10 +358,7 @@ void decay_chunk_kernel(DecayArgs a) {
   for (int n = tid; n <= C; n += NT) {
     const double p = n == 0 ? 1.0 : exp(n * ld);
     pow_sh[n] = (float)(p * (double)a.scale);
-    if (n < C) {
-      end_sh[C - 1 - n] = (float)p;
-      end_sh[C + n] = 0.0f;
-    }
+    if (n < C) plain_sh[n] = end_sh[C - 1 - n] = (float)p;
   }
   // The rounding of w^C would add up over the chunks: every eighth makes up
   // for eight of them.
@@ -435,53 +396,38 @@ void decay_chunk_kernel(DecayArgs a) {
   constexpr int UK = C * (DKP / 8) / NT, UV = C * (DVW / 8) / NT;   // units of a thread
   static_assert(UK * NT == C * (DKP / 8) && UV * NT == C * (DVW / 8), "whole units");
   Unit<T> ku[UK], vu[UV], qu[OUT ? UK : 1];
-  int image = 0;                             // where the next chunk's lies
   auto load_chunk = [&]() {
     const int n = left < C ? left : C;
-    if constexpr (ASYNC) {
-      copy_units<UK, DKP, NW>(lds + image, kp, n, a.kt, a.dk, wave, lane);
-      if constexpr (OUT) copy_units<UK, DKP, NW>(lds + image + Q_AT, qp, n, a.qt, a.dk, wave, lane);
-      copy_units<UV, DVW, NW>(lds + image + V_AT, vp, n, a.vt, dvs, wave, lane);
-    } else {
-      load_units<T, UK, DKP, NT, VEC>(ku, kp, n, a.kt, a.dk);
-      load_units<T, UV, DVW, NT, VEC>(vu, vp, n, a.vt, dvs);
-      if constexpr (OUT) load_units<T, UK, DKP, NT, VEC>(qu, qp, n, a.qt, a.dk);
-    }
+    load_units<T, UK, DKP, NT, VEC>(ku, kp, n, a.kt, a.dk);
+    load_units<T, UV, DVW, NT, VEC>(vu, vp, n, a.vt, dvs);
+    if constexpr (OUT) load_units<T, UK, DKP, NT, VEC>(qu, qp, n, a.qt, a.dk);
   };
 
+  const uint32_t at_row = row_base<DKP>(lane), at_key = token_base<DKP>(lane, true);
+  const uint32_t at_value = token_base<DVW>(lane, false) ^ (uint32_t)(wave << 6);
+
   if (left > 0) load_chunk();
-  if constexpr (ASYNC) wait_copies<0>();
   while (left > 0) {
     const int n = left < C ? left : C;
-    const uint32_t at_row = row_base<DKP>(lane) + (ASYNC ? image : 0);
-    const uint32_t at_key = token_base<DKP>(lane, true) + (ASYNC ? image : 0);
-    const uint32_t at_value = (token_base<DVW>(lane, false) ^ (uint32_t)(wave << 6)) +
-                              (ASYNC ? image : 0);
-    if constexpr (ASYNC) {
-      // this chunk's copies are older than the last one's stores (2 CT)
-      wait_copies<OUT ? 2 * CT : 0>();
-      __syncthreads();                       // ... and the other image is read
-      image = IMAGE - image;
-    } else {
-      __syncthreads();                       // the last chunk's images are read
+    __syncthreads();                         // the last chunk's images are read
 #pragma unroll
-      for (int i = 0; i < UK; ++i) {
-        const int u = tid + NT * i, row = u / (DKP / 8), piece = u % (DKP / 8);
-        store_unit<T, C, DKP>(lds, ku[i], row, piece);
-        if constexpr (OUT) store_unit<T, C, DKP>(lds + Q_AT, qu[i], row, piece);
-      }
-#pragma unroll
-      for (int i = 0; i < UV; ++i) {
-        const int u = tid + NT * i, row = u / (DVW / 8), piece = u % (DVW / 8);
-        store_unit<T, C, DVW>(lds + V_AT, vu[i], row, piece);
-      }
-      __syncthreads();
+    for (int i = 0; i < UK; ++i) {
+      const int u = tid + NT * i, row = u / (DKP / 8), piece = u % (DKP / 8);
+      store_unit<T, C, DKP>(lds, ku[i], row, piece);
+      if constexpr (OUT) store_unit<T, C, DKP>(lds + Q_AT, qu[i], row, piece);
     }
+#pragma unroll
+    for (int i = 0; i < UV; ++i) {
+      const int u = tid + NT * i, row = u / (DVW / 8), piece = u % (DVW / 8);
+      store_unit<T, C, DVW>(lds + V_AT, vu[i], row, piece);
+    }
+    if (n < C)                               // (the last chunk: its predecessor's powers are read)
+      for (int j = tid; j < C; j += NT) end_sh[j] = j < n ? plain_sh[n - 1 - j] : 0.0f;
+    __syncthreads();
     left -= n;
     kp += C * a.kt;
     vp += C * a.vt;
     qp += C * a.qt;
-    if (left > 0) load_chunk();
 
     u32x4 vop[CS][NL];                       // lane: column sc, tokens as token_operand
 #pragma unroll
@@ -492,8 +438,9 @@ void decay_chunk_kernel(DecayArgs a) {
     // A value that is not finite would give NaN wherever it meets a masked
     // score's zero: it is taken out, and what depends on it set to NaN below
     // (this lane's column: the queries from its token on, and the state).
+    // (The segments' own states have no masked scores: there NaN goes its way.)
     int bad_from = C;
-    {
+    if constexpr (OUT) {
       uint32_t any = 0u;                     // exponents of all ones, of the leading parts
 #pragma unroll
       for (int s = 0; s < CS; ++s)
@@ -516,9 +463,9 @@ void decay_chunk_kernel(DecayArgs a) {
         if (other < bad_from) bad_from = other;
       }
     }
-    const bool any_bad = __ballot(bad_from < C) != 0;
+    const bool any_bad = OUT && __ballot(bad_from < C) != 0;
 
-    const float fade = n == C ? wch : end_sh[C - 1 - n];
+    const float fade = n == C ? wch : plain_sh[n];
     if ((++chunk & 7) == 0 && n == C) {
 #pragma unroll
       for (int t = 0; t < KT; ++t)
@@ -526,56 +473,73 @@ void decay_chunk_kernel(DecayArgs a) {
         for (int r = 0; r < 16; ++r) S[t][r] = __builtin_fmaf(S[t][r], wc8, S[t][r]);
     }
 
-    // two tokens (2 p, 2 p + 1 of a lane's eight) of the operand w^(n-1-j) v_j of
-    // S's update
+    // The operand w^(n-1-j) v_j of S's update, 16 tokens of it: its weights, and
+    // two tokens (2 p, 2 p + 1 of a lane's eight) at a time.
+    Vec<float, 4> wt[2];
+    auto weights = [&](int s) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        wt[e] = *reinterpret_cast<const Vec<float, 4>*>(end_sh + 16 * s + 8 * e + 4 * hi);
+    };
     auto weigh = [&](int s, int p, u32x4* to) {
       float y[2];
 #pragma unroll
       for (int l = 0; l < NL; ++l) {
         const uint32_t word = vop[s][l][p];
-        const float a = __builtin_bit_cast(float, word << 16);
-        const float b = __builtin_bit_cast(float, word & 0xffff0000u);
-        y[0] = l == 0 ? a : y[0] + a;
-        y[1] = l == 0 ? b : y[1] + b;
+        const float lo = __builtin_bit_cast(float, word << 16);
+        const float up = __builtin_bit_cast(float, word & 0xffff0000u);
+        y[0] = l == 0 ? lo : y[0] + lo;
+        y[1] = l == 0 ? up : y[1] + up;
       }
-      const int tok = 16 * s + 8 * (p >> 1) + 4 * hi + 2 * (p & 1);
-      split2<3>(y[0] * end_sh[tok + C - n], y[1] * end_sh[tok + 1 + C - n], to, p);
+      split2<3>(y[0] * wt[p >> 1].v[2 * (p & 1)], y[1] * wt[p >> 1].v[2 * (p & 1) + 1], to, p);
     };
     f16v acc[CT];
 
+    // In what follows the operands of the next products are read, and made,
+    // between the products at hand, and the compiler is held to that order
+    // (step()): left alone, short of registers, it reads each operand right
+    // before its use and waits for LDS some eighty times a chunk.
     if constexpr (OUT) {
       // Scores K Q^T of 32 keys (rows) x 32 queries (columns): eight registers
       // on end are an operand of V^T P^T as they lie.  One tile: every wave
       // for itself; three: a tile a wave, exchanged in LDS.
       u32x4 pop[CT > 1 ? 1 : 2][NP];
       auto score_tile = [&](int kt, int qt, u32x4 (*ops)[NP]) {
-        f16v acc = {};
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          u32x4 ak[NL], bq[NL];
-#pragma unroll
-          for (int p = 0; p < NL; ++p) {
-            ak[p] = row_operand<C, DKP>(lds, at_row, p, kt, s);
-            bq[p] = row_operand<C, DKP>(lds + Q_AT, at_row, p, qt, s);
-          }
-#pragma unroll
-          for (int x = 0; x < NL; ++x)
-#pragma unroll
-            for (int y = 0; y < NL; ++y)
-              if (x + y < (NL == 1 ? 1 : NP)) acc = mfma(ak[x], bq[y], acc);
-        }
         // query minus key, less a constant of the register; opaque: 16 powers and
         // masks kept over the chunks cost more registers than there are
         int gap0 = 32 * (qt - kt) + col - 4 * hi;
         asm volatile("" : "+v"(gap0));
         const float* const powers = pow_sh + gap0;
+        u32x4 ak[2][NL], bq[2][NL];
+        auto read = [&](int s) {
+#pragma unroll
+          for (int p = 0; p < NL; ++p) {
+            ak[s & 1][p] = row_operand<C, DKP>(lds, at_row, p, kt, s);
+            bq[s & 1][p] = row_operand<C, DKP>(lds + Q_AT, at_row, p, qt, s);
+          }
+        };
+        read(0);
+        float f[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) f[r] = powers[-(8 * (r >> 2) + (r & 3))];
+        f16v acc = {};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          if (s + 1 < KS) read(s + 1);
+#pragma unroll
+          for (int x = 0; x < NL; ++x)
+#pragma unroll
+            for (int y = 0; y < NL; ++y)
+              if (x + y < (NL == 1 ? 1 : NP)) acc = mfma(ak[s & 1][x], bq[s & 1][y], acc);
+          step();
+        }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           float x[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const int key = 16 * s + 8 * (j >> 2) + (j & 3);
-            const float y = acc[8 * s + j] * powers[-key];
+            const float y = acc[8 * s + j] * f[8 * s + j];
             x[j] = gap0 >= key ? y : 0.0f;
           }
           split8<NP>(x, ops[s]);
@@ -599,26 +563,43 @@ void decay_chunk_kernel(DecayArgs a) {
 
       // O^T = scale w^(i+1) S^T Q^T + V^T P^T: rows columns of the values,
       // columns queries (P holds the scale).
+      {
+        u32x4 as[2][NP], bq[2][CT][NL];
+        auto state_part = [&](int s) {       // S's operand, and S faded
+          float x[8];
 #pragma unroll
-      for (int qt = 0; qt < CT; ++qt) acc[qt] = f16v{};
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = S[s / 2][8 * (s & 1) + j];
-        u32x4 as[NP];
-        split8<NP>(x, as);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) S[s / 2][8 * (s & 1) + j] = x[j] * fade;
-#pragma unroll
-        for (int qt = 0; qt < CT; ++qt) {
-#pragma unroll
-          for (int y = 0; y < NL; ++y) {
-            const u32x4 bq = row_operand<C, DKP>(lds + Q_AT, at_row, y, qt, s);
-#pragma unroll
-            for (int x2 = 0; x2 < NP; ++x2)
-              if (x2 + y < NP) acc[qt] = mfma(as[x2], bq, acc[qt]);
+          for (int j = 0; j < 8; ++j) {
+            x[j] = S[s / 2][8 * (s & 1) + j];
+            S[s / 2][8 * (s & 1) + j] = x[j] * fade;
           }
+          split8<NP>(x, as[s & 1]);
+        };
+        auto read = [&](int s) {
+#pragma unroll
+          for (int qt = 0; qt < CT; ++qt)
+#pragma unroll
+            for (int y = 0; y < NL; ++y)
+              bq[s & 1][qt][y] = row_operand<C, DKP>(lds + Q_AT, at_row, y, qt, s);
+        };
+        read(0);
+        state_part(0);
+#pragma unroll
+        for (int qt = 0; qt < CT; ++qt) acc[qt] = f16v{};
+        step();
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          if (s + 1 < KS) {
+            read(s + 1);
+            state_part(s + 1);
+          }
+#pragma unroll
+          for (int x = 0; x < NP; ++x)
+#pragma unroll
+            for (int y = 0; y < NL; ++y)
+#pragma unroll
+              for (int qt = 0; qt < CT; ++qt)
+                if (x + y < NP) acc[qt] = mfma(as[s & 1][x], bq[s & 1][qt][y], acc[qt]);
+          step();
         }
       }
 #pragma unroll
@@ -627,23 +608,36 @@ void decay_chunk_kernel(DecayArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[qt][r] *= f;
       }
-      if constexpr (CT > 1) __syncthreads();
+      if constexpr (CT > 1) {
+        __syncthreads();
+        u32x4 bp[2][NP];
+        constexpr int STEPS = TILES * 2;     // (tile, s)
+        auto read = [&](int i) {
 #pragma unroll
-      for (int kt = 0; kt < CT; ++kt)
+          for (int y = 0; y < NP; ++y)
+            bp[i & 1][y] = *reinterpret_cast<const u32x4*>(psh + ((i * NP + y) * 64 + lane) * 16);
+        };
+        read(0);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
+        for (int i = 0; i < STEPS; ++i) {
+          if (i + 1 < STEPS) read(i + 1);
+          const int qt = i / 2 == 0 ? 0 : 1, kt = i / 2 == 2 ? 1 : 0, s = i & 1;
 #pragma unroll
-          for (int qt = kt; qt < CT; ++qt)
+          for (int y = 0; y < NP; ++y)
 #pragma unroll
-            for (int y = 0; y < NP; ++y) {
-              const u32x4 bp = CT > 1 ? *reinterpret_cast<const u32x4*>(
-                                            psh + ((((kt + qt) * 2 + s) * NP + y) * 64 + lane) * 16)
-                                      : pop[CT > 1 ? 0 : s][y];
-#pragma unroll
-              for (int p = 0; p < NL; ++p)
-                if (p + y < NP) acc[qt] = mfma(vop[2 * kt + s][p], bp, acc[qt]);
-            }
+            for (int p = 0; p < NL; ++p)
+              if (p + y < NP) acc[qt] = mfma(vop[2 * kt + s][p], bp[i & 1][y], acc[qt]);
+          step();
         }
+      } else {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int y = 0; y < NP; ++y)
+#pragma unroll
+            for (int p = 0; p < NL; ++p)
+              if (p + y < NP) acc[0] = mfma(vop[s][p], pop[s][y], acc[0]);
+      }
     } else {
 #pragma unroll
       for (int t = 0; t < KT; ++t)
@@ -720,21 +714,40 @@ void decay_chunk_kernel(DecayArgs a) {
       }
       op += C * a.ot;
     }
+
+    // The next chunk's rows, now that the outputs' registers are free.
+    if (left > 0) load_chunk();
+
     // S <- w^n S (above) + K^T (w^(n-1-j) V)
+    {
+      u32x4 bv[2][3], ak[2][NL];
+      auto key_tile = [&](int i) {
 #pragma unroll
-    for (int s = 0; s < CS; ++s) {
-      u32x4 bv[3];
+        for (int y = 0; y < NL; ++y)
+          ak[i & 1][y] = token_operand<C, DKP>(lds, at_key, y, i % KT, i / KT);
+      };
+      weights(0);
+      key_tile(0);
 #pragma unroll
-      for (int p = 0; p < 4; ++p) weigh(s, p, bv);
+      for (int p = 0; p < 4; ++p) weigh(0, p, bv[0]);
+      if (CS > 1) weights(1);
+      step();
 #pragma unroll
-      for (int t = 0; t < KT; ++t)
+      for (int i = 0; i < CS * KT; ++i) {
+        const int s = i / KT, t = i % KT;
+        if (i + 1 < CS * KT) key_tile(i + 1);
 #pragma unroll
-        for (int y = 0; y < NL; ++y) {
-          const u32x4 ak = token_operand<C, DKP>(lds, at_key, y, t, s);
+        for (int y = 0; y < NL; ++y)
 #pragma unroll
           for (int p = 0; p < 3; ++p)
-            if (p + y < 3) S[t] = mfma(ak, bv[p], S[t]);
+            if (p + y < 3) S[t] = mfma(ak[i & 1][y], bv[s & 1][p], S[t]);
+        if (s + 1 < CS) {
+#pragma unroll
+          for (int p = t * 4 / KT; p < (t + 1) * 4 / KT; ++p) weigh(s + 1, p, bv[(s + 1) & 1]);
+          if (t == KT - 1 && s + 2 < CS) weights(s + 2);
         }
+        step();
+      }
     }
     if (any_bad && bad_from < C) {
 #pragma unroll
@@ -837,7 +850,7 @@ hipError_t launch_chunks(DecayArgs a, hipStream_t st) {
 
 template <typename T, bool VEC>
 hipError_t launch_decay_v(const DecayArgs& a, hipStream_t st) {
-  constexpr int C = 32;
+  constexpr int C = sizeof(T) == 2 && parts_of<T>() == 1 ? 64 : 32;
   if (a.dk <= 32) return launch_chunks<T, 32, 1, C, VEC>(a, st);
   if (a.dk <= 64) return launch_chunks<T, 64, 2, C, VEC>(a, st);
   if (a.dk <= 128) return launch_chunks<T, 128, 4, C, VEC>(a, st);

@@ -170,14 +170,26 @@ def _call(fn, what: str, dev, args) -> None:
 # attention with a decay for each head
 # ---------------------------------------------------------------------------
 
-def _segment(seqs: int, tokens: int, packed: bool, heads: int, dk: int, dv: int):
-    """(tokens a segment, segments in all); (0, 0): whole sequences."""
+def _segment(seqs: int, tokens: int, packed: bool, heads: int, dk: int, dv: int, wide: bool):
+    """(tokens a segment, segments in all); (0, 0): whole sequences.
+
+    A workgroup takes a segment of one head and `width` columns; the segments'
+    own states cost a further pass over k and v (about half of the outputs'
+    time), so sequences are split where they leave most of the card idle, into
+    about as many workgroups as run at once.  Measured (us, bf16, heads of
+    128): one sequence of 65536 tokens, 32 heads: segments of 2048 tokens 756,
+    4096 739, 8192 1190; 24 packed ones of 24011 tokens, 16 heads: whole 266,
+    384 183, 768 176; fp32, 3 sequences of 1237, 8 heads of 80: whole 280, 64
+    51, 128 47, 256 75; one of 196, 12 heads of 32: whole 22, 64 18."""
     width = 32 if dk <= 32 else 64 if dk <= 64 else 128
     columns = heads * -(-dv // width)          # workgroups of one segment
+    at_once = (2048 if dk <= 32 else 1024 if dk <= 64 else 512 if dk <= 128 else 256) // \
+        (2 if wide and 32 < dk <= 128 else 1)
+    if tokens <= 2 * CHUNK or seqs * columns * (1 if packed else 8) > 4 * at_once:
+        return 0, 0
     total = tokens if packed else seqs * tokens
-    wanted = -(-512 // columns)
-    segment = max(256, -(-total // (wanted * CHUNK)) * CHUNK)
-    if segment >= tokens or (not packed and seqs * columns >= 512):
+    segment = max(1, -(-total * columns // (at_once * CHUNK))) * CHUNK
+    if segment >= tokens:
         return 0, 0
     return segment, tokens // segment + seqs if packed else seqs * -(-tokens // segment)
 
@@ -241,7 +253,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
         if zero_rest:
             out.zero_()
         return (out, left) if return_state else out
-    segment, segments = _segment(B, N, cu_seqlens is not None, H, dk, dv)
+    segment, segments = _segment(B, N, cu_seqlens is not None, H, dk, dv,
+                                 q.dtype == torch.float32)
     ws_bytes = segments * (4 * H * dk * dv + SPAN_BYTES)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if segments else None
     ev = _t0()
