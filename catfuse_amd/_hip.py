@@ -140,11 +140,12 @@ class ConvHaloPairArgs(ctypes.Structure):
 
 
 # The argument blocks of the sequence operators (include/catfuse_amd.h:
-# CfDecayAttentionArgs, CfDecayStepArgs, CfRotaryArgs), packed as bytes by one
-# call: Q a pointer, q an int64, d a double, every field 8 bytes.
-DECAY_ATTENTION_ARGS = struct.Struct("=8Q21qQ2qdQ")
-DECAY_STEP_ARGS = struct.Struct("=7Q17qdQ")
-ROTARY_ARGS = struct.Struct("=8Q33qdQ")
+# CfDecayAttentionArgs, CfDecayStepArgs, CfRotaryArgs), packed as bytes: first
+# the pointers and the stream (Q), which differ from call to call, then what a
+# launch plan keeps (q an int64, d a double), every field 8 bytes.
+DECAY_ATTENTION_ARGS = struct.Struct("=10Q"), struct.Struct("=23qd")
+DECAY_STEP_ARGS = struct.Struct("=8Q"), struct.Struct("=17qd")
+ROTARY_ARGS = struct.Struct("=9Q"), struct.Struct("=33qd")
 _RESTYPES = {"cf_error_string": c_char_p}
 
 _lib = None

@@ -32,11 +32,35 @@ MAX_HEADS = 4096            # CF_SEQ_MAX_HEADS
 MAX_KEY_DIM = 256           # CF_DECAY_MAX_DK
 MAX_VALUE_DIM = 1024        # CF_DECAY_MAX_DV
 MAX_SEQUENCES = 65535       # CF_DECAY_MAX_SEQS
+MAX_TOKENS = 2000000000     # CF_DECAY_MAX_TOKENS
 CHUNK = 64                  # CF_DECAY_CHUNK
 SPAN_BYTES = 48             # CF_DECAY_SPAN_BYTES
 MAX_TOKEN_STRIDE = 8000000  # CF_DECAY_MAX_TOKEN_STRIDE
 MAX_ROTARY_DIM = 512        # CF_ROTARY_MAX_DIM
 MAX_AXES = 3                # CF_ROTARY_MAX_AXES
+
+
+# Launch plans: the checked, packed static arguments of a call by what its
+# tensors look like (shapes, strides, types, devices), so that a repeated call
+# skips the checks; addresses are taken anew for each call.
+_PLANS: dict = {}
+_Tensor = torch.Tensor
+
+
+def _looks(t):
+    """What a plan depends on of a tensor (or of None)."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device, t.requires_grad)
+
+
+def _keep(key, plan):
+    if len(_PLANS) >= 512:
+        _PLANS.clear()
+    _PLANS[key] = plan
+    return plan
+
+
+def _at(t) -> int:
+    return 0 if t is None else t.data_ptr() if type(t) is _Tensor else ptr(t)
 
 
 # ---------------------------------------------------------------------------
@@ -113,16 +137,14 @@ def _require_distinct(t, name: str) -> None:
         reach += (n - 1) * s
 
 
-def _output(out, name: str, shape, like, inputs):
+def _require_output(out, name: str, shape, like) -> None:
     if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
+        return
     _require(out, name, (like.dtype,), like.device)
     if tuple(out.shape) != tuple(shape):
         raise ValueError(f"{name} has shape {tuple(out.shape)}, expected {tuple(shape)}")
     _require_rows(out, name)
     _require_distinct(out, name)
-    _require_apart(out, name, inputs)
-    return out
 
 
 def _require_attention(q, k, v, log_decay, ndims):
@@ -222,57 +244,84 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     Returns (out [.., H, dv], state after the last token), or out alone
     without return_state.  Sums and states are fp32; a token that holds an
     infinity or NaN does not reach the tokens before it."""
-    dev = _require_attention(q, k, v, log_decay, (4,) if cu_seqlens is None else (3,))
-    H, dk, dv = q.shape[-2], q.shape[-1], v.shape[-1]
-    if cu_seqlens is None:
-        B, N = q.shape[:2]
-        qb, kb, vb = q.stride(0), k.stride(0), v.stride(0)
+    try:
+        key = (decay_attention, _looks(q), _looks(k), _looks(v), _looks(log_decay), _looks(state),
+               _looks(cu_seqlens), _looks(out), scale, return_state, torch.is_grad_enabled())
+        plan = _PLANS.get(key)
+    except (AttributeError, TypeError):      # not tensors: the checks say which
+        key = plan = None
+    if plan is None:
+        plan = _attention_plan(q, k, v, log_decay, scale, state, cu_seqlens, out)
+        if key is not None:
+            _keep(key, plan)
+    dev, shape, state_shape, ws_bytes, tail = plan
+    given = out is not None
+    if given:
+        _require_apart(out, "out", (q, k, v, log_decay, state, cu_seqlens))
     else:
+        out = torch.empty(shape, dtype=q.dtype, device=dev)
+    _require_gpu(q, "q")
+    left = torch.empty(state_shape, dtype=torch.float32, device=dev) if return_state else None
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    if state_shape[0] == 0:                  # no sequences: no row belongs to one
+        if not given:
+            out.zero_()
+        return (out, left) if return_state else out
+    ev = _t0()
+    args = _hip.DECAY_ATTENTION_ARGS[0].pack(
+        _at(q), _at(k), _at(v), _at(log_decay), _at(state), _at(left), _at(out), _at(cu_seqlens),
+        _at(ws), _hip.stream(dev)) + tail
+    _call(_hip.lib().cf_decay_attention, "cf_decay_attention", dev, args)
+    if ev is not None:
+        H, Hk, dk, dv = q.shape[-2], k.shape[-2], q.shape[-1], v.shape[-1]
+        rows = q.numel() // (H * dk)
+        _t1("decay_attention", ev, flops=4 * rows * H * dk * dv,
+            nbytes=q.element_size() * rows * (H + Hk) * (dk + dv) +
+            4 * state_shape[0] * H * dk * dv * ((state is not None) + return_state))
+    return (out, left) if return_state else out
+
+
+def _attention_plan(q, k, v, log_decay, scale, state, cu_seqlens, out):
+    """(device, shapes of the output and of the states, workspace bytes, packed
+    arguments) of a checked call."""
+    dev = _require_attention(q, k, v, log_decay, (4,) if cu_seqlens is None else (3,))
+    H, Hk, dk, dv = q.shape[-2], k.shape[-2], q.shape[-1], v.shape[-1]
+    packed = cu_seqlens is not None
+    if packed:
         if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.ndim != 1 or \
                 cu_seqlens.shape[0] < 1:
             raise ValueError("cu_seqlens must be a one-dimensional tensor of offsets")
         B, N = cu_seqlens.shape[0] - 1, q.shape[0]
         _require_index(cu_seqlens, "cu_seqlens", B + 1, dev)
-        qb = kb = vb = 0
+    else:
+        B, N = q.shape[:2]
     if B > MAX_SEQUENCES:
         raise ValueError(f"{B} sequences (at most {MAX_SEQUENCES})")
     if state is not None:
         _require(state, "state", (torch.float32,), dev)
         if state.shape != (B, H, dk, dv) or not state.is_contiguous():
             raise ValueError(f"state must be contiguous [{B}, {H}, {dk}, {dv}]")
+    shape = tuple(q.shape[:-1]) + (dv,)
+    _require_output(out, "out", shape, q)
     for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
         if t is not None and t.stride(-3) > MAX_TOKEN_STRIDE and t.shape[-3] > 1:
             raise ValueError(f"tokens of {name} lie {t.stride(-3)} elements apart (at most "
                              f"{MAX_TOKEN_STRIDE})")
-    zero_rest = out is None
-    out = _output(out, "out", q.shape[:-1] + (dv,), q,
-                  (q, k, v, log_decay, state, cu_seqlens))
-    _require_gpu(q, "q")
-    left = torch.empty((B, H, dk, dv), dtype=torch.float32, device=dev) if return_state else None
-    if B == 0:
-        if zero_rest:
-            out.zero_()
-        return (out, left) if return_state else out
-    segment, segments = _segment(B, N, cu_seqlens is not None, H, dk, dv,
-                                 q.dtype == torch.float32)
+    if N > MAX_TOKENS:
+        raise ValueError(f"{N} tokens (at most {MAX_TOKENS})")
+
+    def steps(t):
+        # (a dimension of one element may have any stride)
+        return (0 if packed else t.stride(0), t.stride(-3) if t.shape[-3] > 1 else 0, t.stride(-2))
+    # a new output is contiguous
+    o = steps(out) if out is not None else (0 if packed else N * H * dv, H * dv, dv)
+    segment, segments = _segment(B, N, packed, H, dk, dv, q.dtype == torch.float32)
     ws_bytes = segments * (4 * H * dk * dv + SPAN_BYTES)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if segments else None
-    ev = _t0()
-    args = _hip.DECAY_ATTENTION_ARGS.pack(
-        ptr(q), ptr(k), ptr(v), ptr(log_decay), ptr(state) or 0, ptr(left) or 0, ptr(out),
-        ptr(cu_seqlens) or 0, cu_seqlens is not None and cu_seqlens.dtype == torch.int64,
-        zero_rest, _DTYPES[q.dtype], B, N, H, k.shape[-2], dk, dv, qb, q.stride(-3), q.stride(-2),
-        kb, k.stride(-3), k.stride(-2), vb, v.stride(-3), v.stride(-2),
-        out.stride(0) if cu_seqlens is None else 0, out.stride(-3), out.stride(-2),
-        ptr(ws) or 0, segment, ws_bytes,
-        float(dk ** -0.5 if scale is None else scale), _hip.stream(dev))
-    _call(_hip.lib().cf_decay_attention, "cf_decay_attention", dev, args)
-    if ev is not None:
-        rows = q.numel() // (H * dk)
-        _t1("decay_attention", ev, flops=4 * rows * H * dk * dv,
-            nbytes=q.element_size() * rows * (H + k.shape[-2]) * (dk + dv) +
-            4 * B * H * dk * dv * ((state is not None) + return_state))
-    return (out, left) if return_state else out
+    tail = _hip.DECAY_ATTENTION_ARGS[1].pack(
+        packed and cu_seqlens.dtype == torch.int64, out is None, _DTYPES[q.dtype], B, N, H, Hk, dk,
+        dv, *steps(q), *steps(k), *steps(v), *o, segment, ws_bytes,
+        float(dk ** -0.5 if scale is None else scale))
+    return dev, shape, (B, H, dk, dv), ws_bytes, tail
 
 
 def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -294,6 +343,43 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     the same slot are taken as consecutive tokens of one sequence.
 
     Returns out [rows, H, dv]."""
+    try:
+        key = (decay_attention_step, _looks(q), _looks(k), _looks(v), _looks(log_decay),
+               _looks(state), _looks(slots), _looks(out), scale, torch.is_grad_enabled())
+        plan = _PLANS.get(key)
+    except (AttributeError, TypeError):      # not tensors: the checks say which
+        key = plan = None
+    if plan is None:
+        plan = _step_plan(q, k, v, log_decay, state, slots, scale, out)
+        if key is not None:
+            _keep(key, plan)
+    dev, shape, spans, tail = plan
+    first = state.data_ptr()
+    last = first + spans[0]
+    for t, n in zip((q, k, v, log_decay, slots), spans[1:]):
+        if n and t.data_ptr() < last and first < t.data_ptr() + n:
+            raise ValueError("state overlaps the memory of an input")
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=dev)
+    else:
+        _require_apart(out, "out", (q, k, v, log_decay, slots, state))
+    _require_gpu(q, "q")
+    if shape[0] == 0:
+        return out
+    ev = _t0()
+    args = _hip.DECAY_STEP_ARGS[0].pack(_at(q), _at(k), _at(v), _at(log_decay), _at(state), _at(out),
+                                        _at(slots), _hip.stream(dev)) + tail
+    _call(_hip.lib().cf_decay_attention_step, "cf_decay_attention_step", dev, args)
+    if ev is not None:
+        (rows, H, dk), Hk, dv = q.shape, k.shape[1], v.shape[2]
+        _t1("decay_attention_step", ev, flops=4 * rows * H * dk * dv,
+            nbytes=8 * rows * H * dk * dv + q.element_size() * rows * (H + Hk) * (dk + dv))
+    return out
+
+
+def _step_plan(q, k, v, log_decay, state, slots, scale, out):
+    """(device, output shape, bytes that state and the inputs lie over, packed
+    arguments) of a checked call."""
     dev = _require_attention(q, k, v, log_decay, (3,))
     rows, H, dk = q.shape
     dv = v.shape[-1]
@@ -309,25 +395,18 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         raise ValueError(f"{rows} rows but {state.shape[0]} states: slots are needed")
     if rows > MAX_SEQUENCES:
         raise ValueError(f"{rows} rows (at most {MAX_SEQUENCES})")
-    inputs = (q, k, v, log_decay, slots)
-    _require_apart(state, "state", inputs)
-    out = _output(out, "out", (rows, H, dv), q, inputs + (state,))
-    _require_gpu(q, "q")
-    if rows == 0:
-        return out
-    ev = _t0()
-    args = _hip.DECAY_STEP_ARGS.pack(
-        ptr(q), ptr(k), ptr(v), ptr(log_decay), ptr(state), ptr(out), ptr(slots) or 0,
+    shape = (rows, H, dv)
+    _require_output(out, "out", shape, q)
+    o = (H * dv, dv) if out is None else (out.stride(0), out.stride(1))
+    spans = []
+    for t in (state, q, k, v, log_decay, slots):
+        a, b = (0, 0) if t is None else _span(t)
+        spans.append(b - a)
+    tail = _hip.DECAY_STEP_ARGS[1].pack(
         slots is not None and slots.dtype == torch.int64, _DTYPES[q.dtype], rows, H, k.shape[1],
         dk, dv, state.shape[0], state.stride(0), q.stride(0), q.stride(1), k.stride(0),
-        k.stride(1), v.stride(0), v.stride(1), out.stride(0), out.stride(1),
-        float(dk ** -0.5 if scale is None else scale), _hip.stream(dev))
-    _call(_hip.lib().cf_decay_attention_step, "cf_decay_attention_step", dev, args)
-    if ev is not None:
-        _t1("decay_attention_step", ev, flops=4 * rows * H * dk * dv,
-            nbytes=8 * rows * H * dk * dv +
-            q.element_size() * rows * (H + k.shape[1]) * (dk + dv))
-    return out
+        k.stride(1), v.stride(0), v.stride(1), *o, float(dk ** -0.5 if scale is None else scale))
+    return dev, shape, tuple(spans), tail
 
 
 # ---------------------------------------------------------------------------
@@ -379,18 +458,61 @@ def _split_tokens(shape, tensors):
 
 
 def _weight(w, name, x):
-    """(pointer, fp32?, stride between heads) of the norm weights of x's heads."""
+    """(fp32?, stride between heads) of the norm weights of x's heads."""
     if w is None:
-        return 0, 1, 0
+        return 1, 0
     _require(w, name, (torch.float32, x.dtype), x.device)
     H, d = x.shape[-2:]
     if w.shape not in ((d,), (H, d)) or not w.is_contiguous():
         raise ValueError(f"{name} must be contiguous [{d}] or [{H}, {d}]")
-    return ptr(w), w.dtype == torch.float32, d if w.ndim == 2 else 0
+    return w.dtype == torch.float32, d if w.ndim == 2 else 0
 
 
 def _rotate(x, k, positions, freqs, sections, interleaved, inverse, norm, eps, weights, outs,
             names):
+    try:
+        key = (_rotate, _looks(x), _looks(k), _looks(positions), _looks(freqs), sections,
+               interleaved, inverse, norm, eps, _looks(weights[0]), _looks(weights[1]),
+               _looks(outs[0]), _looks(outs[1]), torch.is_grad_enabled())
+        plan = _PLANS.get(key)
+    except (AttributeError, TypeError):      # not tensors (or sections a list): checked below
+        key = plan = None
+    if plan is None:
+        plan = _rotary_plan(x, k, positions, freqs, sections, interleaved, inverse, norm, eps,
+                            weights, outs, names)
+        if key is not None:
+            _keep(key, plan)
+    dev, tail = plan
+    ys = []
+    for t, out in zip((x, k), outs):
+        if t is None:
+            ys.append(None)
+        elif out is None:
+            ys.append(torch.empty(t.shape, dtype=t.dtype, device=dev))
+        else:
+            in_place = out.data_ptr() == t.data_ptr() and out.stride() == t.stride()
+            inputs = (x, k, positions, freqs) + weights
+            _require_apart(out, "out", tuple(o for o in inputs if not (in_place and o is t)))
+            ys.append(out)
+    if outs[0] is not None and outs[1] is not None:
+        _require_apart(ys[0], "out", (ys[1],))
+    _require_gpu(x, names[0])
+    if x.numel() == 0:
+        return ys
+    ev = _t0()
+    args = _hip.ROTARY_ARGS[0].pack(_at(x), _at(ys[0]), _at(weights[0]), _at(k), _at(ys[1]),
+                                    _at(weights[1]), _at(positions), _at(freqs),
+                                    _hip.stream(dev)) + tail
+    _call(_hip.lib().cf_rotary, "cf_rotary", dev, args)
+    if ev is not None:
+        m = x.numel() + (0 if k is None else k.numel())
+        _t1("qk_norm_rotary" if norm else "rotary", ev, nbytes=2 * m * x.element_size())
+    return ys
+
+
+def _rotary_plan(x, k, positions, freqs, sections, interleaved, inverse, norm, eps, weights, outs,
+                 names):
+    """(device, packed arguments) of a checked call."""
     _require(x, names[0], _DTYPES)
     dev = x.device
     xs = (x,) if k is None else (x, k)
@@ -428,41 +550,30 @@ def _rotate(x, k, positions, freqs, sections, interleaved, inverse, norm, eps, w
     if not (eps >= 0):
         raise ValueError(f"eps {eps} is negative")
     ws = [_weight(w, n + "_weight", t) for t, w, n in zip(xs, weights, names)]
-    inputs = xs + (positions, freqs) + tuple(weights)
-    ys = []
-    for i, (t, out) in enumerate(zip(xs, outs)):
-        if out is not None and out.data_ptr() == t.data_ptr() and out.shape == t.shape and \
-                out.stride() == t.stride():           # in place
-            others = tuple(o for o in inputs if o is not t)
-        else:
-            others = inputs
-        ys.append(_output(out, "out", t.shape, t, others))
-    if len(ys) == 2 and outs[0] is not None and outs[1] is not None:
-        _require_apart(ys[0], "out", (ys[1],))
-    strides = [t.stride()[:-2] for t in xs] + [t.stride()[:-2] for t in ys] + \
+    for t, out in zip(xs, outs):
+        _require_output(out, "out", t.shape, t)
+
+    def contiguous(t):                       # strides of a new output
+        got, n = [], 1
+        for m in reversed(t.shape):
+            got.insert(0, n)
+            n *= m
+        return tuple(got)
+    out_strides = [contiguous(t) if out is None else out.stride() for t, out in zip(xs, outs)]
+    strides = [t.stride()[:-2] for t in xs] + [st[:-2] for st in out_strides] + \
         [positions.stride()[1:]]
     outer, inner, at = _split_tokens(lead, strides)
-    _require_gpu(x, names[0])
-    if x.numel() == 0:
-        return ys
     n = len(xs)
     second = (0, 0, 0, 0, 0, 0) if k is None else \
-        at[1] + (k.stride(-2),) + at[3] + (ys[1].stride(-2),)
-    wk = (0, 1, 0) if k is None else ws[1]
-    ev = _t0()
-    args = _hip.ROTARY_ARGS.pack(
-        ptr(x), ptr(ys[0]), ws[0][0], 0 if k is None else ptr(k), 0 if k is None else ptr(ys[1]),
-        wk[0], ptr(positions), ptr(freqs), ws[0][1], ws[0][2], wk[1], wk[2],
-        _POSITIONS[positions.dtype], _DTYPES[x.dtype], outer, inner, x.shape[-2],
+        at[1] + (k.stride(-2),) + at[3] + (out_strides[1][-2],)
+    wk = (1, 0) if k is None else ws[1]
+    tail = _hip.ROTARY_ARGS[1].pack(
+        *ws[0], *wk, _POSITIONS[positions.dtype], _DTYPES[x.dtype], outer, inner, x.shape[-2],
         0 if k is None else k.shape[-2], d, pairs, axes, parts[0] if axes > 1 else 0,
         parts[0] + parts[1] if axes > 2 else 0, bool(interleaved), norm, bool(inverse),
-        positions.stride(0), *at[2 * n], *at[0], x.stride(-2), *at[n], ys[0].stride(-2), *second,
-        float(eps), _hip.stream(dev))
-    _call(_hip.lib().cf_rotary, "cf_rotary", dev, args)
-    if ev is not None:
-        m = sum(t.numel() for t in xs)
-        _t1("qk_norm_rotary" if norm else "rotary", ev, nbytes=2 * m * x.element_size())
-    return ys
+        positions.stride(0), *at[2 * n], *at[0], x.stride(-2), *at[n], out_strides[0][-2], *second,
+        float(eps))
+    return dev, tail
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *,
@@ -481,7 +592,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, *,
     inverse turns back.  out: a tensor for the output, x itself to turn in
     place."""
     return _rotate(x, None, positions, freqs, sections, interleaved, inverse, False, 0.0,
-                   (None,), (out,), ("x",))[0]
+                   (None, None), (out, None), ("x",))[0]
 
 
 def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,

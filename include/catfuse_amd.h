@@ -823,13 +823,13 @@ typedef struct CfDecayAttentionArgs {
   float* state_out;
   void* out;
   const void* cu_seqlens;
+  void* workspace;
+  void* stream;
   int64_t cu_wide, zero_rest, dtype, seqs, tokens, heads, kv_heads, dk, dv;
   int64_t q_batch, q_token, q_head, k_batch, k_token, k_head;
   int64_t v_batch, v_token, v_head, out_batch, out_token, out_head;
-  void* workspace;
   int64_t segment, workspace_bytes;
   double scale;
-  void* stream;
 } CfDecayAttentionArgs;
 int cf_decay_attention(const CfDecayAttentionArgs* args);
 
@@ -846,10 +846,10 @@ typedef struct CfDecayStepArgs {
   float* state;
   void* out;
   const void* slots;
+  void* stream;
   int64_t slots_wide, dtype, rows, heads, kv_heads, dk, dv, pool, state_slot;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
   double scale;
-  void* stream;
 } CfDecayStepArgs;
 int cf_decay_attention_step(const CfDecayStepArgs* args);
 
@@ -873,6 +873,7 @@ typedef struct CfRotaryArgs {
   const void* k_weight;
   const void* positions;
   const double* freqs;
+  void* stream;
   int64_t x_weight_f32, x_weight_head, k_weight_f32, k_weight_head, pos_kind, dtype;
   int64_t outer, inner, x_heads, k_heads, d, pairs, axes, section1, section2;
   int64_t interleaved, norm, inverse;
@@ -880,7 +881,6 @@ typedef struct CfRotaryArgs {
   int64_t x_outer, x_inner, x_head, x_out_outer, x_out_inner, x_out_head;
   int64_t k_outer, k_inner, k_head, k_out_outer, k_out_inner, k_out_head;
   double eps;
-  void* stream;
 } CfRotaryArgs;
 int cf_rotary(const CfRotaryArgs* args);
 

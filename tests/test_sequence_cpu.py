@@ -29,8 +29,8 @@ def test_blocks_mirror_the_header(cname, block):
             kinds += kind * (line.count(",") + 1)
     want = "".join(f"{n}{c}" if n > 1 else c
                    for c, n in ((c, len(list(g))) for c, g in itertools.groupby(kinds)))
-    assert block.format == "=" + want
-    assert block.size == 8 * len(kinds)
+    assert block[0].format + block[1].format[1:] == "=" + want
+    assert block[0].size + block[1].size == 8 * len(kinds)
 
 
 def test_limits_mirror_the_header():
@@ -41,6 +41,7 @@ def test_limits_mirror_the_header():
     assert sequence.MAX_VALUE_DIM == limit("CF_DECAY_MAX_DV")
     assert sequence.MAX_SEQUENCES == limit("CF_DECAY_MAX_SEQS")
     assert sequence.MAX_ROTARY_DIM == limit("CF_ROTARY_MAX_DIM")
+    assert sequence.MAX_TOKENS == limit("CF_DECAY_MAX_TOKENS")
     assert sequence.SPAN_BYTES == limit("CF_DECAY_SPAN_BYTES")
     assert sequence.CHUNK == limit("CF_DECAY_CHUNK")
     assert sequence.MAX_TOKEN_STRIDE == limit("CF_DECAY_MAX_TOKEN_STRIDE")
@@ -58,7 +59,9 @@ def _block(cname, block, **fields):
     """A block whose every field is 1 (a pointer that is never read) or as given."""
     names = _fields(cname)
     assert set(fields) <= set(names)
-    return block.pack(*(fields.get(n, 1.0 if n in ("scale", "eps") else 1) for n in names))
+    values = [fields.get(n, 1.0 if n in ("scale", "eps") else 1) for n in names]
+    pointers = block[0].size // 8
+    return block[0].pack(*values[:pointers]) + block[1].pack(*values[pointers:])
 
 
 def test_c_entries_refuse():
