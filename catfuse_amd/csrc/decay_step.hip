@@ -56,7 +56,10 @@ __global__ __launch_bounds__(256) void decay_step_kernel(StepArgs a) {
       for (int i = 0; i < VEC; ++i) out[row * a.orow + c + i] = from_f<T>(0.0f);
     return;
   }
-  const float w = (float)exp((double)a.log_decay[h]);
+  // w as a sum of two floats: the rounding of one would shift the horizon of a
+  // slow decay by the token (1e-4 of a state after 4096 tokens)
+  const double wd = exp((double)a.log_decay[h]);
+  const float w = (float)wd, wl = wd < 1e300 ? (float)(wd - (double)w) : 0.0f;
   float* const s = a.state + slot * a.state_slot + (int64_t)h * a.dk * a.dv + c;
   for (;;) {
     // the next row of this slot; nothing to do if an earlier row has it
@@ -101,7 +104,7 @@ __global__ __launch_bounds__(256) void decay_step_kernel(StepArgs a) {
           if (d >= a.dk) break;
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
-            y[u].v[i] = __builtin_fmaf(y[u].v[i], w, ks[d] * x[i]);
+            y[u].v[i] = __builtin_fmaf(y[u].v[i], w, __builtin_fmaf(y[u].v[i], wl, ks[d] * x[i]));
             p[i] = __builtin_fmaf(qs[d], y[u].v[i], p[i]);
           }
           *reinterpret_cast<Vec<float, VEC>*>(s + (int64_t)d * a.dv) = y[u];

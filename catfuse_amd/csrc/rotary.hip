@@ -62,35 +62,61 @@ __device__ __forceinline__ float2 rotary_angle(double pos, double freq) {
 // Rows (a token's head) of LG lanes; a lane holds PU pair units (VE pairs: two
 // vectors of VE elements) and RU vectors of channels that are not turned.
 // A workgroup takes TT tokens: their angles first, one a thread, into LDS, so
-// that the sines are computed once for all heads.
+// that the sines are computed once for all heads; also there where each token's
+// heads lie (64-bit divisions) and the weights that the heads share, as fp32.
 template <typename T, int VE, int PU, int RU>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a, int lg, int tt, int head_split) {
-  extern __shared__ float2 cs_sh[];          // [tt][pairs]
-  const int tid = threadIdx.x;
+  extern __shared__ __attribute__((aligned(32))) char lds[];
+  const int tid = threadIdx.x, shared_d = (a.d + 7) / 8 * 8;
+  int64_t* const at_sh = reinterpret_cast<int64_t*>(lds);              // [tt][4]: x, y, k, k's y
+  float2* const cs_sh = reinterpret_cast<float2*>(at_sh + 4 * tt);     // [tt][pairs]
+  float* const w_sh = reinterpret_cast<float*>(cs_sh + (tt * a.pairs + 3) / 4 * 4);  // [2][shared_d]
   const int64_t tokens = a.outer * a.inner, tok0 = (int64_t)blockIdx.x * tt;
   const int ntok = (int)(tokens - tok0 < tt ? tokens - tok0 : tt);
   for (int i = tid; i < ntok * a.pairs; i += 256) {
     const int t = i / a.pairs, p = i % a.pairs;
     int axis = 0;
     while (axis + 1 < a.axes && p >= a.sec[axis + 1]) ++axis;
-    const int64_t tok = tok0 + t, o = tok / a.inner, n = tok % a.inner;
+    const int64_t tok = tok0 + t, o = a.outer == 1 ? 0 : tok / a.inner, n = tok - o * a.inner;
     float2 cs = rotary_angle(rotary_pos(a, axis * a.pa + o * a.po + n * a.pi), a.freqs[p]);
     cs.y *= a.sign;
     cs_sh[i] = cs;
   }
+  for (int i = tid; i < ntok; i += 256) {
+    const int64_t tok = tok0 + i, o = a.outer == 1 ? 0 : tok / a.inner, n = tok - o * a.inner;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      at_sh[4 * i + 2 * j] = o * a.t[j].xo + n * a.t[j].xi;
+      at_sh[4 * i + 2 * j + 1] = o * a.t[j].yo + n * a.t[j].yi;
+    }
+  }
+  if (a.norm) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const RotaryTensor& r = a.t[j];
+      if (r.weight == nullptr || r.weight_head == 0)
+        for (int i = tid; i < a.d; i += 256)
+          w_sh[j * shared_d + i] =
+              r.weight == nullptr ? 1.0f
+              : r.weight_f32      ? reinterpret_cast<const float*>(r.weight)[i]
+                                  : to_f(reinterpret_cast<const T*>(r.weight)[i]);
+    }
+  }
   __syncthreads();
   const int lane = tid % lg, heads = a.t[0].heads + a.t[1].heads;
   const int upairs = a.pairs / VE, urest = (a.d - 2 * a.pairs) / VE;
-  const int rows = ntok * heads, step = 256 / lg * head_split;
-  for (int row = tid / lg + 256 / lg * (int)blockIdx.y; row < rows; row += step) {
-    const int t = row / heads;
-    int h = row % heads;
-    const bool second = h >= a.t[0].heads;
-    const RotaryTensor& r = second ? a.t[1] : a.t[0];
-    if (second) h -= a.t[0].heads;
-    const int64_t tok = tok0 + t, o = tok / a.inner, n = tok % a.inner;
-    const T* const x = (const T*)r.x + o * r.xo + n * r.xi + h * r.xh;
-    T* const y = (T*)r.y + o * r.yo + n * r.yi + h * r.yh;
+  const int step = 256 / lg * head_split;
+  int t = 0, head = tid / lg + 256 / lg * (int)blockIdx.y;   // the row: token and head of both
+  for (;; head += step) {
+    while (head >= heads) {
+      head -= heads;
+      ++t;
+    }
+    if (t >= ntok) break;
+    const int second = head >= a.t[0].heads ? 1 : 0, h = head - (second ? a.t[0].heads : 0);
+    const RotaryTensor& r = a.t[second];
+    const T* const x = (const T*)r.x + at_sh[4 * t + 2 * second] + h * r.xh;
+    T* const y = (T*)r.y + at_sh[4 * t + 2 * second + 1] + h * r.yh;
     float va[PU][VE], vb[PU][VE], vr[RU > 0 ? RU : 1][VE];
     float sum = 0.0f;
 #pragma unroll
@@ -126,33 +152,34 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a, int lg, int t
       // (the lanes of a row run together: rows are whole groups of lg lanes)
       for (int m = lg >> 1; m > 0; m >>= 1) sum += __shfl_xor(sum, m, 64);
       const float inv = 1.0f / __builtin_sqrtf(sum / (float)a.d + a.eps);
-      auto weight = [&](int c) {
-        if (r.weight == nullptr) return 1.0f;
-        const int64_t at = h * r.weight_head + c;
-        return r.weight_f32 ? reinterpret_cast<const float*>(r.weight)[at]
-                            : to_f(reinterpret_cast<const T*>(r.weight)[at]);
+      // the weights of VE channels from c on, times the norm
+      auto scale = [&](float* v, int c) {
+        if (r.weight == nullptr || r.weight_head == 0) {
+          const Vec<float, VE> w =
+              *reinterpret_cast<const Vec<float, VE>*>(w_sh + second * shared_d + c);
+#pragma unroll
+          for (int i = 0; i < VE; ++i) v[i] = v[i] * inv * w.v[i];
+        } else {
+          const int64_t from = h * r.weight_head + c;
+#pragma unroll
+          for (int i = 0; i < VE; ++i)
+            v[i] = v[i] * inv * (r.weight_f32 ? reinterpret_cast<const float*>(r.weight)[from + i]
+                                              : to_f(reinterpret_cast<const T*>(r.weight)[from + i]));
+        }
       };
 #pragma unroll
       for (int u = 0; u < PU; ++u) {
         const int unit = lane + u * lg;
         if (unit < upairs) {
           const int ca = a.interleaved ? 2 * unit * VE : unit * VE;
-          const int cb = a.interleaved ? ca + VE : a.pairs + unit * VE;
-#pragma unroll
-          for (int i = 0; i < VE; ++i) {
-            va[u][i] = va[u][i] * inv * weight(ca + i);
-            vb[u][i] = vb[u][i] * inv * weight(cb + i);
-          }
+          scale(va[u], ca);
+          scale(vb[u], a.interleaved ? ca + VE : a.pairs + unit * VE);
         }
       }
 #pragma unroll
       for (int u = 0; u < RU; ++u) {
         const int unit = lane + u * lg;
-        if (unit < urest) {
-#pragma unroll
-          for (int i = 0; i < VE; ++i)
-            vr[u][i] = vr[u][i] * inv * weight(2 * a.pairs + unit * VE + i);
-        }
+        if (unit < urest) scale(vr[u], 2 * a.pairs + unit * VE);
       }
     }
 #pragma unroll
@@ -202,6 +229,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a, int lg, int t
 }
 
 constexpr int ROTARY_LDS = 32768;   // bytes of angles a workgroup holds at most
+constexpr int ROTARY_TOKENS = 256;  // tokens of a workgroup at most (32 bytes of LDS each)
 
 template <typename T, int VE, int PU, int RU>
 hipError_t launch_rotary_v(const RotaryArgs& a, int lg, hipStream_t st) {
@@ -211,6 +239,7 @@ hipError_t launch_rotary_v(const RotaryArgs& a, int lg, hipStream_t st) {
   int tt = (4 * (256 / lg) + heads - 1) / heads;
   const int fit = a.pairs > 0 ? ROTARY_LDS / (8 * a.pairs) : tt;
   if (tt > fit) tt = fit;
+  if (tt > ROTARY_TOKENS) tt = ROTARY_TOKENS;
   if (tt < 1) tt = 1;
   // few tokens: their rows over several workgroups
   const int64_t groups = (tokens + tt - 1) / tt;
@@ -218,7 +247,8 @@ hipError_t launch_rotary_v(const RotaryArgs& a, int lg, hipStream_t st) {
   while (split < 16 && groups * split < 256 && split * (256 / lg) < tt * heads) split *= 2;
   if (groups > 0x7fffffff) return hipErrorInvalidValue;
   hipLaunchKernelGGL((rotary_kernel<T, VE, PU, RU>), dim3((unsigned)groups, (unsigned)split),
-                     dim3(256), (size_t)tt * a.pairs * 8, st, a, lg, tt, split);
+                     dim3(256), (size_t)tt * 32 + (tt * a.pairs + 3) / 4 * 32 + (a.d + 7) / 8 * 64, st,
+                     a, lg, tt, split);
   return hipGetLastError();
 }
 

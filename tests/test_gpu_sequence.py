@@ -350,6 +350,26 @@ def test_step_many_rows(cuda):
     assert torch.equal(out[::2], a) and torch.equal(out[1::2], b) and torch.equal(state, pool)
 
 
+def test_step_many_tokens(cuda):
+    """4096 tokens, one after another: the rounding of the decay does not add up."""
+    f = torch.tensor([-2.0 ** -12, -2.0 ** -5])
+    g = torch.Generator().manual_seed(3)
+    N = 4096
+    k, v = torch.randn(N, 2, 16, generator=g), torch.randn(N, 2, 8, generator=g)
+    state = torch.zeros(1, 2, 16, 8, device=cuda)
+    kg, vg, fg = k.to(cuda), v.to(cuda), f.to(cuda)
+    for t in range(N):
+        kernels.decay_attention_step(kg[t:t + 1], kg[t:t + 1], vg[t:t + 1], fg, state)
+    left = torch.exp(f.double() * (N - 1 - torch.arange(N, dtype=torch.float64))[:, None])
+    def total(k, v):
+        return torch.einsum("th,thi,thj->hij", left, k, v)
+    want, big = total(k.double(), v.double()), total(k.double().abs(), v.double().abs())
+    # two roundings a token of a state that fades: at most 2 u sum_t |S_t| w^(N-1-t);
+    # |S_t| is bound by big (1 - w^t) / (1 - w^N), so the sum by big times the
+    # horizon 1 / (1 - w), of random signs by its root: 64, and six deviations
+    _close(state[0], want, big, F32, 2 * 6 * 64 * U32)
+
+
 def test_step_strides(cuda):
     """States of one layer among others, heads of a fused projection, an
     output among other columns, misaligned states."""
@@ -418,7 +438,7 @@ def _norm(d):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("d,rot", [(2, 2), (8, 4), (32, 32), (64, 64), (80, 80), (128, 128),
+@pytest.mark.parametrize("d,rot", [(2, 2), (8, 4), (8, 8), (16, 16), (32, 32), (64, 64), (80, 80), (128, 128),
                                    (128, 32), (256, 256), (96, 48), (70, 70), (100, 36), (33, 32),
                                    (512, 512), (512, 2), (511, 16), (256, 16)])
 @pytest.mark.parametrize("interleaved", [False, True])
@@ -431,6 +451,9 @@ def test_rotary_sizes(cuda, dtype, d, rot, interleaved):
     want, size = _turned(x, pos[None], freqs, (rot // 2,), interleaved)
     _close(y, want, size, dtype, TURN)
     assert torch.equal(y[..., rot:].cpu(), x[..., rot:])
+    many = x.repeat(97, 1, 1)[:, :1].to(cuda)         # more tokens than a workgroup takes, one head
+    z = kernels.rotary(many, pos.repeat(97).to(cuda), freqs.to(cuda), interleaved=interleaved)
+    assert torch.equal(z, y[:, :1].repeat(97, 1, 1))
     back = kernels.rotary(y, pos.to(cuda), freqs.to(cuda), interleaved=interleaved, inverse=True)
     want, size = _turned(y.cpu(), pos[None], freqs, (rot // 2,), interleaved, inverse=True)
     _close(back, want, size, dtype, TURN)
