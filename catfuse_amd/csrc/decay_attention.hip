@@ -44,7 +44,7 @@ struct DecayArgs {
   int64_t segment, segments; // tokens a segment; segments in all at most
   int heads, group, dk, dv, slices;
   int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, ob, ot, oh;
-  int vec;                   // 16-byte accesses are aligned and whole
+  int vec;                   // 16-byte accesses are aligned and whole, rows apart
   float scale;
 };
 
@@ -128,24 +128,22 @@ struct Unit { u32x4 w[sizeof(T) / 2]; };
 // This thread's units of a chunk's image: piece tid % (D / 8) of the rows
 // tid / (D / 8) + i NT / (D / 8).  Rows from n on and channels from d on are
 // zeros: out of the buffer's range (VEC: 16-byte loads, from aligned rows of
-// whole 16-byte pieces) or not read.
+// whole 16-byte pieces that do not overlap) or not read.
 template <typename T, int U, int D, int NT, bool VEC>
 __device__ __forceinline__ void load_units(Unit<T>* u, const T* base, int n, int64_t stride, int d) {
   constexpr int PER = 16 / sizeof(T), ROWS = NT / (D / 8);
   const int row = threadIdx.x / (D / 8), c0 = threadIdx.x % (D / 8) * 8;
   if constexpr (VEC) {
-    const int st = (int)stride * (int)sizeof(T);
+    const int st = (int)stride * (int)sizeof(T);   // at least d's: rows from n on are beyond the range
     const __amdgpu_buffer_rsrc_t rsrc =
         rows_rsrc(base, (uint32_t)((n - 1) * st + d * (int)sizeof(T)));
-    const uint32_t at = (uint32_t)(row * st + c0 * (int)sizeof(T));
 #pragma unroll
-    for (int i = 0; i < U; ++i)
+    for (int p = 0; p < (int)(sizeof(T) / 2); ++p) {
+      const uint32_t at = c0 + p * PER < d ? (uint32_t)(row * st + (c0 + p * PER) * (int)sizeof(T)) : OOB;
 #pragma unroll
-      for (int p = 0; p < (int)(sizeof(T) / 2); ++p) {
-        const uint32_t off = at + (uint32_t)(i * ROWS * st + 16 * p);
-        u[i].w[p] = __builtin_amdgcn_raw_buffer_load_b128(
-            rsrc, row + i * ROWS < n && c0 + p * PER < d ? off : OOB, 0, 0);
-      }
+      for (int i = 0; i < U; ++i)
+        u[i].w[p] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at + (uint32_t)(i * ROWS * st), 0, 0);
+    }
   } else {
     typedef Vec<T, 8> V8;
 #pragma unroll 1
@@ -661,7 +659,7 @@ void decay_chunk_kernel(DecayArgs a) {
         const __amdgpu_buffer_rsrc_t ro =
             rows_rsrc(op, (uint32_t)((n - 1) * st + dvs * (int)sizeof(T)));
         auto at = [&](int i, int c) {
-          return i < n && c < dvs ? (uint32_t)(i * st + c * (int)sizeof(T)) : OOB;
+          return c < dvs ? (uint32_t)(i * st + c * (int)sizeof(T)) : OOB;
         };
 #pragma unroll
         for (int qt = 0; qt < CT; ++qt) {
@@ -908,7 +906,7 @@ CF_API int cf_decay_attention(const CfDecayAttentionArgs* p) {
   const int size = x.dtype == SEQ_F32 ? 4 : 2, per = 16 / size;
   auto vec = [&](const void* base, int64_t b, int64_t t, int64_t h, int64_t d) {
     return (uintptr_t)base % 16 == 0 && b % per == 0 && t % per == 0 && h % per == 0 &&
-           d % per == 0;
+           d % per == 0 && t >= d;
   };
   a.vec = vec(x.q, a.qb, a.qt, a.qh, x.dk) && vec(x.k, a.kb, a.kt, a.kh, x.dk) &&
           vec(x.v, a.vb, a.vt, a.vh, x.dv) && vec(x.out, a.ob, a.ot, a.oh, x.dv);

@@ -311,8 +311,10 @@ def _attention_plan(q, k, v, log_decay, scale, state, cu_seqlens, out):
         raise ValueError(f"{N} tokens (at most {MAX_TOKENS})")
 
     def steps(t):
-        # (a dimension of one element may have any stride)
-        return (0 if packed else t.stride(0), t.stride(-3) if t.shape[-3] > 1 else 0, t.stride(-2))
+        # (a dimension of one element may have any stride: a plain one)
+        return (t.stride(0) if not packed and B > 1 else 0,
+                t.stride(-3) if N > 1 else t.shape[-1],
+                t.stride(-2) if t.shape[-2] > 1 else 0)
     # a new output is contiguous
     o = steps(out) if out is not None else (0 if packed else N * H * dv, H * dv, dv)
     segment, segments = _segment(B, N, packed, H, dk, dv, q.dtype == torch.float32)

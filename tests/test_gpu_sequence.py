@@ -178,6 +178,15 @@ def test_attention_strides(cuda):
         for other in (qt, flat):
             out, left = kernels.decay_attention(other, k, v, f)
             assert torch.equal(out, want) and torch.equal(left, s)
+        twice = k.as_strided(k.shape, (k.stride(0), 8, 16, 1))     # rows that overlap
+        want, s = kernels.decay_attention(q, twice.contiguous(), v, f)
+        out, left = kernels.decay_attention(q, twice, v, f)
+        assert torch.equal(out, want) and torch.equal(left, s)
+        row = q[:1, :1].contiguous()          # one token: its strides mean nothing
+        odd = row.as_strided(row.shape, (7, 0, 40, 1))
+        a = kernels.decay_attention(row, k[:1, :1].contiguous(), v[:1, :1].contiguous(), f)
+        b = kernels.decay_attention(odd, k[:1, :1], v[:1, :1], f)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
         one = k[:, :1].expand(2, 70, 2, 40)
         want, s = kernels.decay_attention(q, one.contiguous(), v, f)
         out, left = kernels.decay_attention(q, one, v, f)
