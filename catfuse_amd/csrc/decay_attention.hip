@@ -145,14 +145,27 @@ __device__ __forceinline__ void load_units(Unit<T>* u, const T* base, int n, int
         u[i].w[p] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at + (uint32_t)(i * ROWS * st), 0, 0);
     }
   } else {
-    typedef Vec<T, 8> V8;
-#pragma unroll 1
-    for (int i = 0; i < U; ++i) {
-      V8 x{};
-      const int r = row + i * ROWS;
+    // element by element, from a base brought to 16 bytes
+    const uintptr_t p = (uintptr_t)base, skip = p & 15;
+    const int st = (int)stride * (int)sizeof(T);
+    const __amdgpu_buffer_rsrc_t rsrc =
+        rows_rsrc((const void*)(p - skip), (uint32_t)((n - 1) * st + d * (int)sizeof(T) + (int)skip));
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (r < n && c0 + j < d) x.v[j] = base[(int64_t)r * stride + c0 + j];
+    for (int i = 0; i < U; ++i) {
+      const int r = row + i * ROWS;
+      const uint32_t at = (uint32_t)(r * st + c0 * (int)sizeof(T) + (int)skip);
+      Vec<T, 8> x;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t off = r < n && c0 + j < d ? at + (uint32_t)(j * sizeof(T)) : OOB;
+        if constexpr (sizeof(T) == 2) {
+          const uint16_t e = __builtin_amdgcn_raw_buffer_load_b16(rsrc, off, 0, 0);
+          x.v[j] = __builtin_bit_cast(T, e);
+        } else {
+          const uint32_t e = __builtin_amdgcn_raw_buffer_load_b32(rsrc, off, 0, 0);
+          x.v[j] = __builtin_bit_cast(T, e);
+        }
+      }
       u[i] = __builtin_bit_cast(Unit<T>, x);
     }
   }
@@ -304,9 +317,12 @@ __device__ __forceinline__ Span read_span(const DecayArgs& a, int64_t w) {
 // operand are taken in that order, so that eight registers on end are an
 // operand of the next chunk's q S as they lie.
 template <typename T, int DKP, int NW, int C, bool OUT, bool VEC>
-__global__ __launch_bounds__(64 * NW, DKP <= 128 && sizeof(T) == 2 ? 2 : 1)
+__global__ __launch_bounds__(64 * NW, DKP <= 128 ? 2 : 1)
 void decay_chunk_kernel(DecayArgs a) {
   constexpr int NL = parts_of<T>(), NP = NL == 3 ? 3 : 2, NT = 64 * NW;
+  // operands read ahead: one set; none of three parts, whose products take long
+  // enough and whose registers would cost the second workgroup of a CU
+  constexpr int AHEAD = NL == 3 ? 0 : 1, SETS = AHEAD + 1;
   constexpr int KT = DKP / 32, KS = DKP / 16, CT = C / 32, CS = C / 16, DVW = 32 * NW;
   constexpr int QK_BYTES = NL * C * DKP * 2, V_BYTES = NL * C * DVW * 2;
   constexpr int TILES = CT * (CT + 1) / 2;                     // score tiles that are not masked
@@ -508,28 +524,28 @@ void decay_chunk_kernel(DecayArgs a) {
         int gap0 = 32 * (qt - kt) + col - 4 * hi;
         asm volatile("" : "+v"(gap0));
         const float* const powers = pow_sh + gap0;
-        u32x4 ak[2][NL], bq[2][NL];
+        u32x4 ak[SETS][NL], bq[SETS][NL];
         auto read = [&](int s) {
 #pragma unroll
           for (int p = 0; p < NL; ++p) {
-            ak[s & 1][p] = row_operand<C, DKP>(lds, at_row, p, kt, s);
-            bq[s & 1][p] = row_operand<C, DKP>(lds + Q_AT, at_row, p, qt, s);
+            ak[s % SETS][p] = row_operand<C, DKP>(lds, at_row, p, kt, s);
+            bq[s % SETS][p] = row_operand<C, DKP>(lds + Q_AT, at_row, p, qt, s);
           }
         };
-        read(0);
+        if (AHEAD) read(0);
         float f[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) f[r] = powers[-(8 * (r >> 2) + (r & 3))];
         f16v acc = {};
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          if (s + 1 < KS) read(s + 1);
+          if (s + AHEAD < KS) read(s + AHEAD);
 #pragma unroll
           for (int x = 0; x < NL; ++x)
 #pragma unroll
             for (int y = 0; y < NL; ++y)
-              if (x + y < (NL == 1 ? 1 : NP)) acc = mfma(ak[s & 1][x], bq[s & 1][y], acc);
-          step();
+              if (x + y < (NL == 1 ? 1 : NP)) acc = mfma(ak[s % SETS][x], bq[s % SETS][y], acc);
+          if (AHEAD) step();
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -562,7 +578,7 @@ void decay_chunk_kernel(DecayArgs a) {
       // O^T = scale w^(i+1) S^T Q^T + V^T P^T: rows columns of the values,
       // columns queries (P holds the scale).
       {
-        u32x4 as[2][NP], bq[2][CT][NL];
+        u32x4 as[SETS][NP], bq[SETS][CT][NL];
         auto state_part = [&](int s) {       // S's operand, and S faded
           float x[8];
 #pragma unroll
@@ -570,25 +586,27 @@ void decay_chunk_kernel(DecayArgs a) {
             x[j] = S[s / 2][8 * (s & 1) + j];
             S[s / 2][8 * (s & 1) + j] = x[j] * fade;
           }
-          split8<NP>(x, as[s & 1]);
+          split8<NP>(x, as[s % SETS]);
         };
         auto read = [&](int s) {
 #pragma unroll
           for (int qt = 0; qt < CT; ++qt)
 #pragma unroll
             for (int y = 0; y < NL; ++y)
-              bq[s & 1][qt][y] = row_operand<C, DKP>(lds + Q_AT, at_row, y, qt, s);
+              bq[s % SETS][qt][y] = row_operand<C, DKP>(lds + Q_AT, at_row, y, qt, s);
         };
-        read(0);
-        state_part(0);
+        if (AHEAD) {
+          read(0);
+          state_part(0);
+        }
 #pragma unroll
         for (int qt = 0; qt < CT; ++qt) acc[qt] = f16v{};
         step();
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          if (s + 1 < KS) {
-            read(s + 1);
-            state_part(s + 1);
+          if (s + AHEAD < KS) {
+            read(s + AHEAD);
+            state_part(s + AHEAD);
           }
 #pragma unroll
           for (int x = 0; x < NP; ++x)
@@ -596,8 +614,8 @@ void decay_chunk_kernel(DecayArgs a) {
             for (int y = 0; y < NL; ++y)
 #pragma unroll
               for (int qt = 0; qt < CT; ++qt)
-                if (x + y < NP) acc[qt] = mfma(as[s & 1][x], bq[s & 1][qt][y], acc[qt]);
-          step();
+                if (x + y < NP) acc[qt] = mfma(as[s % SETS][x], bq[s % SETS][qt][y], acc[qt]);
+          if (AHEAD) step();
         }
       }
 #pragma unroll
@@ -718,33 +736,40 @@ void decay_chunk_kernel(DecayArgs a) {
 
     // S <- w^n S (above) + K^T (w^(n-1-j) V)
     {
-      u32x4 bv[2][3], ak[2][NL];
+      u32x4 bv[SETS][3], ak[SETS][NL];
       auto key_tile = [&](int i) {
 #pragma unroll
         for (int y = 0; y < NL; ++y)
-          ak[i & 1][y] = token_operand<C, DKP>(lds, at_key, y, i % KT, i / KT);
+          ak[i % SETS][y] = token_operand<C, DKP>(lds, at_key, y, i % KT, i / KT);
       };
       weights(0);
-      key_tile(0);
+      if (AHEAD) {
+        key_tile(0);
 #pragma unroll
-      for (int p = 0; p < 4; ++p) weigh(0, p, bv[0]);
-      if (CS > 1) weights(1);
+        for (int p = 0; p < 4; ++p) weigh(0, p, bv[0]);
+        if (CS > 1) weights(1);
+      }
       step();
 #pragma unroll
       for (int i = 0; i < CS * KT; ++i) {
         const int s = i / KT, t = i % KT;
-        if (i + 1 < CS * KT) key_tile(i + 1);
+        if (i + AHEAD < CS * KT) key_tile(i + AHEAD);
+        if (!AHEAD && t == 0) {
+          if (s > 0) weights(s);
+#pragma unroll
+          for (int p = 0; p < 4; ++p) weigh(s, p, bv[0]);
+        }
 #pragma unroll
         for (int y = 0; y < NL; ++y)
 #pragma unroll
           for (int p = 0; p < 3; ++p)
-            if (p + y < 3) S[t] = mfma(ak[i & 1][y], bv[s & 1][p], S[t]);
-        if (s + 1 < CS) {
+            if (p + y < 3) S[t] = mfma(ak[i % SETS][y], bv[s % SETS][p], S[t]);
+        if (AHEAD && s + 1 < CS) {
 #pragma unroll
-          for (int p = t * 4 / KT; p < (t + 1) * 4 / KT; ++p) weigh(s + 1, p, bv[(s + 1) & 1]);
+          for (int p = t * 4 / KT; p < (t + 1) * 4 / KT; ++p) weigh(s + 1, p, bv[(s + 1) % SETS]);
           if (t == KT - 1 && s + 2 < CS) weights(s + 2);
         }
-        step();
+        if (AHEAD) step();
       }
     }
     if (any_bad && bad_from < C) {

@@ -192,21 +192,20 @@ def _call(fn, what: str, dev, args) -> None:
 # attention with a decay for each head
 # ---------------------------------------------------------------------------
 
-def _segment(seqs: int, tokens: int, packed: bool, heads: int, dk: int, dv: int, wide: bool):
+def _segment(seqs: int, tokens: int, packed: bool, heads: int, dk: int, dv: int):
     """(tokens a segment, segments in all); (0, 0): whole sequences.
 
     A workgroup takes a segment of one head and `width` columns; the segments'
     own states cost a further pass over k and v (about half of the outputs'
     time), so sequences are split where they leave most of the card idle, into
     about as many workgroups as run at once.  Measured (us, bf16, heads of
-    128): one sequence of 65536 tokens, 32 heads: segments of 2048 tokens 756,
-    4096 739, 8192 1190; 24 packed ones of 24011 tokens, 16 heads: whole 266,
-    384 183, 768 176; fp32, 3 sequences of 1237, 8 heads of 80: whole 280, 64
-    51, 128 47, 256 75; one of 196, 12 heads of 32: whole 22, 64 18."""
+    128): one sequence of 65536 tokens, 32 heads: segments of 2048 tokens 729,
+    4096 719, 8192 1190; 24 packed ones of 24011 tokens, 16 heads: whole 266,
+    384 185, 768 180, 1024 175; fp32, 3 sequences of 1237, 8 heads of 80: whole
+    280, 64 43, 128 46, 192 58; one of 196, 12 heads of 32: whole 21, 64 17."""
     width = 32 if dk <= 32 else 64 if dk <= 64 else 128
     columns = heads * -(-dv // width)          # workgroups of one segment
-    at_once = (2048 if dk <= 32 else 1024 if dk <= 64 else 512 if dk <= 128 else 256) // \
-        (2 if wide and 32 < dk <= 128 else 1)
+    at_once = 2048 if dk <= 32 else 1024 if dk <= 64 else 512 if dk <= 128 else 256
     if tokens <= 2 * CHUNK or seqs * columns * (1 if packed else 8) > 4 * at_once:
         return 0, 0
     total = tokens if packed else seqs * tokens
@@ -317,7 +316,7 @@ def _attention_plan(q, k, v, log_decay, scale, state, cu_seqlens, out):
                 t.stride(-2) if t.shape[-2] > 1 else 0)
     # a new output is contiguous
     o = steps(out) if out is not None else (0 if packed else N * H * dv, H * dv, dv)
-    segment, segments = _segment(B, N, packed, H, dk, dv, q.dtype == torch.float32)
+    segment, segments = _segment(B, N, packed, H, dk, dv)
     ws_bytes = segments * (4 * H * dk * dv + SPAN_BYTES)
     tail = _hip.DECAY_ATTENTION_ARGS[1].pack(
         packed and cu_seqlens.dtype == torch.int64, out is None, _DTYPES[q.dtype], B, N, H, Hk, dk,
