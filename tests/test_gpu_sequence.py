@@ -490,6 +490,17 @@ def test_rotary_axes(cuda, dtype, sections, kind):
     _close(y.flatten(0, 2), want, size, dtype, TURN)
 
 
+def test_rotary_large(cuda):
+    """More output than the caches hold (streaming stores): the bits of the same
+    rows in small launches."""
+    N = 13000
+    x = torch.randn(N, 32, 128, device=cuda).bfloat16()
+    pos, freqs = torch.arange(N, device=cuda), kernels.rotary_freqs(64, device=cuda)
+    y = kernels.rotary(x, pos, freqs)
+    for i in range(0, N, 4001):
+        assert torch.equal(y[i:i + 4001], kernels.rotary(x[i:i + 4001], pos[i:i + 4001], freqs))
+
+
 def test_rotary_far_positions(cuda):
     """Positions of up to 2^31 keep an angle within 2^-52 of the turns."""
     x = torch.ones(4, 1, 8, device=cuda)
