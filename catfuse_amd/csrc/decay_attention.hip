@@ -258,6 +258,26 @@ __device__ __forceinline__ Span find_span(const DecayArgs& a, int64_t w) {
     return s;
   }
   const int lane = threadIdx.x & 63;
+  if (a.segments == a.seqs) {
+    // whole sequences (a segment holds every token): the largest offset up to
+    // the sequence's, all loads in flight
+    int64_t m = 0;
+    for (int64_t i = lane; i <= w; i += 64) {
+      const int64_t x = seq_offset(a.cu, a.cu_wide, i, a.tokens);
+      if (x > m) m = x;
+    }
+    for (int d = 1; d < 64; d *= 2) {
+      const int64_t o = __shfl_xor(m, d, 64);
+      if (o > m) m = o;
+    }
+    const int64_t end = seq_offset(a.cu, a.cu_wide, w + 1, a.tokens);
+    s.seq = w;
+    s.part = 0;
+    s.parts = 1;
+    s.begin = uniform(m);
+    s.len = uniform(end > m ? end - m : 0);
+    return s;
+  }
   int64_t before = 0, top = 0;               // segments and the largest offset so far
   for (int64_t b0 = 0; b0 < a.seqs; b0 += 64) {
     const int64_t b = b0 + lane;
@@ -919,7 +939,8 @@ CF_API int cf_decay_attention(const CfDecayAttentionArgs* p) {
     a.segments = x.cu_seqlens ? x.tokens / x.segment + x.seqs
                               : x.seqs * ((x.tokens + x.segment - 1) / x.segment);
     const int64_t state = 4 * x.heads * x.dk * x.dv;
-    if (!x.workspace || x.workspace_bytes / (state + CF_DECAY_SPAN_BYTES) < a.segments)
+    if (!x.workspace || (uintptr_t)x.workspace % 16 != 0 ||
+        x.workspace_bytes / (state + CF_DECAY_SPAN_BYTES) < a.segments)
       return (int)hipErrorInvalidValue;
     a.spans = x.workspace;
     a.ws = (float*)((char*)x.workspace + a.segments * CF_DECAY_SPAN_BYTES);

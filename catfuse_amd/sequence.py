@@ -231,7 +231,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     number b the rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1.  Query head h
     reads key head h // (H // Hk).  fp32, fp16 or bf16, all of one type; the
     last dimension contiguous, other strides free.  dk <= 256, dv <= 1024.
-    log_decay fp32 [H]: 0 keeps everything, -inf only the token itself.
+    log_decay fp32 [H]: 0 keeps everything, -inf only the token itself; above 0
+    the past grows (exp(64 log_decay) has to be finite).
     scale: dk ** -0.5 if None.
     state: fp32 [sequences, H, dk, dv], S before the first token (None: zeros).
     cu_seqlens: int32 or int64 [sequences + 1], in device memory and therefore
@@ -243,6 +244,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     Returns (out [.., H, dv], state after the last token), or out alone
     without return_state.  Sums and states are fp32; a token that holds an
     infinity or NaN does not reach the tokens before it."""
+    scale = None if scale is None else float(scale)
     try:
         key = (decay_attention, _looks(q), _looks(k), _looks(v), _looks(log_decay), _looks(state),
                _looks(cu_seqlens), _looks(out), scale, return_state, torch.is_grad_enabled())
@@ -344,6 +346,7 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     the same slot are taken as consecutive tokens of one sequence.
 
     Returns out [rows, H, dv]."""
+    scale = None if scale is None else float(scale)
     try:
         key = (decay_attention_step, _looks(q), _looks(k), _looks(v), _looks(log_decay),
                _looks(state), _looks(slots), _looks(out), scale, torch.is_grad_enabled())
@@ -471,12 +474,14 @@ def _weight(w, name, x):
 
 def _rotate(x, k, positions, freqs, sections, interleaved, inverse, norm, eps, weights, outs,
             names):
+    sections = None if sections is None else tuple(int(n) for n in sections)
+    interleaved, inverse = bool(interleaved), bool(inverse)
     try:
         key = (_rotate, _looks(x), _looks(k), _looks(positions), _looks(freqs), sections,
                interleaved, inverse, norm, eps, _looks(weights[0]), _looks(weights[1]),
                _looks(outs[0]), _looks(outs[1]), torch.is_grad_enabled())
         plan = _PLANS.get(key)
-    except (AttributeError, TypeError):      # not tensors (or sections a list): checked below
+    except (AttributeError, TypeError):      # not tensors: the checks say which
         key = plan = None
     if plan is None:
         plan = _rotary_plan(x, k, positions, freqs, sections, interleaved, inverse, norm, eps,
@@ -485,15 +490,15 @@ def _rotate(x, k, positions, freqs, sections, interleaved, inverse, norm, eps, w
             _keep(key, plan)
     dev, tail = plan
     ys = []
-    for t, out in zip((x, k), outs):
+    for i, (t, out) in enumerate(zip((x, k), outs)):
         if t is None:
             ys.append(None)
         elif out is None:
             ys.append(torch.empty(t.shape, dtype=t.dtype, device=dev))
         else:
             in_place = out.data_ptr() == t.data_ptr() and out.stride() == t.stride()
-            inputs = (x, k, positions, freqs) + weights
-            _require_apart(out, "out", tuple(o for o in inputs if not (in_place and o is t)))
+            others = (positions, freqs, k if i == 0 else x) + weights
+            _require_apart(out, "out", others if in_place else others + (t,))
             ys.append(out)
     if outs[0] is not None and outs[1] is not None:
         _require_apart(ys[0], "out", (ys[1],))
@@ -535,7 +540,7 @@ def _rotary_plan(x, k, positions, freqs, sections, interleaved, inverse, norm, e
     pairs = freqs.shape[0]
     if not 1 <= d <= MAX_ROTARY_DIM or not 1 <= pairs or 2 * pairs > d:
         raise ValueError(f"{pairs} pairs in heads of {d} channels (at most {MAX_ROTARY_DIM})")
-    parts = (pairs,) if sections is None else tuple(int(n) for n in sections)
+    parts = (pairs,) if sections is None else sections
     axes = len(parts)
     if not 1 <= axes <= MAX_AXES or sum(parts) != pairs or min(parts) < 0:
         raise ValueError(f"sections {parts} do not make {pairs} pairs of up to {MAX_AXES} axes")
@@ -571,7 +576,7 @@ def _rotary_plan(x, k, positions, freqs, sections, interleaved, inverse, norm, e
     tail = _hip.ROTARY_ARGS[1].pack(
         *ws[0], *wk, _POSITIONS[positions.dtype], _DTYPES[x.dtype], outer, inner, x.shape[-2],
         0 if k is None else k.shape[-2], d, pairs, axes, parts[0] if axes > 1 else 0,
-        parts[0] + parts[1] if axes > 2 else 0, bool(interleaved), norm, bool(inverse),
+        parts[0] + parts[1] if axes > 2 else 0, interleaved, norm, inverse,
         positions.stride(0), *at[2 * n], *at[0], x.stride(-2), *at[n], out_strides[0][-2], *second,
         float(eps))
     return dev, tail

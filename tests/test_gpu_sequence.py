@@ -156,6 +156,39 @@ def test_attention_rest_rows(cuda):
     assert torch.equal(o[0], out[20:]) and torch.equal(s[0], left[2])
 
 
+@pytest.mark.parametrize("B,N,H", [(3000, 9000, 2), (1500, 9000, 1), (130, 70000, 2)])
+def test_attention_many_sequences(cuda, B, N, H):
+    """Offsets beyond one scan of a wave, whole sequences and split ones (of any
+    length, many empty), some out of order: each as by itself."""
+    g = torch.Generator().manual_seed(B)
+    q, k, v = (x.to(cuda) for x in _inputs((N, H, 16), (N, 1, 16), 16, F32, B))
+    f = _decays(H).to(cuda)
+    cu = torch.randint(0, N + 1, (B + 1,), generator=g).sort()[0]
+    cu[0], cu[-1] = 0, N
+    want = cu.clone()
+    cu[B // 2], cu[B // 3] = -7, 5                   # count as their predecessors
+    want[B // 2], want[B // 3] = want[B // 2 - 1], want[B // 3 - 1]
+    out, left = kernels.decay_attention(q, k, v, f, cu_seqlens=cu.to(cuda))
+    for b in [0, 1, 63, 64, 65, B // 3 - 1, B // 3, B // 2 - 1, B // 2, B - 2, B - 1]:
+        i, j = int(want[b]), int(want[b + 1])
+        o, s = kernels.decay_attention(q[None, i:j], k[None, i:j], v[None, i:j], f)
+        # (split in other places: both within the tolerance of the definition's bound)
+        big, sbig = kernels.decay_attention(q[None, i:j].abs(), k[None, i:j].abs(),
+                                            v[None, i:j].abs(), f)
+        assert bool(((out[i:j] - o[0]).abs() <= 150 * U32 * big[0]).all())
+        assert bool(((left[b] - s[0]).abs() <= 150 * U32 * sbig[0]).all())
+
+
+def test_attention_scale(cuda):
+    """A scale of another value in the same tensor is another scale."""
+    q, k, v = (x.to(cuda) for x in _inputs((1, 40, 2, 16), (1, 40, 2, 16), 16, F32, 1))
+    f, scale = _decays(2).to(cuda), torch.tensor(0.5)
+    a, _ = kernels.decay_attention(q, k, v, f, scale=scale)
+    scale *= 4
+    b, _ = kernels.decay_attention(q, k, v, f, scale=scale)
+    assert torch.equal(b, 4 * a) and bool((a != 0).any())
+
+
 def test_attention_strides(cuda):
     """Heads of one fused projection, transposed heads, expanded keys, an
     output among other columns, misaligned rows: all the values of contiguous

@@ -78,7 +78,8 @@ def test_c_entries_refuse():
                 dict(log_decay=0), dict(segment=100), dict(segment=-64), dict(q_token=-1),
                 dict(out_token=8000001), dict(segment=64, tokens=65, workspace=0),
                 # 65 tokens of a packed sequence in segments of 64: up to two states of 1 x 1
-                dict(segment=64, tokens=65, workspace_bytes=2 * 52 - 1)):
+                dict(segment=64, tokens=65, workspace=64, workspace_bytes=2 * 52 - 1),
+                dict(segment=64, tokens=65, workspace=8, workspace_bytes=2 * 52)):
         assert attention(**dict(dict(segment=0), **bad)) == INVALID, bad
     assert attention(seqs=0, segment=0) == 0          # nothing to do, nothing launched
 
@@ -242,6 +243,10 @@ def test_rotary_in_place_and_overlaps():
     with pytest.raises(ValueError, match="overlaps"):
         kernels.qk_norm_rotary(q, k, *args, out=(rows[:, 24:].unflatten(1, (2, 8)),
                                                  rows[:, 32:].unflatten(1, (1, 8))))
+    with pytest.raises(ValueError, match="overlaps"):      # one tensor as both, one in place
+        kernels.qk_norm_rotary(q, q, *args, out=(q, None))
+    with pytest.raises(ValueError, match="overlaps"):
+        kernels.qk_norm_rotary(k, k, *args, out=(k, k))
     with pytest.raises(ValueError, match="two strides"):
         _turn(x=torch.zeros(2, 2, 2, 2, 8).transpose(0, 2), positions=torch.zeros(2, 2, 2))
 
