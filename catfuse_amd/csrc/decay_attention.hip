@@ -236,7 +236,8 @@ __device__ __forceinline__ void step() { __builtin_amdgcn_sched_barrier(0); }
 
 // Which (sequence, segment) a segment number is.  Packed sequences: every
 // wave scans the offsets, 64 a time, each offset at least its predecessor.
-struct alignas(16) Span { int64_t seq, part, parts, begin, len; };   // seq < 0: none
+// `turn`, of the i-th: the segment whose outputs are the i-th to be made.
+struct alignas(16) Span { int64_t seq, part, parts, begin, len, turn; };   // seq < 0: none
 static_assert(sizeof(Span) == CF_DECAY_SPAN_BYTES, "the workspace has one a segment");
 
 // The same value in every lane, kept in scalar registers.
@@ -323,7 +324,7 @@ __device__ __forceinline__ Span find_span(const DecayArgs& a, int64_t w) {
 // The same, as the launch of the segments' own states noted it.
 __device__ __forceinline__ Span read_span(const DecayArgs& a, int64_t w) {
   const Span s = reinterpret_cast<const Span*>(a.spans)[w];
-  return {uniform(s.seq), uniform(s.part), uniform(s.parts), uniform(s.begin), uniform(s.len)};
+  return {uniform(s.seq), uniform(s.part), uniform(s.parts), uniform(s.begin), uniform(s.len), 0};
 }
 
 // A workgroup takes a segment of a sequence, one head, 32 NW columns of the
@@ -363,13 +364,21 @@ void decay_chunk_kernel(DecayArgs a) {
   const unsigned shared = (unsigned)(a.group * a.slices), kv_heads = (unsigned)(a.heads / a.group);
   const unsigned slot = blockIdx.x >> 3;
   const unsigned super = slot / shared * 8 + (blockIdx.x & 7), inner = slot % shared;
-  const int64_t w = super / kv_heads;
+  int64_t w = super / kv_heads;
   if (w >= a.segments) return;
+  if (OUT && a.ws != nullptr) w = uniform(reinterpret_cast<const Span*>(a.spans)[w].turn);
   const int hk = (int)(super % kv_heads), h = hk * a.group + (int)(inner / (unsigned)a.slices);
   const int dv0 = (int)(inner % (unsigned)a.slices) * DVW;
 
   const Span sp = OUT && a.ws != nullptr ? read_span(a, w) : find_span(a, w);
-  if (!OUT && hk == 0 && inner == 0 && tid == 0) reinterpret_cast<Span*>(a.spans)[w] = sp;
+  if (!OUT && hk == 0 && inner == 0 && tid == 0) {
+    Span* const note = reinterpret_cast<Span*>(a.spans) + w;
+    note->seq = sp.seq;
+    note->part = sp.part;
+    note->parts = sp.parts;
+    note->begin = sp.begin;
+    note->len = sp.len;
+  }
   if (sp.seq < 0) return;
   const bool last = sp.part == sp.parts - 1;
   if (!OUT && last) return;                  // no segment reads it
@@ -827,10 +836,43 @@ void decay_chunk_kernel(DecayArgs a) {
 // all earlier segments in every workgroup of the outputs' kernel instead took
 // as long as the outputs from 32 segments on).
 constexpr int JOIN_AHEAD = 8;
+// One workgroup more sorts the segments for the outputs, whole ones first and the
+// ends of sequences by eighths of a segment: the last workgroups to start are
+// then the shortest.
+__device__ __forceinline__ void order_segments(const DecayArgs& a) {
+  __shared__ int place[10];
+  Span* const spans = reinterpret_cast<Span*>(a.spans);
+  const int tid = threadIdx.x;
+  auto rank = [&](int64_t i) {               // 0: whole, 8: empty, 9: not one
+    const Span& s = spans[i];
+    if (s.seq < 0) return 9;
+    const int64_t left = s.len - s.part * a.segment, len = left < a.segment ? left : a.segment;
+    return 8 - (int)((8 * len + a.segment - 1) / a.segment);
+  };
+  if (tid < 10) place[tid] = 0;
+  __syncthreads();
+  for (int64_t i = tid; i < a.segments; i += 256) atomicAdd(&place[rank(i)], 1);
+  __syncthreads();
+  if (tid == 0) {
+    int at = 0;
+    for (int r = 0; r < 10; ++r) {
+      const int n = place[r];
+      place[r] = at;
+      at += n;
+    }
+  }
+  __syncthreads();
+  for (int64_t i = tid; i < a.segments; i += 256) spans[atomicAdd(&place[rank(i)], 1)].turn = i;
+}
+
 template <int N>
 __global__ __launch_bounds__(256) void decay_join_kernel(DecayArgs a) {
   typedef Vec<float, N> V;
   const int64_t w = blockIdx.y;
+  if (w == a.segments) {
+    if (blockIdx.x == 0 && blockIdx.z == 0) order_segments(a);
+    return;
+  }
   const Span sp = read_span(a, w);
   if (sp.seq < 0 || sp.part != 0 || sp.parts < 2) return;
   const int h = blockIdx.z;
@@ -864,7 +906,7 @@ __global__ __launch_bounds__(256) void decay_join_kernel(DecayArgs a) {
 hipError_t launch_join(const DecayArgs& a, hipStream_t st) {
   const int64_t size = (int64_t)a.dk * a.dv;
   const bool wide = size % 4 == 0 && (uintptr_t)a.ws % 16 == 0 && (uintptr_t)a.state_in % 16 == 0;
-  const dim3 grid((unsigned)((size / (wide ? 4 : 1) + 255) / 256), (unsigned)a.segments,
+  const dim3 grid((unsigned)((size / (wide ? 4 : 1) + 255) / 256), (unsigned)a.segments + 1,
                   (unsigned)a.heads);
   if (wide) hipLaunchKernelGGL(decay_join_kernel<4>, grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL(decay_join_kernel<1>, grid, dim3(256), 0, st, a);
@@ -876,7 +918,7 @@ hipError_t launch_chunks(DecayArgs a, hipStream_t st) {
   a.slices = (a.dv + 32 * NW - 1) / (32 * NW);
   const int64_t shared = (int64_t)a.group * a.slices, kv_heads = a.heads / a.group;
   const int64_t grid = (a.segments * kv_heads + 7) / 8 * 8 * shared;
-  if (grid * 64 * NW > 0xffffffffll || (a.ws != nullptr && a.segments > 65535))
+  if (grid * 64 * NW > 0xffffffffll || (a.ws != nullptr && a.segments >= 65535))
     return hipErrorInvalidValue;
   if (a.ws != nullptr) {
     hipLaunchKernelGGL((decay_chunk_kernel<T, DKP, NW, C, false, VEC>), dim3((unsigned)grid),
