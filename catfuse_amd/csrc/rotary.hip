@@ -272,29 +272,46 @@ int pow2_at_least(int n) {
   return p;
 }
 
+// The widest vectors that the channels, strides and addresses allow: 16 bytes
+// (one pair unit and up to two others a lane), 8 or 4 bytes or single elements,
+// several units a lane.  Measured (us, 20000 tokens x 24 heads, bf16): heads of 52,
+// single elements in 64 lanes 129, vectors of 4 bytes in 8 lanes 29; heads of 46,
+// single elements in 64 lanes 125, in 8 lanes 35.
 template <typename T>
 hipError_t launch_rotary(const RotaryArgs& a, bool stream, hipStream_t st) {
-  constexpr int VE = 16 / sizeof(T);
+  constexpr int V16 = 16 / sizeof(T), V8 = 8 / sizeof(T);
   const int rest = a.d - 2 * a.pairs;
-  bool wide = a.pairs % VE == 0 && rest % VE == 0;
-  for (int i = 0; i < 2; ++i) {
-    const RotaryTensor& r = a.t[i];
-    if (r.heads == 0) continue;
-    wide = wide && (uintptr_t)r.x % 16 == 0 && (uintptr_t)r.y % 16 == 0;
-    for (int64_t s : {r.xo, r.xi, r.xh, r.yo, r.yi, r.yh}) wide = wide && s % VE == 0;
-  }
-  const int up = a.pairs / VE, ur = rest / VE;
-  if (wide && up <= 64 && ur <= 128) {
-    const int lg = pow2_at_least(up > (ur + 1) / 2 ? up : (ur + 1) / 2);
+  auto fits = [&](int ve) {
+    bool ok = a.pairs % ve == 0 && rest % ve == 0;
+    for (int i = 0; i < 2; ++i) {
+      const RotaryTensor& r = a.t[i];
+      if (r.heads == 0) continue;
+      const uintptr_t bytes = ve * sizeof(T);
+      ok = ok && (uintptr_t)r.x % bytes == 0 && (uintptr_t)r.y % bytes == 0;
+      for (int64_t s : {r.xo, r.xi, r.xh, r.yo, r.yi, r.yh}) ok = ok && s % ve == 0;
+    }
+    return ok;
+  };
+  // lanes of a row for pu pair units and ru others a lane
+  auto lanes = [&](int ve, int pu, int ru) {
+    const int up = (a.pairs / ve + pu - 1) / pu, ur = (rest / ve + ru - 1) / ru;
+    return pow2_at_least(up > ur ? up : ur);
+  };
+  if (fits(V16)) {
+    const int lg = lanes(V16, 1, 2);
     if (rest == 0)
-      return stream ? launch_rotary_v<T, VE, 1, 0, true>(a, lg, st)
-                    : launch_rotary_v<T, VE, 1, 0, false>(a, lg, st);
-    return stream ? launch_rotary_v<T, VE, 1, 2, true>(a, lg, st)
-                  : launch_rotary_v<T, VE, 1, 2, false>(a, lg, st);
+      return stream ? launch_rotary_v<T, V16, 1, 0, true>(a, lg, st)
+                    : launch_rotary_v<T, V16, 1, 0, false>(a, lg, st);
+    return stream ? launch_rotary_v<T, V16, 1, 2, true>(a, lg, st)
+                  : launch_rotary_v<T, V16, 1, 2, false>(a, lg, st);
   }
-  return launch_rotary_v<T, 1, 4, 8, false>(a, 64, st);
+  if (fits(V8)) return launch_rotary_v<T, V8, 2, 4, false>(a, lanes(V8, 2, 4), st);
+  if (sizeof(T) == 2 && fits(2)) return launch_rotary_v<T, 2, 2, 4, false>(a, lanes(2, 2, 4), st);
+  return launch_rotary_v<T, 1, 4, 8, false>(a, lanes(1, 4, 8), st);
 }
-static_assert(CF_ROTARY_MAX_DIM <= 512, "the element form holds 4 x 64 pairs and 8 x 64 channels");
+// (16 bytes: 64 x 4 pairs and 2 x 64 x 4 channels of fp32; 4 bytes: 2 x 64 x 2 and
+// 4 x 64 x 2; single ones: 4 x 64 and 8 x 64)
+static_assert(CF_ROTARY_MAX_DIM <= 512, "a row takes at most 64 lanes");
 
 }  // namespace
 
