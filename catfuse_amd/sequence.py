@@ -201,7 +201,7 @@ def _segment(seqs: int, tokens: int, packed: bool, heads: int, dk: int, dv: int)
     about as many workgroups as run at once.  Measured (us, bf16, heads of
     128): one sequence of 65536 tokens, 32 heads: segments of 2048 tokens 729,
     4096 719, 8192 1190; 24 packed ones of 24011 tokens, 16 heads: whole 266,
-    384 185, 768 180, 1024 175; fp32, 3 sequences of 1237, 8 heads of 80: whole
+    384 185, 512 170, 768 160, 1024 161; fp32, 3 sequences of 1237, 8 heads of 80: whole
     280, 64 43, 128 46, 192 58; one of 196, 12 heads of 32: whole 21, 64 17."""
     width = 32 if dk <= 32 else 64 if dk <= 64 else 128
     columns = heads * -(-dv // width)          # workgroups of one segment
