@@ -337,6 +337,15 @@ __device__ __forceinline__ Span read_span(const DecayArgs& a, int64_t w) {
 // 32 t + 16 (r / 8) + 8 (lane / 32) + r % 8, column lane % 32: the rows of K's
 // operand are taken in that order, so that eight registers on end are an
 // operand of the next chunk's q S as they lie.
+//
+// Four waves of 32 columns share a chunk's images of q, k and its scores; S for
+// 128 channels takes 64 registers of a wave, so that two workgroups fit a CU.
+// Chunks of 64 for bf16 (one image a tensor); two or three parts leave LDS for 32.
+// Bound by issue, not by memory: 65536 tokens x 32 heads x 128 bf16, outputs
+// 472-578 us, segments' own states 200-247 (matrix cores 42 and 45 % of the
+// cycles, vector issue 47 and 43 %, at 1.75-1.91 GHz); one pass over the data
+// at the rate of a copy would take 263.  bf16 chunks of 32, three waves a SIMD,
+// images copied straight to LDS: the whole call 769 us against 719.
 template <typename T, int DKP, int NW, int C, bool OUT, bool VEC>
 __global__ __launch_bounds__(64 * NW, DKP <= 128 ? 2 : 1)
 void decay_chunk_kernel(DecayArgs a) {
@@ -865,6 +874,12 @@ __device__ __forceinline__ void order_segments(const DecayArgs& a) {
   for (int64_t i = tid; i < a.segments; i += 256) spans[atomicAdd(&place[rank(i)], 1)].turn = i;
 }
 
+// The segments' own states become the states before them, in place:
+//   S_0 = state_in,  S_{m+1} = w^segment S_m + (own state of m)
+// A thread carries N numbers along a sequence, JOIN_AHEAD loads in flight.
+// Bound by the latency of those loads: 16 segments of 32 heads of 128 x 128 take
+// 15 us; with the sum in every workgroup of the outputs instead the call was
+// slower (65536 tokens: 871 us, this launch with reads ahead there 740).
 template <int N>
 __global__ __launch_bounds__(256) void decay_join_kernel(DecayArgs a) {
   typedef Vec<float, N> V;

@@ -37,7 +37,9 @@ constexpr int STEP_MAX_DK = CF_DECAY_MAX_DK;
 
 // Bound by HBM: every state is read and written once.  A workgroup takes a
 // slice of CL * VEC columns of one row and head: thread = VEC columns, 256 /
-// CL row groups, U rows in flight each.
+// CL row groups, U rows in flight each.  256 rows x 32 heads of 128 x 128:
+// 214 us, 5.0 TB/s read and written, a large copy's rate; loads of the states
+// before the scan of the slots, or streaming stores, were no faster.
 template <typename T, int VEC, int CL>
 __global__ __launch_bounds__(256) void decay_step_kernel(StepArgs a) {
   constexpr int RG = 256 / CL, U = 8;
