@@ -19,6 +19,10 @@ from __future__ import annotations
 from typing import Optional, Sequence
 
 import torch
+# Tensors that a kernel writes count as changed, as after an in-place operation
+# of torch: the package's copies of a fused output and autograd's saved tensors
+# go by that count.
+from torch.autograd.graph import increment_version as _changed
 
 from catfuse_amd import _hip
 from catfuse_amd._hip import check, ptr
@@ -273,6 +277,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
         _at(q), _at(k), _at(v), _at(log_decay), _at(state), _at(left), _at(out), _at(cu_seqlens),
         _at(ws), _hip.stream(dev)) + tail
     _call(_hip.lib().cf_decay_attention, "cf_decay_attention", dev, args)
+    if given:
+        _changed(out)
     if ev is not None:
         H, Hk, dk, dv = q.shape[-2], k.shape[-2], q.shape[-1], v.shape[-1]
         rows = q.numel() // (H * dk)
@@ -363,6 +369,7 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     for t, n in zip((q, k, v, log_decay, slots), spans[1:]):
         if n and t.data_ptr() < last and first < t.data_ptr() + n:
             raise ValueError("state overlaps the memory of an input")
+    written = (state,) if out is None else (state, out)
     if out is None:
         out = torch.empty(shape, dtype=q.dtype, device=dev)
     else:
@@ -374,6 +381,7 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     args = _hip.DECAY_STEP_ARGS[0].pack(_at(q), _at(k), _at(v), _at(log_decay), _at(state), _at(out),
                                         _at(slots), _hip.stream(dev)) + tail
     _call(_hip.lib().cf_decay_attention_step, "cf_decay_attention_step", dev, args)
+    _changed(written)
     if ev is not None:
         (rows, H, dk), Hk, dv = q.shape, k.shape[1], v.shape[2]
         _t1("decay_attention_step", ev, flops=4 * rows * H * dk * dv,
@@ -510,6 +518,9 @@ def _rotate(x, k, positions, freqs, sections, interleaved, inverse, norm, eps, w
                                     _at(weights[1]), _at(positions), _at(freqs),
                                     _hip.stream(dev)) + tail
     _call(_hip.lib().cf_rotary, "cf_rotary", dev, args)
+    for out in outs:
+        if out is not None:
+            _changed(out)
     if ev is not None:
         m = x.numel() + (0 if k is None else k.numel())
         _t1("qk_norm_rotary" if norm else "rotary", ev, nbytes=2 * m * x.element_size())

@@ -1,4 +1,5 @@
-"""Edges of the sequence operators: precision where terms cancel.
+"""Edges of the sequence operators: precision where terms cancel, tensors that
+other parts of the package or autograd keep track of.
 
 Tolerances as in test_gpu_sequence: an output's own rounding plus 72 * 2^-24
 (a sum's depth and the roundings of its terms) of the definition evaluated
@@ -9,7 +10,7 @@ import pytest
 import torch
 
 from catfuse_amd import kernels
-from test_gpu_sequence import BF16, F16, F32, U32, _close, _definition
+from test_gpu_sequence import BF16, F16, F32, U32, _close, _decays, _definition
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +90,76 @@ def test_attention_keeps_products_of_second_parts(cuda):
     v = torch.ones(1, 64, 1, 32)
     v[:, 1::2] = -1
     _check(cuda, q, k, v, None, F16)
+
+
+# ---------------------------------------------------------------------------
+# tensors that others keep track of
+# ---------------------------------------------------------------------------
+
+def test_written_tensors_change_versions(cuda):
+    """Outputs that are given and states in place count as changed, inputs and
+    other outputs do not; tensors of inference mode have no count."""
+    q, k, v = (torch.randn(3, n, 16, device=cuda) for n in (4, 2, 2))
+    f, pos = _decays(4).to(cuda), torch.arange(3, device=cuda)
+    freqs = kernels.rotary_freqs(8, device=cuda)
+    pool, out = torch.zeros(3, 4, 16, 16, device=cuda), torch.empty(3, 4, 16, device=cuda)
+    cu = torch.tensor([0, 3], dtype=torch.int32, device=cuda)
+
+    def changed(call, written):
+        every = [q, k, v, f, pos, freqs, pool, out, cu]
+        before = [t._version for t in every]
+        call()
+        assert [t._version > n for t, n in zip(every, before)] == \
+            [any(t is w for w in written) for t in every]
+    for _ in range(2):                                   # planned anew, and again
+        changed(lambda: kernels.decay_attention(q, k, v, f, cu_seqlens=cu), [])
+        changed(lambda: kernels.decay_attention(q, k, v, f, cu_seqlens=cu, out=out), [out])
+        changed(lambda: kernels.decay_attention(q, k, v, f, cu_seqlens=cu, out=out,
+                                                return_state=False), [out])
+        changed(lambda: kernels.decay_attention_step(q, k, v, f, pool), [pool])
+        changed(lambda: kernels.decay_attention_step(q, k, v, f, pool[:], slots=pos, out=out),
+                [pool, out])
+        changed(lambda: kernels.rotary(q, pos, freqs), [])
+        changed(lambda: kernels.rotary(q, pos, freqs, out=out), [out])
+        changed(lambda: kernels.rotary(q[:, :2], pos, freqs, out=q[:, :2]), [q])
+        changed(lambda: kernels.qk_norm_rotary(q, k, pos, freqs, out=(None, k)), [k])
+        changed(lambda: kernels.qk_norm_rotary(q, k, pos, freqs, out=(q, k)), [q, k])
+    with torch.inference_mode():
+        x = torch.randn(3, 4, 16, device=cuda)
+        want = kernels.rotary(x, pos, freqs)
+        assert torch.equal(kernels.rotary(x, pos, freqs, out=x), want)
+
+
+def test_saved_activation_turned_in_place(cuda):
+    """A head that autograd has saved, turned in place through a detached view:
+    the backward pass refuses it, as after any change in place."""
+    x = torch.randn(5, 2, 8, device=cuda)
+    w = torch.randn(8, device=cuda, requires_grad=True)
+    y = (x * w).sum()                                    # saves x for w's gradient
+    kernels.rotary(x.detach(), torch.arange(5, device=cuda), kernels.rotary_freqs(4, device=cuda),
+                   out=x.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_fused_output_turned_in_place(cuda):
+    """The output of a fused token layer, turned in place through a view of its
+    heads: the next fused layer reads the turned values, not the copy that the
+    first one left for it."""
+    from catfuse_amd.transformer import FusedLinearBNLIF
+    from test_gpu_transformer import _triple
+    first, second = (FusedLinearBNLIF.from_sj_modules(*_triple(64, 64, s)).to(cuda) for s in (3, 4))
+    x = (torch.rand(2, 2, 49, 64, generator=torch.Generator().manual_seed(5)) < 0.3).float().to(cuda)
+    pos, freqs = torch.arange(49, device=cuda).view(1, 1, 49), kernels.rotary_freqs(16, device=cuda)
+    with torch.no_grad():
+        y = first(x)
+        plain = second(y).clone()
+        heads = y.unflatten(-1, (2, 32))
+        turned = kernels.rotary(heads, pos, freqs).flatten(-2)
+        kernels.rotary(heads, pos, freqs, out=heads)
+        assert torch.equal(y, turned)
+        second.reset()
+        got = second(y).clone()
+        second.reset()
+        want = second(turned).clone()
+    assert torch.equal(got, want) and not torch.equal(got, plain)
