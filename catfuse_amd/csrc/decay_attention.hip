@@ -883,9 +883,11 @@ __global__ __launch_bounds__(256) void decay_join_kernel(DecayArgs a) {
   const int h = blockIdx.z;
   const int64_t size = (int64_t)a.dk * a.dv, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N;
   if (i >= size) return;
-  // w^segment as a sum of two floats: its rounding would add up
+  // In 64 bits: the rounding of w^segment would add up, and where w > 1 it passes
+  // the range of fp32 (exp(64 log_decay) is in it) although the state times it
+  // may not.  A state of zero stays one even if it passes that of fp64; any other
+  // one leaves fp32 then.
   const double f = exp((double)a.segment * (double)a.log_decay[h]);
-  const float fh = (float)f, fl = f < 1e300 ? (float)(f - (double)fh) : 0.0f;
   float* const p = a.ws + (w * a.heads + h) * size + i;
   const int64_t step = a.heads * size, n = sp.parts - 1;      // the last one has none of its own
   V s{};
@@ -902,7 +904,7 @@ __global__ __launch_bounds__(256) void decay_join_kernel(DecayArgs a) {
       *reinterpret_cast<V*>(p + (m0 + j) * step) = s;
 #pragma unroll
       for (int c = 0; c < N; ++c)
-        s.v[c] = __builtin_fmaf(s.v[c], fh, __builtin_fmaf(s.v[c], fl, x[j].v[c]));
+        s.v[c] = s.v[c] == 0.0f ? x[j].v[c] : (float)__builtin_fma((double)s.v[c], f, (double)x[j].v[c]);
     }
   }
   *reinterpret_cast<V*>(p + n * step) = s;

@@ -236,7 +236,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     reads key head h // (H // Hk).  fp32, fp16 or bf16, all of one type; the
     last dimension contiguous, other strides free.  dk <= 256, dv <= 1024.
     log_decay fp32 [H]: 0 keeps everything, -inf only the token itself; above 0
-    the past grows (exp(64 log_decay) has to be finite).
+    the past grows (exp(64 log_decay), scale times it too, has to be a number of
+    fp32: log_decay up to 1.38).
     scale: dk ** -0.5 if None.
     state: fp32 [sequences, H, dk, dv], S before the first token (None: zeros).
     cu_seqlens: int32 or int64 [sequences + 1], in device memory and therefore

@@ -801,6 +801,8 @@ int cf_conv_sparse_noalloc(const void* x, int64_t Cin, const void* w_packed, con
  * for every sequence and head, from S = state_in[seq][h] (nullable: zeros);
  * the last S goes to state_out (nullable).  States fp32 [seqs][heads][dk][dv].
  * Query head h reads key and value head h / (heads / kv_heads).
+ * log_decay may be above 0 as far as exp(64 log_decay), and scale times it, are
+ * numbers of fp32.
  * cu_seqlens null: `seqs` sequences of `tokens` rows, the strides *_batch
  * apart.  Else int32 (cu_wide 0) or int64 offsets [seqs + 1] in device memory:
  * sequence b is rows cu[b] .. cu[b + 1] - 1 of `tokens` rows; offsets are

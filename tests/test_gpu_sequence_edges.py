@@ -1,5 +1,5 @@
 """Edges of the sequence operators: precision where terms cancel, tensors that
-other parts of the package or autograd keep track of.
+other parts of the package or autograd keep track of, decays that grow.
 
 Tolerances as in test_gpu_sequence: an output's own rounding plus 72 * 2^-24
 (a sum's depth and the roundings of its terms) of the definition evaluated
@@ -9,10 +9,25 @@ one it stands there with its reason.
 import pytest
 import torch
 
-from catfuse_amd import kernels
-from test_gpu_sequence import BF16, F16, F32, U32, _close, _decays, _definition
+from catfuse_amd import kernels, sequence
+from test_gpu_sequence import (BF16, F16, F32, U32, _check_attention, _close, _decays, _definition,
+                               _inputs)
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def segments(monkeypatch):
+    """Makes the calls that follow split sequences into segments of so many
+    tokens (0: whole sequences), whatever the rule on sizes says."""
+    def force(tokens):
+        def split(seqs, n, packed, heads, dk, dv):
+            if tokens == 0 or tokens >= n:
+                return 0, 0
+            return tokens, n // tokens + seqs if packed else seqs * -(-n // tokens)
+        monkeypatch.setattr(sequence, "_segment", split)
+        monkeypatch.setattr(sequence, "_PLANS", {})
+    return force
 
 
 # ---------------------------------------------------------------------------
@@ -163,3 +178,48 @@ def test_fused_output_turned_in_place(cuda):
         second.reset()
         want = second(turned).clone()
     assert torch.equal(got, want) and not torch.equal(got, plain)
+
+
+# ---------------------------------------------------------------------------
+# decays that grow
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dk", [16, 40])
+@pytest.mark.parametrize("segment", [0, 64, 256, 448])
+def test_attention_growth_past_a_segment(cuda, segments, dtype, dk, segment):
+    """Decays above 0 whose powers leave the range of fp32 (and of fp64) within
+    a segment, on heads that are silent at first: the definition's zeros and
+    what grows out of the first token that is not silent (by up to exp(69): with
+    a scale that brings it into the range of fp16 there)."""
+    segments(segment)
+    N, start, scale = 700, 650, 2.0 ** -100 if dtype == F16 else None
+    q, k, v = _inputs((1, N, 3, dk), (1, N, 3, dk), 24, dtype, dk)
+    k[:, :start] = 0
+    f = torch.tensor([1.0, 0.35, 1.38])                 # exp(64 * 1.38) = 2e38
+    _check_attention(cuda, q, k, v, f, scale, None, None, dtype)
+    out, left = _check_attention(cuda, q, torch.zeros_like(k), v, f, scale, None, None,
+                                 dtype)
+    assert bool((out == 0).all()) and bool((left == 0).all())
+
+
+@pytest.mark.parametrize("segment", [0, 64, 256])
+def test_attention_growth_of_a_small_state(cuda, segments, segment):
+    """A state of 1e-20 times a power past 3.4e38 is a number of fp32 again."""
+    segments(segment)
+    N, f = 300, torch.tensor([0.35])                    # exp(0.35 * 256) = 8e38
+    q, k, v = _inputs((1, N, 1, 32), (1, N, 1, 32), 32, F32, 1)
+    state = 1e-20 * torch.randn(1, 1, 32, 32, generator=torch.Generator().manual_seed(6))
+    out, left = _check_attention(cuda, q, torch.zeros_like(k), v, f, None, state, None, F32)
+    assert bool(left.isfinite().all()) and bool((left != 0).any())
+
+
+def test_attention_growth_in_the_segments_of_a_long_batch(cuda):
+    """The same at a size that the rule splits by itself."""
+    N, H = 8192, 32
+    tokens, _ = sequence._segment(1, N, False, H, 8, 8)
+    assert tokens > 64
+    f = torch.full((H,), 90.0 / tokens, device=cuda)    # its power: past 3.4e38
+    q, k, v = (torch.randn(1, N, H, 8, device=cuda) for _ in range(3))
+    out, left = kernels.decay_attention(q, torch.zeros_like(k), v, f)
+    assert bool((out == 0).all()) and bool((left == 0).all())
