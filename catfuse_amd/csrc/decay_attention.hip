@@ -354,6 +354,8 @@ void decay_chunk_kernel(DecayArgs a) {
   float* const pow_sh = pow_all + 32;
   __shared__ float plain_sh[C];              // w^n
   __shared__ __attribute__((aligned(16))) float end_sh[C];   // w^(n - 1 - j) of a chunk of n tokens
+  __shared__ double fade_sh[3];              // w^C, its inverse, error carried on
+  __shared__ float chunk_fade_sh[2];         // w^C of the chunk at hand and the next one
 
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -402,12 +404,17 @@ void decay_chunk_kernel(DecayArgs a) {
     pow_sh[n] = (float)(p * (double)a.scale);
     if (n < C) plain_sh[n] = end_sh[C - 1 - n] = (float)p;
   }
-  // The rounding of w^C would add up over the chunks: every eighth makes up
-  // for eight of them.
-  const double wc = exp(C * ld);
-  const float wch = (float)wc;
-  const float wc8 = wc > 1e-30 && wc < 1e30 ? (float)(8.0 * (wc - (double)wch) / wc) : 0.0f;
-  int chunk = 0;
+  // The rounding of w^C would add up over the chunks (2^-25 each, all of one
+  // sign): what a chunk's power was off by goes into the next one's, so that the
+  // powers' product never is off by more than one rounding.
+  if (tid == 0) {
+    const double wc = exp(C * ld), inverse = wc > 1e-30 && wc < 1e30 ? 1.0 / wc : 0.0;
+    chunk_fade_sh[0] = (float)wc;
+    fade_sh[0] = wc;
+    fade_sh[1] = inverse;
+    fade_sh[2] = (wc - (double)(float)wc) * inverse;
+  }
+  int odd = 0;                               // which of the two is at hand
 
   f16v S[KT];
 #pragma unroll
@@ -507,12 +514,13 @@ void decay_chunk_kernel(DecayArgs a) {
     }
     const bool any_bad = OUT && __ballot(bad_from < C) != 0;
 
-    const float fade = n == C ? wch : plain_sh[n];
-    if ((++chunk & 7) == 0 && n == C) {
-#pragma unroll
-      for (int t = 0; t < KT; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) S[t][r] = __builtin_fmaf(S[t][r], wc8, S[t][r]);
+    const float fade = n == C ? chunk_fade_sh[odd] : plain_sh[n];
+    odd ^= 1;
+    if (tid == 0) {                          // the next chunk's, which no one reads before a barrier
+      const double p = __builtin_fma(fade_sh[0], fade_sh[2], fade_sh[0]);
+      const float w = (float)p;
+      chunk_fade_sh[odd] = w;
+      fade_sh[2] = (p - (double)w) * fade_sh[1];
     }
 
     // The operand w^(n-1-j) v_j of S's update, 16 tokens of it: its weights, and
@@ -928,8 +936,12 @@ hipError_t launch_chunks(DecayArgs a, hipStream_t st) {
   if (grid * 64 * NW > 0xffffffffll || (a.ws != nullptr && a.segments >= 65535))
     return hipErrorInvalidValue;
   if (a.ws != nullptr) {
+    // bf16 heads of 65-128: LDS for two workgroups a CU, though the registers would
+    // let three in: where all start at once, some CUs would get three and others one
+    // (24 packed prompts of 24011 tokens, 16 heads of 128: 55 us, with two 46).
+    constexpr size_t pad = DKP == 128 && C == 64 ? 24576 : 0;
     hipLaunchKernelGGL((decay_chunk_kernel<T, DKP, NW, C, false, VEC>), dim3((unsigned)grid),
-                       dim3(64 * NW), 0, st, a);
+                       dim3(64 * NW), pad, st, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     e = launch_join(a, st);

@@ -1,11 +1,14 @@
 """Edges of the sequence operators: precision where terms cancel, tensors that
-other parts of the package or autograd keep track of, decays that grow.
+other parts of the package or autograd keep track of, decays that grow, and
+many chunks in a row.
 
 Tolerances as in test_gpu_sequence: an output's own rounding plus 72 * 2^-24
 (a sum's depth and the roundings of its terms) of the definition evaluated
 with absolute values, for outputs of 16 bits too; where a test needs another
 one it stands there with its reason.
 """
+import math
+
 import pytest
 import torch
 
@@ -223,3 +226,39 @@ def test_attention_growth_in_the_segments_of_a_long_batch(cuda):
     q, k, v = (torch.randn(1, N, H, 8, device=cuda) for _ in range(3))
     out, left = kernels.decay_attention(q, torch.zeros_like(k), v, f)
     assert bool((out == 0).all()) and bool((left == 0).all())
+
+
+# ---------------------------------------------------------------------------
+# many chunks and segments in a row
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("segment", [0, 512])
+def test_attention_decay_does_not_drift(cuda, segments, dtype, segment):
+    """65536 tokens of nothing: the state fades by w^65536 and no rounding of
+    w^64 or w^32 adds up over the chunks.
+
+    M chunks each multiply a state by a power, rounded (u of it at most, of
+    either sign): errors with a deviation of at most u / sqrt(3) that are
+    unrelated between the 4096 elements of a head, so their mean has one of
+    sqrt(M / 3 / 4096) u; six of those, and 2 u for the powers' product and the
+    joins.  Powers that were all off the same way would be off by M times their
+    error; here by a half u and by a twentieth of it."""
+    segments(segment)
+    N, H, d = 65536, 4, 64
+    chunk = 64 if dtype == BF16 else 32
+    n = (segment or N) // chunk
+    near = -2.0 ** -14 * (1 + torch.arange(4096) / 8192)
+    power = torch.exp(chunk * near.double())
+    off = (power.float().double() - power) / power
+    at = torch.stack([off.argmin(), off.argmax(), (off - U32 / 20).abs().argmin(),
+                      (off + U32 / 20).abs().argmin()])
+    f, off = near[at], off[at]
+    tol = (6 * math.sqrt(N // chunk / 3 / d ** 2) + 2) * U32
+    assert segment or bool((n * off.abs() > 10 * tol).all())
+    q, k, v = (torch.zeros(1, N, H, d, dtype=dtype, device=cuda) for _ in range(3))
+    state = 1 + torch.rand(1, H, d, d, generator=torch.Generator().manual_seed(9))
+    out, left = kernels.decay_attention(q, k, v, f.to(cuda), state=state.to(cuda))
+    want = state[0].double() * torch.exp(N * f.double())[:, None, None]
+    rel = ((left[0].double().cpu() - want) / want).mean((-2, -1))
+    assert bool((rel.abs() <= tol).all()), (rel / U32, tol / U32)
