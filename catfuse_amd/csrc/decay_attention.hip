@@ -44,6 +44,7 @@ struct DecayArgs {
   int64_t seqs, tokens;      // tokens: rows in all (packed) or of each sequence
   int64_t segment, segments; // tokens a segment; segments in all at most
   int heads, group, dk, dv, slices;
+  unsigned first;            // of the launch's pairs of a segment and a key head
   int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, ob, ot, oh;
   int vec;                   // 16-byte accesses are aligned and whole, rows apart
   float scale;
@@ -364,7 +365,7 @@ void decay_chunk_kernel(DecayArgs a) {
   // rows: consecutive workgroups of one XCD (workgroup number mod 8).
   const unsigned shared = (unsigned)(a.group * a.slices), kv_heads = (unsigned)(a.heads / a.group);
   const unsigned slot = blockIdx.x >> 3;
-  const unsigned super = slot / shared * 8 + (blockIdx.x & 7), inner = slot % shared;
+  const unsigned super = a.first + slot / shared * 8 + (blockIdx.x & 7), inner = slot % shared;
   int64_t w = super / kv_heads;
   if (w >= a.segments) return;
   if (OUT && a.ws != nullptr) w = uniform(reinterpret_cast<const Span*>(a.spans)[w].turn);
@@ -931,25 +932,33 @@ hipError_t launch_join(const DecayArgs& a, hipStream_t st) {
 template <typename T, int DKP, int NW, int C, bool VEC>
 hipError_t launch_chunks(DecayArgs a, hipStream_t st) {
   a.slices = (a.dv + 32 * NW - 1) / (32 * NW);
-  const int64_t shared = (int64_t)a.group * a.slices, kv_heads = a.heads / a.group;
-  const int64_t grid = (a.segments * kv_heads + 7) / 8 * 8 * shared;
-  if (grid * 64 * NW > 0xffffffffll || (a.ws != nullptr && a.segments >= 65535))
-    return hipErrorInvalidValue;
+  const int64_t shared = (int64_t)a.group * a.slices;
+  const int64_t pairs = a.segments * (a.heads / a.group);      // of a segment and a key head
+  // a launch has fewer than 2^32 threads: more pairs take several
+  const int64_t most = 0xffffffffll / (64 * NW) / (8 * shared) * 8;
+  if (a.ws != nullptr && a.segments >= 65535) return hipErrorInvalidValue;   // the join's grid
+  auto launch = [&](auto kernel, size_t lds) {
+    for (int64_t first = 0; first < pairs; first += most) {
+      const int64_t n = pairs - first < most ? pairs - first : most;
+      a.first = (unsigned)first;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)((n + 7) / 8 * 8 * shared)), dim3(64 * NW), lds, st,
+                         a);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  };
   if (a.ws != nullptr) {
     // bf16 heads of 65-128: LDS for two workgroups a CU, though the registers would
     // let three in: where all start at once, some CUs would get three and others one
     // (24 packed prompts of 24011 tokens, 16 heads of 128: 55 us, with two 46).
-    constexpr size_t pad = DKP == 128 && C == 64 ? 24576 : 0;
-    hipLaunchKernelGGL((decay_chunk_kernel<T, DKP, NW, C, false, VEC>), dim3((unsigned)grid),
-                       dim3(64 * NW), pad, st, a);
-    hipError_t e = hipGetLastError();
+    hipError_t e = launch(decay_chunk_kernel<T, DKP, NW, C, false, VEC>,
+                          DKP == 128 && C == 64 ? 24576 : 0);
     if (e != hipSuccess) return e;
     e = launch_join(a, st);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((decay_chunk_kernel<T, DKP, NW, C, true, VEC>), dim3((unsigned)grid),
-                     dim3(64 * NW), 0, st, a);
-  return hipGetLastError();
+  return launch(decay_chunk_kernel<T, DKP, NW, C, true, VEC>, 0);
 }
 
 template <typename T, bool VEC>
@@ -991,6 +1000,7 @@ CF_API int cf_decay_attention(const CfDecayAttentionArgs* p) {
   a.seqs = x.seqs; a.tokens = x.tokens;
   a.heads = (int)x.heads; a.group = (int)(x.heads / x.kv_heads);
   a.dk = (int)x.dk; a.dv = (int)x.dv;
+  a.first = 0;
   a.ws = nullptr;
   a.spans = nullptr;
   a.segment = x.tokens > 0 ? x.tokens : 1;

@@ -813,8 +813,8 @@ int cf_conv_sparse_noalloc(const void* x, int64_t Cin, const void* w_packed, con
  * segments of so many tokens that run side by side, with CF_DECAY_SPAN_BYTES
  * and a state [heads][dk][dv] a segment in the workspace (16-byte aligned, as
  * hipMalloc gives it), n of both: n = tokens / segment + seqs of packed
- * sequences, seqs * ceil(tokens / segment) of equal ones; unused where segment
- * is 0 or not below tokens.  Token strides are 0 ..
+ * sequences, seqs * ceil(tokens / segment) of equal ones, at most 65534; unused
+ * where segment is 0 or not below tokens.  Token strides are 0 ..
  * CF_DECAY_MAX_TOKEN_STRIDE. */
 typedef struct CfDecayAttentionArgs {
   const void* q;

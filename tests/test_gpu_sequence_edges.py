@@ -1,6 +1,6 @@
 """Edges of the sequence operators: precision where terms cancel, tensors that
-other parts of the package or autograd keep track of, decays that grow, and
-many chunks in a row.
+other parts of the package or autograd keep track of, decays that grow, many
+chunks and workgroups in a row.
 
 Tolerances as in test_gpu_sequence: an output's own rounding plus 72 * 2^-24
 (a sum's depth and the roundings of its terms) of the definition evaluated
@@ -262,3 +262,15 @@ def test_attention_decay_does_not_drift(cuda, segments, dtype, segment):
     want = state[0].double() * torch.exp(N * f.double())[:, None, None]
     rel = ((left[0].double().cpu() - want) / want).mean((-2, -1))
     assert bool((rel.abs() <= tol).all()), (rel / U32, tol / U32)
+
+
+def test_attention_more_workgroups_than_a_launch(cuda):
+    """As many sequences as are allowed, of one token, on 1025 heads: more than
+    2^32 threads.  Small integers: every value is exact."""
+    B, H = 65535, 1025
+    g = torch.Generator(device=cuda).manual_seed(1)
+    q = torch.randint(-8, 9, (B, 1, H, 1), generator=g, device=cuda).to(BF16)
+    k, v = (torch.randint(-3, 4, (B, 1, 1, 1), generator=g, device=cuda).to(BF16) for _ in range(2))
+    out, left = kernels.decay_attention(q, k, v, torch.zeros(H, device=cuda), scale=1.0)
+    assert torch.equal(out, q * (k * v))
+    assert torch.equal(left, (k * v).float().expand(B, H, 1, 1))
