@@ -233,6 +233,54 @@ def test_attention_growth_in_the_segments_of_a_long_batch(cuda):
 # ---------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dk,dv", [(32, 32), (64, 40), (128, 128), (160, 64)])
+@pytest.mark.parametrize("segment", [0, 64, 512, 1024])
+def test_attention_chunks_in_a_row(cuda, segments, dtype, dk, dv, segment):
+    """Whole sequences of 33 (bf16) and 66 chunks, and segments of 1 to 32, over
+    states, no decay, a slow one and a fast one.
+
+    A sum of N terms without a decay: the matrix cores add 16 products to a
+    state at a time, N / 16 times one after another, each time rounded (the sum
+    of the 16 and the sum with the state: 2 u of what is there)."""
+    segments(segment)
+    N = 2100
+    q, k, v = _inputs((1, N, 3, dk), (1, N, 1, dk), dv, dtype, dk + segment)
+    f = torch.tensor([0.0, -2.0 ** -12, -2.0 ** -5])
+    state = torch.randn(1, 3, dk, dv, generator=torch.Generator().manual_seed(2))
+    out, left = kernels.decay_attention(q.to(cuda), k.to(cuda), v.to(cuda), f.to(cuda),
+                                        state=state.to(cuda))
+    a = [x[0].double() for x in (q, k, v)]
+    want, s = _definition(*a, f.double(), dk ** -0.5, state[0].double())
+    big, sbig = _definition(*(x.abs() for x in a), f.double(), dk ** -0.5, state[0].double().abs())
+    depth = (N / 8 + 72) * U32
+    _close(out[0], want, big, dtype, depth)
+    _close(left[0], s, sbig, F32, depth)
+
+
+@pytest.mark.parametrize("lens", [[1000, 0, 1, 640, 63, 1025], [700] * 4])
+@pytest.mark.parametrize("segment", [0, 128, 512])
+def test_attention_packed_in_segments(cuda, segments, lens, segment):
+    """Full segments, ends of every length and sequences without any, in one
+    launch."""
+    segments(segment)
+    N, dk = sum(lens), 64
+    q, k, v = _inputs((N, 2, dk), (N, 1, dk), dk, BF16, segment)
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32)
+    state = torch.randn(len(lens), 2, dk, dk, generator=torch.Generator().manual_seed(3))
+    f = torch.tensor([-2.0 ** -9, -2.0 ** -3])
+    out, left = kernels.decay_attention(q.to(cuda), k.to(cuda), v.to(cuda), f.to(cuda),
+                                        state=state.to(cuda), cu_seqlens=cu.to(cuda))
+    for b, (i, j) in enumerate(zip(cu.tolist(), cu.tolist()[1:])):
+        a = [x[i:j].double() for x in (q, k, v)]
+        want, s = _definition(*a, f.double(), dk ** -0.5, state[b].double())
+        big, sbig = _definition(*(x.abs() for x in a), f.double(), dk ** -0.5,
+                                state[b].double().abs())
+        depth = (1025 / 8 + 72) * U32
+        _close(out[i:j], want, big, BF16, depth)
+        _close(left[b], s, sbig, F32, depth)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("segment", [0, 512])
 def test_attention_decay_does_not_drift(cuda, segments, dtype, segment):
     """65536 tokens of nothing: the state fades by w^65536 and no rounding of
@@ -262,6 +310,35 @@ def test_attention_decay_does_not_drift(cuda, segments, dtype, segment):
     want = state[0].double() * torch.exp(N * f.double())[:, None, None]
     rel = ((left[0].double().cpu() - want) / want).mean((-2, -1))
     assert bool((rel.abs() <= tol).all()), (rel / U32, tol / U32)
+
+
+@pytest.mark.parametrize("B,H,wide", [(5000, 2, False), (3000, 4, True)])
+def test_attention_many_whole_sequences(cuda, B, H, wide):
+    """Whole packed sequences whose first rows are found over many offsets,
+    some of them decreasing, negative and past the tokens."""
+    N, d = 9000, 16
+    assert sequence._segment(B, N, True, H, d, d) == (0, 0)
+    g = torch.Generator().manual_seed(B)
+    q, k, v = _inputs((N, H, d), (N, 1, d), d, F32, B)
+    f = _decays(H)
+    cu = torch.randint(0, N + 1, (B + 1,), generator=g).sort()[0]
+    cu[B // 2], cu[B // 3], cu[70], cu[130] = -7, 5, 3, cu[125]
+    cu[-4], cu[-2], cu[-1] = N + 100, 12, N - 3
+    ends = cu.clamp(0, N).cummax(0)[0].tolist()
+    out, left = kernels.decay_attention(
+        q.to(cuda), k.to(cuda), v.to(cuda), f.to(cuda),
+        cu_seqlens=cu.to(torch.int64 if wide else torch.int32).to(cuda))
+    want, big = (torch.zeros(N, H, d, dtype=torch.float64) for _ in range(2))
+    s, sbig = (torch.zeros(B, H, d, d, dtype=torch.float64) for _ in range(2))
+    for b, (i, j) in enumerate(zip(ends, ends[1:])):
+        if j > i:
+            a = [x[i:j].double() for x in (q, k, v)]
+            want[i:j], s[b] = _definition(*a, f.double(), d ** -0.5, None)
+            big[i:j], sbig[b] = _definition(*(x.abs() for x in a), f.double(), d ** -0.5, None)
+    _close(out, want, big, F32, 72 * U32)
+    _close(left, s, sbig, F32, 72 * U32)
+    assert bool((out[:ends[0]] == 0).all())
+
 
 
 def test_attention_more_workgroups_than_a_launch(cuda):
