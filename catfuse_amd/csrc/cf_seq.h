@@ -27,9 +27,9 @@ __device__ __forceinline__ T from_f(float x) { return (T)x; }   // to nearest ev
 template <typename T, int N>
 struct alignas(sizeof(T) * N) Vec { T v[N]; };
 
-// The row range [begin, end) of sequence b: packed sequences have their
-// offsets in device memory, where nothing has checked them, so each is
-// clamped to the tensors' rows (offsets that decrease give an empty range).
+// Offset i of packed sequences, int32 or int64 (wide) in device memory, where
+// nothing has checked it: clamped to the tensors' rows 0 .. tokens.  (That one
+// below its predecessor counts as that is left to the caller.)
 __device__ __forceinline__ int64_t seq_offset(const void* cu, int wide, int64_t i, int64_t tokens) {
   const int64_t o = wide ? reinterpret_cast<const int64_t*>(cu)[i]
                          : (int64_t)reinterpret_cast<const int32_t*>(cu)[i];

@@ -17,11 +17,13 @@
 // exact).  Products of parts below 2^-24 of the whole are left out.  For 16-bit
 // outputs too: two parts of the state and the scores hide behind the output's
 // rounding only where their terms do not cancel (channels that share a mean: 2^-16
-// of it in the output), and took 718 us instead of 791 at 65536 tokens
+// of it in the output); they took 718 us where three take 777 at 65536 tokens
 // x 32 heads x 128 bf16.
 //
 // A value that is not finite must not reach the tokens before it, where the
-// product has a zero for it (0 * inf is NaN): see below at `bad_from`.
+// product has a zero for it (0 * inf is NaN): see below at `bad_from`.  What it
+// does reach is NaN as a rule, also where the formula gives an infinity: an
+// infinity's second part is inf - inf.
 //
 // No counterpart in the reference; the causal, ordered relative of the
 // spiking attention core in attention.hip.
@@ -333,10 +335,11 @@ __device__ __forceinline__ Span read_span(const DecayArgs& a, int64_t w) {
 // 128 channels takes 64 registers of a wave, so that two workgroups fit a CU.
 // Chunks of 64 for bf16 (one image a tensor); two or three parts leave LDS for 32.
 // Bound by issue, not by memory: 65536 tokens x 32 heads x 128 bf16, outputs
-// 472-578 us, segments' own states 200-247 (matrix cores 42 and 45 % of the
-// cycles, vector issue 47 and 43 %, at 1.75-1.91 GHz); one pass over the data
+// 544-647 us, segments' own states 202-234 (matrix cores 45 % of the cycles in
+// both, vector issue 50 and 43 %, at 1.72-1.94 GHz); one pass over the data
 // at the rate of a copy would take 263.  bf16 chunks of 32, three waves a SIMD,
-// images copied straight to LDS: the whole call 769 us against 719.
+// images copied straight to LDS: the whole call 769 us against 719 (both with
+// two parts of the state).
 template <typename T, int DKP, int NW, int C, bool OUT, bool VEC>
 __global__ __launch_bounds__(64 * NW, DKP <= 128 ? 2 : 1)
 void decay_chunk_kernel(DecayArgs a) {
@@ -838,13 +841,7 @@ void decay_chunk_kernel(DecayArgs a) {
   }
 }
 
-// The states before the segments of a sequence from the segments' own: an
-// element of the state a thread, over the segments in their order, in place.
-// Reads and writes the workspace once, JOIN_AHEAD segments in flight (a sum over
-// all earlier segments in every workgroup of the outputs' kernel instead took
-// as long as the outputs from 32 segments on).
-constexpr int JOIN_AHEAD = 8;
-// One workgroup more sorts the segments for the outputs, whole ones first and the
+// Sorts the segments for the outputs (one workgroup), whole ones first and the
 // ends of sequences by eighths of a segment: the last workgroups to start are
 // then the shortest.
 __device__ __forceinline__ void order_segments(const DecayArgs& a) {
@@ -875,10 +872,12 @@ __device__ __forceinline__ void order_segments(const DecayArgs& a) {
 
 // The segments' own states become the states before them, in place:
 //   S_0 = state_in,  S_{m+1} = w^segment S_m + (own state of m)
-// A thread carries N numbers along a sequence, JOIN_AHEAD loads in flight.
+// A thread carries N numbers along a sequence, JOIN_AHEAD loads in flight; one
+// workgroup more orders the segments.
 // Bound by the latency of those loads: 16 segments of 32 heads of 128 x 128 take
-// 15 us; with the sum in every workgroup of the outputs instead the call was
+// 15-17 us; with the sum in every workgroup of the outputs instead the call was
 // slower (65536 tokens: 871 us, this launch with reads ahead there 740).
+constexpr int JOIN_AHEAD = 8;
 template <int N>
 __global__ __launch_bounds__(256) void decay_join_kernel(DecayArgs a) {
   typedef Vec<float, N> V;

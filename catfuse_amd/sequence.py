@@ -203,10 +203,12 @@ def _segment(seqs: int, tokens: int, packed: bool, heads: int, dk: int, dv: int)
     own states cost a further pass over k and v (about half of the outputs'
     time), so sequences are split where they leave most of the card idle, into
     about as many workgroups as run at once.  Measured (us, bf16, heads of
-    128): one sequence of 65536 tokens, 32 heads: segments of 2048 tokens 729,
-    4096 719, 8192 1190; 24 packed ones of 24011 tokens, 16 heads: whole 266,
-    384 185, 512 170, 768 160, 1024 161; fp32, 3 sequences of 1237, 8 heads of 80: whole
-    280, 64 43, 128 46, 192 58; one of 196, 12 heads of 32: whole 21, 64 17."""
+    128): one sequence of 65536 tokens, 32 heads: segments of 2048 tokens 777,
+    4096 766, 8192 852; 24 packed ones of 24011 tokens, 16 heads: whole 205,
+    384 187, 512 179, 768 173, 1024 177; fp32, 3 sequences of 1237, 8 heads of 80: whole
+    212, 64 42, 128 45, 192 58; one of 196, 12 heads of 32: whole 22, 64 18.
+    (Where splitting ends, 4 at_once workgroups of packed sequences and an eighth
+    of that of equal rows, is not measured.)"""
     width = 32 if dk <= 32 else 64 if dk <= 64 else 128
     columns = heads * -(-dv // width)          # workgroups of one segment
     at_once = 2048 if dk <= 32 else 1024 if dk <= 64 else 512 if dk <= 128 else 256
@@ -234,7 +236,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     tokens; or, with cu_seqlens, [tokens, H, dk] and so on: packed sequences,
     number b the rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1.  Query head h
     reads key head h // (H // Hk).  fp32, fp16 or bf16, all of one type; the
-    last dimension contiguous, other strides free.  dk <= 256, dv <= 1024.
+    last dimension contiguous, other strides free (tokens of a sequence at most
+    8,000,000 elements apart).  dk <= 256, dv <= 1024.
     log_decay fp32 [H]: 0 keeps everything, -inf only the token itself; above 0
     the past grows (exp(64 log_decay), scale times it too, has to be a number of
     fp32: log_decay up to 1.38).
@@ -247,8 +250,13 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     out: a tensor for the output, apart from the inputs.
 
     Returns (out [.., H, dv], state after the last token), or out alone
-    without return_state.  Sums and states are fp32; a token that holds an
-    infinity or NaN does not reach the tokens before it."""
+    without return_state.  Sums and states are fp32, products exact to 2^-24 of
+    their factors for every type; a token that holds an infinity or NaN does not
+    reach the tokens before it, and what an infinity (or an overflow) does reach
+    may be NaN where the formula gives an infinity.
+    Long sequences of a small batch are computed in segments side by side, with
+    a workspace of a state [H, dk, dv] for each, from torch's allocator (32 heads
+    of 128: 36 MB for one prompt of 65536 tokens, 168 MB for 64 packed ones)."""
     scale = None if scale is None else float(scale)
     try:
         key = (decay_attention, _looks(q), _looks(k), _looks(v), _looks(log_decay), _looks(state),

@@ -802,7 +802,8 @@ int cf_conv_sparse_noalloc(const void* x, int64_t Cin, const void* w_packed, con
  * the last S goes to state_out (nullable).  States fp32 [seqs][heads][dk][dv].
  * Query head h reads key and value head h / (heads / kv_heads).
  * log_decay may be above 0 as far as exp(64 log_decay), and scale times it, are
- * numbers of fp32.
+ * numbers of fp32.  A token that is not finite does not reach the tokens before
+ * it; what an infinity does reach may be NaN where the formula gives an infinity.
  * cu_seqlens null: `seqs` sequences of `tokens` rows, the strides *_batch
  * apart.  Else int32 (cu_wide 0) or int64 offsets [seqs + 1] in device memory:
  * sequence b is rows cu[b] .. cu[b + 1] - 1 of `tokens` rows; offsets are
