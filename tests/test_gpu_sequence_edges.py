@@ -163,17 +163,21 @@ def test_saved_activation_turned_in_place(cuda):
 def test_fused_output_turned_in_place(cuda):
     """The output of a fused token layer, turned in place through a view of its
     heads: the next fused layer reads the turned values, not the copy that the
-    first one left for it."""
+    first one left for it.  A quarter turn: spikes stay numbers that the fused
+    layers take exactly."""
+    import catfuse_amd
     from catfuse_amd.transformer import FusedLinearBNLIF
     from test_gpu_transformer import _triple
     first, second = (FusedLinearBNLIF.from_sj_modules(*_triple(64, 64, s)).to(cuda) for s in (3, 4))
     x = (torch.rand(2, 2, 49, 64, generator=torch.Generator().manual_seed(5)) < 0.3).float().to(cuda)
-    pos, freqs = torch.arange(49, device=cuda).view(1, 1, 49), kernels.rotary_freqs(16, device=cuda)
+    pos = torch.ones(1, 1, 49, dtype=torch.int64, device=cuda)
+    freqs = torch.full((16,), math.pi / 2, dtype=torch.float64, device=cuda)
     with torch.no_grad():
         y = first(x)
         plain = second(y).clone()
         heads = y.unflatten(-1, (2, 32))
         turned = kernels.rotary(heads, pos, freqs).flatten(-2)
+        assert torch.equal(turned.abs().unflatten(-1, (2, 32)), heads.roll(16, -1))
         kernels.rotary(heads, pos, freqs, out=heads)
         assert torch.equal(y, turned)
         second.reset()
@@ -181,6 +185,7 @@ def test_fused_output_turned_in_place(cuda):
         second.reset()
         want = second(turned).clone()
     assert torch.equal(got, want) and not torch.equal(got, plain)
+    catfuse_amd.check_status()
 
 
 # ---------------------------------------------------------------------------
