@@ -1,5 +1,5 @@
 // Device helpers shared by the sequence operators (decay_attention.hip,
-// decay_step.hip, rotary.hip): element types and their conversions.  These
+// decay_step.hip, delta_attention.hip, delta_step.hip, rotary.hip): element types and their conversions.  These
 // files take their argument blocks and limits from the C-ABI header itself
 // (cf_common.h restates its constants as enumerators, so they do not include
 // it).
@@ -34,6 +34,20 @@ __device__ __forceinline__ int64_t seq_offset(const void* cu, int wide, int64_t 
   const int64_t o = wide ? reinterpret_cast<const int64_t*>(cu)[i]
                          : (int64_t)reinterpret_cast<const int32_t*>(cu)[i];
   return o < 0 ? 0 : (o > tokens ? tokens : o);
+}
+
+// Number i of a tensor that is fp32 (f32) or of the operator's type.
+template <typename T>
+__device__ __forceinline__ double load_double(const void* p, int64_t i, int f32) {
+  return f32 ? (double)reinterpret_cast<const float*>(p)[i]
+             : (double)to_f(reinterpret_cast<const T*>(p)[i]);
+}
+
+// Head h of the delta rule's states reads head h / (heads / n) of the n of each
+// input.
+static inline bool delta_heads_fit(int64_t heads, int64_t q, int64_t k, int64_t v) {
+  return heads >= 1 && heads <= CF_SEQ_MAX_HEADS && q >= 1 && k >= 1 && v >= 1 && heads % q == 0 &&
+         heads % k == 0 && heads % v == 0;
 }
 
 }  // namespace

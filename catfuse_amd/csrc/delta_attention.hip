@@ -1,0 +1,946 @@
+// Softmax-free causal attention whose state fades and corrects itself, over
+// whole sequences:
+//   S_t = w_t S_{t-1} + k_t u_t^T,  u_t = beta_t (v_t - w_t S_{t-1}^T k_t),
+//   o_t = scale q_t S_t,            w_t = exp(log_decay_t)
+// per sequence and head, S a dk x dv matrix in fp32; beta and log_decay are each
+// token's and head's own.
+//
+// By chunks of C tokens (t, s the places in a chunk, S the state before it, g_t
+// the sum of the chunk's log decays up to t):
+//   u_t + sum_{s < t} L_ts u_s = r_t,   L_ts = beta_t e^(g_t - g_s) (k_t . k_s)
+//   r_t = beta_t (v_t - e^(g_t) S^T k_t)
+//   o_t = scale (e^(g_t) q_t S + sum_{s <= t} e^(g_t - g_s) (q_t . k_s) u_s)
+//   S  <- e^(g_end) S + sum_s e^(g_end - g_s) k_s u_s^T
+// T = (I + L)^-1 does not depend on the state: delta_solve_kernel makes it for
+// all chunks side by side.  What is left for the walk over the chunks are
+// products for the matrix cores.  Every power has an exponent of at most zero
+// where the log decays have.
+//
+// Long sequences of few heads are walked in segments side by side.  A segment
+// takes the state before it to  M S + N,  N what it makes of zeros and M what it
+// makes of the unit matrix without values: the same walk on dv and on dk
+// columns; delta_join_kernel goes from segment to segment.
+//
+// Precision as in decay_attention.hip: numbers that are not bf16 ones enter a
+// product as parts of eight bits, products of parts below 2^-24 of the whole
+// left out; T by fp32 forward substitution and products of its blocks.
+//
+// No counterpart in the reference.
+#include "cf_chunk.h"
+
+namespace {
+
+struct DeltaArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* beta;
+  const void* log_decay;
+  const float* state_in;
+  float* state_out;
+  void* out;
+  const void* cu;
+  // workspace: rows that the sequences begin at [seqs + 1] (packed ones); of each
+  // chunk and head T, the running sums of its log decays and its betas; of each
+  // segment and head N, later the state before it, and M
+  int64_t* begins;
+  float* solved;
+  double* falls;
+  float* betas;
+  float* own;
+  float* moves;
+  int cu_wide, zero_rest, beta_f32, decay_f32;
+  int64_t seqs, tokens;      // tokens: rows in all (packed) or of each sequence
+  int64_t chunks;            // numbers of chunks, some of none
+  int64_t segment, segments; // tokens a segment (0: whole sequences); their numbers, some of none
+  int heads, q_group, k_group, v_group, dk, dv, slices, value_slices;
+  int64_t first;             // of the launch's pairs of a segment and a key head, or a chunk and a head
+  int64_t qb, qt, qh, kb, kt, kh, vb, vt, vh, bb, bt, bh, lb, lt, lh, ob, ot, oh;
+  int vec;                   // 16-byte accesses are aligned and whole, rows apart
+  float scale;
+};
+
+// Chunks or segments of `unit` tokens, numbered through: the first one of a
+// sequence has the number  seq + begin / unit  (equal rows: seq times those of
+// a sequence), which is beyond all of the sequence before it, since
+// ceil(len / unit) <= floor(len / unit) + 1, so that no sums over the
+// sequences' lengths are needed.  An empty sequence has one.
+__host__ __device__ inline int64_t units_of(int64_t tokens, int64_t unit) {
+  return tokens > 0 ? (tokens + unit - 1) / unit : 1;
+}
+
+struct Place { int64_t seq, part, parts, begin, len; };   // seq < 0: none has the number
+
+__device__ __forceinline__ Place find_place(const DeltaArgs& a, int64_t w, int64_t unit) {
+  Place s;
+  if (a.cu == nullptr) {
+    s.parts = uniform(units_of(a.tokens, unit));
+    s.seq = uniform(w / s.parts);
+    s.part = uniform(w % s.parts);
+    s.begin = 0;
+    s.len = a.tokens;
+    if (s.seq >= a.seqs) s.seq = -1;
+    return s;
+  }
+  // the last sequence whose first number is at most w: 64 probes a time
+  const int lane = threadIdx.x & 63;
+  int64_t lo = 0, n = a.seqs;
+  s.seq = -1;
+  s.part = s.parts = s.begin = s.len = 0;
+  for (;;) {
+    const int64_t step = (n + 63) / 64, i = lo + lane * step;
+    const bool in = lane * step < n && i + a.begins[lane * step < n ? i : lo] / unit <= w;
+    const uint64_t hit = __ballot(in);
+    if (hit == 0) return s;                  // before the first sequence's
+    const int l = 63 - __clzll((long long)hit);
+    lo = uniform(lo + l * step);
+    n = uniform(n - l * step < step ? n - l * step : step);
+    if (step == 1) break;
+  }
+  const int64_t begin = uniform(a.begins[lo]), len = uniform(a.begins[lo + 1]) - begin;
+  const int64_t part = uniform(w - (lo + begin / unit)), parts = uniform(units_of(len, unit));
+  if (part >= parts) return s;
+  s.seq = lo;
+  s.part = part;
+  s.parts = parts;
+  s.begin = begin;
+  s.len = len;
+  return s;
+}
+
+// The rows that packed sequences begin at: the offsets clamped to the tensors'
+// rows, each at least its predecessor.  One workgroup.
+__global__ __launch_bounds__(1024) void delta_begins_kernel(DeltaArgs a) {
+  __shared__ int64_t top_sh[2][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int64_t before = 0;
+  int odd = 0;
+  for (int64_t i0 = 0; i0 <= a.seqs; i0 += 1024, odd ^= 1) {
+    const int64_t i = i0 + tid;
+    int64_t m = i <= a.seqs ? seq_offset(a.cu, a.cu_wide, i, a.tokens) : 0;
+    for (int d = 1; d < 64; d *= 2) {
+      const int64_t o = __shfl_up(m, d, 64);
+      if (lane >= d && o > m) m = o;
+    }
+    if (lane == 63) top_sh[odd][wave] = m;
+    __syncthreads();
+    if (before > m) m = before;
+    for (int w = 0; w < 16; ++w) {
+      const int64_t o = top_sh[odd][w];
+      if (w < wave && o > m) m = o;
+      if (o > before) before = o;
+    }
+    if (i <= a.seqs) a.begins[i] = m;
+  }
+}
+
+// T of one chunk and head.  In the workspace T lies as the walk's operands: for
+// each tile of 32 x 32 that is not above the diagonal ((0,0) (1,0) (1,1)) and
+// each half of its columns the eight numbers of each lane: row lane % 32,
+// columns 4 (lane / 32) + 0 .. 3 and the same plus 8 of the half's sixteen.
+//
+// The products k_t . k_s on the matrix cores; blocks of 16 inverted column by
+// column in registers, then joined in pairs:
+//   (A 0; B D)^-1 = (A^-1 0; -D^-1 B A^-1 D^-1).
+template <int C> constexpr int solved_size() { return (C / 32) * (C / 32 + 1) / 2 * 1024; }
+
+template <typename T, int DKP, int C, int NT, bool VEC>
+__global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
+  constexpr int NL = parts_of<T>(), NP = 3, KS = DKP / 16, CT = C / 32, TILES = CT * (CT + 1) / 2;
+  constexpr int P = C + 1;
+  __shared__ __attribute__((aligned(512))) char lds[NL * C * DKP * 2];
+  __shared__ float low[C * P], inv[C * P];
+  __shared__ double fall[C];
+  __shared__ float beta[C];
+  const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  const int64_t pair = a.first + blockIdx.x;
+  const int64_t w = pair / a.heads;
+  const int h = (int)(pair % a.heads);
+  const Place pl = find_place(a, w, C);
+  if (pl.seq < 0 || pl.len == 0) return;
+  const int64_t row0 = a.cu != nullptr ? 0 : pl.seq, begin = pl.begin + pl.part * C;
+  const int n = (int)(pl.len - pl.part * C < C ? pl.len - pl.part * C : C);
+
+  constexpr int UK = C * (DKP / 8) / NT;
+  static_assert(UK * NT == C * (DKP / 8), "whole units");
+  Unit<T> ku[UK];
+  load_units<T, UK, DKP, NT, VEC>(ku, (const T*)a.k + row0 * a.kb + begin * a.kt + (h / a.k_group) * a.kh,
+                                  n, a.kt, a.dk);
+  if (tid < C) {
+    double g = 0.0;
+    float b = 0.0f;
+    if (tid < n) {
+      if (a.log_decay != nullptr)
+        g = load_double<T>(a.log_decay, row0 * a.lb + (begin + tid) * a.lt + h * a.lh, a.decay_f32);
+      b = (float)load_double<T>(a.beta, row0 * a.bb + (begin + tid) * a.bt + h * a.bh, a.beta_f32);
+    }
+    // in powers of two; -inf (only the token itself is kept) as one whose sums
+    // and differences are numbers and whose power is zero
+    g = g < -1e4 ? -1e4 : g;
+    g *= 1.44269504088896340736;
+    for (int d = 1; d < C; d *= 2) {
+      const double o = __shfl_up(g, d, 64);
+      if (tid >= d) g += o;
+    }
+    fall[tid] = g;
+    beta[tid] = b;
+    a.falls[pair * C + tid] = g;
+    a.betas[pair * C + tid] = b;
+  }
+#pragma unroll
+  for (int i = 0; i < UK; ++i) {
+    const int u = tid + NT * i;
+    store_unit<T, C, DKP>(lds, ku[i], u / (DKP / 8), u % (DKP / 8));
+  }
+  __syncthreads();
+
+  const uint32_t at_row = row_base<DKP>(lane);
+  for (int tile = wave; tile < TILES; tile += NT / 64) {
+    const int tt = tile == 0 ? 0 : 1, ts = tile == 2 ? 1 : 0;
+    f16v acc = {};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      u32x4 x[NL], y[NL];
+#pragma unroll
+      for (int p = 0; p < NL; ++p) {
+        x[p] = row_operand<C, DKP>(lds, at_row, p, tt, s);
+        y[p] = row_operand<C, DKP>(lds, at_row, p, ts, s);
+      }
+#pragma unroll
+      for (int i = 0; i < NL; ++i)
+#pragma unroll
+        for (int j = 0; j < NL; ++j)
+          if (i + j < (NL == 1 ? 1 : NP)) acc = mfma(x[i], y[j], acc);
+    }
+    const int s = 32 * ts + col;
+    const double gs = fall[s];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int t = 32 * tt + 8 * (r >> 2) + 4 * hi + (r & 3);
+      const float f = beta[t] * __builtin_amdgcn_exp2f((float)(fall[t] - gs));
+      low[t * P + s] = t > s ? f * acc[r] : 0.0f;
+    }
+  }
+  __syncthreads();
+
+  // blocks of 16: thread = block and column
+  if (tid < C) {
+    const int b0 = tid & ~15, c = tid & 15;
+    float x[16];
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+      float y = 0.0f;
+#pragma unroll
+      for (int s = 0; s < t; ++s) y = __builtin_fmaf(-low[(b0 + t) * P + b0 + s], x[s], y);
+      x[t] = t < c ? 0.0f : t == c ? 1.0f : y;
+      inv[(b0 + t) * P + b0 + c] = x[t];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int size = 16; size < C; size *= 2) {
+    // B A^-1 where the pair's upper right block would be, then its product
+    const int per = size * size, all = C / (2 * size) * per;
+    for (int i = tid; i < all; i += NT) {
+      const int b0 = i / per * 2 * size, r = i % per / size, c = i % size;
+      float y = 0.0f;
+      for (int m = 0; m < size; ++m) {
+        const float x = low[(b0 + size + r) * P + b0 + m] * inv[(b0 + m) * P + b0 + c];
+        y += m >= c ? x : 0.0f;
+      }
+      inv[(b0 + r) * P + b0 + size + c] = y;
+    }
+    __syncthreads();
+    for (int i = tid; i < all; i += NT) {
+      const int b0 = i / per * 2 * size, r = i % per / size, c = i % size;
+      float y = 0.0f;
+      for (int m = 0; m < size; ++m) {
+        const float x = inv[(b0 + size + r) * P + b0 + size + m] * inv[(b0 + m) * P + b0 + size + c];
+        y += m <= r ? x : 0.0f;
+      }
+      inv[(b0 + size + r) * P + b0 + c] = -y;
+    }
+    __syncthreads();
+  }
+
+  float* const to = a.solved + pair * solved_size<C>();
+  for (int u = tid; u < TILES * 128; u += NT) {
+    const int tile = u >> 7, half = (u >> 6) & 1, l = u & 63;
+    const int t = 32 * (tile == 0 ? 0 : 1) + (l & 31);
+    const int s0 = 32 * (tile == 2 ? 1 : 0) + 16 * half + 4 * (l >> 5);
+    Vec<float, 4> y[2];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int s = s0 + 8 * (j >> 2) + (j & 3);
+      const float x = inv[t * P + s];
+      y[j >> 2].v[j & 3] = s <= t ? x : 0.0f;
+    }
+    *reinterpret_cast<Vec<float, 4>*>(to + u * 8) = y[0];
+    *reinterpret_cast<Vec<float, 4>*>(to + u * 8 + 4) = y[1];
+  }
+}
+
+// The walk.  A workgroup takes a segment of a sequence, one head, 32 NW columns
+// of the values; wave w the columns 32 w .. + 31 with their part of S (all DKP
+// rows, in accumulators) throughout: a column of u, r and S depends on no other
+// column, so the waves share only the chunk's images.  OUT: outputs, from the
+// state before the segment; else the segment's N (slices of the values) and M
+// (further slices: columns of the unit matrix, no values).
+//
+// S as accumulators: tile t, register r of a lane is row (channel of k)
+// 32 t + 16 (r / 8) + 8 (lane / 32) + r % 8, column lane % 32 (the rows of K's
+// operand are taken in that order): eight registers on end are an operand of the
+// next products as they lie.  So are eight registers of r and u, tokens
+// 16 s + 4 (lane / 32) + 0 .. 3 and the same plus 8, the order in which T, the
+// scores and K's turned operand have them.
+template <typename T, int DKP, int NW, int C, bool OUT, bool VEC>
+__global__ __launch_bounds__(64 * NW, DKP <= 128 ? 2 : 1)
+void delta_walk_kernel(DeltaArgs a) {
+  constexpr int NL = parts_of<T>(), NP = 3, NT = 64 * NW;
+  constexpr int KT = DKP / 32, KS = DKP / 16, CT = C / 32, CS = C / 16, DVW = 32 * NW;
+  constexpr int QK_BYTES = NL * C * DKP * 2, V_BYTES = NL * C * DVW * 2;
+  constexpr int TILES = CT * (CT + 1) / 2, T_BYTES = TILES * 2 * NP * 1024;
+  static_assert(CT == 1 || NW >= TILES, "a score tile a wave");
+  constexpr int Q_AT = QK_BYTES, V_AT = Q_AT + (OUT ? QK_BYTES : 0), IMAGE = V_AT + V_BYTES;
+  __shared__ __attribute__((aligned(512))) char lds[IMAGE];     // of K, Q and V
+  __shared__ __attribute__((aligned(16))) char tsh[T_BYTES];    // T, later the scores
+  __shared__ double fall_sh[C];
+  // beta; beta e^g; scale e^g; e^(g_end - g)
+  __shared__ __attribute__((aligned(16))) float beta_sh[C], since_sh[C], query_sh[C], end_sh[C];
+  __shared__ float fade_sh[2];               // e^(g_end) as a sum of two
+
+  const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  // Heads of one key head and the slices of their columns read the same rows:
+  // consecutive workgroups of one XCD (workgroup number mod 8).
+  const unsigned shared = (unsigned)(a.k_group * a.slices), k_heads = (unsigned)(a.heads / a.k_group);
+  const unsigned slot = blockIdx.x >> 3;
+  const int64_t super = a.first + slot / shared * 8 + (blockIdx.x & 7);
+  const unsigned inner = slot % shared;
+  const int64_t w = uniform(super / k_heads);
+  if (w >= a.segments) return;
+  const int hk = (int)uniform(super % k_heads), h = hk * a.k_group + (int)(inner / (unsigned)a.slices);
+  const int slice = (int)(inner % (unsigned)a.slices);
+  const bool move = !OUT && slice >= a.value_slices;            // columns of M
+  const int c0 = (move ? slice - a.value_slices : slice) * DVW, cols = move ? a.dk : a.dv;
+
+  const Place pl = find_place(a, w, a.segment > 0 ? a.segment : INT64_MAX / 2);
+  if (pl.seq < 0) return;
+  const bool last = pl.part == pl.parts - 1;
+  if (!OUT && last) return;                  // no segment reads it
+  const int dvs = cols - c0 < DVW ? cols - c0 : DVW;            // columns of this slice
+  const T *kp, *vp, *qp;
+  T* op;
+  int left;                                  // tokens from here to the segment's end
+  int64_t pair;                              // of the chunk and the head
+  {
+    const int64_t tok0 = pl.part * a.segment, row0 = a.cu != nullptr ? 0 : pl.seq;
+    const int64_t begin = pl.begin + tok0, rest = pl.len - tok0;
+    left = (int)(a.segment > 0 && rest > a.segment ? a.segment : rest);
+    qp = (const T*)a.q + row0 * a.qb + begin * a.qt + (h / a.q_group) * a.qh;
+    kp = (const T*)a.k + row0 * a.kb + begin * a.kt + hk * a.kh;
+    vp = (const T*)a.v + row0 * a.vb + begin * a.vt + (h / a.v_group) * a.vh + (move ? 0 : c0);
+    op = (T*)a.out + row0 * a.ob + begin * a.ot + h * a.oh + c0;
+    const int64_t chunk = tok0 / C + (a.cu != nullptr ? pl.seq + pl.begin / C
+                                                      : pl.seq * units_of(a.tokens, C));
+    pair = uniform(chunk * a.heads + h);
+  }
+
+  f16v S[KT];
+#pragma unroll
+  for (int t = 0; t < KT; ++t) S[t] = f16v{};
+  const int sc = 32 * wave + col;            // this lane's column of the slice
+  // this lane's place in a state: of its first row; the others are dv apart,
+  // rows from dk on and columns from dvs on out of the buffer's range
+  const uint32_t s_at = sc < dvs ? 4u * (uint32_t)(8 * hi * a.dv + c0 + sc) : OOB;
+  auto s_off = [&](int t, int r) {
+    return s_at + 4u * (uint32_t)((32 * t + 16 * (r >> 3) + (r & 7)) * a.dv);
+  };
+  auto state_of = [&](const float* base, int64_t i) {
+    return rows_rsrc(base + (i * a.heads + h) * (int64_t)a.dk * a.dv, 4u * a.dk * a.dv);
+  };
+  if (OUT) {
+    const float* const from = pl.part > 0 ? a.own : a.state_in;
+    if (from != nullptr) {
+      const __amdgpu_buffer_rsrc_t rs = state_of(from, pl.part > 0 ? w : pl.seq);
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          S[t][r] = __builtin_bit_cast(
+              float, __builtin_amdgcn_raw_buffer_load_b32(rs, s_off(t, r), 0, 0));
+    }
+  } else if (move) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        S[t][r] = 32 * t + 16 * (r >> 3) + 8 * hi + (r & 7) == c0 + sc ? 1.0f : 0.0f;
+  }
+
+  constexpr int UK = C * (DKP / 8) / NT, UV = C * (DVW / 8) / NT;   // units of a thread
+  static_assert(UK * NT == C * (DKP / 8) && UV * NT == C * (DVW / 8), "whole units");
+  // Of T: threads past the last unit take their first one again.  (Here and at
+  // the powers below no lane is masked off: a register that the compiler spills
+  // inside such a branch is saved for the lanes in it alone.)
+  constexpr int UT = (TILES * 128 + NT - 1) / NT;
+  auto unit = [&](int i) { return tid + NT * i < TILES * 128 ? tid + NT * i : tid; };
+  Unit<T> ku[UK], vu[UV], qu[OUT ? UK : 1];
+  Vec<float, 4> tu[UT][2];
+  double fall = 0.0;
+  float beta = 0.0f;
+  auto load_chunk = [&]() {
+    const int n = left < C ? left : C;
+    load_units<T, UK, DKP, NT, VEC>(ku, kp, n, a.kt, a.dk);
+    if (OUT || !move) load_units<T, UV, DVW, NT, VEC>(vu, vp, n, a.vt, dvs);
+    if constexpr (OUT) load_units<T, UK, DKP, NT, VEC>(qu, qp, n, a.qt, a.dk);
+    const float* const from = a.solved + pair * solved_size<C>();
+#pragma unroll
+    for (int i = 0; i < UT; ++i) {
+      tu[i][0] = *reinterpret_cast<const Vec<float, 4>*>(from + unit(i) * 8);
+      tu[i][1] = *reinterpret_cast<const Vec<float, 4>*>(from + unit(i) * 8 + 4);
+    }
+    fall = a.falls[pair * C + tid % C];
+    beta = a.betas[pair * C + tid % C];
+  };
+  if (!OUT && move)
+#pragma unroll
+    for (int i = 0; i < UV; ++i) vu[i] = Unit<T>{};
+
+  const uint32_t at_row = row_base<DKP>(lane), at_key = token_base<DKP>(lane, true);
+  const uint32_t at_value = token_base<DVW>(lane, false) ^ (uint32_t)(wave << 6);
+
+  if (left > 0) load_chunk();
+  while (left > 0) {
+    const int n = left < C ? left : C;
+    __syncthreads();                         // the last chunk's images are read
+#pragma unroll
+    for (int i = 0; i < UK; ++i) {
+      const int u = tid + NT * i, row = u / (DKP / 8), piece = u % (DKP / 8);
+      store_unit<T, C, DKP>(lds, ku[i], row, piece);
+      if constexpr (OUT) store_unit<T, C, DKP>(lds + Q_AT, qu[i], row, piece);
+    }
+#pragma unroll
+    for (int i = 0; i < UV; ++i) {
+      const int u = tid + NT * i, row = u / (DVW / 8), piece = u % (DVW / 8);
+      store_unit<T, C, DVW>(lds + V_AT, vu[i], row, piece);
+    }
+#pragma unroll
+    for (int i = 0; i < UT; ++i) {
+      const int u = unit(i);
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = tu[i][j >> 2].v[j & 3];
+      u32x4 parts[NP];
+      split8<NP>(x, parts);
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+        *reinterpret_cast<u32x4*>(tsh + (((u >> 6) * NP + p) * 64 + (u & 63)) * 16) = parts[p];
+    }
+    if (wave == 0) {                         // lane: token lane % C
+      const double end = __shfl(fall, C - 1, 64), f = exp2(end);
+      const float e = __builtin_amdgcn_exp2f((float)fall);
+      fall_sh[lane % C] = fall;
+      beta_sh[lane % C] = beta;
+      since_sh[lane % C] = beta * e;
+      query_sh[lane % C] = a.scale * e;
+      end_sh[lane % C] = __builtin_amdgcn_exp2f((float)(end - fall));
+      fade_sh[0] = (float)f;
+      fade_sh[1] = f < 1e300 ? (float)(f - (double)(float)f) : 0.0f;
+    }
+    __syncthreads();
+    left -= n;
+    kp += C * a.kt;
+    vp += C * a.vt;
+    qp += C * a.qt;
+    pair += a.heads;
+
+    const float fade = fade_sh[0], fade_low = fade_sh[1];
+
+    // Scores K Q^T of 32 keys (rows) x 32 queries (columns): eight registers
+    // on end are an operand of U^T P^T as they lie.  One tile: every wave for
+    // itself; three: a tile a wave, exchanged in LDS.
+    u32x4 pop[OUT ? 2 : 1][NP];
+    if constexpr (OUT) {
+      if (CT == 1 || wave < TILES) {
+        const int qt = CT == 1 || wave == 0 ? 0 : 1, kt = CT > 1 && wave == 2 ? 1 : 0;
+        f16v acc = {};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          u32x4 ak[NL], bq[NL];
+#pragma unroll
+          for (int p = 0; p < NL; ++p) {
+            ak[p] = row_operand<C, DKP>(lds, at_row, p, kt, s);
+            bq[p] = row_operand<C, DKP>(lds + Q_AT, at_row, p, qt, s);
+          }
+#pragma unroll
+          for (int x = 0; x < NL; ++x)
+#pragma unroll
+            for (int y = 0; y < NL; ++y)
+              if (x + y < (NL == 1 ? 1 : NP)) acc = mfma(ak[x], bq[y], acc);
+        }
+        const int i = 32 * qt + col;
+        const double gi = fall_sh[i];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          float x[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int key = 32 * kt + 16 * s + 8 * (j >> 2) + 4 * hi + (j & 3);
+            const float y = acc[8 * s + j] * (a.scale * __builtin_amdgcn_exp2f((float)(gi - fall_sh[key])));
+            x[j] = i >= key ? y : 0.0f;
+          }
+          split8<NP>(x, pop[s]);
+        }
+      }
+    }
+
+    // r = beta v - beta e^g (K S), rows tokens;  O^T = S^T Q^T, rows columns of
+    // the values: both of S's parts.
+    f16v R[CT], O[OUT ? CT : 1];
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      R[t] = f16v{};
+      if constexpr (OUT) O[t] = f16v{};
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] = S[s / 2][8 * (s & 1) + j];
+        S[s / 2][8 * (s & 1) + j] = __builtin_fmaf(x[j], fade, x[j] * fade_low);
+      }
+      u32x4 sp[NP];
+      split8<NP>(x, sp);
+#pragma unroll
+      for (int t = 0; t < CT; ++t) {
+        u32x4 y[NL];
+#pragma unroll
+        for (int p = 0; p < NL; ++p) y[p] = row_operand<C, DKP>(lds, at_row, p, t, s);
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+          for (int l = 0; l < NL; ++l)
+            if (p + l < NP) R[t] = mfma(y[l], sp[p], R[t]);
+        if constexpr (OUT) {
+#pragma unroll
+          for (int p = 0; p < NL; ++p) y[p] = row_operand<C, DKP>(lds + Q_AT, at_row, p, t, s);
+#pragma unroll
+          for (int p = 0; p < NP; ++p)
+#pragma unroll
+            for (int l = 0; l < NL; ++l)
+              if (p + l < NP) O[t] = mfma(sp[p], y[l], O[t]);
+        }
+      }
+    }
+    if constexpr (OUT) {
+#pragma unroll
+      for (int t = 0; t < CT; ++t) {
+        const float f = query_sh[32 * t + col];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) O[t][r] *= f;
+      }
+    }
+
+    // A value that is not finite would give NaN wherever it meets a zero of T or
+    // of the scores: it is taken out of r (then u), and what depends on it set to
+    // NaN below: this lane's column, the queries from its token on and the state.
+    // (The segments' own states keep it: there NaN goes its way.)
+    int bad_from = C;
+    auto take_out = [&](f16v* x) {
+      float z = 0.0f;                        // NaN if any is not finite
+#pragma unroll
+      for (int t = 0; t < CT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z = __builtin_fmaf(x[t][r], 0.0f, z);
+      if (__ballot(z != z) != 0) {
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (!(__builtin_fabsf(x[t][r]) < __builtin_inff())) {
+              const int tok = 32 * t + 8 * (r >> 2) + 4 * hi + (r & 3);
+              if (tok < bad_from) bad_from = tok;
+              x[t][r] = 0.0f;
+            }
+        const int other = __shfl_xor(bad_from, 32, 64);
+        if (other < bad_from) bad_from = other;
+      }
+    };
+
+    u32x4 rop[CS][NP];                       // r, then u, as operands
+#pragma unroll
+    for (int s = 0; s < CS; ++s) {
+      u32x4 vop[NL];
+#pragma unroll
+      for (int p = 0; p < NL; ++p) vop[p] = token_operand<C, DVW>(lds + V_AT, at_value, p, 0, s);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const Vec<float, 4> b = *reinterpret_cast<const Vec<float, 4>*>(beta_sh + 16 * s + 8 * e + 4 * hi);
+        const Vec<float, 4> f = *reinterpret_cast<const Vec<float, 4>*>(since_sh + 16 * s + 8 * e + 4 * hi);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float y = 0.0f;
+#pragma unroll
+          for (int p = 0; p < NL; ++p) {
+            const uint32_t word = vop[p][2 * e + (j >> 1)];
+            y += __builtin_bit_cast(float, j & 1 ? word & 0xffff0000u : word << 16);
+          }
+          const int r = 8 * (s & 1) + 4 * e + j;
+          R[s / 2][r] = __builtin_fmaf(-f.v[j], R[s / 2][r], b.v[j] * y);
+        }
+      }
+    }
+    if constexpr (OUT) take_out(R);
+#pragma unroll
+    for (int s = 0; s < CS; ++s) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = R[s / 2][8 * (s & 1) + j];
+      split8<NP>(x, rop[s]);
+    }
+
+    // u = T r
+    f16v U[CT];
+#pragma unroll
+    for (int t = 0; t < CT; ++t) U[t] = f16v{};
+#pragma unroll
+    for (int i = 0; i < TILES * 2; ++i) {
+      const int tt = i / 2 == 0 ? 0 : 1, ts = i / 2 == 2 ? 1 : 0, s = 2 * ts + (i & 1);
+      u32x4 x[NP];
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+        x[p] = *reinterpret_cast<const u32x4*>(tsh + ((i * NP + p) * 64 + lane) * 16);
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int y = 0; y < NP; ++y)
+          if (p + y < NP) U[tt] = mfma(x[p], rop[s][y], U[tt]);
+    }
+
+    bool any_bad = false;
+    if constexpr (OUT) {
+      take_out(U);
+      if constexpr (CT > 1) {
+        __syncthreads();                     // T is read
+        if (wave < TILES) {
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+              *reinterpret_cast<u32x4*>(tsh + (((wave * 2 + s) * NP + p) * 64 + lane) * 16) = pop[s][p];
+        }
+        __syncthreads();
+      }
+#pragma unroll
+      for (int s = 0; s < CS; ++s) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = U[s / 2][8 * (s & 1) + j];
+        split8<NP>(x, rop[s]);
+      }
+      // O^T += U^T P^T
+#pragma unroll
+      for (int i = 0; i < TILES * 2; ++i) {
+        const int qt = i / 2 == 0 ? 0 : 1, kt = i / 2 == 2 ? 1 : 0, s = 2 * kt + (i & 1);
+        u32x4 y[NP];
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          y[p] = CT == 1 ? pop[i & 1][p]
+                         : *reinterpret_cast<const u32x4*>(tsh + ((i * NP + p) * 64 + lane) * 16);
+#pragma unroll
+        for (int x = 0; x < NP; ++x)
+#pragma unroll
+          for (int p = 0; p < NP; ++p)
+            if (p + x < NP) O[qt] = mfma(rop[s][x], y[p], O[qt]);
+      }
+      any_bad = __ballot(bad_from < C) != 0;
+      if (any_bad) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int from = __shfl(bad_from, 8 * (r >> 2) + 4 * hi + (r & 3), 64);
+#pragma unroll
+          for (int qt = 0; qt < CT; ++qt)
+            if (32 * qt + col >= from) O[qt][r] = __builtin_nanf("");
+        }
+      }
+      store_columns<T, CT, VEC>(O, op, n, dvs, a.ot, wave);
+      op += C * a.ot;
+    }
+
+    // The next chunk's rows, now that the outputs' registers are free.
+    if (left > 0) load_chunk();
+
+    // S <- e^(g_end) S (above) + K^T (e^(g_end - g) u)
+#pragma unroll
+    for (int s = 0; s < CS; ++s) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const Vec<float, 4> f = *reinterpret_cast<const Vec<float, 4>*>(end_sh + 16 * s + 8 * e + 4 * hi);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[4 * e + j] = U[s / 2][8 * (s & 1) + 4 * e + j] * f.v[j];
+      }
+      u32x4 bu[NP];
+      split8<NP>(x, bu);
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        u32x4 ak[NL];
+#pragma unroll
+        for (int y = 0; y < NL; ++y) ak[y] = token_operand<C, DKP>(lds, at_key, y, t, s);
+#pragma unroll
+        for (int y = 0; y < NL; ++y)
+#pragma unroll
+          for (int p = 0; p < NP; ++p)
+            if (p + y < NP) S[t] = mfma(ak[y], bu[p], S[t]);
+      }
+    }
+    if (any_bad) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[t][r] = bad_from < C ? __builtin_nanf("") : S[t][r];
+    }
+  }
+
+  if (move) {
+    // M turned: row = column of M, so that the join reads it in lines
+    float* const m = a.moves + (w * a.heads + h) * (int64_t)a.dk * a.dk;
+    if (sc < dvs) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int d = 32 * t + 16 * (r >> 3) + 8 * hi + (r & 7);
+          if (d < a.dk) m[(int64_t)(c0 + sc) * a.dk + d] = S[t][r];
+        }
+    }
+    return;
+  }
+  float* const to = OUT ? (last ? a.state_out : nullptr) : a.own;
+  if (to != nullptr) {
+    const __amdgpu_buffer_rsrc_t rs = state_of(to, OUT ? pl.seq : w);
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, (float)S[t][r]), rs,
+                                              s_off(t, r), 0, 0);
+  }
+  if (OUT && a.cu != nullptr && a.zero_rest) {   // rows of no sequence
+    T* const all = (T*)a.out + h * a.oh + c0;
+    auto clear = [&](int64_t from, int64_t to) {
+      for (int64_t t = from + tid / DVW; t < to; t += NT / DVW)
+        if (tid % DVW < dvs) all[t * a.ot + tid % DVW] = from_f<T>(0.0f);
+    };
+    if (pl.seq == 0 && pl.part == 0) clear(0, pl.begin);
+    if (pl.seq == a.seqs - 1 && last) clear(pl.begin + pl.len, a.tokens);
+  }
+}
+
+// The segments' N become the states before them, in place:
+//   S_0 = state_in,  S_{m+1} = M_m S_m + N_m.
+// A workgroup carries 8 columns of a head along a sequence.
+constexpr int JOIN_COLS = 8;
+__global__ __launch_bounds__(256) void delta_join_kernel(DeltaArgs a) {
+  __shared__ __attribute__((aligned(16))) float s_sh[2][CF_DECAY_MAX_DK * JOIN_COLS];
+  const int64_t w = blockIdx.y;
+  const Place pl = find_place(a, w, a.segment);
+  if (pl.seq < 0 || pl.part != 0 || pl.parts < 2) return;
+  const int h = blockIdx.z, c0 = blockIdx.x * JOIN_COLS, tid = threadIdx.x;
+  const int cols = a.dv - c0 < JOIN_COLS ? a.dv - c0 : JOIN_COLS;
+  const int64_t size = (int64_t)a.dk * a.dv;
+  for (int i = tid; i < a.dk * JOIN_COLS; i += 256) {
+    const int r = i / JOIN_COLS, c = i % JOIN_COLS;
+    s_sh[0][i] = a.state_in != nullptr && c < cols
+                     ? a.state_in[(pl.seq * a.heads + h) * size + (int64_t)r * a.dv + c0 + c] : 0.0f;
+  }
+  __syncthreads();
+  for (int64_t m = 0; m < pl.parts; ++m) {
+    const float* const s = s_sh[m & 1];
+    float* const next = s_sh[(m + 1) & 1];
+    float* const own = a.own + ((w + m) * a.heads + h) * size + c0;
+    const float* const mt = a.moves + ((w + m) * a.heads + h) * (int64_t)a.dk * a.dk;
+    const bool more = m + 1 < pl.parts;      // (the last one has no M and N)
+    for (int i = tid; i < 2 * a.dk; i += 256) {
+      const int r = i % a.dk, quad = i / a.dk * 4;
+      float y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = more && quad + j < cols ? own[(int64_t)r * a.dv + quad + j] : 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (quad + j < cols) own[(int64_t)r * a.dv + quad + j] = s[r * JOIN_COLS + quad + j];
+      if (more) {
+#pragma unroll 8
+        for (int k = 0; k < a.dk; ++k) {
+          const float x = mt[(int64_t)k * a.dk + r];
+          const Vec<float, 4> z = *reinterpret_cast<const Vec<float, 4>*>(s + k * JOIN_COLS + quad);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[j] = __builtin_fmaf(x, z.v[j], y[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) next[r * JOIN_COLS + quad + j] = y[j];
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// A launch has fewer than 2^32 threads: more workgroups take several, in
+// multiples of `unit`.
+template <typename F>
+hipError_t in_launches(int64_t count, int64_t most, F launch) {
+  for (int64_t first = 0; first < count; first += most) {
+    launch(first, count - first < most ? count - first : most);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+template <typename T, int DKP, int NW, int C, bool VEC>
+hipError_t launch_chunks(DeltaArgs a, hipStream_t st) {
+  constexpr int NT = C == 64 ? 256 : 64;
+  if (a.tokens > 0) {
+    const hipError_t e = in_launches(a.chunks * a.heads, 0x7fffff00ll / NT, [&](int64_t first, int64_t n) {
+      a.first = first;
+      hipLaunchKernelGGL((delta_solve_kernel<T, DKP, C, NT, VEC>), dim3((unsigned)n), dim3(NT), 0, st, a);
+    });
+    if (e != hipSuccess) return e;
+  }
+  a.value_slices = (a.dv + 32 * NW - 1) / (32 * NW);
+  const int64_t pairs = a.segments * (a.heads / a.k_group);    // of a segment and a key head
+  auto launch = [&](auto kernel, int slices) {
+    a.slices = slices;
+    const int64_t shared = (int64_t)a.k_group * slices;
+    return in_launches(pairs, 0xffffffffll / (64 * NW) / (8 * shared) * 8, [&](int64_t first, int64_t n) {
+      a.first = first;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)((n + 7) / 8 * 8 * shared)), dim3(64 * NW), 0, st, a);
+    });
+  };
+  if (a.segment > 0) {
+    hipError_t e = launch(delta_walk_kernel<T, DKP, NW, C, false, VEC>,
+                          a.value_slices + (a.dk + 32 * NW - 1) / (32 * NW));
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(delta_join_kernel, dim3((unsigned)((a.dv + JOIN_COLS - 1) / JOIN_COLS),
+                                               (unsigned)a.segments, (unsigned)a.heads),
+                       dim3(256), 0, st, a);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return launch(delta_walk_kernel<T, DKP, NW, C, true, VEC>, a.value_slices);
+}
+
+// bf16 heads of 65 to 128 channels have room for chunks of 64 (CF_DELTA_CHUNK)
+inline int chunk_of(int64_t dtype, int64_t dk) { return dtype == SEQ_BF16 && dk > 64 && dk <= 128 ? 64 : 32; }
+
+template <typename T, bool VEC>
+hipError_t launch_delta_v(const DeltaArgs& a, hipStream_t st) {
+  constexpr int C = parts_of<T>() == 1 ? 64 : 32;
+  if (a.dk <= 32) return launch_chunks<T, 32, 1, 32, VEC>(a, st);
+  if (a.dk <= 64) return launch_chunks<T, 64, 2, 32, VEC>(a, st);
+  if (a.dk <= 128) return launch_chunks<T, 128, 4, C, VEC>(a, st);
+  return launch_chunks<T, 256, 4, 32, VEC>(a, st);
+}
+
+template <typename T>
+hipError_t launch_delta(const DeltaArgs& a, hipStream_t st) {
+  return a.vec ? launch_delta_v<T, true>(a, st) : launch_delta_v<T, false>(a, st);
+}
+
+}  // namespace
+
+CF_API int64_t cf_delta_workspace(const CfDeltaAttentionArgs* p) {
+  if (!p || p->heads < 1 || p->seqs < 0 || p->tokens < 0 || p->segment < 0) return -1;
+  const CfDeltaAttentionArgs& x = *p;
+  const int64_t C = chunk_of(x.dtype, x.dk);
+  const int64_t solved = (C / 32) * (C / 32 + 1) / 2 * 1024;
+  const int64_t chunks = x.cu_seqlens ? x.tokens / C + x.seqs : x.seqs * units_of(x.tokens, C);
+  int64_t bytes = x.cu_seqlens ? (8 * (x.seqs + 1) + 255) / 256 * 256 : 0;
+  if (x.tokens > 0) bytes += chunks * x.heads * (4 * solved + 12 * C);
+  if (x.segment > 0 && x.segment < x.tokens) {
+    const int64_t segments = x.cu_seqlens ? x.tokens / x.segment + x.seqs
+                                          : x.seqs * units_of(x.tokens, x.segment);
+    bytes += segments * x.heads * 4 * x.dk * (x.dv + x.dk);
+  }
+  return bytes;
+}
+
+CF_API int cf_delta_attention(const CfDeltaAttentionArgs* p) {
+  if (!p) return (int)hipErrorInvalidValue;
+  const CfDeltaAttentionArgs& x = *p;
+  if (x.seqs < 0 || x.tokens < 0 || !delta_heads_fit(x.heads, x.q_heads, x.k_heads, x.v_heads) ||
+      x.dk < 1 || x.dk > CF_DECAY_MAX_DK || x.dv < 1 || x.dv > CF_DECAY_MAX_DV || x.dtype < 0 ||
+      x.dtype > 2 || x.seqs > CF_DECAY_MAX_SEQS || x.tokens > CF_DECAY_MAX_TOKENS || x.segment < 0 ||
+      x.segment % CF_DECAY_CHUNK != 0 || x.workspace_bytes < 0)
+    return (int)hipErrorInvalidValue;
+  for (int64_t s : {x.q_token, x.k_token, x.v_token, x.out_token})
+    if (s < 0 || s > CF_DECAY_MAX_TOKEN_STRIDE) return (int)hipErrorInvalidValue;
+  if (x.seqs == 0) return 0;
+  if (x.tokens > 0 && (!x.q || !x.k || !x.v || !x.beta || !x.out)) return (int)hipErrorInvalidValue;
+  const int64_t need = cf_delta_workspace(p);
+  if (x.workspace_bytes < need || (need > 0 && (!x.workspace || (uintptr_t)x.workspace % 256 != 0)))
+    return (int)hipErrorInvalidValue;
+  DeltaArgs a;
+  a.q = x.q; a.k = x.k; a.v = x.v;
+  a.beta = x.beta; a.log_decay = x.log_decay;
+  a.state_in = x.state_in; a.state_out = x.state_out;
+  a.out = x.out;
+  a.cu = x.cu_seqlens;
+  a.cu_wide = x.cu_wide != 0; a.zero_rest = x.zero_rest != 0;
+  a.beta_f32 = x.beta_f32 != 0; a.decay_f32 = x.decay_f32 != 0;
+  a.seqs = x.seqs; a.tokens = x.tokens;
+  a.heads = (int)x.heads;
+  a.q_group = (int)(x.heads / x.q_heads);
+  a.k_group = (int)(x.heads / x.k_heads);
+  a.v_group = (int)(x.heads / x.v_heads);
+  a.dk = (int)x.dk; a.dv = (int)x.dv;
+  a.first = 0;
+  a.slices = a.value_slices = 0;
+  const int64_t C = chunk_of(x.dtype, x.dk);
+  a.chunks = a.cu ? x.tokens / C + x.seqs : x.seqs * units_of(x.tokens, C);
+  a.segment = x.segment > 0 && x.segment < x.tokens ? x.segment : 0;
+  a.segments = a.segment == 0 ? x.seqs
+               : a.cu ? x.tokens / a.segment + x.seqs : x.seqs * units_of(x.tokens, a.segment);
+  if (a.segment > 0 && a.segments > 65535) return (int)hipErrorInvalidValue;   // the join's grid
+  char* at = (char*)x.workspace;
+  a.begins = (int64_t*)at;
+  if (a.cu) at += (8 * (x.seqs + 1) + 255) / 256 * 256;
+  a.solved = (float*)at;
+  if (x.tokens > 0) at += a.chunks * a.heads * ((C / 32) * (C / 32 + 1) / 2 * 4096);
+  a.falls = (double*)at;
+  if (x.tokens > 0) at += a.chunks * a.heads * 8 * C;
+  a.betas = (float*)at;
+  if (x.tokens > 0) at += a.chunks * a.heads * 4 * C;
+  a.own = (float*)at;
+  a.moves = a.own + a.segments * a.heads * (int64_t)a.dk * a.dv;
+  a.qb = x.q_batch; a.qt = x.q_token; a.qh = x.q_head;
+  a.kb = x.k_batch; a.kt = x.k_token; a.kh = x.k_head;
+  a.vb = x.v_batch; a.vt = x.v_token; a.vh = x.v_head;
+  a.bb = x.beta_batch; a.bt = x.beta_token; a.bh = x.beta_head;
+  a.lb = x.decay_batch; a.lt = x.decay_token; a.lh = x.decay_head;
+  a.ob = x.out_batch; a.ot = x.out_token; a.oh = x.out_head;
+  const int size = x.dtype == SEQ_F32 ? 4 : 2, per = 16 / size;
+  auto vec = [&](const void* base, int64_t b, int64_t t, int64_t h, int64_t d) {
+    return (uintptr_t)base % 16 == 0 && b % per == 0 && t % per == 0 && h % per == 0 &&
+           d % per == 0 && t >= d;
+  };
+  a.vec = vec(x.q, a.qb, a.qt, a.qh, x.dk) && vec(x.k, a.kb, a.kt, a.kh, x.dk) &&
+          vec(x.v, a.vb, a.vt, a.vh, x.dv) && vec(x.out, a.ob, a.ot, a.oh, x.dv);
+  a.scale = (float)x.scale;
+  hipStream_t st = (hipStream_t)x.stream;
+  if (a.cu) {
+    hipLaunchKernelGGL(delta_begins_kernel, dim3(1), dim3(1024), 0, st, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
+  }
+  hipError_t e;
+  if (x.dtype == SEQ_F32) e = launch_delta<float>(a, st);
+  else if (x.dtype == SEQ_F16) e = launch_delta<_Float16>(a, st);
+  else e = launch_delta<bf16_t>(a, st);
+  return (int)e;
+}

@@ -856,6 +856,67 @@ typedef struct CfDecayStepArgs {
 } CfDecayStepArgs;
 int cf_decay_attention_step(const CfDecayStepArgs* args);
 
+/* The delta rule, whose state corrects itself before it adds:
+ *   S_t = w_t S_{t-1} + k_t u_t^T,  u_t = beta_t (v_t - w_t S_{t-1}^T k_t),
+ *   out_t = scale q_t S_t,          w_t = exp(log_decay_t)
+ * for every sequence and each of `heads` heads; head h reads head
+ * h / (heads / n) of the n of each of q, k and v (n divides heads).  beta and
+ * log_decay (nullable: zeros) [token][heads] are fp32 (beta_f32, decay_f32) or
+ * of dtype; log_decay is 0 or less as a rule, -inf keeps only the token itself.
+ * States, cu_seqlens, zero_rest, strides and limits as in
+ * CfDecayAttentionArgs; the strides of beta and log_decay are free.  A token that
+ * is not finite does not reach the tokens before it; what it does reach may be
+ * NaN where the formula gives an infinity.
+ * segment (0, or a multiple of CF_DECAY_CHUNK): sequences are split into
+ * segments of so many tokens that run side by side; unused where it is not below
+ * tokens; at most 65535 segments in all.  The workspace (256-byte aligned) has
+ * at least the bytes that cf_delta_workspace gives for the same block (-1: the
+ * block makes no sense); every call needs one, and it is free again when the
+ * call's work on the stream is done. */
+typedef struct CfDeltaAttentionArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* beta;
+  const void* log_decay;
+  const float* state_in;
+  float* state_out;
+  void* out;
+  const void* cu_seqlens;
+  void* workspace;
+  void* stream;
+  int64_t cu_wide, zero_rest, dtype, beta_f32, decay_f32, seqs, tokens;
+  int64_t heads, q_heads, k_heads, v_heads, dk, dv;
+  int64_t q_batch, q_token, q_head, k_batch, k_token, k_head;
+  int64_t v_batch, v_token, v_head, beta_batch, beta_token, beta_head;
+  int64_t decay_batch, decay_token, decay_head, out_batch, out_token, out_head;
+  int64_t segment, workspace_bytes;
+  double scale;
+} CfDeltaAttentionArgs;
+int64_t cf_delta_workspace(const CfDeltaAttentionArgs* args);
+int cf_delta_attention(const CfDeltaAttentionArgs* args);
+
+/* One token for each of `rows` sequences through the delta rule, S = state +
+ * slot * state_slot updated in place; slots as in CfDecayStepArgs, heads, beta
+ * and log_decay as in CfDeltaAttentionArgs. */
+typedef struct CfDeltaStepArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* beta;
+  const void* log_decay;
+  float* state;
+  void* out;
+  const void* slots;
+  void* stream;
+  int64_t slots_wide, dtype, beta_f32, decay_f32, rows, heads, q_heads, k_heads, v_heads;
+  int64_t dk, dv, pool, state_slot;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, beta_row, beta_head;
+  int64_t decay_row, decay_head, out_row, out_head;
+  double scale;
+} CfDeltaStepArgs;
+int cf_delta_attention_step(const CfDeltaStepArgs* args);
+
 /* Rotation of the heads x [outer][inner][x_heads][d] and, with k_heads > 0, k
  * (same tokens and d) by the angle position * freqs[pair], pairs (i, i +
  * pairs) or (2 i, 2 i + 1) interleaved, channels past 2 * pairs passed on;
