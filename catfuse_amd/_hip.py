@@ -107,6 +107,8 @@ _SIGNATURES = {
     "cf_delta_workspace": [_P],
     "cf_delta_attention": [_P],
     "cf_delta_attention_step": [_P],
+    "cf_linear_workspace": [_P],
+    "cf_linear": [_P],
 }
 
 _D = c_double
@@ -144,14 +146,16 @@ class ConvHaloPairArgs(ctypes.Structure):
 
 # The argument blocks of the sequence operators (include/catfuse_amd.h:
 # CfDecayAttentionArgs, CfDecayStepArgs, CfRotaryArgs, CfDeltaAttentionArgs,
-# CfDeltaStepArgs), packed as bytes: first the pointers and the stream (Q), which differ from call to call, then what a
+# CfDeltaStepArgs) and of the dense products (CfLinearArgs), packed as bytes:
+# first the pointers and the stream (Q), which differ from call to call, then what a
 # launch plan keeps (q an int64, d a double), every field 8 bytes.
 DECAY_ATTENTION_ARGS = struct.Struct("=10Q"), struct.Struct("=23qd")
 DECAY_STEP_ARGS = struct.Struct("=8Q"), struct.Struct("=17qd")
 ROTARY_ARGS = struct.Struct("=9Q"), struct.Struct("=33qd")
 DELTA_ATTENTION_ARGS = struct.Struct("=11Q"), struct.Struct("=33qd")
 DELTA_STEP_ARGS = struct.Struct("=9Q"), struct.Struct("=25qd")
-_RESTYPES = {"cf_error_string": c_char_p, "cf_delta_workspace": _I}
+LINEAR_ARGS = struct.Struct("=9Q"), struct.Struct("=12q")
+_RESTYPES = {"cf_error_string": c_char_p, "cf_delta_workspace": _I, "cf_linear_workspace": _I}
 
 _lib = None
 

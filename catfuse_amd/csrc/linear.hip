@@ -1,0 +1,589 @@
+// Dense products with an epilogue:
+//   out = act(x w^T + bias) + residual                     (linear)
+//   out = act(x w^T + bias) * (x w2^T + bias2)             (gated)
+// x [rows][inner], w and w2 [cols][inner], out [rows][cols]; fp32, fp16 or bf16
+// with fp32 sums, each output rounded once.
+//
+// Both operands lie with the inner dimension on end, which is how the matrix
+// cores' operands want them: a lane takes 16 bytes of one row.  Products of
+// fp32 numbers run on the fp32 matrix instructions (their products and sums, an
+// infinity stays one), those of 16-bit ones on theirs.
+//
+// No counterpart in the reference.
+#include "cf_seq.h"
+
+namespace {
+
+struct LinearArgs {
+  const void* x;
+  const void* w[2];
+  const void* bias[2];
+  const void* residual;
+  void* out;
+  float* parts;              // sums of the splits [split][product][rows][cols], or null
+  int bias_f32, activation;
+  int64_t rows;
+  int inner, cols;
+  int64_t xr, wr[2], rr, orow;
+  int splits, split_steps;   // along the inner dimension; steps of a split
+  int row_tiles, col_tiles;
+};
+
+typedef float f4v __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+
+// Products of 16 bytes of a row of either operand (`a`: rows of the result,
+// `b`: its columns): 8 numbers of 16 bits, or 4 of 32 taken one at a time (the
+// same ones of both operands, in whatever order).
+template <typename T>
+__device__ __forceinline__ f16v mfma32(u32x4 a, u32x4 b, f16v c) {
+  if constexpr (sizeof(T) == 4) {
+    const f4v x = __builtin_bit_cast(f4v, a), y = __builtin_bit_cast(f4v, b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
+    return c;
+  } else if constexpr (__is_same(T, bf16_t)) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a),
+                                                   __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a),
+                                                  __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  }
+}
+template <typename T>
+__device__ __forceinline__ f4v mfma16(u32x4 a, u32x4 b, f4v c) {
+  if constexpr (sizeof(T) == 4) {
+    const f4v x = __builtin_bit_cast(f4v, a), y = __builtin_bit_cast(f4v, b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
+    return c;
+  } else if constexpr (__is_same(T, bf16_t)) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a),
+                                                   __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a),
+                                                  __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  }
+}
+
+// 16 bytes from wherever they begin (a multiple of the type's size).
+template <typename T>
+__device__ __forceinline__ u32x4 load16(const T* p) {
+  u32x4 r;
+  __builtin_memcpy(&r, p, 16);
+  return r;
+}
+// The first n (0 to all) of the numbers there, zeros behind.
+template <typename T>
+__device__ __forceinline__ u32x4 load_some(const T* p, int n) {
+  constexpr int PER = 16 / sizeof(T);
+  Vec<T, PER> v;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) v.v[i] = i < n ? p[i] : from_f<T>(0.0f);
+  return __builtin_bit_cast(u32x4, v);
+}
+
+// e^x to about an ulp: the rounding of x log2(e) is put back.
+__device__ __forceinline__ float exp_f(float x) {
+  const float y = x * 1.44269502f;
+  const float low = __builtin_fmaf(x, 1.44269502f, -y) + x * 1.92596299e-8f;
+  const float e = __builtin_amdgcn_exp2f(y);
+  // (an infinite or vanished power stays one)
+  return __builtin_fabsf(y) < 126.0f ? __builtin_fmaf(e, low * 0.693147182f, e) : e;
+}
+__device__ __forceinline__ float sigmoid_times(float z, float t) {   // z / (1 + e^-t)
+  return z * __builtin_amdgcn_rcpf(1.0f + exp_f(-t));
+}
+__device__ __forceinline__ float activate(float z, int kind) {
+  switch (kind) {
+    case CF_ACT_RELU: return z < 0.0f ? 0.0f : z;
+    case CF_ACT_SILU: return sigmoid_times(z, z);
+    case CF_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.707106781f));
+    case CF_ACT_GELU_TANH:     // 1 + tanh(t) = 2 / (1 + e^(-2 t))
+      return sigmoid_times(z, 1.59576912f * __builtin_fmaf(0.044715f * z * z, z, z));
+    default: return z;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float bias_of(const LinearArgs& a, int op, int n) {
+  if (a.bias[op] == nullptr) return 0.0f;
+  return a.bias_f32 ? reinterpret_cast<const float*>(a.bias[op])[n]
+                    : to_f(reinterpret_cast<const T*>(a.bias[op])[n]);
+}
+
+// Four outputs of a row, columns n .. n + 3, from the sums s[product][4]; those
+// from cols on are left alone.  wide: four on end are aligned and whole.
+template <typename T, int OPS>
+__device__ __forceinline__ void finish4(const LinearArgs& a, int64_t m, int n, const float (*s)[4],
+                                        bool wide) {
+  if (n >= a.cols) return;
+  float y[4], r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  T* const to = (T*)a.out + m * a.orow + n;
+  if (OPS == 1 && a.residual != nullptr) {
+    const T* const from = (const T*)a.residual + m * a.rr + n;
+    if (wide) {
+      const Vec<T, 4> v = *reinterpret_cast<const Vec<T, 4>*>(from);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = to_f(v.v[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n + j < a.cols) r[j] = to_f(from[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int c = n + j < a.cols ? n + j : a.cols - 1;
+    y[j] = activate(s[0][j] + bias_of<T>(a, 0, c), a.activation);
+    if constexpr (OPS == 2) y[j] *= s[1][j] + bias_of<T>(a, 1, c);
+    else y[j] += r[j];
+  }
+  if (wide) {
+    Vec<T, 4> v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v.v[j] = from_f<T>(y[j]);
+    *reinterpret_cast<Vec<T, 4>*>(to) = v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (n + j < a.cols) to[j] = from_f<T>(y[j]);
+  }
+}
+
+// Whether four columns on end, from a multiple of four, are aligned and whole.
+template <typename T>
+__device__ __forceinline__ bool wide_columns(const LinearArgs& a) {
+  const uintptr_t by = 4 * sizeof(T) - 1;
+  return a.cols % 4 == 0 && a.orow % 4 == 0 && ((uintptr_t)a.out & by) == 0 &&
+         (a.residual == nullptr || (a.rr % 4 == 0 && ((uintptr_t)a.residual & by) == 0));
+}
+
+// Few rows of x: bound by the bytes of w, each read once.  A workgroup takes 16
+// columns (rows of w) and all rows of x, NW waves a part of the inner dimension
+// each, joined in LDS.  A lane of a product takes 16 bytes of w's row lane % 16,
+// piece lane / 16 of four; U products' loads are in flight.
+template <typename T, int MT, int NW, int OPS>
+__global__ __launch_bounds__(64 * NW) void linear_few_kernel(LinearArgs a) {
+  constexpr int PER = 16 / sizeof(T), STEP = 4 * PER, U = MT * OPS <= 2 ? 8 : 4;
+  __shared__ float part[NW][OPS * MT][4][64];
+  const int tid = threadIdx.x, lane = tid & 63, row = lane & 15, quarter = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n0 = blockIdx.x * 16;
+  const int steps = (a.inner + STEP - 1) / STEP, each = (steps + NW - 1) / NW;
+  const int first = wave * each, whole = a.inner / STEP;
+  int last = first + each < steps ? first + each : steps;
+  const T *wp[OPS], *xp[MT];
+#pragma unroll
+  for (int o = 0; o < OPS; ++o)
+    wp[o] = (const T*)a.w[o] + (n0 + row < a.cols ? n0 + row : a.cols - 1) * a.wr[o] + quarter * PER;
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const int64_t m = 16 * t + row;
+    xp[t] = (const T*)a.x + (m < a.rows ? m : a.rows - 1) * a.xr + quarter * PER;
+  }
+  f4v acc[OPS][MT];
+#pragma unroll
+  for (int o = 0; o < OPS; ++o)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[o][t] = f4v{};
+  int s = first;
+  const int full = last < whole ? last : whole;
+  for (; s + U <= full; s += U) {
+    u32x4 wv[U][OPS], xv[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int o = 0; o < OPS; ++o) wv[u][o] = load16(wp[o] + (int64_t)(s + u) * STEP);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) xv[u][t] = load16(xp[t] + (int64_t)(s + u) * STEP);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int o = 0; o < OPS; ++o)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[o][t] = mfma16<T>(wv[u][o], xv[u][t], acc[o][t]);
+  }
+  for (; s < last; ++s) {                    // the inner dimension's end: zeros behind it
+    const int left = a.inner - s * STEP - quarter * PER;
+    u32x4 wv[OPS], xv[MT];
+#pragma unroll
+    for (int o = 0; o < OPS; ++o) wv[o] = load_some(wp[o] + (int64_t)s * STEP, left);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) xv[t] = load_some(xp[t] + (int64_t)s * STEP, left);
+#pragma unroll
+    for (int o = 0; o < OPS; ++o)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) acc[o][t] = mfma16<T>(wv[o], xv[t], acc[o][t]);
+  }
+#pragma unroll
+  for (int o = 0; o < OPS; ++o)
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) part[wave][o * MT + t][j][lane] = acc[o][t][j];
+  __syncthreads();
+  const bool wide = wide_columns<T>(a);
+  for (int t = wave; t < MT; t += NW) {
+    float y[OPS][4];
+#pragma unroll
+    for (int o = 0; o < OPS; ++o)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float z = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) z += part[i][o * MT + t][j][lane];
+        y[o][j] = z;
+      }
+    const int64_t m = 16 * t + row;
+    if (m < a.rows) finish4<T, OPS>(a, m, n0 + 4 * quarter, y, wide);
+  }
+}
+
+// One copy of 16 bytes a lane from a buffer straight to LDS: byte `at` of the
+// buffer (zeros beyond its range), `add` bytes on, to lds + 16 lane.  In
+// assembly, so that the compiler does not wait for it before every read of LDS;
+// the kernel waits before the barrier that lets the copies be read.
+__device__ __forceinline__ void copy16(i32x4 rsrc, uint32_t at, uint32_t add, uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %3\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %0, %1, %2 offen lds"
+      :
+      : "v"(at), "s"(rsrc), "s"(add), "s"(lds)
+      : "memory", "m0");
+}
+__device__ __forceinline__ i32x4 buffer_of(const void* base, uint32_t bytes) {
+  const uint64_t p = (uint64_t)(uintptr_t)base;
+  i32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)p);
+  r[1] = __builtin_amdgcn_readfirstlane((int)((uint32_t)(p >> 32) & 0xffffu));
+  r[2] = __builtin_amdgcn_readfirstlane((int)bytes);
+  r[3] = 0x00020000;
+  return r;
+}
+
+// Many rows.  A workgroup takes BM rows of x and BN columns, in steps of 128
+// bytes of the inner dimension; two stages of LDS, the next step's rows copied
+// while the present one's are multiplied.  Waves WM x WN, each BM / WM rows and
+// BN / WN columns: results as accumulators of 32 columns (their rows) by 32 rows
+// of x (their columns), so that a lane holds four columns on end.
+//
+// LDS rows of 128 bytes, their eight pieces exchanged by row (piece ^ row % 8),
+// which spreads both the copies' and the operands' accesses over all banks.
+//
+// VEC: rows in pieces of 16 bytes, aligned and whole, not overlapping; else
+// through registers, element by element at the inner dimension's end.
+template <typename T, int BM, int BN, int WM, int WN, int OPS, bool VEC>
+__global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinearArgs a) {
+  constexpr int NW = WM * WN, NT = 64 * NW, PER = 16 / sizeof(T), STEP = 8 * PER;
+  constexpr int ROWS = BM + OPS * BN, STAGE = ROWS * 128;
+  constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
+  static_assert(ROWS % (8 * NW) == 0 && BM % 8 == 0 && BN % 8 == 0, "whole copies");
+  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
+
+  // Tiles in bands of eight rows of them, a band column by column; each XCD
+  // (workgroup number mod 8) takes a run of them, so that its L2 holds what its
+  // tiles share.
+  const int tiles = a.row_tiles * a.col_tiles;
+  int tile = blockIdx.x;
+  {
+    const int each = tiles / 8, rest = tiles % 8, xcd = tile % 8, i = tile / 8;
+    tile = xcd * each + (xcd < rest ? xcd : rest) + i;
+  }
+  const int band = tile / (8 * a.col_tiles), in_band = tile % (8 * a.col_tiles);
+  const int band_rows = a.row_tiles - 8 * band < 8 ? a.row_tiles - 8 * band : 8;
+  const int64_t m0 = (int64_t)(8 * band + in_band % band_rows) * BM;
+  const int n0 = in_band / band_rows * BN;
+
+  const int steps_all = (a.inner + STEP - 1) / STEP, split = blockIdx.y;
+  const int from = split * a.split_steps;
+  const int steps = steps_all - from < a.split_steps ? steps_all - from : a.split_steps;
+
+  // What this thread copies: rows r0 + 8 NW i of the stage, piece lane % 8
+  const int r0 = 8 * wave + (lane >> 3), piece = lane & 7;
+  constexpr int COPIES = ROWS / (8 * NW);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  const int64_t rows_left = a.rows - m0;
+  const int cols_left = a.cols - n0;
+  i32x4 xb, wb[OPS];
+  if constexpr (VEC) {
+    const int64_t rn = rows_left < BM ? rows_left : BM, cn = cols_left < BN ? cols_left : BN;
+    xb = buffer_of((const T*)a.x + m0 * a.xr, (uint32_t)(((rn - 1) * a.xr + a.inner) * sizeof(T)));
+#pragma unroll
+    for (int o = 0; o < OPS; ++o)
+      wb[o] = buffer_of((const T*)a.w[o] + n0 * a.wr[o],
+                        (uint32_t)(((cn - 1) * a.wr[o] + a.inner) * sizeof(T)));
+  }
+  u32x4 regs[VEC ? 1 : COPIES];
+  // Rows beyond x's and w's: out of the buffers' ranges.  (A copy's eight rows
+  // are all of one operand.)
+  auto fetch = [&](int stage, int step) {
+    const int k = (from + step) * STEP + (piece ^ (r0 & 7)) * PER;
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+      const int base = 8 * wave + 8 * NW * i, r = base + (lane >> 3);   // (base: the same in every lane)
+      if constexpr (VEC) {
+        const bool is_x = base < BM;
+        const int o = OPS == 2 && base >= BM + BN ? 1 : 0;
+        const int row = is_x ? r : r - BM - o * BN;
+        const int64_t stride = is_x ? a.xr : a.wr[o];
+        uint32_t at = (uint32_t)(row * (int)stride * (int)sizeof(T)) + (uint32_t)((piece ^ (r & 7)) * 16);
+        if (k >= a.inner) at = 0x80000000u;
+        copy16(is_x ? xb : wb[o], at, (uint32_t)((from + step) * 128), lds0 + stage * STAGE + base * 128);
+      } else {
+        const bool is_x = base < BM;
+        const int o = OPS == 2 && base >= BM + BN ? 1 : 0;
+        int64_t row = is_x ? m0 + r : n0 + r - BM - o * BN;
+        const int64_t end = is_x ? a.rows : a.cols;
+        row = row < end ? row : end - 1;     // (its results are not stored)
+        const T* const p = (is_x ? (const T*)a.x + row * a.xr : (const T*)a.w[o] + row * a.wr[o]) + k;
+        regs[i] = k + PER <= a.inner ? load16(p) : load_some(p, a.inner - k);
+      }
+    }
+  };
+  auto deposit = [&](int stage) {
+    if constexpr (!VEC) {
+#pragma unroll
+      for (int i = 0; i < COPIES; ++i) {
+        const int r = 8 * wave + 8 * NW * i + (lane >> 3);
+        *reinterpret_cast<u32x4*>(lds + stage * STAGE + r * 128 + piece * 16) = regs[i];
+      }
+    }
+  };
+
+  f16v acc[OPS][TN][TM];
+#pragma unroll
+  for (int o = 0; o < OPS; ++o)
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int j = 0; j < TM; ++j) acc[o][i][j] = f16v{};
+
+  const char* const xs = lds + (wm * (BM / WM) + col) * 128;
+  const char* const ws = lds + (BM + wn * (BN / WN) + col) * 128;
+  fetch(0, 0);
+  deposit(0);
+  for (int step = 0; step < steps; ++step) {
+    if constexpr (VEC) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    const int stage = step & 1;
+    if (step + 1 < steps) fetch(stage ^ 1, step + 1);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int at = stage * STAGE + (((2 * s + hi) ^ (col & 7)) << 4);
+      u32x4 xv[TM], wv[OPS][TN];
+#pragma unroll
+      for (int j = 0; j < TM; ++j) xv[j] = *reinterpret_cast<const u32x4*>(xs + j * 32 * 128 + at);
+#pragma unroll
+      for (int o = 0; o < OPS; ++o)
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+          wv[o][i] = *reinterpret_cast<const u32x4*>(ws + (o * BN + i * 32) * 128 + at);
+#pragma unroll
+      for (int o = 0; o < OPS; ++o)
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+          for (int j = 0; j < TM; ++j) acc[o][i][j] = mfma32<T>(wv[o][i], xv[j], acc[o][i][j]);
+    }
+    if (step + 1 < steps) deposit(stage ^ 1);
+  }
+
+  const bool wide = wide_columns<T>(a);
+#pragma unroll
+  for (int j = 0; j < TM; ++j) {
+    const int64_t m = m0 + wm * (BM / WM) + 32 * j + col;
+    if (m >= a.rows) continue;
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int n = n0 + wn * (BN / WN) + 32 * i + 8 * g + 4 * hi;
+        float y[OPS][4];
+#pragma unroll
+        for (int o = 0; o < OPS; ++o)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[o][e] = acc[o][i][j][4 * g + e];
+        if (a.parts == nullptr) {
+          finish4<T, OPS>(a, m, n, y, wide);
+        } else {
+#pragma unroll
+          for (int o = 0; o < OPS; ++o) {
+            float* const to = a.parts + (((int64_t)split * OPS + o) * a.rows + m) * a.cols + n;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (n + e < a.cols) to[e] = y[o][e];
+          }
+        }
+      }
+  }
+}
+
+// The sums of the splits, in their order, and the epilogue: four columns a thread.
+template <typename T, int OPS>
+__global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a) {
+  const int quads = (a.cols + 3) / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.rows * quads) return;
+  const int64_t m = i / quads;
+  const int n = (int)(i % quads) * 4;
+  float y[OPS][4];
+#pragma unroll
+  for (int o = 0; o < OPS; ++o)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[o][e] = 0.0f;
+  for (int s = 0; s < a.splits; ++s)
+#pragma unroll
+    for (int o = 0; o < OPS; ++o) {
+      const float* const from = a.parts + (((int64_t)s * OPS + o) * a.rows + m) * a.cols + n;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < a.cols) y[o][e] += from[e];
+    }
+  finish4<T, OPS>(a, m, n, y, wide_columns<T>(a));
+}
+
+// How a product is taken.
+struct Plan { int few, size, splits, split_steps; };   // few: waves of the few-rows kernel, or 0
+
+constexpr int FEW_ROWS = 32;
+constexpr int CUS = 256;
+
+inline Plan plan_of(const CfLinearArgs& x, bool gated) {
+  Plan p = {0, 0, 1, 0};
+  const int64_t step = x.dtype == SEQ_F32 ? 32 : 64, steps = (x.inner + step - 1) / step;
+  if (x.rows <= FEW_ROWS) {
+    p.few = (x.cols + 15) / 16 >= 2 * CUS ? 4 : 8;
+    return p;
+  }
+  auto tiles = [&](int64_t bm, int64_t bn) {
+    return ((x.rows + bm - 1) / bm) * ((x.cols + bn - 1) / bn);
+  };
+  const int big = gated ? 64 : 128;
+  p.size = tiles(128, big) >= CUS ? 128 : 64;
+  const int64_t n = p.size == 128 ? tiles(128, big) : tiles(64, gated ? 32 : 64);
+  if (n < CUS && steps >= 16) {
+    int64_t splits = CUS / n;
+    if (splits > steps / 8) splits = steps / 8;
+    if (splits > 1) {
+      p.split_steps = (int)((steps + splits - 1) / splits);
+      p.splits = (int)((steps + p.split_steps - 1) / p.split_steps);
+    }
+  }
+  if (p.splits <= 1) p.splits = 1, p.split_steps = (int)steps;
+  return p;
+}
+
+inline int64_t workspace_of(const CfLinearArgs& x, const Plan& p, bool gated) {
+  return p.few || p.splits < 2 ? 0 : 4 * (gated ? 2 : 1) * p.splits * x.rows * x.cols;
+}
+
+template <typename T, int OPS>
+hipError_t launch_few(const LinearArgs& a, int waves, hipStream_t st) {
+  const dim3 grid((unsigned)((a.cols + 15) / 16));
+  if (a.rows <= 16) {
+    if (waves == 4) hipLaunchKernelGGL((linear_few_kernel<T, 1, 4, OPS>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((linear_few_kernel<T, 1, 8, OPS>), grid, dim3(512), 0, st, a);
+  } else {
+    if (waves == 4) hipLaunchKernelGGL((linear_few_kernel<T, 2, 4, OPS>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((linear_few_kernel<T, 2, 8, OPS>), grid, dim3(512), 0, st, a);
+  }
+  return hipGetLastError();
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int OPS, bool VEC>
+hipError_t launch_tiles(LinearArgs a, hipStream_t st) {
+  const int64_t rt = (a.rows + BM - 1) / BM, ct = (a.cols + BN - 1) / BN;
+  if (rt * ct > 0xffffffffll / (64 * WM * WN) / a.splits) return hipErrorInvalidValue;
+  a.row_tiles = (int)rt;
+  a.col_tiles = (int)ct;
+  hipLaunchKernelGGL((linear_tile_kernel<T, BM, BN, WM, WN, OPS, VEC>),
+                     dim3((unsigned)(rt * ct), (unsigned)a.splits), dim3(64 * WM * WN), 0, st, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.parts == nullptr) return e;
+  const int64_t n = a.rows * ((a.cols + 3) / 4);
+  hipLaunchKernelGGL((linear_join_kernel<T, OPS>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+template <typename T, int OPS, bool VEC>
+hipError_t launch_sizes(const LinearArgs& a, const Plan& p, hipStream_t st) {
+  constexpr int N = OPS == 2 ? 2 : 1;
+  if (p.size == 128) return launch_tiles<T, 128, 128 / N, 2, 2, OPS, VEC>(a, st);
+  return launch_tiles<T, 64, 64 / N, 2, 2 / N, OPS, VEC>(a, st);
+}
+
+template <typename T, int OPS>
+hipError_t launch_linear(const LinearArgs& a, const Plan& p, bool vec, hipStream_t st) {
+  if (p.few) return launch_few<T, OPS>(a, p.few, st);
+  return vec ? launch_sizes<T, OPS, true>(a, p, st) : launch_sizes<T, OPS, false>(a, p, st);
+}
+
+template <typename T>
+hipError_t launch_ops(const LinearArgs& a, const Plan& p, bool vec, hipStream_t st) {
+  return a.w[1] ? launch_linear<T, 2>(a, p, vec, st) : launch_linear<T, 1>(a, p, vec, st);
+}
+
+inline bool sizes_make_sense(const CfLinearArgs& x) {
+  return x.dtype >= 0 && x.dtype <= 2 && x.rows >= 0 && x.rows <= CF_LINEAR_MAX_ROWS && x.inner >= 0 &&
+         x.inner <= CF_LINEAR_MAX_WIDTH && x.cols >= 1 && x.cols <= CF_LINEAR_MAX_WIDTH;
+}
+
+}  // namespace
+
+CF_API int64_t cf_linear_workspace(const CfLinearArgs* p) {
+  if (!p || !sizes_make_sense(*p)) return -1;
+  const bool gated = p->w2 != nullptr;
+  return workspace_of(*p, plan_of(*p, gated), gated);
+}
+
+CF_API int cf_linear(const CfLinearArgs* p) {
+  if (!p) return (int)hipErrorInvalidValue;
+  const CfLinearArgs& x = *p;
+  if (!sizes_make_sense(x) || x.activation < 0 || x.activation > CF_ACT_GELU_TANH || x.x_row < 0 ||
+      x.w_row < 0 || x.w2_row < 0 || x.residual_row < 0 || x.out_row < x.cols || x.workspace_bytes < 0)
+    return (int)hipErrorInvalidValue;
+  if (x.rows == 0) return 0;
+  const bool gated = x.w2 != nullptr;
+  if (!x.out || (x.inner > 0 && (!x.x || !x.w)) || (gated && x.residual))
+    return (int)hipErrorInvalidValue;
+  const Plan plan = plan_of(x, gated);
+  const int64_t need = workspace_of(x, plan, gated);
+  if (need > 0 && (!x.workspace || (uintptr_t)x.workspace % 16 != 0 || x.workspace_bytes < need))
+    return (int)hipErrorInvalidValue;
+  LinearArgs a;
+  a.x = x.x;
+  a.w[0] = x.w; a.w[1] = x.w2;
+  a.bias[0] = x.bias; a.bias[1] = x.bias2;
+  a.residual = x.residual;
+  a.out = x.out;
+  a.parts = need > 0 ? (float*)x.workspace : nullptr;
+  a.bias_f32 = x.bias_f32 != 0;
+  a.activation = (int)x.activation;
+  a.rows = x.rows; a.inner = (int)x.inner; a.cols = (int)x.cols;
+  a.xr = x.x_row; a.wr[0] = x.w_row; a.wr[1] = x.w2_row; a.rr = x.residual_row; a.orow = x.out_row;
+  a.splits = plan.splits; a.split_steps = plan.split_steps;
+  a.row_tiles = a.col_tiles = 0;
+  const int size = x.dtype == SEQ_F32 ? 4 : 2, per = 16 / size;
+  // rows of whole 16-byte pieces that do not overlap, 256 of them within 2^31 bytes
+  auto vec = [&](const void* base, int64_t stride) {
+    return (uintptr_t)base % 16 == 0 && stride % per == 0 && stride >= x.inner &&
+           stride * size * 256 < 0x7fffffffll;
+  };
+  const bool v = x.inner % per == 0 && vec(x.x, x.x_row) && vec(x.w, x.w_row) &&
+                 (!gated || vec(x.w2, x.w2_row));
+  hipStream_t st = (hipStream_t)x.stream;
+  hipError_t e;
+  if (x.dtype == SEQ_F32) e = launch_ops<float>(a, plan, v, st);
+  else if (x.dtype == SEQ_F16) e = launch_ops<_Float16>(a, plan, v, st);
+  else e = launch_ops<bf16_t>(a, plan, v, st);
+  return (int)e;
+}

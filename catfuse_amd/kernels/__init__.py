@@ -21,6 +21,10 @@ The delta rule's attention (catfuse_amd.delta):
   delta_attention(q, k, v, beta, log_decay, ...),
                   delta_attention_step(q, k, v, beta, log_decay, state, ...)
 
+Dense products with their epilogue (catfuse_amd.dense):
+  linear(x, w, bias, activation, residual, ...),
+                  gated_linear(x, w_gate, w_up, ...)
+
 Each LIF call starts from the initial membrane state (v = v_reset), like the
 reference's single-block (K = T) launchers, unless a carry tensor is given;
 the `*_lif` tails return (spikes, v_final).  Packed weights are cached by
@@ -30,6 +34,7 @@ from __future__ import annotations
 
 import torch
 
+from catfuse_amd.dense import gated_linear, linear
 from catfuse_amd.delta import delta_attention, delta_attention_step
 from catfuse_amd.runtime import ID_ADD_Z, ConvLIFRunner, avgpool2x2_lif, lif_multistep
 from catfuse_amd.sequence import (decay_attention, decay_attention_step, qk_norm_rotary, rotary,
@@ -140,4 +145,4 @@ def linear_lif(x, w, bias=None, v_carry=None, tau=2.0, v_th=1.0, v_reset=0.0, de
 __all__ = ["partial_fusion_conv_lif", "partial_fusion_conv_bn_lif",
            "partial_fusion_conv_bn_add_lif", "add_lif", "add_bn_lif", "bn_lif", "avgpool_lif",
            "linear_lif", "decay_attention", "decay_attention_step", "qk_norm_rotary", "rotary",
-           "rotary_freqs", "delta_attention", "delta_attention_step"]
+           "rotary_freqs", "delta_attention", "delta_attention_step", "linear", "gated_linear"]

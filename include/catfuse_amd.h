@@ -948,6 +948,39 @@ typedef struct CfRotaryArgs {
 } CfRotaryArgs;
 int cf_rotary(const CfRotaryArgs* args);
 
+/* Dense products with their epilogue, x [rows][inner], w (and w2) [cols][inner],
+ * out [rows][cols], fp32 sums:
+ *   out = act(x w^T + bias) + residual          (w2 null; bias, residual nullable)
+ *   out = act(x w^T + bias) * (x w2^T + bias2)  (residual null)
+ * Rows are *_row elements apart (0 and overlaps allowed for inputs), elements of
+ * a row on end; bias and bias2 [cols] fp32 (bias_f32) or of dtype.  out may be
+ * the residual itself (the same rows) and must not overlap the inputs otherwise.
+ * Small products are split along the inner dimension: the workspace (16-byte
+ * aligned) has at least the bytes that cf_linear_workspace gives for the same
+ * block (0: none is needed, -1: the sizes make no sense). */
+#define CF_LINEAR_MAX_ROWS 1000000000
+#define CF_LINEAR_MAX_WIDTH 16000000
+#define CF_ACT_NONE 0
+#define CF_ACT_RELU 1
+#define CF_ACT_SILU 2
+#define CF_ACT_GELU 3
+#define CF_ACT_GELU_TANH 4
+typedef struct CfLinearArgs {
+  const void* x;
+  const void* w;
+  const void* w2;
+  const void* bias;
+  const void* bias2;
+  const void* residual;
+  void* out;
+  void* workspace;
+  void* stream;
+  int64_t dtype, bias_f32, activation, rows, inner, cols;
+  int64_t x_row, w_row, w2_row, residual_row, out_row, workspace_bytes;
+} CfLinearArgs;
+int64_t cf_linear_workspace(const CfLinearArgs* args);
+int cf_linear(const CfLinearArgs* args);
+
 /* Diagnostic: one wave computes D(32x32 fp32) = A(32x16 fp16) * B(16x32
  * fp16) through the matrix-core lane mapping cf_conv_mfma relies on.
  * No reference counterpart (layout self-test). */
