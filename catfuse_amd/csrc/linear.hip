@@ -98,14 +98,21 @@ __device__ __forceinline__ float exp_f(float x) {
 __device__ __forceinline__ float sigmoid_times(float z, float t) {   // z / (1 + e^-t)
   return z * __builtin_amdgcn_rcpf(1.0f + exp_f(-t));
 }
-__device__ __forceinline__ float activate(float z, int kind) {
-  switch (kind) {
-    case CF_ACT_RELU: return z < 0.0f ? 0.0f : z;
-    case CF_ACT_SILU: return sigmoid_times(z, z);
-    case CF_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.707106781f));
-    case CF_ACT_GELU_TANH:     // 1 + tanh(t) = 2 / (1 + e^(-2 t))
-      return sigmoid_times(z, 1.59576912f * __builtin_fmaf(0.044715f * z * z, z, z));
-    default: return z;
+template <int N>
+__device__ __forceinline__ void activate(float* z, int kind) {
+  if (kind == CF_ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) z[j] = z[j] < 0.0f ? 0.0f : z[j];
+  } else if (kind == CF_ACT_SILU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) z[j] = sigmoid_times(z[j], z[j]);
+  } else if (kind == CF_ACT_GELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) z[j] = 0.5f * z[j] * (1.0f + erff(z[j] * 0.707106781f));
+  } else if (kind == CF_ACT_GELU_TANH) {     // 1 + tanh(t) = 2 / (1 + e^(-2 t))
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      z[j] = sigmoid_times(z[j], 1.59576912f * __builtin_fmaf(0.044715f * z[j] * z[j], z[j], z[j]));
   }
 }
 
@@ -116,51 +123,92 @@ __device__ __forceinline__ float bias_of(const LinearArgs& a, int op, int n) {
                     : to_f(reinterpret_cast<const T*>(a.bias[op])[n]);
 }
 
-// Four outputs of a row, columns n .. n + 3, from the sums s[product][4]; those
-// from cols on are left alone.  wide: four on end are aligned and whole.
-template <typename T, int OPS>
-__device__ __forceinline__ void finish4(const LinearArgs& a, int64_t m, int n, const float (*s)[4],
-                                        bool wide) {
-  if (n >= a.cols) return;
-  float y[4], r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+// Outputs of a row, columns n .. n + 7 (COUNT of them), from the sums and the
+// biases of each product; those from cols on are left alone.  wide: eight on end,
+// from a multiple of eight, are aligned and whole.  given: the residual, if the
+// caller has it.
+template <typename T, int OPS, int COUNT>
+__device__ __forceinline__ void finish(const LinearArgs& a, int64_t m, int n, const float (*s)[COUNT],
+                                       const float (*b)[COUNT], const Vec<T, COUNT>& given, bool have, bool wide) {
+  float y[COUNT], r[COUNT];
+  constexpr int PER = COUNT * sizeof(T) > 16 ? 16 / sizeof(T) : COUNT;   // of an access
   T* const to = (T*)a.out + m * a.orow + n;
+#pragma unroll
+  for (int j = 0; j < COUNT; ++j) r[j] = 0.0f;
   if (OPS == 1 && a.residual != nullptr) {
     const T* const from = (const T*)a.residual + m * a.rr + n;
-    if (wide) {
-      const Vec<T, 4> v = *reinterpret_cast<const Vec<T, 4>*>(from);
+    if (have) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r[j] = to_f(v.v[j]);
+      for (int j = 0; j < COUNT; ++j) r[j] = to_f(given.v[j]);
+    } else if (wide) {
+#pragma unroll
+      for (int i = 0; i < COUNT; i += PER) {
+        const Vec<T, PER> v = *reinterpret_cast<const Vec<T, PER>*>(from + i);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) r[i + j] = to_f(v.v[j]);
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < COUNT; ++j)
         if (n + j < a.cols) r[j] = to_f(from[j]);
     }
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int c = n + j < a.cols ? n + j : a.cols - 1;
-    y[j] = activate(s[0][j] + bias_of<T>(a, 0, c), a.activation);
-    if constexpr (OPS == 2) y[j] *= s[1][j] + bias_of<T>(a, 1, c);
+  for (int j = 0; j < COUNT; ++j) y[j] = s[0][j] + b[0][j];
+  activate<COUNT>(y, a.activation);
+#pragma unroll
+  for (int j = 0; j < COUNT; ++j) {
+    if constexpr (OPS == 2) y[j] *= s[1][j] + b[1][j];
     else y[j] += r[j];
   }
   if (wide) {
-    Vec<T, 4> v;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v.v[j] = from_f<T>(y[j]);
-    *reinterpret_cast<Vec<T, 4>*>(to) = v;
+    for (int i = 0; i < COUNT; i += PER) {
+      Vec<T, PER> v;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) v.v[j] = from_f<T>(y[i + j]);
+      *reinterpret_cast<Vec<T, PER>*>(to + i) = v;
+    }
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < COUNT; ++j)
       if (n + j < a.cols) to[j] = from_f<T>(y[j]);
   }
 }
 
-// Whether four columns on end, from a multiple of four, are aligned and whole.
+// The same of eight, or the sums themselves to the workspace.
+template <typename T, int OPS>
+__device__ __forceinline__ void finish8(const LinearArgs& a, int64_t m, int n, int split,
+                                        const float (*s)[8], const float (*b)[8],
+                                        const Vec<T, 8>& given, bool have, bool wide) {
+  if (a.parts == nullptr) {
+    finish<T, OPS, 8>(a, m, n, s, b, given, have, wide);
+    return;
+  }
+#pragma unroll
+  for (int o = 0; o < OPS; ++o) {
+    float* const to = a.parts + (((int64_t)split * OPS + o) * a.rows + m) * a.cols + n;
+    if (a.cols % 8 == 0) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const Vec<float, 4> v = {s[o][e], s[o][e + 1], s[o][e + 2], s[o][e + 3]};
+        *reinterpret_cast<Vec<float, 4>*>(to + e) = v;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (n + e < a.cols) to[e] = s[o][e];
+    }
+  }
+}
+
+// Whether eight columns on end, from a multiple of eight, are aligned (to 16
+// bytes; four of 16 bits to 8) and whole.
 template <typename T>
 __device__ __forceinline__ bool wide_columns(const LinearArgs& a) {
-  const uintptr_t by = 4 * sizeof(T) - 1;
-  return a.cols % 4 == 0 && a.orow % 4 == 0 && ((uintptr_t)a.out & by) == 0 &&
-         (a.residual == nullptr || (a.rr % 4 == 0 && ((uintptr_t)a.residual & by) == 0));
+  constexpr int PER = 16 / sizeof(T);
+  return a.cols % 8 == 0 && a.orow % PER == 0 && ((uintptr_t)a.out & 15) == 0 &&
+         (a.residual == nullptr || (a.rr % PER == 0 && ((uintptr_t)a.residual & 15) == 0));
 }
 
 // Few rows of x: bound by the bytes of w, each read once.  A workgroup takes 16
@@ -241,7 +289,15 @@ __global__ __launch_bounds__(64 * NW) void linear_few_kernel(LinearArgs a) {
         y[o][j] = z;
       }
     const int64_t m = 16 * t + row;
-    if (m < a.rows) finish4<T, OPS>(a, m, n0 + 4 * quarter, y, wide);
+    const int n = n0 + 4 * quarter;
+    if (m < a.rows && n < a.cols) {
+      float b[OPS][4];
+#pragma unroll
+      for (int o = 0; o < OPS; ++o)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[o][j] = bias_of<T>(a, o, n + j < a.cols ? n + j : a.cols - 1);
+      finish<T, OPS, 4>(a, m, n, y, b, {}, false, wide);
+    }
   }
 }
 
@@ -256,7 +312,7 @@ __device__ __forceinline__ void copy16(i32x4 rsrc, uint32_t at, uint32_t add, ui
       "buffer_load_dwordx4 %0, %1, %2 offen lds"
       :
       : "v"(at), "s"(rsrc), "s"(add), "s"(lds)
-      : "memory", "m0");
+      : "memory");
 }
 __device__ __forceinline__ i32x4 buffer_of(const void* base, uint32_t bytes) {
   const uint64_t p = (uint64_t)(uintptr_t)base;
@@ -269,23 +325,32 @@ __device__ __forceinline__ i32x4 buffer_of(const void* base, uint32_t bytes) {
 }
 
 // Many rows.  A workgroup takes BM rows of x and BN columns, in steps of 128
-// bytes of the inner dimension; two stages of LDS, the next step's rows copied
-// while the present one's are multiplied.  Waves WM x WN, each BM / WM rows and
-// BN / WN columns: results as accumulators of 32 columns (their rows) by 32 rows
-// of x (their columns), so that a lane holds four columns on end.
+// bytes of the inner dimension, two stages of LDS.  Waves WM x WN, each BM / WM
+// rows and BN / WN columns of each product: results as accumulators of 32 columns
+// (their rows) by 32 rows of x (their columns).
+//
+// A step has four parts (32 bytes of a row for a lane pair).  A part's operands
+// are read from LDS between the products of the part before; before a step's last
+// products the waves meet, when all its operands are in registers and the next
+// stage's copies have landed: the last products then cover the first reads of
+// that stage and the start of the copies into the stage just read.
 //
 // LDS rows of 128 bytes, their eight pieces exchanged by row (piece ^ row % 8),
 // which spreads both the copies' and the operands' accesses over all banks.
 //
-// VEC: rows in pieces of 16 bytes, aligned and whole, not overlapping; else
-// through registers, element by element at the inner dimension's end.
+// VEC: rows in pieces of 16 bytes, aligned and whole, not overlapping, copied
+// straight to LDS; else through registers, element by element at the inner
+// dimension's end.
 template <typename T, int BM, int BN, int WM, int WN, int OPS, bool VEC>
-__global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinearArgs a) {
-  constexpr int NW = WM * WN, NT = 64 * NW, PER = 16 / sizeof(T), STEP = 8 * PER;
+__global__ __launch_bounds__(64 * WM * WN, BM >= 256 ? 1 : 2) void linear_tile_kernel(LinearArgs a) {
+  constexpr int NW = WM * WN, PER = 16 / sizeof(T), STEP = 8 * PER;
   constexpr int ROWS = BM + OPS * BN, STAGE = ROWS * 128;
-  constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
+  constexpr int TM = BM / WM / 32, TN = BN / WN / 32, WIDE = OPS * TN * 32;
   static_assert(ROWS % (8 * NW) == 0 && BM % 8 == 0 && BN % 8 == 0, "whole copies");
-  __shared__ __attribute__((aligned(1024))) char lds[2 * STAGE];
+  // the epilogue turns 32 rows of a wave's results at a time
+  constexpr int PITCH = WIDE + 4, TURN = 32 * PITCH * 4;
+  constexpr int LDS = 2 * STAGE > NW * TURN ? 2 * STAGE : NW * TURN;
+  __shared__ __attribute__((aligned(1024))) char lds[LDS];
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
 
@@ -307,123 +372,177 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_tile_kernel(LinearArgs a)
   const int from = split * a.split_steps;
   const int steps = steps_all - from < a.split_steps ? steps_all - from : a.split_steps;
 
-  // What this thread copies: rows r0 + 8 NW i of the stage, piece lane % 8
-  const int r0 = 8 * wave + (lane >> 3), piece = lane & 7;
+  // What this thread copies: rows 8 wave + lane / 8 + 8 NW i of the stage (a
+  // copy's eight rows are all of one operand), piece lane % 8.
+  const int piece = (lane & 7) ^ (lane >> 3);
   constexpr int COPIES = ROWS / (8 * NW);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-  const int64_t rows_left = a.rows - m0;
-  const int cols_left = a.cols - n0;
   i32x4 xb, wb[OPS];
+  uint32_t at[VEC ? COPIES : 1];             // rows beyond x's and w's: out of the buffers' ranges
   if constexpr (VEC) {
-    const int64_t rn = rows_left < BM ? rows_left : BM, cn = cols_left < BN ? cols_left : BN;
+    const int64_t rn = a.rows - m0 < BM ? a.rows - m0 : BM, cn = a.cols - n0 < BN ? a.cols - n0 : BN;
     xb = buffer_of((const T*)a.x + m0 * a.xr, (uint32_t)(((rn - 1) * a.xr + a.inner) * sizeof(T)));
 #pragma unroll
     for (int o = 0; o < OPS; ++o)
       wb[o] = buffer_of((const T*)a.w[o] + n0 * a.wr[o],
                         (uint32_t)(((cn - 1) * a.wr[o] + a.inner) * sizeof(T)));
-  }
-  u32x4 regs[VEC ? 1 : COPIES];
-  // Rows beyond x's and w's: out of the buffers' ranges.  (A copy's eight rows
-  // are all of one operand.)
-  auto fetch = [&](int stage, int step) {
-    const int k = (from + step) * STEP + (piece ^ (r0 & 7)) * PER;
 #pragma unroll
     for (int i = 0; i < COPIES; ++i) {
-      const int base = 8 * wave + 8 * NW * i, r = base + (lane >> 3);   // (base: the same in every lane)
-      if constexpr (VEC) {
-        const bool is_x = base < BM;
-        const int o = OPS == 2 && base >= BM + BN ? 1 : 0;
-        const int row = is_x ? r : r - BM - o * BN;
-        const int64_t stride = is_x ? a.xr : a.wr[o];
-        uint32_t at = (uint32_t)(row * (int)stride * (int)sizeof(T)) + (uint32_t)((piece ^ (r & 7)) * 16);
-        if (k >= a.inner) at = 0x80000000u;
-        copy16(is_x ? xb : wb[o], at, (uint32_t)((from + step) * 128), lds0 + stage * STAGE + base * 128);
-      } else {
-        const bool is_x = base < BM;
-        const int o = OPS == 2 && base >= BM + BN ? 1 : 0;
-        int64_t row = is_x ? m0 + r : n0 + r - BM - o * BN;
-        const int64_t end = is_x ? a.rows : a.cols;
-        row = row < end ? row : end - 1;     // (its results are not stored)
-        const T* const p = (is_x ? (const T*)a.x + row * a.xr : (const T*)a.w[o] + row * a.wr[o]) + k;
-        regs[i] = k + PER <= a.inner ? load16(p) : load_some(p, a.inner - k);
-      }
+      const int base = 8 * wave + 8 * NW * i;
+      const int o = OPS == 2 && base >= BM + BN ? 1 : 0;
+      const int row = base + (lane >> 3) - (base < BM ? 0 : BM + o * BN);
+      at[i] = (uint32_t)(row * (int)(base < BM ? a.xr : a.wr[o]) * (int)sizeof(T) + piece * 16);
     }
+  }
+  u32x4 regs[VEC ? 1 : COPIES];
+  auto fetch = [&](int stage, int step, int i) {
+    const int base = 8 * wave + 8 * NW * i, k = (from + step) * STEP + piece * PER;
+    const int o = OPS == 2 && base >= BM + BN ? 1 : 0;
+    if constexpr (VEC) {
+      copy16(base < BM ? xb : wb[o], k < a.inner ? at[i] : 0x80000000u, (uint32_t)((from + step) * 128),
+             lds0 + stage * STAGE + base * 128);
+    } else {
+      const int r = base + (lane >> 3);
+      int64_t row = base < BM ? m0 + r : n0 + r - BM - o * BN;
+      const int64_t end = base < BM ? a.rows : a.cols;
+      row = row < end ? row : end - 1;       // (its results are not stored)
+      const T* const p = (base < BM ? (const T*)a.x + row * a.xr : (const T*)a.w[o] + row * a.wr[o]) + k;
+      regs[i] = k + PER <= a.inner ? load16(p) : load_some(p, a.inner - k);
+    }
+  };
+  auto fetch_all = [&](int stage, int step) {
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) fetch(stage, step, i);
   };
   auto deposit = [&](int stage) {
     if constexpr (!VEC) {
 #pragma unroll
-      for (int i = 0; i < COPIES; ++i) {
-        const int r = 8 * wave + 8 * NW * i + (lane >> 3);
-        *reinterpret_cast<u32x4*>(lds + stage * STAGE + r * 128 + piece * 16) = regs[i];
-      }
+      for (int i = 0; i < COPIES; ++i)
+        *reinterpret_cast<u32x4*>(lds + stage * STAGE + (8 * wave + 8 * NW * i) * 128 + lane * 16) = regs[i];
     }
   };
+  auto meet = [&]() {                        // copies have landed, reads are done
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
 
-  f16v acc[OPS][TN][TM];
+  f16v acc[OPS * TN][TM];
 #pragma unroll
-  for (int o = 0; o < OPS; ++o)
+  for (int i = 0; i < OPS * TN; ++i)
 #pragma unroll
-    for (int i = 0; i < TN; ++i)
-#pragma unroll
-      for (int j = 0; j < TM; ++j) acc[o][i][j] = f16v{};
+    for (int j = 0; j < TM; ++j) acc[i][j] = f16v{};
 
   const char* const xs = lds + (wm * (BM / WM) + col) * 128;
   const char* const ws = lds + (BM + wn * (BN / WN) + col) * 128;
-  fetch(0, 0);
-  deposit(0);
+  constexpr int READS = TM + OPS * TN, PRODUCTS = TM * OPS * TN;
+  u32x4 xv[2][TM], wv[2][OPS * TN];
+  auto read = [&](int stage, int s, int i) {
+    const int off = stage * STAGE + (((2 * s + hi) ^ (col & 7)) << 4);
+    if (i < TM) xv[s & 1][i] = *reinterpret_cast<const u32x4*>(xs + i * 32 * 128 + off);
+    else wv[s & 1][i - TM] =
+        *reinterpret_cast<const u32x4*>(ws + ((i - TM) / TN * BN + (i - TM) % TN * 32) * 128 + off);
+  };
+
+  // Results: 32 rows at a time turned through LDS, each wave for itself, so that
+  // eight columns on end of a row are a lane's and a row's lanes lie on end.  The
+  // residual's first rows are loaded here, the others AHEAD turns before they are
+  // added: with one workgroup a CU nothing else would cover their way.
+  float* const turn = reinterpret_cast<float*>(lds + wave * TURN);
+  constexpr int LANES = TN * 4, PARTS = 32 * LANES / 64, TURNS = TM * PARTS;   // LANES of a row
+  constexpr int AHEAD = TURNS < 16 / (int)sizeof(T) ? TURNS : 16 / (int)sizeof(T);
+  const int nc = lane % LANES * 8, n = n0 + wn * (BN / WN) + nc;
+  const int64_t mt = m0 + wm * (BM / WM) + lane / LANES;
+  const bool wide = wide_columns<T>(a);
+  const bool early = OPS == 1 && wide && a.residual != nullptr && a.parts == nullptr;
+  auto residual_at = [&](int t) {
+    const int64_t m = mt + t * (64 / LANES);
+    return *reinterpret_cast<const Vec<T, 8>*>((const T*)a.residual + (m < a.rows ? m : a.rows - 1) * a.rr +
+                                               (n < a.cols ? n : 0));
+  };
+  Vec<T, 8> ahead[AHEAD];
+  if (early) {
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) ahead[d] = residual_at(d);
+  }
+  float b[OPS][8];
+#pragma unroll
+  for (int o = 0; o < OPS; ++o)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[o][e] = bias_of<T>(a, o, n + e < a.cols ? n + e : a.cols - 1);
+
+  if (steps > 0) {
+    fetch_all(0, 0);
+    deposit(0);
+    meet();
+    if (steps > 1) fetch_all(1, 1);
+#pragma unroll
+    for (int i = 0; i < READS; ++i) read(0, 0, i);
+  }
   for (int step = 0; step < steps; ++step) {
-    if constexpr (VEC) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
     const int stage = step & 1;
-    if (step + 1 < steps) fetch(stage ^ 1, step + 1);
+    const bool more = step + 1 < steps, two = step + 2 < steps;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      const int at = stage * STAGE + (((2 * s + hi) ^ (col & 7)) << 4);
-      u32x4 xv[TM], wv[OPS][TN];
-#pragma unroll
-      for (int j = 0; j < TM; ++j) xv[j] = *reinterpret_cast<const u32x4*>(xs + j * 32 * 128 + at);
-#pragma unroll
-      for (int o = 0; o < OPS; ++o)
-#pragma unroll
-        for (int i = 0; i < TN; ++i)
-          wv[o][i] = *reinterpret_cast<const u32x4*>(ws + (o * BN + i * 32) * 128 + at);
-#pragma unroll
-      for (int o = 0; o < OPS; ++o)
-#pragma unroll
-        for (int i = 0; i < TN; ++i)
-#pragma unroll
-          for (int j = 0; j < TM; ++j) acc[o][i][j] = mfma32<T>(wv[o][i], xv[j], acc[o][i][j]);
-    }
-    if (step + 1 < steps) deposit(stage ^ 1);
-  }
-
-  const bool wide = wide_columns<T>(a);
-#pragma unroll
-  for (int j = 0; j < TM; ++j) {
-    const int64_t m = m0 + wm * (BM / WM) + 32 * j + col;
-    if (m >= a.rows) continue;
-#pragma unroll
-    for (int i = 0; i < TN; ++i)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int n = n0 + wn * (BN / WN) + 32 * i + 8 * g + 4 * hi;
-        float y[OPS][4];
-#pragma unroll
-        for (int o = 0; o < OPS; ++o)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) y[o][e] = acc[o][i][j][4 * g + e];
-        if (a.parts == nullptr) {
-          finish4<T, OPS>(a, m, n, y, wide);
-        } else {
-#pragma unroll
-          for (int o = 0; o < OPS; ++o) {
-            float* const to = a.parts + (((int64_t)split * OPS + o) * a.rows + m) * a.cols + n;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (n + e < a.cols) to[e] = y[o][e];
-          }
-        }
+      if (s == 3) {
+        if (more) deposit(stage ^ 1);
+        meet();
       }
+#pragma unroll
+      for (int p = 0; p < PRODUCTS; ++p) {
+        const int i = p / TM, j = p % TM;
+        acc[i][j] = mfma32<T>(wv[s & 1][i], xv[s & 1][j], acc[i][j]);
+        // spread over the products: the next part's reads, and in the last part
+        // the copies of the stage after the next
+#pragma unroll
+        for (int r = p * READS / PRODUCTS; r < (p + 1) * READS / PRODUCTS; ++r) {
+          if (s < 3) read(stage, s + 1, r);
+          else if (more) read(stage ^ 1, 0, r);
+        }
+        if (s == 3 && two)
+#pragma unroll
+          for (int c = p * COPIES / PRODUCTS; c < (p + 1) * COPIES / PRODUCTS; ++c) fetch(stage, step + 2, c);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  meet();                                    // LDS is free for the results
+#pragma unroll 1
+  for (int t = 0; t < TURNS; ++t) {
+    if (t % PARTS == 0) {
+#pragma unroll
+      for (int j = 0; j < TM; ++j)
+        if (t == j * PARTS) {
+#pragma unroll
+          for (int i = 0; i < OPS * TN; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              Vec<float, 4> y;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y.v[e] = acc[i][j][4 * g + e];
+              *reinterpret_cast<Vec<float, 4>*>(turn + col * PITCH + 32 * i + 8 * g + 4 * hi) = y;
+            }
+        }
+    }
+    const int r = t % PARTS * (64 / LANES) + lane / LANES;
+    const int64_t m = mt + t * (64 / LANES);
+    float y[OPS][8];
+#pragma unroll
+    for (int o = 0; o < OPS; ++o)
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const Vec<float, 4> v =
+            *reinterpret_cast<const Vec<float, 4>*>(turn + r * PITCH + o * TN * 32 + nc + e);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) y[o][e + f] = v.v[f];
+      }
+    const Vec<T, 8> now = ahead[0];
+    if (early) {
+#pragma unroll
+      for (int d = 0; d + 1 < AHEAD; ++d) ahead[d] = ahead[d + 1];
+      if (t + AHEAD < TURNS) ahead[AHEAD - 1] = residual_at(t + AHEAD);
+    }
+    if (m < a.rows && n < a.cols) finish8<T, OPS>(a, m, n, split, y, b, now, early, wide);
   }
 }
 
@@ -448,7 +567,12 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a) {
       for (int e = 0; e < 4; ++e)
         if (n + e < a.cols) y[o][e] += from[e];
     }
-  finish4<T, OPS>(a, m, n, y, wide_columns<T>(a));
+  float b[OPS][4];
+#pragma unroll
+  for (int o = 0; o < OPS; ++o)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[o][e] = bias_of<T>(a, o, n + e < a.cols ? n + e : a.cols - 1);
+  finish<T, OPS, 4>(a, m, n, y, b, {}, false, wide_columns<T>(a));
 }
 
 // How a product is taken.
@@ -457,7 +581,7 @@ struct Plan { int few, size, splits, split_steps; };   // few: waves of the few-
 constexpr int FEW_ROWS = 32;
 constexpr int CUS = 256;
 
-inline Plan plan_of(const CfLinearArgs& x, bool gated) {
+inline Plan plan_of(const CfLinearArgs& x, bool gated, bool vec) {
   Plan p = {0, 0, 1, 0};
   const int64_t step = x.dtype == SEQ_F32 ? 32 : 64, steps = (x.inner + step - 1) / step;
   if (x.rows <= FEW_ROWS) {
@@ -467,9 +591,9 @@ inline Plan plan_of(const CfLinearArgs& x, bool gated) {
   auto tiles = [&](int64_t bm, int64_t bn) {
     return ((x.rows + bm - 1) / bm) * ((x.cols + bn - 1) / bn);
   };
-  const int big = gated ? 64 : 128;
-  p.size = tiles(128, big) >= CUS ? 128 : 64;
-  const int64_t n = p.size == 128 ? tiles(128, big) : tiles(64, gated ? 32 : 64);
+  const int half = gated ? 2 : 1;
+  p.size = vec && tiles(256, 256 / half) >= CUS ? 256 : tiles(128, 128 / half) >= CUS ? 128 : 64;
+  const int64_t n = tiles(p.size, p.size / half);
   if (n < CUS && steps >= 16) {
     int64_t splits = CUS / n;
     if (splits > steps / 8) splits = steps / 8;
@@ -517,6 +641,8 @@ hipError_t launch_tiles(LinearArgs a, hipStream_t st) {
 template <typename T, int OPS, bool VEC>
 hipError_t launch_sizes(const LinearArgs& a, const Plan& p, hipStream_t st) {
   constexpr int N = OPS == 2 ? 2 : 1;
+  if constexpr (VEC)
+    if (p.size == 256) return launch_tiles<T, 256, 256 / N, 2, 2, OPS, true>(a, st);
   if (p.size == 128) return launch_tiles<T, 128, 128 / N, 2, 2, OPS, VEC>(a, st);
   return launch_tiles<T, 64, 64 / N, 2, 2 / N, OPS, VEC>(a, st);
 }
@@ -532,6 +658,19 @@ hipError_t launch_ops(const LinearArgs& a, const Plan& p, bool vec, hipStream_t 
   return a.w[1] ? launch_linear<T, 2>(a, p, vec, st) : launch_linear<T, 1>(a, p, vec, st);
 }
 
+// Whether x and w have rows of whole aligned 16-byte pieces that do not overlap,
+// 256 of them within 2^31 bytes.  (The plan of a workspace's size takes addresses
+// for aligned: the plans differ in splits only where there are few tiles, which
+// the tile of 256 never is for.)
+inline bool whole_pieces(const CfLinearArgs& x) {
+  const int size = x.dtype == SEQ_F32 ? 4 : 2, per = 16 / size;
+  auto vec = [&](const void* base, int64_t stride) {
+    return (uintptr_t)base % 16 == 0 && stride % per == 0 && stride >= x.inner &&
+           stride * size * 256 < 0x7fffffffll;
+  };
+  return x.inner % per == 0 && vec(x.x, x.x_row) && vec(x.w, x.w_row) && (!x.w2 || vec(x.w2, x.w2_row));
+}
+
 inline bool sizes_make_sense(const CfLinearArgs& x) {
   return x.dtype >= 0 && x.dtype <= 2 && x.rows >= 0 && x.rows <= CF_LINEAR_MAX_ROWS && x.inner >= 0 &&
          x.inner <= CF_LINEAR_MAX_WIDTH && x.cols >= 1 && x.cols <= CF_LINEAR_MAX_WIDTH;
@@ -542,7 +681,7 @@ inline bool sizes_make_sense(const CfLinearArgs& x) {
 CF_API int64_t cf_linear_workspace(const CfLinearArgs* p) {
   if (!p || !sizes_make_sense(*p)) return -1;
   const bool gated = p->w2 != nullptr;
-  return workspace_of(*p, plan_of(*p, gated), gated);
+  return workspace_of(*p, plan_of(*p, gated, true), gated);
 }
 
 CF_API int cf_linear(const CfLinearArgs* p) {
@@ -555,7 +694,8 @@ CF_API int cf_linear(const CfLinearArgs* p) {
   const bool gated = x.w2 != nullptr;
   if (!x.out || (x.inner > 0 && (!x.x || !x.w)) || (gated && x.residual))
     return (int)hipErrorInvalidValue;
-  const Plan plan = plan_of(x, gated);
+  const bool v = whole_pieces(x);
+  const Plan plan = plan_of(x, gated, v);
   const int64_t need = workspace_of(x, plan, gated);
   if (need > 0 && (!x.workspace || (uintptr_t)x.workspace % 16 != 0 || x.workspace_bytes < need))
     return (int)hipErrorInvalidValue;
@@ -572,14 +712,6 @@ CF_API int cf_linear(const CfLinearArgs* p) {
   a.xr = x.x_row; a.wr[0] = x.w_row; a.wr[1] = x.w2_row; a.rr = x.residual_row; a.orow = x.out_row;
   a.splits = plan.splits; a.split_steps = plan.split_steps;
   a.row_tiles = a.col_tiles = 0;
-  const int size = x.dtype == SEQ_F32 ? 4 : 2, per = 16 / size;
-  // rows of whole 16-byte pieces that do not overlap, 256 of them within 2^31 bytes
-  auto vec = [&](const void* base, int64_t stride) {
-    return (uintptr_t)base % 16 == 0 && stride % per == 0 && stride >= x.inner &&
-           stride * size * 256 < 0x7fffffffll;
-  };
-  const bool v = x.inner % per == 0 && vec(x.x, x.x_row) && vec(x.w, x.w_row) &&
-                 (!gated || vec(x.w2, x.w2_row));
   hipStream_t st = (hipStream_t)x.stream;
   hipError_t e;
   if (x.dtype == SEQ_F32) e = launch_ops<float>(a, plan, v, st);

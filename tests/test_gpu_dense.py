@@ -98,7 +98,8 @@ def test_shapes(cuda, dtype, M, K, N, gated):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("M,K,N", [(2000, 600, 1100), (4100, 256, 2050), (513, 4096, 520)])
+@pytest.mark.parametrize("M,K,N", [(2000, 600, 1100), (4100, 256, 2050), (513, 4096, 520),
+                                   (4100, 328, 4200), (8200, 72, 2056)])
 @pytest.mark.parametrize("gated", [False, True])
 def test_large(cuda, dtype, M, K, N, gated):
     x, ws, bs, r = _make(cuda, M, K, N, dtype, M, gated, dtype, residual=not gated)
