@@ -98,6 +98,16 @@ __device__ __forceinline__ float exp_f(float x) {
 __device__ __forceinline__ float sigmoid_times(float z, float t) {   // z / (1 + e^-t)
   return z * __builtin_amdgcn_rcpf(1.0f + exp_f(-t));
 }
+// 1 + erf(x / sqrt(2)) by Abramowitz and Stegun's formula 7.1.26, to 1.5e-7.
+__device__ __forceinline__ float one_plus_erf(float x) {
+  const float y = __builtin_fabsf(x) * 0.707106781f, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, y, 1.0f));
+  float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+  p = __builtin_fmaf(p, t, 1.421413741f);
+  p = __builtin_fmaf(p, t, -0.284496736f);
+  p = __builtin_fmaf(p, t, 0.254829592f) * t;
+  const float tail = p * __builtin_amdgcn_exp2f(y * y * -1.44269504f);    // 1 - erf(y)
+  return x < 0.0f ? tail : 2.0f - tail;
+}
 template <int N>
 __device__ __forceinline__ void activate(float* z, int kind) {
   if (kind == CF_ACT_RELU) {
@@ -108,7 +118,7 @@ __device__ __forceinline__ void activate(float* z, int kind) {
     for (int j = 0; j < N; ++j) z[j] = sigmoid_times(z[j], z[j]);
   } else if (kind == CF_ACT_GELU) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) z[j] = 0.5f * z[j] * (1.0f + erff(z[j] * 0.707106781f));
+    for (int j = 0; j < N; ++j) z[j] = 0.5f * z[j] * one_plus_erf(z[j]);
   } else if (kind == CF_ACT_GELU_TANH) {     // 1 + tanh(t) = 2 / (1 + e^(-2 t))
 #pragma unroll
     for (int j = 0; j < N; ++j)
@@ -325,9 +335,10 @@ __device__ __forceinline__ i32x4 buffer_of(const void* base, uint32_t bytes) {
 }
 
 // Many rows.  A workgroup takes BM rows of x and BN columns, in steps of 128
-// bytes of the inner dimension, two stages of LDS.  Waves WM x WN, each BM / WM
-// rows and BN / WN columns of each product: results as accumulators of 32 columns
-// (their rows) by 32 rows of x (their columns).
+// bytes of the inner dimension (whole lines: half as many a step, four stages,
+// took 642 us where this takes 570, 16384 x 4096 x 4096 bf16), two stages of LDS.
+// Waves WM x WN, each BM / WM rows and BN / WN columns of each product: results as
+// accumulators of 32 columns (their rows) by 32 rows of x (their columns).
 //
 // A step has four parts (32 bytes of a row for a lane pair).  A part's operands
 // are read from LDS between the products of the part before; before a step's last
@@ -335,18 +346,18 @@ __device__ __forceinline__ i32x4 buffer_of(const void* base, uint32_t bytes) {
 // stage's copies have landed: the last products then cover the first reads of
 // that stage and the start of the copies into the stage just read.
 //
-// LDS rows of 128 bytes, their eight pieces exchanged by row (piece ^ row % 8),
-// which spreads both the copies' and the operands' accesses over all banks.
+// LDS rows of 128 bytes, their eight pieces exchanged by row (piece ^ row / 2 % 8):
+// sixteen rows on end then spread over all 64 banks.
 //
 // VEC: rows in pieces of 16 bytes, aligned and whole, not overlapping, copied
 // straight to LDS; else through registers, element by element at the inner
 // dimension's end.
 template <typename T, int BM, int BN, int WM, int WN, int OPS, bool VEC>
-__global__ __launch_bounds__(64 * WM * WN, BM >= 256 ? 1 : 2) void linear_tile_kernel(LinearArgs a) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile_kernel(LinearArgs a) {
   constexpr int NW = WM * WN, PER = 16 / sizeof(T), STEP = 8 * PER;
   constexpr int ROWS = BM + OPS * BN, STAGE = ROWS * 128;
   constexpr int TM = BM / WM / 32, TN = BN / WN / 32, WIDE = OPS * TN * 32;
-  static_assert(ROWS % (8 * NW) == 0 && BM % 8 == 0 && BN % 8 == 0, "whole copies");
+  static_assert(ROWS % (8 * NW) == 0 && BM % 8 == 0 && BN % 8 == 0 && NW % 2 == 0, "whole copies");
   // the epilogue turns 32 rows of a wave's results at a time
   constexpr int PITCH = WIDE + 4, TURN = 32 * PITCH * 4;
   constexpr int LDS = 2 * STAGE > NW * TURN ? 2 * STAGE : NW * TURN;
@@ -373,8 +384,8 @@ __global__ __launch_bounds__(64 * WM * WN, BM >= 256 ? 1 : 2) void linear_tile_k
   const int steps = steps_all - from < a.split_steps ? steps_all - from : a.split_steps;
 
   // What this thread copies: rows 8 wave + lane / 8 + 8 NW i of the stage (a
-  // copy's eight rows are all of one operand), piece lane % 8.
-  const int piece = (lane & 7) ^ (lane >> 3);
+  // copy's eight rows are all of one operand), place lane % 8.
+  const int piece = (lane & 7) ^ (((8 * wave + (lane >> 3)) >> 1) & 7);
   constexpr int COPIES = ROWS / (8 * NW);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   i32x4 xb, wb[OPS];
@@ -438,7 +449,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM >= 256 ? 1 : 2) void linear_tile_k
   constexpr int READS = TM + OPS * TN, PRODUCTS = TM * OPS * TN;
   u32x4 xv[2][TM], wv[2][OPS * TN];
   auto read = [&](int stage, int s, int i) {
-    const int off = stage * STAGE + (((2 * s + hi) ^ (col & 7)) << 4);
+    const int off = stage * STAGE + (((2 * s + hi) ^ ((col >> 1) & 7)) << 4);
     if (i < TM) xv[s & 1][i] = *reinterpret_cast<const u32x4*>(xs + i * 32 * 128 + off);
     else wv[s & 1][i - TM] =
         *reinterpret_cast<const u32x4*>(ws + ((i - TM) / TN * BN + (i - TM) % TN * 32) * 128 + off);
@@ -480,12 +491,12 @@ __global__ __launch_bounds__(64 * WM * WN, BM >= 256 ? 1 : 2) void linear_tile_k
     for (int i = 0; i < READS; ++i) read(0, 0, i);
   }
   for (int step = 0; step < steps; ++step) {
-    const int stage = step & 1;
+    const int stage = step & 1, next = stage ^ 1;
     const bool more = step + 1 < steps, two = step + 2 < steps;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       if (s == 3) {
-        if (more) deposit(stage ^ 1);
+        if (more) deposit(next);
         meet();
       }
 #pragma unroll
@@ -493,20 +504,21 @@ __global__ __launch_bounds__(64 * WM * WN, BM >= 256 ? 1 : 2) void linear_tile_k
         const int i = p / TM, j = p % TM;
         acc[i][j] = mfma32<T>(wv[s & 1][i], xv[s & 1][j], acc[i][j]);
         // spread over the products: the next part's reads, and in the last part
-        // the copies of the stage after the next
+        // the copies of the stage that takes this one's place
 #pragma unroll
         for (int r = p * READS / PRODUCTS; r < (p + 1) * READS / PRODUCTS; ++r) {
           if (s < 3) read(stage, s + 1, r);
-          else if (more) read(stage ^ 1, 0, r);
+          else if (more) read(next, 0, r);
         }
         if (s == 3 && two)
 #pragma unroll
-          for (int c = p * COPIES / PRODUCTS; c < (p + 1) * COPIES / PRODUCTS; ++c) fetch(stage, step + 2, c);
+          for (int c = p * COPIES / PRODUCTS; c < (p + 1) * COPIES / PRODUCTS; ++c)
+            fetch(stage, step + 2, c);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
-  meet();                                    // LDS is free for the results
+  meet();                               // LDS is free for the results
 #pragma unroll 1
   for (int t = 0; t < TURNS; ++t) {
     if (t % PARTS == 0) {
@@ -642,7 +654,7 @@ template <typename T, int OPS, bool VEC>
 hipError_t launch_sizes(const LinearArgs& a, const Plan& p, hipStream_t st) {
   constexpr int N = OPS == 2 ? 2 : 1;
   if constexpr (VEC)
-    if (p.size == 256) return launch_tiles<T, 256, 256 / N, 2, 2, OPS, true>(a, st);
+    if (p.size == 256) return launch_tiles<T, 256, 256 / N, 2, 4, OPS, true>(a, st);
   if (p.size == 128) return launch_tiles<T, 128, 128 / N, 2, 2, OPS, VEC>(a, st);
   return launch_tiles<T, 64, 64 / N, 2, 2 / N, OPS, VEC>(a, st);
 }
