@@ -299,6 +299,9 @@ template <typename T, int DKP, int NW, int C, bool OUT, bool VEC>
 __global__ __launch_bounds__(64 * NW, DKP <= 128 ? 2 : 1)
 void delta_walk_kernel(DeltaArgs a) {
   constexpr int NL = parts_of<T>(), NP = 3, NT = 64 * NW;
+  // operands read ahead: one set; none of three parts, whose products take long
+  // enough and whose registers would cost the second workgroup of a CU
+  constexpr int AHEAD = NL == 3 ? 0 : 1, SETS = AHEAD + 1;
   constexpr int KT = DKP / 32, KS = DKP / 16, CT = C / 32, CS = C / 16, DVW = 32 * NW;
   constexpr int QK_BYTES = NL * C * DKP * 2, V_BYTES = NL * C * DVW * 2;
   constexpr int TILES = CT * (CT + 1) / 2, T_BYTES = TILES * 2 * NP * 1024;
@@ -383,38 +386,55 @@ void delta_walk_kernel(DeltaArgs a) {
 
   constexpr int UK = C * (DKP / 8) / NT, UV = C * (DVW / 8) / NT;   // units of a thread
   static_assert(UK * NT == C * (DKP / 8) && UV * NT == C * (DVW / 8), "whole units");
-  // Of T: threads past the last unit take their first one again.  (Here and at
+  // Of T: threads past the last unit take one of another's again.  (Here and at
   // the powers below no lane is masked off: a register that the compiler spills
   // inside such a branch is saved for the lanes in it alone.)
   constexpr int UT = (TILES * 128 + NT - 1) / NT;
-  auto unit = [&](int i) { return tid + NT * i < TILES * 128 ? tid + NT * i : tid; };
+  auto unit = [&](int i) { return tid + NT * i < TILES * 128 ? tid + NT * i : tid % (TILES * 128); };
   Unit<T> ku[UK], vu[UV], qu[OUT ? UK : 1];
   Vec<float, 4> tu[UT][2];
   double fall = 0.0;
   float beta = 0.0f;
-  auto load_chunk = [&]() {
-    const int n = left < C ? left : C;
-    load_units<T, UK, DKP, NT, VEC>(ku, kp, n, a.kt, a.dk);
-    if (OUT || !move) load_units<T, UV, DVW, NT, VEC>(vu, vp, n, a.vt, dvs);
-    if constexpr (OUT) load_units<T, UK, DKP, NT, VEC>(qu, qp, n, a.qt, a.dk);
-    const float* const from = a.solved + pair * solved_size<C>();
+  // The next chunk's rows; behind the last chunk the segment's first row again, so
+  // that no load is conditional: the registers of one that is not made would stay
+  // taken from one chunk to the next.
+  const T *const k_first = kp, *const v_first = vp, *const q_first = qp;
+  const int64_t pair_first = pair;
+  auto rows = [&]() { return left >= C ? C : left > 0 ? left : 1; };
+  auto load_keys = [&]() {
+    load_units<T, UK, DKP, NT, VEC>(ku, left > 0 ? kp : k_first, rows(), a.kt, a.dk);
+    const int64_t at = left > 0 ? pair : pair_first;
+    const float* const from = a.solved + at * solved_size<C>();
 #pragma unroll
     for (int i = 0; i < UT; ++i) {
       tu[i][0] = *reinterpret_cast<const Vec<float, 4>*>(from + unit(i) * 8);
       tu[i][1] = *reinterpret_cast<const Vec<float, 4>*>(from + unit(i) * 8 + 4);
     }
-    fall = a.falls[pair * C + tid % C];
-    beta = a.betas[pair * C + tid % C];
+    fall = a.falls[at * C + tid % C];
+    beta = a.betas[at * C + tid % C];
+  };
+  auto load_values = [&]() {
+    if (OUT || !move) load_units<T, UV, DVW, NT, VEC>(vu, left > 0 ? vp : v_first, rows(), a.vt, dvs);
+  };
+  auto load_queries = [&]() {
+    if constexpr (OUT) load_units<T, UK, DKP, NT, VEC>(qu, left > 0 ? qp : q_first, rows(), a.qt, a.dk);
   };
   if (!OUT && move)
 #pragma unroll
     for (int i = 0; i < UV; ++i) vu[i] = Unit<T>{};
 
-  const uint32_t at_row = row_base<DKP>(lane), at_key = token_base<DKP>(lane, true);
-  const uint32_t at_value = token_base<DVW>(lane, false) ^ (uint32_t)(wave << 6);
+  uint32_t at_row = row_base<DKP>(lane), at_key = token_base<DKP>(lane, true);
+  uint32_t at_value = token_base<DVW>(lane, false) ^ (uint32_t)(wave << 6);
 
-  if (left > 0) load_chunk();
+  if (left > 0) {
+    load_keys();
+    load_values();
+    load_queries();
+  }
   while (left > 0) {
+    // opaque: the places derived from them, kept over the chunks, cost more
+    // registers than there are
+    asm volatile("" : "+v"(at_row), "+v"(at_key), "+v"(at_value));
     const int n = left < C ? left : C;
     __syncthreads();                         // the last chunk's images are read
 #pragma unroll
@@ -460,81 +480,59 @@ void delta_walk_kernel(DeltaArgs a) {
 
     const float fade = fade_sh[0], fade_low = fade_sh[1];
 
-    // Scores K Q^T of 32 keys (rows) x 32 queries (columns): eight registers
-    // on end are an operand of U^T P^T as they lie.  One tile: every wave for
-    // itself; three: a tile a wave, exchanged in LDS.
-    u32x4 pop[OUT ? 2 : 1][NP];
-    if constexpr (OUT) {
-      if (CT == 1 || wave < TILES) {
-        const int qt = CT == 1 || wave == 0 ? 0 : 1, kt = CT > 1 && wave == 2 ? 1 : 0;
-        f16v acc = {};
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          u32x4 ak[NL], bq[NL];
-#pragma unroll
-          for (int p = 0; p < NL; ++p) {
-            ak[p] = row_operand<C, DKP>(lds, at_row, p, kt, s);
-            bq[p] = row_operand<C, DKP>(lds + Q_AT, at_row, p, qt, s);
-          }
-#pragma unroll
-          for (int x = 0; x < NL; ++x)
-#pragma unroll
-            for (int y = 0; y < NL; ++y)
-              if (x + y < (NL == 1 ? 1 : NP)) acc = mfma(ak[x], bq[y], acc);
-        }
-        const int i = 32 * qt + col;
-        const double gi = fall_sh[i];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          float x[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int key = 32 * kt + 16 * s + 8 * (j >> 2) + 4 * hi + (j & 3);
-            const float y = acc[8 * s + j] * (a.scale * __builtin_amdgcn_exp2f((float)(gi - fall_sh[key])));
-            x[j] = i >= key ? y : 0.0f;
-          }
-          split8<NP>(x, pop[s]);
-        }
-      }
-    }
+    // In what follows the operands of the next products are read, and made, between
+    // the products at hand, and the compiler is held to that order (step()).
 
     // r = beta v - beta e^g (K S), rows tokens;  O^T = S^T Q^T, rows columns of
     // the values: both of S's parts.
     f16v R[CT], O[OUT ? CT : 1];
+    {
+      u32x4 sp[SETS][NP], ky[SETS][CT][NL], qy[OUT ? SETS : 1][CT][NL];
+      auto state_part = [&](int s) {         // S's operand, and S faded
+        float x[8];
 #pragma unroll
-    for (int t = 0; t < CT; ++t) {
-      R[t] = f16v{};
-      if constexpr (OUT) O[t] = f16v{};
-    }
+        for (int j = 0; j < 8; ++j) {
+          x[j] = S[s / 2][8 * (s & 1) + j];
+          S[s / 2][8 * (s & 1) + j] = __builtin_fmaf(x[j], fade, x[j] * fade_low);
+        }
+        split8<NP>(x, sp[s % SETS]);
+      };
+      auto read = [&](int s) {
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      float x[8];
+        for (int t = 0; t < CT; ++t)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = S[s / 2][8 * (s & 1) + j];
-        S[s / 2][8 * (s & 1) + j] = __builtin_fmaf(x[j], fade, x[j] * fade_low);
+          for (int p = 0; p < NL; ++p) {
+            ky[s % SETS][t][p] = row_operand<C, DKP>(lds, at_row, p, t, s);
+            if constexpr (OUT) qy[s % SETS][t][p] = row_operand<C, DKP>(lds + Q_AT, at_row, p, t, s);
+          }
+      };
+      if (AHEAD) {
+        read(0);
+        state_part(0);
       }
-      u32x4 sp[NP];
-      split8<NP>(x, sp);
 #pragma unroll
       for (int t = 0; t < CT; ++t) {
-        u32x4 y[NL];
+        R[t] = f16v{};
+        if constexpr (OUT) O[t] = f16v{};
+      }
+      if (AHEAD) step();
 #pragma unroll
-        for (int p = 0; p < NL; ++p) y[p] = row_operand<C, DKP>(lds, at_row, p, t, s);
+      for (int s = 0; s < KS; ++s) {
+        if (s + AHEAD < KS) {
+          read(s + AHEAD);
+          state_part(s + AHEAD);
+        }
 #pragma unroll
         for (int p = 0; p < NP; ++p)
 #pragma unroll
           for (int l = 0; l < NL; ++l)
-            if (p + l < NP) R[t] = mfma(y[l], sp[p], R[t]);
-        if constexpr (OUT) {
 #pragma unroll
-          for (int p = 0; p < NL; ++p) y[p] = row_operand<C, DKP>(lds + Q_AT, at_row, p, t, s);
-#pragma unroll
-          for (int p = 0; p < NP; ++p)
-#pragma unroll
-            for (int l = 0; l < NL; ++l)
-              if (p + l < NP) O[t] = mfma(sp[p], y[l], O[t]);
-        }
+            for (int t = 0; t < CT; ++t)
+              if (p + l < NP) {
+                R[t] = mfma(ky[s % SETS][t][l], sp[s % SETS][p], R[t]);
+                if constexpr (OUT) O[t] = mfma(sp[s % SETS][p], qy[s % SETS][t][l], O[t]);
+              }
+        if (AHEAD) step();
       }
     }
     if constexpr (OUT) {
@@ -545,32 +543,6 @@ void delta_walk_kernel(DeltaArgs a) {
         for (int r = 0; r < 16; ++r) O[t][r] *= f;
       }
     }
-
-    // A value that is not finite would give NaN wherever it meets a zero of T or
-    // of the scores: it is taken out of r (then u), and what depends on it set to
-    // NaN below: this lane's column, the queries from its token on and the state.
-    // (The segments' own states keep it: there NaN goes its way.)
-    int bad_from = C;
-    auto take_out = [&](f16v* x) {
-      float z = 0.0f;                        // NaN if any is not finite
-#pragma unroll
-      for (int t = 0; t < CT; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) z = __builtin_fmaf(x[t][r], 0.0f, z);
-      if (__ballot(z != z) != 0) {
-#pragma unroll
-        for (int t = 0; t < CT; ++t)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (!(__builtin_fabsf(x[t][r]) < __builtin_inff())) {
-              const int tok = 32 * t + 8 * (r >> 2) + 4 * hi + (r & 3);
-              if (tok < bad_from) bad_from = tok;
-              x[t][r] = 0.0f;
-            }
-        const int other = __shfl_xor(bad_from, 32, 64);
-        if (other < bad_from) bad_from = other;
-      }
-    };
 
     u32x4 rop[CS][NP];                       // r, then u, as operands
 #pragma unroll
@@ -588,14 +560,48 @@ void delta_walk_kernel(DeltaArgs a) {
 #pragma unroll
           for (int p = 0; p < NL; ++p) {
             const uint32_t word = vop[p][2 * e + (j >> 1)];
-            y += __builtin_bit_cast(float, j & 1 ? word & 0xffff0000u : word << 16);
+            const float part = __builtin_bit_cast(float, j & 1 ? word & 0xffff0000u : word << 16);
+            y = p == 0 ? part : y + part;
           }
           const int r = 8 * (s & 1) + 4 * e + j;
           R[s / 2][r] = __builtin_fmaf(-f.v[j], R[s / 2][r], b.v[j] * y);
         }
       }
     }
-    if constexpr (OUT) take_out(R);
+    // A value that is not finite would give NaN wherever it meets a zero of T or
+    // of the scores: r and u are zeros from its token on, and what depends on them
+    // set to NaN below: this lane's column, the queries from the token on and the
+    // state.  (A k, beta or decay that is not finite shows in r too.  The segments'
+    // own states keep it: there NaN goes its way.)
+    int bad_from = C;
+    bool any_bad = false;
+    auto take_out = [&](f16v* x) {
+#pragma unroll
+      for (int t = 0; t < CT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          x[t][r] = 32 * t + 8 * (r >> 2) + 4 * hi + (r & 3) >= bad_from ? 0.0f : x[t][r];
+    };
+    if constexpr (OUT) {
+      float z = 0.0f;                        // NaN if any is not finite
+#pragma unroll
+      for (int t = 0; t < CT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z = __builtin_fmaf(R[t][r], 0.0f, z);
+      any_bad = __ballot(z != z) != 0;
+      if (any_bad) {
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int tok = 32 * t + 8 * (r >> 2) + 4 * hi + (r & 3);
+            bad_from = !(__builtin_fabsf(R[t][r]) < __builtin_inff()) && tok < bad_from ? tok : bad_from;
+          }
+        const int other = __shfl_xor(bad_from, 32, 64);
+        bad_from = other < bad_from ? other : bad_from;
+        take_out(R);
+      }
+    }
 #pragma unroll
     for (int s = 0; s < CS; ++s) {
       float x[8];
@@ -604,37 +610,75 @@ void delta_walk_kernel(DeltaArgs a) {
       split8<NP>(x, rop[s]);
     }
 
-    // u = T r
+    // u = T r, from T's operands in LDS (below O^T from the scores' in their place)
     f16v U[CT];
+    u32x4 tile_op[2][NP];
+    auto read_tile = [&](int i) {
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+        tile_op[i & 1][p] = *reinterpret_cast<const u32x4*>(tsh + ((i * NP + p) * 64 + lane) * 16);
+    };
+    read_tile(0);
 #pragma unroll
     for (int t = 0; t < CT; ++t) U[t] = f16v{};
 #pragma unroll
     for (int i = 0; i < TILES * 2; ++i) {
       const int tt = i / 2 == 0 ? 0 : 1, ts = i / 2 == 2 ? 1 : 0, s = 2 * ts + (i & 1);
-      u32x4 x[NP];
-#pragma unroll
-      for (int p = 0; p < NP; ++p)
-        x[p] = *reinterpret_cast<const u32x4*>(tsh + ((i * NP + p) * 64 + lane) * 16);
+      if (i + 1 < TILES * 2) read_tile(i + 1);
 #pragma unroll
       for (int p = 0; p < NP; ++p)
 #pragma unroll
         for (int y = 0; y < NP; ++y)
-          if (p + y < NP) U[tt] = mfma(x[p], rop[s][y], U[tt]);
+          if (p + y < NP) U[tt] = mfma(tile_op[i & 1][p], rop[s][y], U[tt]);
+      step();
     }
 
-    bool any_bad = false;
     if constexpr (OUT) {
-      take_out(U);
-      if constexpr (CT > 1) {
-        __syncthreads();                     // T is read
-        if (wave < TILES) {
+      if (CT > 1) __syncthreads();           // T is read
+      if (any_bad) take_out(U);
+      // Scores K Q^T of 32 keys (rows) x 32 queries (columns): eight registers
+      // on end are an operand of U^T P^T as they lie.  One tile: every wave for
+      // itself; three: a tile a wave, exchanged in LDS.
+      u32x4 pop[2][NP];
+      if (CT == 1 || wave < TILES) {
+        const int qt = CT == 1 || wave == 0 ? 0 : 1, kt = CT > 1 && wave == 2 ? 1 : 0;
+        u32x4 ak[SETS][NL], bq[SETS][NL];
+        auto read = [&](int s) {
 #pragma unroll
-          for (int s = 0; s < 2; ++s)
+          for (int p = 0; p < NL; ++p) {
+            ak[s % SETS][p] = row_operand<C, DKP>(lds, at_row, p, kt, s);
+            bq[s % SETS][p] = row_operand<C, DKP>(lds + Q_AT, at_row, p, qt, s);
+          }
+        };
+        if (AHEAD) read(0);
+        f16v acc = {};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          if (s + AHEAD < KS) read(s + AHEAD);
+#pragma unroll
+          for (int x = 0; x < NL; ++x)
+#pragma unroll
+            for (int y = 0; y < NL; ++y)
+              if (x + y < (NL == 1 ? 1 : NP)) acc = mfma(ak[s % SETS][x], bq[s % SETS][y], acc);
+          if (AHEAD) step();
+        }
+        const int i = 32 * qt + col;
+        const double gi = fall_sh[i];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          float x[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int key = 32 * kt + 16 * s + 8 * (j >> 2) + 4 * hi + (j & 3);
+            const float y = acc[8 * s + j] * (a.scale * __builtin_amdgcn_exp2f((float)(gi - fall_sh[key])));
+            x[j] = i >= key ? y : 0.0f;
+          }
+          split8<NP>(x, pop[s]);
+          if constexpr (CT > 1)
 #pragma unroll
             for (int p = 0; p < NP; ++p)
               *reinterpret_cast<u32x4*>(tsh + (((wave * 2 + s) * NP + p) * 64 + lane) * 16) = pop[s][p];
         }
-        __syncthreads();
       }
 #pragma unroll
       for (int s = 0; s < CS; ++s) {
@@ -644,59 +688,87 @@ void delta_walk_kernel(DeltaArgs a) {
         split8<NP>(x, rop[s]);
       }
       // O^T += U^T P^T
+      if constexpr (CT > 1) {
+        __syncthreads();
+        read_tile(0);
+      }
 #pragma unroll
       for (int i = 0; i < TILES * 2; ++i) {
         const int qt = i / 2 == 0 ? 0 : 1, kt = i / 2 == 2 ? 1 : 0, s = 2 * kt + (i & 1);
-        u32x4 y[NP];
-#pragma unroll
-        for (int p = 0; p < NP; ++p)
-          y[p] = CT == 1 ? pop[i & 1][p]
-                         : *reinterpret_cast<const u32x4*>(tsh + ((i * NP + p) * 64 + lane) * 16);
+        if (CT > 1 && i + 1 < TILES * 2) read_tile(i + 1);
 #pragma unroll
         for (int x = 0; x < NP; ++x)
 #pragma unroll
           for (int p = 0; p < NP; ++p)
-            if (p + x < NP) O[qt] = mfma(rop[s][x], y[p], O[qt]);
+            if (p + x < NP) O[qt] = mfma(rop[s][x], CT == 1 ? pop[i & 1][p] : tile_op[i & 1][p], O[qt]);
+        step();
       }
-      any_bad = __ballot(bad_from < C) != 0;
       if (any_bad) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int from = __shfl(bad_from, 8 * (r >> 2) + 4 * hi + (r & 3), 64);
 #pragma unroll
           for (int qt = 0; qt < CT; ++qt)
-            if (32 * qt + col >= from) O[qt][r] = __builtin_nanf("");
+            O[qt][r] = 32 * qt + col >= from ? __builtin_nanf("") : O[qt][r];
         }
       }
       store_columns<T, CT, VEC>(O, op, n, dvs, a.ot, wave);
       op += C * a.ot;
     }
 
-    // The next chunk's rows, now that the outputs' registers are free.
-    if (left > 0) load_chunk();
+    // The next chunk's rows, now that the outputs' registers are free, the values
+    // and queries as u's get free.
+    load_keys();
 
     // S <- e^(g_end) S (above) + K^T (e^(g_end - g) u)
+    {
+      u32x4 bu[SETS][NP], ak[SETS][NL];
+      auto key_tile = [&](int i) {
 #pragma unroll
-    for (int s = 0; s < CS; ++s) {
-      float x[8];
+        for (int y = 0; y < NL; ++y)
+          ak[i % SETS][y] = token_operand<C, DKP>(lds, at_key, y, i % KT, i / KT);
+      };
+      Vec<float, 4> wt[2];
+      auto weights = [&](int s) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const Vec<float, 4> f = *reinterpret_cast<const Vec<float, 4>*>(end_sh + 16 * s + 8 * e + 4 * hi);
+        for (int e = 0; e < 2; ++e)
+          wt[e] = *reinterpret_cast<const Vec<float, 4>*>(end_sh + 16 * s + 8 * e + 4 * hi);
+      };
+      auto weigh = [&](int s, int p) {       // two tokens' of a lane's eight
+        const int r = 8 * (s & 1) + 2 * p;
+        split2<NP>(U[s / 2][r] * wt[p >> 1].v[2 * (p & 1)], U[s / 2][r + 1] * wt[p >> 1].v[2 * (p & 1) + 1],
+                   bu[s % SETS], p);
+      };
+      weights(0);
+      if (AHEAD) {
+        key_tile(0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[4 * e + j] = U[s / 2][8 * (s & 1) + 4 * e + j] * f.v[j];
+        for (int p = 0; p < 4; ++p) weigh(0, p);
+        if (CS > 1) weights(1);
       }
-      u32x4 bu[NP];
-      split8<NP>(x, bu);
+      step();
 #pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        u32x4 ak[NL];
+      for (int i = 0; i < CS * KT; ++i) {
+        const int s = i / KT, t = i % KT;
+        if (i + AHEAD < CS * KT) key_tile(i + AHEAD);
+        if (!AHEAD && t == 0) {
+          if (s > 0) weights(s);
 #pragma unroll
-        for (int y = 0; y < NL; ++y) ak[y] = token_operand<C, DKP>(lds, at_key, y, t, s);
+          for (int p = 0; p < 4; ++p) weigh(s, p);
+        }
 #pragma unroll
         for (int y = 0; y < NL; ++y)
 #pragma unroll
           for (int p = 0; p < NP; ++p)
-            if (p + y < NP) S[t] = mfma(ak[y], bu[p], S[t]);
+            if (p + y < NP) S[t] = mfma(ak[i % SETS][y], bu[s % SETS][p], S[t]);
+        if (AHEAD && s + 1 < CS) {
+#pragma unroll
+          for (int p = t * 4 / KT; p < (t + 1) * 4 / KT; ++p) weigh(s + 1, p);
+          if (t == KT - 1 && s + 2 < CS) weights(s + 2);
+        }
+        if (AHEAD) step();
+        if (i == CS * KT / 2 - 1) load_values();
+        if (i == CS * KT * 3 / 4 - 1) load_queries();
       }
     }
     if (any_bad) {
