@@ -140,24 +140,28 @@ __global__ __launch_bounds__(1024) void delta_begins_kernel(DeltaArgs a) {
 // columns 4 (lane / 32) + 0 .. 3 and the same plus 8 of the half's sixteen.
 //
 // The products k_t . k_s on the matrix cores; blocks of 16 inverted column by
-// column in registers, then joined in pairs:
+// column in registers, then joined in pairs by fp32 matrix instructions:
 //   (A 0; B D)^-1 = (A^-1 0; -D^-1 B A^-1 D^-1).
+// Rows of L from the first one that is not finite on are left out, and of T NaN.
 template <int C> constexpr int solved_size() { return (C / 32) * (C / 32 + 1) / 2 * 1024; }
+
+typedef float f4v __attribute__((ext_vector_type(4)));
 
 template <typename T, int DKP, int C, int NT, bool VEC>
 __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
   constexpr int NL = parts_of<T>(), NP = 3, KS = DKP / 16, CT = C / 32, TILES = CT * (CT + 1) / 2;
-  constexpr int P = C + 1;
+  constexpr int P = C + 4;
   __shared__ __attribute__((aligned(512))) char lds[NL * C * DKP * 2];
-  __shared__ float low[C * P], inv[C * P];
+  __shared__ __attribute__((aligned(16))) float low[C * P], inv[C * P];
   __shared__ double fall[C];
   __shared__ float beta[C];
+  __shared__ int bad_sh;
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   const int64_t pair = a.first + blockIdx.x;
-  const int64_t w = pair / a.heads;
-  const int h = (int)(pair % a.heads);
+  const int64_t w = uniform(pair / a.heads);
+  const int h = (int)(pair - w * a.heads);
   const Place pl = find_place(a, w, C);
   if (pl.seq < 0 || pl.len == 0) return;
   const int64_t row0 = a.cu != nullptr ? 0 : pl.seq, begin = pl.begin + pl.part * C;
@@ -189,6 +193,7 @@ __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
     a.falls[pair * C + tid] = g;
     a.betas[pair * C + tid] = b;
   }
+  if (tid == 0) bad_sh = C;
 #pragma unroll
   for (int i = 0; i < UK; ++i) {
     const int u = tid + NT * i;
@@ -216,52 +221,91 @@ __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
     }
     const int s = 32 * ts + col;
     const double gs = fall[s];
+    float z = 0.0f;                          // NaN if any is not finite
+    int bad = C;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int t = 32 * tt + 8 * (r >> 2) + 4 * hi + (r & 3);
       const float f = beta[t] * __builtin_amdgcn_exp2f((float)(fall[t] - gs));
-      low[t * P + s] = t > s ? f * acc[r] : 0.0f;
+      const float x = t > s ? f * acc[r] : 0.0f;
+      low[t * P + s] = x;
+      z = __builtin_fmaf(x, 0.0f, z);
+      bad = !(__builtin_fabsf(x) < __builtin_inff()) && t < bad ? t : bad;
     }
+    if (__ballot(z != z) != 0) atomicMin(&bad_sh, bad);
   }
   __syncthreads();
+  const int bad_from = bad_sh;
+  if (bad_from < C) {
+    for (int i = tid; i < (C - bad_from) * C; i += NT) low[(bad_from + i / C) * P + i % C] = 0.0f;
+    __syncthreads();
+  }
 
-  // blocks of 16: thread = block and column
+  // Blocks of 16: thread = block and column.  x_t takes what the earlier ones
+  // leave of it as soon as each is known.
   if (tid < C) {
     const int b0 = tid & ~15, c = tid & 15;
     float x[16];
 #pragma unroll
-    for (int t = 0; t < 16; ++t) {
-      float y = 0.0f;
+    for (int t = 0; t < 16; ++t) x[t] = t == c ? 1.0f : 0.0f;
+    Vec<float, 4> l[16][4];
 #pragma unroll
-      for (int s = 0; s < t; ++s) y = __builtin_fmaf(-low[(b0 + t) * P + b0 + s], x[s], y);
-      x[t] = t < c ? 0.0f : t == c ? 1.0f : y;
-      inv[(b0 + t) * P + b0 + c] = x[t];
-    }
+    for (int t = 1; t < 16; ++t)
+#pragma unroll
+      for (int q = 0; q < (t + 3) / 4; ++q)
+        l[t][q] = *reinterpret_cast<const Vec<float, 4>*>(low + (b0 + t) * P + b0 + 4 * q);
+#pragma unroll
+    for (int s = 0; s < 15; ++s)
+#pragma unroll
+      for (int t = s + 1; t < 16; ++t) x[t] = __builtin_fmaf(-l[t][s / 4].v[s % 4], x[s], x[t]);
+#pragma unroll
+    for (int t = 0; t < 16; ++t) inv[(b0 + t) * P + b0 + c] = x[t];
+  } else if (C > 32) {
+    // the blocks above them in the pairs' upper left and lower right
+    for (int i = tid - C; i < 512; i += NT - C)
+      inv[(i / 256 * 32 + i % 256 / 16) * P + i / 256 * 32 + 16 + i % 16] = 0.0f;
   }
   __syncthreads();
+  const int c16 = lane & 15, q16 = lane >> 4;
+  // pairs of 16: B A^-1 (its accumulators are the next product's operand as they
+  // lie, if that takes its inner indices 4 q16 + j), then -D^-1 times it
+  if (wave < C / 32) {
+    const int b0 = 32 * wave;
+    f4v m = {}, y = {};
 #pragma unroll
-  for (int size = 16; size < C; size *= 2) {
-    // B A^-1 where the pair's upper right block would be, then its product
-    const int per = size * size, all = C / (2 * size) * per;
-    for (int i = tid; i < all; i += NT) {
-      const int b0 = i / per * 2 * size, r = i % per / size, c = i % size;
-      float y = 0.0f;
-      for (int m = 0; m < size; ++m) {
-        const float x = low[(b0 + size + r) * P + b0 + m] * inv[(b0 + m) * P + b0 + c];
-        y += m >= c ? x : 0.0f;
-      }
-      inv[(b0 + r) * P + b0 + size + c] = y;
+    for (int j = 0; j < 4; ++j) {
+      const int k = 4 * j + q16;
+      m = __builtin_amdgcn_mfma_f32_16x16x4f32(low[(b0 + 16 + c16) * P + b0 + k],
+                                               inv[(b0 + k) * P + b0 + c16], m, 0, 0, 0);
     }
-    __syncthreads();
-    for (int i = tid; i < all; i += NT) {
-      const int b0 = i / per * 2 * size, r = i % per / size, c = i % size;
-      float y = 0.0f;
-      for (int m = 0; m < size; ++m) {
-        const float x = inv[(b0 + size + r) * P + b0 + size + m] * inv[(b0 + m) * P + b0 + size + c];
-        y += m <= r ? x : 0.0f;
-      }
-      inv[(b0 + size + r) * P + b0 + c] = -y;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      y = __builtin_amdgcn_mfma_f32_16x16x4f32(inv[(b0 + 16 + c16) * P + b0 + 16 + 4 * q16 + j], m[j], y,
+                                               0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) inv[(b0 + 16 + 4 * q16 + j) * P + b0 + c16] = -y[j];
+  }
+  __syncthreads();
+  if constexpr (C > 32) {
+    // the pair of 32: wave = 16 rows (i) and 16 columns (j) of its lower left block
+    const int i0 = 32 + 16 * (wave & 1), j0 = 16 * (wave >> 1);
+    f4v m[2] = {{}, {}}, y = {};
+#pragma unroll
+    for (int k0 = 0; k0 < 32; k0 += 4) {
+      const float x = inv[(k0 + q16) * P + j0 + c16];
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        m[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(low[(32 + 16 * e + c16) * P + k0 + q16], x, m[e],
+                                                    0, 0, 0);
     }
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        y = __builtin_amdgcn_mfma_f32_16x16x4f32(inv[(i0 + c16) * P + 32 + 16 * e + 4 * q16 + j], m[e][j],
+                                                 y, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) inv[(i0 + 4 * q16 + j) * P + j0 + c16] = -y[j];
     __syncthreads();
   }
 
@@ -270,15 +314,16 @@ __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
     const int tile = u >> 7, half = (u >> 6) & 1, l = u & 63;
     const int t = 32 * (tile == 0 ? 0 : 1) + (l & 31);
     const int s0 = 32 * (tile == 2 ? 1 : 0) + 16 * half + 4 * (l >> 5);
-    Vec<float, 4> y[2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int s = s0 + 8 * (j >> 2) + (j & 3);
-      const float x = inv[t * P + s];
-      y[j >> 2].v[j & 3] = s <= t ? x : 0.0f;
+    for (int e = 0; e < 2; ++e) {
+      Vec<float, 4> y = *reinterpret_cast<const Vec<float, 4>*>(inv + t * P + s0 + 8 * e);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = t >= bad_from ? __builtin_nanf("") : y.v[j];
+        y.v[j] = s0 + 8 * e + j <= t ? x : 0.0f;
+      }
+      *reinterpret_cast<Vec<float, 4>*>(to + u * 8 + 4 * e) = y;
     }
-    *reinterpret_cast<Vec<float, 4>*>(to + u * 8) = y[0];
-    *reinterpret_cast<Vec<float, 4>*>(to + u * 8 + 4) = y[1];
   }
 }
 
@@ -356,14 +401,14 @@ void delta_walk_kernel(DeltaArgs a) {
 #pragma unroll
   for (int t = 0; t < KT; ++t) S[t] = f16v{};
   const int sc = 32 * wave + col;            // this lane's column of the slice
-  // this lane's place in a state: of its first row; the others are dv apart,
-  // rows from dk on and columns from dvs on out of the buffer's range
-  const uint32_t s_at = sc < dvs ? 4u * (uint32_t)(8 * hi * a.dv + c0 + sc) : OOB;
+  // this lane's place in a state (or M): of its first row; the others are cols
+  // apart, rows from dk on and columns from dvs on out of the buffer's range
+  const uint32_t s_at = sc < dvs ? 4u * (uint32_t)(8 * hi * cols + c0 + sc) : OOB;
   auto s_off = [&](int t, int r) {
-    return s_at + 4u * (uint32_t)((32 * t + 16 * (r >> 3) + (r & 7)) * a.dv);
+    return s_at + 4u * (uint32_t)((32 * t + 16 * (r >> 3) + (r & 7)) * cols);
   };
   auto state_of = [&](const float* base, int64_t i) {
-    return rows_rsrc(base + (i * a.heads + h) * (int64_t)a.dk * a.dv, 4u * a.dk * a.dv);
+    return rows_rsrc(base + (i * a.heads + h) * (int64_t)a.dk * cols, 4u * a.dk * cols);
   };
   if (OUT) {
     const float* const from = pl.part > 0 ? a.own : a.state_in;
@@ -779,21 +824,7 @@ void delta_walk_kernel(DeltaArgs a) {
     }
   }
 
-  if (move) {
-    // M turned: row = column of M, so that the join reads it in lines
-    float* const m = a.moves + (w * a.heads + h) * (int64_t)a.dk * a.dk;
-    if (sc < dvs) {
-#pragma unroll
-      for (int t = 0; t < KT; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int d = 32 * t + 16 * (r >> 3) + 8 * hi + (r & 7);
-          if (d < a.dk) m[(int64_t)(c0 + sc) * a.dk + d] = S[t][r];
-        }
-    }
-    return;
-  }
-  float* const to = OUT ? (last ? a.state_out : nullptr) : a.own;
+  float* const to = OUT ? (last ? a.state_out : nullptr) : move ? a.moves : a.own;
   if (to != nullptr) {
     const __amdgpu_buffer_rsrc_t rs = state_of(to, OUT ? pl.seq : w);
 #pragma unroll
@@ -816,49 +847,106 @@ void delta_walk_kernel(DeltaArgs a) {
 
 // The segments' N become the states before them, in place:
 //   S_0 = state_in,  S_{m+1} = M_m S_m + N_m.
-// A workgroup carries 8 columns of a head along a sequence.
-constexpr int JOIN_COLS = 8;
-__global__ __launch_bounds__(256) void delta_join_kernel(DeltaArgs a) {
-  __shared__ __attribute__((aligned(16))) float s_sh[2][CF_DECAY_MAX_DK * JOIN_COLS];
+// A workgroup carries 32 columns of a head along a sequence, wave t their rows
+// 32 t .. + 31 in an accumulator (in the walk's order of rows).  Each step puts S
+// into LDS as operands, all rows for all waves; M's rows and N of the next step are
+// loaded meanwhile.  16 segments of 32 heads of 128 x 128: 24 us; with the products
+// of single numbers in lanes, M read by every 8 columns, 620.
+template <int DKP, bool VEC>
+__global__ __launch_bounds__(2 * DKP) void delta_join_kernel(DeltaArgs a) {
+  constexpr int KT = DKP / 32, KS = DKP / 16, NP = 3;
+  __shared__ __attribute__((aligned(16))) char ssh[2][KS * NP * 1024];
   const int64_t w = blockIdx.y;
   const Place pl = find_place(a, w, a.segment);
   if (pl.seq < 0 || pl.part != 0 || pl.parts < 2) return;
-  const int h = blockIdx.z, c0 = blockIdx.x * JOIN_COLS, tid = threadIdx.x;
-  const int cols = a.dv - c0 < JOIN_COLS ? a.dv - c0 : JOIN_COLS;
-  const int64_t size = (int64_t)a.dk * a.dv;
-  for (int i = tid; i < a.dk * JOIN_COLS; i += 256) {
-    const int r = i / JOIN_COLS, c = i % JOIN_COLS;
-    s_sh[0][i] = a.state_in != nullptr && c < cols
-                     ? a.state_in[(pl.seq * a.heads + h) * size + (int64_t)r * a.dv + c0 + c] : 0.0f;
-  }
-  __syncthreads();
-  for (int64_t m = 0; m < pl.parts; ++m) {
-    const float* const s = s_sh[m & 1];
-    float* const next = s_sh[(m + 1) & 1];
-    float* const own = a.own + ((w + m) * a.heads + h) * size + c0;
-    const float* const mt = a.moves + ((w + m) * a.heads + h) * (int64_t)a.dk * a.dk;
-    const bool more = m + 1 < pl.parts;      // (the last one has no M and N)
-    for (int i = tid; i < 2 * a.dk; i += 256) {
-      const int r = i % a.dk, quad = i / a.dk * 4;
-      float y[4];
+  const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, col = lane & 31;
+  const int t = __builtin_amdgcn_readfirstlane(tid >> 6), h = blockIdx.z, c0 = blockIdx.x * 32;
+  // rows of an operand in the order in which an accumulator's are the state's
+  const int row = 32 * t + 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
+  const uint32_t s_at = c0 + col < a.dv ? 4u * (uint32_t)((32 * t + 8 * hi) * a.dv + c0 + col) : OOB;
+  auto place = [&](const float* base, int64_t i, int cols) {
+    return rows_rsrc(base + (i * a.heads + h) * (int64_t)a.dk * cols, 4u * a.dk * cols);
+  };
+  auto load_state = [&](const float* base, int64_t i) {
+    const __amdgpu_buffer_rsrc_t rs = place(base, i, a.dv);
+    f16v x;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = more && quad + j < cols ? own[(int64_t)r * a.dv + quad + j] : 0.0f;
+    for (int r = 0; r < 16; ++r) {
+      const uint32_t e = __builtin_amdgcn_raw_buffer_load_b32(
+          rs, s_at + 4u * (uint32_t)((16 * (r >> 3) + (r & 7)) * a.dv), 0, 0);
+      x[r] = __builtin_bit_cast(float, e);
+    }
+    return x;
+  };
+  // this lane's numbers of M: its row, columns 16 s + 8 hi .. + 7
+  u32x4 m[KS][2];
+  auto load_move = [&](int64_t i) {
+    const __amdgpu_buffer_rsrc_t rs = place(a.moves, i, a.dk);
+    const uint32_t at = 4u * (uint32_t)(row * a.dk + 8 * hi);     // rows from dk on: out of the range
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (quad + j < cols) own[(int64_t)r * a.dv + quad + j] = s[r * JOIN_COLS + quad + j];
-      if (more) {
-#pragma unroll 8
-        for (int k = 0; k < a.dk; ++k) {
-          const float x = mt[(int64_t)k * a.dk + r];
-          const Vec<float, 4> z = *reinterpret_cast<const Vec<float, 4>*>(s + k * JOIN_COLS + quad);
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) y[j] = __builtin_fmaf(x, z.v[j], y[j]);
+      for (int e = 0; e < 2; ++e) {
+        const int c = 16 * s + 8 * hi + 4 * e;
+        if constexpr (VEC) {
+          m[s][e] = __builtin_amdgcn_raw_buffer_load_b128(rs, c < a.dk ? at + 4u * (16 * s + 4 * e) : OOB,
+                                                          0, 0);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            m[s][e][j] = __builtin_amdgcn_raw_buffer_load_b32(
+                rs, c + j < a.dk ? at + 4u * (16 * s + 4 * e + j) : OOB, 0, 0);
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) next[r * JOIN_COLS + quad + j] = y[j];
       }
+  };
+  f16v S = {};
+  if (a.state_in != nullptr) S = load_state(a.state_in, pl.seq);
+  load_move(w);
+  f16v next = load_state(a.own, w);
+  for (int64_t i = 0; i < pl.parts; ++i) {
+    const __amdgpu_buffer_rsrc_t rs = place(a.own, w + i, a.dv);
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, (float)S[r]), rs,
+                                            s_at + 4u * (uint32_t)((16 * (r >> 3) + (r & 7)) * a.dv), 0, 0);
+    if (i + 1 == pl.parts) return;           // (the last one has no M and N)
+    char* const image = ssh[i & 1];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = S[8 * e + j];
+      u32x4 parts[NP];
+      split8<NP>(x, parts);
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+        *reinterpret_cast<u32x4*>(image + (((2 * t + e) * NP + p) * 64 + lane) * 16) = parts[p];
     }
     __syncthreads();
+    S = next;
+    // (the last segment has none: the first one's again)
+    const int64_t ahead = w + (i + 2 < pl.parts ? i + 1 : 0);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t e = m[s][j >> 2][j & 3];
+        x[j] = __builtin_bit_cast(float, e);
+      }
+      u32x4 mp[NP], sp[NP];
+      split8<NP>(x, mp);
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+        sp[p] = *reinterpret_cast<const u32x4*>(image + ((s * NP + p) * 64 + lane) * 16);
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int q = 0; q < NP; ++q)
+          if (p + q < NP) S = mfma(mp[p], sp[q], S);
+    }
+    load_move(ahead);
+    next = load_state(a.own, ahead);
   }
 }
 
@@ -898,9 +986,9 @@ hipError_t launch_chunks(DeltaArgs a, hipStream_t st) {
     hipError_t e = launch(delta_walk_kernel<T, DKP, NW, C, false, VEC>,
                           a.value_slices + (a.dk + 32 * NW - 1) / (32 * NW));
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(delta_join_kernel, dim3((unsigned)((a.dv + JOIN_COLS - 1) / JOIN_COLS),
-                                               (unsigned)a.segments, (unsigned)a.heads),
-                       dim3(256), 0, st, a);
+    const dim3 grid((unsigned)((a.dv + 31) / 32), (unsigned)a.segments, (unsigned)a.heads);
+    if (a.dk % 4 == 0) hipLaunchKernelGGL((delta_join_kernel<DKP, true>), grid, dim3(2 * DKP), 0, st, a);
+    else hipLaunchKernelGGL((delta_join_kernel<DKP, false>), grid, dim3(2 * DKP), 0, st, a);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
