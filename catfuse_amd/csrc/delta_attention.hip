@@ -44,7 +44,7 @@ struct DeltaArgs {
   // chunk and head T, the running sums of its log decays and its betas; of each
   // segment and head N, later the state before it, and M
   int64_t* begins;
-  float* solved;
+  char* solved;
   double* falls;
   float* betas;
   float* own;
@@ -135,15 +135,15 @@ __global__ __launch_bounds__(1024) void delta_begins_kernel(DeltaArgs a) {
 }
 
 // T of one chunk and head.  In the workspace T lies as the walk's operands: for
-// each tile of 32 x 32 that is not above the diagonal ((0,0) (1,0) (1,1)) and
-// each half of its columns the eight numbers of each lane: row lane % 32,
-// columns 4 (lane / 32) + 0 .. 3 and the same plus 8 of the half's sixteen.
+// each tile of 32 x 32 that is not above the diagonal ((0,0) (1,0) (1,1)), each half
+// of its columns and each of three parts the eight numbers of each lane: row
+// lane % 32, columns 4 (lane / 32) + 0 .. 3 and the same plus 8 of the half's sixteen.
 //
 // The products k_t . k_s on the matrix cores; blocks of 16 inverted column by
 // column in registers, then joined in pairs by fp32 matrix instructions:
 //   (A 0; B D)^-1 = (A^-1 0; -D^-1 B A^-1 D^-1).
 // Rows of L from the first one that is not finite on are left out, and of T NaN.
-template <int C> constexpr int solved_size() { return (C / 32) * (C / 32 + 1) / 2 * 1024; }
+template <int C> constexpr int solved_size() { return (C / 32) * (C / 32 + 1) / 2 * 6144; }   // bytes
 
 typedef float f4v __attribute__((ext_vector_type(4)));
 
@@ -309,21 +309,26 @@ __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
     __syncthreads();
   }
 
-  float* const to = a.solved + pair * solved_size<C>();
+  char* const to = a.solved + pair * solved_size<C>();
   for (int u = tid; u < TILES * 128; u += NT) {
     const int tile = u >> 7, half = (u >> 6) & 1, l = u & 63;
     const int t = 32 * (tile == 0 ? 0 : 1) + (l & 31);
     const int s0 = 32 * (tile == 2 ? 1 : 0) + 16 * half + 4 * (l >> 5);
+    float x[8];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      Vec<float, 4> y = *reinterpret_cast<const Vec<float, 4>*>(inv + t * P + s0 + 8 * e);
+      const Vec<float, 4> y = *reinterpret_cast<const Vec<float, 4>*>(inv + t * P + s0 + 8 * e);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float x = t >= bad_from ? __builtin_nanf("") : y.v[j];
-        y.v[j] = s0 + 8 * e + j <= t ? x : 0.0f;
+        const float z = t >= bad_from ? __builtin_nanf("") : y.v[j];
+        x[4 * e + j] = s0 + 8 * e + j <= t ? z : 0.0f;
       }
-      *reinterpret_cast<Vec<float, 4>*>(to + u * 8 + 4 * e) = y;
     }
+    u32x4 parts[NP];
+    split8<NP>(x, parts);
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+      *reinterpret_cast<u32x4*>(to + (((u >> 6) * NP + p) * 64 + l) * 16) = parts[p];
   }
 }
 
@@ -354,13 +359,17 @@ void delta_walk_kernel(DeltaArgs a) {
   constexpr int Q_AT = QK_BYTES, V_AT = Q_AT + (OUT ? QK_BYTES : 0), IMAGE = V_AT + V_BYTES;
   __shared__ __attribute__((aligned(512))) char lds[IMAGE];     // of K, Q and V
   __shared__ __attribute__((aligned(16))) char tsh[T_BYTES];    // T, later the scores
-  __shared__ double fall_sh[C];
-  // beta; beta e^g; scale e^g; e^(g_end - g)
+  // S is kept as 2^G times what is stored, G with the decays that went by: most
+  // chunks then need not fade its numbers.
+  __shared__ Vec<float, 2> fall_sh[C];       // a token's sum of log2 decays, of two floats
+  // beta; beta 2^(G + fall); scale 2^(G + fall); 2^(G' - fall), G' after the chunk
   __shared__ __attribute__((aligned(16))) float beta_sh[C], since_sh[C], query_sh[C], end_sh[C];
-  __shared__ float fade_sh[2];               // e^(g_end) as a sum of two
+  // what the numbers fade by (of two floats) if G is set back; whether; 2^G' (of two)
+  __shared__ float fade_sh[5];
 
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t t_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)tsh;
 
   // Heads of one key head and the slices of their columns read the same rows:
   // consecutive workgroups of one XCD (workgroup number mod 8).
@@ -431,14 +440,8 @@ void delta_walk_kernel(DeltaArgs a) {
 
   constexpr int UK = C * (DKP / 8) / NT, UV = C * (DVW / 8) / NT;   // units of a thread
   static_assert(UK * NT == C * (DKP / 8) && UV * NT == C * (DVW / 8), "whole units");
-  // Of T: threads past the last unit take one of another's again.  (Here and at
-  // the powers below no lane is masked off: a register that the compiler spills
-  // inside such a branch is saved for the lanes in it alone.)
-  constexpr int UT = (TILES * 128 + NT - 1) / NT;
-  auto unit = [&](int i) { return tid + NT * i < TILES * 128 ? tid + NT * i : tid % (TILES * 128); };
   Unit<T> ku[UK], vu[UV], qu[OUT ? UK : 1];
-  Vec<float, 4> tu[UT][2];
-  double fall = 0.0;
+  double fall = 0.0, gone = 0.0;             // (G: wave 0's)
   float beta = 0.0f;
   // The next chunk's rows; behind the last chunk the segment's first row again, so
   // that no load is conditional: the registers of one that is not made would stay
@@ -449,12 +452,6 @@ void delta_walk_kernel(DeltaArgs a) {
   auto load_keys = [&]() {
     load_units<T, UK, DKP, NT, VEC>(ku, left > 0 ? kp : k_first, rows(), a.kt, a.dk);
     const int64_t at = left > 0 ? pair : pair_first;
-    const float* const from = a.solved + at * solved_size<C>();
-#pragma unroll
-    for (int i = 0; i < UT; ++i) {
-      tu[i][0] = *reinterpret_cast<const Vec<float, 4>*>(from + unit(i) * 8);
-      tu[i][1] = *reinterpret_cast<const Vec<float, 4>*>(from + unit(i) * 8 + 4);
-    }
     fall = a.falls[at * C + tid % C];
     beta = a.betas[at * C + tid % C];
   };
@@ -482,6 +479,11 @@ void delta_walk_kernel(DeltaArgs a) {
     asm volatile("" : "+v"(at_row), "+v"(at_key), "+v"(at_value));
     const int n = left < C ? left : C;
     __syncthreads();                         // the last chunk's images are read
+    {                                        // T, straight to LDS: landed before it is read
+      const i32x4 from = buffer_of(a.solved + pair * solved_size<C>(), T_BYTES);
+      for (int i = wave; i < T_BYTES / 1024; i += NW)
+        copy16(from, (uint32_t)(lane * 16), (uint32_t)(i * 1024), t_lds + i * 1024);
+    }
 #pragma unroll
     for (int i = 0; i < UK; ++i) {
       const int u = tid + NT * i, row = u / (DKP / 8), piece = u % (DKP / 8);
@@ -493,28 +495,23 @@ void delta_walk_kernel(DeltaArgs a) {
       const int u = tid + NT * i, row = u / (DVW / 8), piece = u % (DVW / 8);
       store_unit<T, C, DVW>(lds + V_AT, vu[i], row, piece);
     }
-#pragma unroll
-    for (int i = 0; i < UT; ++i) {
-      const int u = unit(i);
-      float x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = tu[i][j >> 2].v[j & 3];
-      u32x4 parts[NP];
-      split8<NP>(x, parts);
-#pragma unroll
-      for (int p = 0; p < NP; ++p)
-        *reinterpret_cast<u32x4*>(tsh + (((u >> 6) * NP + p) * 64 + (u & 63)) * 16) = parts[p];
-    }
-    if (wave == 0) {                         // lane: token lane % C
-      const double end = __shfl(fall, C - 1, 64), f = exp2(end);
-      const float e = __builtin_amdgcn_exp2f((float)fall);
-      fall_sh[lane % C] = fall;
+    if (wave == 0) {                         // lane: token lane % C; no lane is masked off
+      const double x = fall + gone, end = __shfl(x, C - 1, 64);
+      const bool fold = __ballot(!(__builtin_fabs(x) <= 24.0)) == 0;
+      const float e = __builtin_amdgcn_exp2f((float)x), high = (float)fall;
+      fall_sh[lane % C] = {high, (float)(fall - (double)high)};
       beta_sh[lane % C] = beta;
       since_sh[lane % C] = beta * e;
       query_sh[lane % C] = a.scale * e;
-      end_sh[lane % C] = __builtin_amdgcn_exp2f((float)(end - fall));
-      fade_sh[0] = (float)f;
-      fade_sh[1] = f < 1e300 ? (float)(f - (double)(float)f) : 0.0f;
+      end_sh[lane % C] = __builtin_amdgcn_exp2f((float)(fold ? -x : end - x));
+      gone = fold ? end : 0.0;
+      auto two = [&](float* to, double f) {
+        to[0] = (float)f;
+        to[1] = f < 1e300 ? (float)(f - (double)to[0]) : 0.0f;
+      };
+      two(fade_sh, exp2(end));
+      fade_sh[2] = fold ? 1.0f : 0.0f;
+      two(fade_sh + 3, exp2(gone));
     }
     __syncthreads();
     left -= n;
@@ -522,8 +519,6 @@ void delta_walk_kernel(DeltaArgs a) {
     vp += C * a.vt;
     qp += C * a.qt;
     pair += a.heads;
-
-    const float fade = fade_sh[0], fade_low = fade_sh[1];
 
     // In what follows the operands of the next products are read, and made, between
     // the products at hand, and the compiler is held to that order (step()).
@@ -533,13 +528,10 @@ void delta_walk_kernel(DeltaArgs a) {
     f16v R[CT], O[OUT ? CT : 1];
     {
       u32x4 sp[SETS][NP], ky[SETS][CT][NL], qy[OUT ? SETS : 1][CT][NL];
-      auto state_part = [&](int s) {         // S's operand, and S faded
+      auto state_part = [&](int s) {
         float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x[j] = S[s / 2][8 * (s & 1) + j];
-          S[s / 2][8 * (s & 1) + j] = __builtin_fmaf(x[j], fade, x[j] * fade_low);
-        }
+        for (int j = 0; j < 8; ++j) x[j] = S[s / 2][8 * (s & 1) + j];
         split8<NP>(x, sp[s % SETS]);
       };
       auto read = [&](int s) {
@@ -656,6 +648,8 @@ void delta_walk_kernel(DeltaArgs a) {
     }
 
     // u = T r, from T's operands in LDS (below O^T from the scores' in their place)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
     f16v U[CT];
     u32x4 tile_op[2][NP];
     auto read_tile = [&](int i) {
@@ -708,14 +702,16 @@ void delta_walk_kernel(DeltaArgs a) {
           if (AHEAD) step();
         }
         const int i = 32 * qt + col;
-        const double gi = fall_sh[i];
+        const Vec<float, 2> gi = fall_sh[i];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           float x[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const int key = 32 * kt + 16 * s + 8 * (j >> 2) + 4 * hi + (j & 3);
-            const float y = acc[8 * s + j] * (a.scale * __builtin_amdgcn_exp2f((float)(gi - fall_sh[key])));
+            const Vec<float, 2> gk = fall_sh[key];
+            const float f = __builtin_amdgcn_exp2f((gi.v[0] - gk.v[0]) + (gi.v[1] - gk.v[1]));
+            const float y = acc[8 * s + j] * (a.scale * f);
             x[j] = i >= key ? y : 0.0f;
           }
           split8<NP>(x, pop[s]);
@@ -765,7 +761,14 @@ void delta_walk_kernel(DeltaArgs a) {
     // and queries as u's get free.
     load_keys();
 
-    // S <- e^(g_end) S (above) + K^T (e^(g_end - g) u)
+    // S <- S + K^T (2^(G' - fall) u), faded first if G is set back
+    if (__builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, fade_sh[2])) == 0) {
+      const float fade = fade_sh[0], low = fade_sh[1];
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[t][r] = __builtin_fmaf(S[t][r], fade, S[t][r] * low);
+    }
     {
       u32x4 bu[SETS][NP], ak[SETS][NL];
       auto key_tile = [&](int i) {
@@ -826,6 +829,13 @@ void delta_walk_kernel(DeltaArgs a) {
 
   float* const to = OUT ? (last ? a.state_out : nullptr) : move ? a.moves : a.own;
   if (to != nullptr) {
+    if (pl.len > 0) {
+      const float fade = fade_sh[3], low = fade_sh[4];
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[t][r] = __builtin_fmaf(S[t][r], fade, S[t][r] * low);
+    }
     const __amdgpu_buffer_rsrc_t rs = state_of(to, OUT ? pl.seq : w);
 #pragma unroll
     for (int t = 0; t < KT; ++t)
@@ -1018,10 +1028,10 @@ CF_API int64_t cf_delta_workspace(const CfDeltaAttentionArgs* p) {
   if (!p || p->heads < 1 || p->seqs < 0 || p->tokens < 0 || p->segment < 0) return -1;
   const CfDeltaAttentionArgs& x = *p;
   const int64_t C = chunk_of(x.dtype, x.dk);
-  const int64_t solved = (C / 32) * (C / 32 + 1) / 2 * 1024;
+  const int64_t solved = (C / 32) * (C / 32 + 1) / 2 * 6144;
   const int64_t chunks = x.cu_seqlens ? x.tokens / C + x.seqs : x.seqs * units_of(x.tokens, C);
   int64_t bytes = x.cu_seqlens ? (8 * (x.seqs + 1) + 255) / 256 * 256 : 0;
-  if (x.tokens > 0) bytes += chunks * x.heads * (4 * solved + 12 * C);
+  if (x.tokens > 0) bytes += chunks * x.heads * (solved + 12 * C);
   if (x.segment > 0 && x.segment < x.tokens) {
     const int64_t segments = x.cu_seqlens ? x.tokens / x.segment + x.seqs
                                           : x.seqs * units_of(x.tokens, x.segment);
@@ -1070,8 +1080,8 @@ CF_API int cf_delta_attention(const CfDeltaAttentionArgs* p) {
   char* at = (char*)x.workspace;
   a.begins = (int64_t*)at;
   if (a.cu) at += (8 * (x.seqs + 1) + 255) / 256 * 256;
-  a.solved = (float*)at;
-  if (x.tokens > 0) at += a.chunks * a.heads * ((C / 32) * (C / 32 + 1) / 2 * 4096);
+  a.solved = at;
+  if (x.tokens > 0) at += a.chunks * a.heads * ((C / 32) * (C / 32 + 1) / 2 * 6144);
   a.falls = (double*)at;
   if (x.tokens > 0) at += a.chunks * a.heads * 8 * C;
   a.betas = (float*)at;

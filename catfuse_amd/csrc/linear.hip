@@ -32,7 +32,6 @@ struct LinearArgs {
 typedef float f4v __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
@@ -309,29 +308,6 @@ __global__ __launch_bounds__(64 * NW) void linear_few_kernel(LinearArgs a) {
       finish<T, OPS, 4>(a, m, n, y, b, {}, false, wide);
     }
   }
-}
-
-// One copy of 16 bytes a lane from a buffer straight to LDS: byte `at` of the
-// buffer (zeros beyond its range), `add` bytes on, to lds + 16 lane.  In
-// assembly, so that the compiler does not wait for it before every read of LDS;
-// the kernel waits before the barrier that lets the copies be read.
-__device__ __forceinline__ void copy16(i32x4 rsrc, uint32_t at, uint32_t add, uint32_t lds) {
-  asm volatile(
-      "s_mov_b32 m0, %3\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %0, %1, %2 offen lds"
-      :
-      : "v"(at), "s"(rsrc), "s"(add), "s"(lds)
-      : "memory");
-}
-__device__ __forceinline__ i32x4 buffer_of(const void* base, uint32_t bytes) {
-  const uint64_t p = (uint64_t)(uintptr_t)base;
-  i32x4 r;
-  r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)p);
-  r[1] = __builtin_amdgcn_readfirstlane((int)((uint32_t)(p >> 32) & 0xffffu));
-  r[2] = __builtin_amdgcn_readfirstlane((int)bytes);
-  r[3] = 0x00020000;
-  return r;
 }
 
 // Many rows.  A workgroup takes BM rows of x and BN columns, in steps of 128

@@ -84,7 +84,7 @@ def test_workspace(dtype, dk, seqs, tokens, cu):
     def count(unit):
         return tokens // unit + seqs if cu else seqs * max(1, -(-tokens // unit))
     begins = (8 * (seqs + 1) + 255) // 256 * 256 if cu else 0
-    chunks = count(C) * H * ((12288 if C == 64 else 4096) + 12 * C) if tokens else 0
+    chunks = count(C) * H * ((18432 if C == 64 else 6144) + 12 * C) if tokens else 0
     for segment in (0, 64, 128, 1024):
         own = count(segment) * H * 4 * dk * (dv + dk) if 0 < segment < tokens else 0
         f = dict(dtype=dtype, dk=dk, dv=dv, heads=H, seqs=seqs, tokens=tokens, cu_seqlens=cu,
