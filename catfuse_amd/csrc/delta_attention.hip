@@ -151,11 +151,14 @@ template <typename T, int DKP, int C, int NT, bool VEC>
 __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
   constexpr int NL = parts_of<T>(), NP = 3, KS = DKP / 16, CT = C / 32, TILES = CT * (CT + 1) / 2;
   constexpr int P = C + 4;
-  __shared__ __attribute__((aligned(512))) char lds[NL * C * DKP * 2];
-  __shared__ __attribute__((aligned(16))) float low[C * P], inv[C * P];
+  constexpr int IMAGE = NL * C * DKP * 2, INVERSE = C * P * 4;
+  // K's image, after the products the inverse
+  __shared__ __attribute__((aligned(512))) char lds[IMAGE > INVERSE ? IMAGE : INVERSE];
+  __shared__ __attribute__((aligned(16))) float low[C * P];
   __shared__ double fall[C];
   __shared__ float beta[C];
   __shared__ int bad_sh;
+  float* const inv = reinterpret_cast<float*>(lds);
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
@@ -248,16 +251,18 @@ __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
     float x[16];
 #pragma unroll
     for (int t = 0; t < 16; ++t) x[t] = t == c ? 1.0f : 0.0f;
-    Vec<float, 4> l[16][4];
+    Vec<float, 4> l[16];
 #pragma unroll
-    for (int t = 1; t < 16; ++t)
+    for (int s = 0; s < 15; ++s) {
+      if (s % 4 == 0) {
 #pragma unroll
-      for (int q = 0; q < (t + 3) / 4; ++q)
-        l[t][q] = *reinterpret_cast<const Vec<float, 4>*>(low + (b0 + t) * P + b0 + 4 * q);
+        for (int t = 1; t < 16; ++t)
+          if (t > s) l[t] = *reinterpret_cast<const Vec<float, 4>*>(low + (b0 + t) * P + b0 + s);
+      }
 #pragma unroll
-    for (int s = 0; s < 15; ++s)
-#pragma unroll
-      for (int t = s + 1; t < 16; ++t) x[t] = __builtin_fmaf(-l[t][s / 4].v[s % 4], x[s], x[t]);
+      for (int t = 1; t < 16; ++t)
+        if (t > s) x[t] = __builtin_fmaf(-l[t].v[s % 4], x[s], x[t]);
+    }
 #pragma unroll
     for (int t = 0; t < 16; ++t) inv[(b0 + t) * P + b0 + c] = x[t];
   } else if (C > 32) {
@@ -440,6 +445,12 @@ void delta_walk_kernel(DeltaArgs a) {
 
   constexpr int UK = C * (DKP / 8) / NT, UV = C * (DVW / 8) / NT;   // units of a thread
   static_assert(UK * NT == C * (DKP / 8) && UV * NT == C * (DVW / 8), "whole units");
+  // T: with the keys where registers are free (the products before it is read are
+  // few there, too few to hide its way), else straight to LDS
+  constexpr bool T_AHEAD = CT == 1;
+  constexpr int UT = T_AHEAD ? (T_BYTES / 16 + NT - 1) / NT : 1;
+  auto unit = [&](int i) { return (tid + NT * i) % (T_BYTES / 16); };   // (some twice)
+  u32x4 tu[UT];
   Unit<T> ku[UK], vu[UV], qu[OUT ? UK : 1];
   double fall = 0.0, gone = 0.0;             // (G: wave 0's)
   float beta = 0.0f;
@@ -452,6 +463,10 @@ void delta_walk_kernel(DeltaArgs a) {
   auto load_keys = [&]() {
     load_units<T, UK, DKP, NT, VEC>(ku, left > 0 ? kp : k_first, rows(), a.kt, a.dk);
     const int64_t at = left > 0 ? pair : pair_first;
+    if constexpr (T_AHEAD)
+#pragma unroll
+      for (int i = 0; i < UT; ++i)
+        tu[i] = *reinterpret_cast<const u32x4*>(a.solved + at * solved_size<C>() + unit(i) * 16);
     fall = a.falls[at * C + tid % C];
     beta = a.betas[at * C + tid % C];
   };
@@ -479,7 +494,10 @@ void delta_walk_kernel(DeltaArgs a) {
     asm volatile("" : "+v"(at_row), "+v"(at_key), "+v"(at_value));
     const int n = left < C ? left : C;
     __syncthreads();                         // the last chunk's images are read
-    {                                        // T, straight to LDS: landed before it is read
+    if constexpr (T_AHEAD) {
+#pragma unroll
+      for (int i = 0; i < UT; ++i) *reinterpret_cast<u32x4*>(tsh + unit(i) * 16) = tu[i];
+    } else {                                 // landed before it is read
       const i32x4 from = buffer_of(a.solved + pair * solved_size<C>(), T_BYTES);
       for (int i = wave; i < T_BYTES / 1024; i += NW)
         copy16(from, (uint32_t)(lane * 16), (uint32_t)(i * 1024), t_lds + i * 1024);
@@ -648,8 +666,10 @@ void delta_walk_kernel(DeltaArgs a) {
     }
 
     // u = T r, from T's operands in LDS (below O^T from the scores' in their place)
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+    if constexpr (!T_AHEAD) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+    }
     f16v U[CT];
     u32x4 tile_op[2][NP];
     auto read_tile = [&](int i) {
@@ -890,28 +910,29 @@ __global__ __launch_bounds__(2 * DKP) void delta_join_kernel(DeltaArgs a) {
   };
   // this lane's numbers of M: its row, columns 16 s + 8 hi .. + 7
   u32x4 m[KS][2];
-  auto load_move = [&](int64_t i) {
-    const __amdgpu_buffer_rsrc_t rs = place(a.moves, i, a.dk);
-    const uint32_t at = 4u * (uint32_t)(row * a.dk + 8 * hi);     // rows from dk on: out of the range
+  const uint32_t m_at = 4u * (uint32_t)(row * a.dk + 8 * hi);     // rows from dk on: out of the range
+  auto load_move = [&](const __amdgpu_buffer_rsrc_t& rs, int s) {
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+    for (int e = 0; e < 2; ++e) {
+      const int c = 16 * s + 8 * hi + 4 * e;
+      if constexpr (VEC) {
+        m[s][e] = __builtin_amdgcn_raw_buffer_load_b128(rs, c < a.dk ? m_at + 4u * (16 * s + 4 * e) : OOB,
+                                                        0, 0);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int c = 16 * s + 8 * hi + 4 * e;
-        if constexpr (VEC) {
-          m[s][e] = __builtin_amdgcn_raw_buffer_load_b128(rs, c < a.dk ? at + 4u * (16 * s + 4 * e) : OOB,
-                                                          0, 0);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            m[s][e][j] = __builtin_amdgcn_raw_buffer_load_b32(
-                rs, c + j < a.dk ? at + 4u * (16 * s + 4 * e + j) : OOB, 0, 0);
-        }
+        for (int j = 0; j < 4; ++j)
+          m[s][e][j] = __builtin_amdgcn_raw_buffer_load_b32(
+              rs, c + j < a.dk ? m_at + 4u * (16 * s + 4 * e + j) : OOB, 0, 0);
       }
+    }
   };
   f16v S = {};
   if (a.state_in != nullptr) S = load_state(a.state_in, pl.seq);
-  load_move(w);
+  {
+    const __amdgpu_buffer_rsrc_t rm = place(a.moves, w, a.dk);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) load_move(rm, s);
+  }
   f16v next = load_state(a.own, w);
   for (int64_t i = 0; i < pl.parts; ++i) {
     const __amdgpu_buffer_rsrc_t rs = place(a.own, w + i, a.dv);
@@ -936,6 +957,8 @@ __global__ __launch_bounds__(2 * DKP) void delta_join_kernel(DeltaArgs a) {
     S = next;
     // (the last segment has none: the first one's again)
     const int64_t ahead = w + (i + 2 < pl.parts ? i + 1 : 0);
+    const __amdgpu_buffer_rsrc_t rm = place(a.moves, ahead, a.dk);
+    next = load_state(a.own, ahead);
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       float x[8];
@@ -946,6 +969,7 @@ __global__ __launch_bounds__(2 * DKP) void delta_join_kernel(DeltaArgs a) {
       }
       u32x4 mp[NP], sp[NP];
       split8<NP>(x, mp);
+      load_move(rm, s);                      // the next step's, in the place of this one's
 #pragma unroll
       for (int p = 0; p < NP; ++p)
         sp[p] = *reinterpret_cast<const u32x4*>(image + ((s * NP + p) * 64 + lane) * 16);
@@ -954,9 +978,8 @@ __global__ __launch_bounds__(2 * DKP) void delta_join_kernel(DeltaArgs a) {
 #pragma unroll
         for (int q = 0; q < NP; ++q)
           if (p + q < NP) S = mfma(mp[p], sp[q], S);
+      step();
     }
-    load_move(ahead);
-    next = load_state(a.own, ahead);
   }
 }
 
