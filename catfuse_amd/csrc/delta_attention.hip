@@ -599,12 +599,21 @@ void delta_walk_kernel(DeltaArgs a) {
       }
     }
 
-    u32x4 rop[CS][NP];                       // r, then u, as operands
-#pragma unroll
-    for (int s = 0; s < CS; ++s) {
+    // u = T r, sixteen tokens of r at a time, made while those before are multiplied.
+    //
+    // A value that is not finite would give NaN wherever it meets a zero of T or
+    // of the scores: r and u are zeros from its token on, and what depends on them
+    // set to NaN below: this lane's column, the queries from the token on and the
+    // state.  (A k, beta or decay that is not finite shows in r too.  The segments'
+    // own states keep it: there NaN goes its way.)
+    int bad_from = C;
+    bool any_bad = false;
+    u32x4 rop[2][NP];                        // r, then u, as operands
+    auto make_r = [&](int s) {
       u32x4 vop[NL];
 #pragma unroll
       for (int p = 0; p < NL; ++p) vop[p] = token_operand<C, DVW>(lds + V_AT, at_value, p, 0, s);
+      float x[8], z = 0.0f;                  // z: NaN if any is not finite
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const Vec<float, 4> b = *reinterpret_cast<const Vec<float, 4>*>(beta_sh + 16 * s + 8 * e + 4 * hi);
@@ -618,83 +627,75 @@ void delta_walk_kernel(DeltaArgs a) {
             const float part = __builtin_bit_cast(float, j & 1 ? word & 0xffff0000u : word << 16);
             y = p == 0 ? part : y + part;
           }
-          const int r = 8 * (s & 1) + 4 * e + j;
-          R[s / 2][r] = __builtin_fmaf(-f.v[j], R[s / 2][r], b.v[j] * y);
+          x[4 * e + j] = __builtin_fmaf(-f.v[j], R[s / 2][8 * (s & 1) + 4 * e + j], b.v[j] * y);
+          if constexpr (OUT) z = __builtin_fmaf(x[4 * e + j], 0.0f, z);
         }
       }
-    }
-    // A value that is not finite would give NaN wherever it meets a zero of T or
-    // of the scores: r and u are zeros from its token on, and what depends on them
-    // set to NaN below: this lane's column, the queries from the token on and the
-    // state.  (A k, beta or decay that is not finite shows in r too.  The segments'
-    // own states keep it: there NaN goes its way.)
-    int bad_from = C;
-    bool any_bad = false;
-    auto take_out = [&](f16v* x) {
+      if constexpr (OUT) {
+        any_bad = any_bad || __ballot(z != z) != 0;
+        if (any_bad) {
 #pragma unroll
-      for (int t = 0; t < CT; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          x[t][r] = 32 * t + 8 * (r >> 2) + 4 * hi + (r & 3) >= bad_from ? 0.0f : x[t][r];
-    };
-    if constexpr (OUT) {
-      float z = 0.0f;                        // NaN if any is not finite
-#pragma unroll
-      for (int t = 0; t < CT; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) z = __builtin_fmaf(R[t][r], 0.0f, z);
-      any_bad = __ballot(z != z) != 0;
-      if (any_bad) {
-#pragma unroll
-        for (int t = 0; t < CT; ++t)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int tok = 32 * t + 8 * (r >> 2) + 4 * hi + (r & 3);
-            bad_from = !(__builtin_fabsf(R[t][r]) < __builtin_inff()) && tok < bad_from ? tok : bad_from;
+          for (int j = 0; j < 8; ++j) {
+            const int tok = 16 * s + 8 * (j >> 2) + 4 * hi + (j & 3);
+            bad_from = !(__builtin_fabsf(x[j]) < __builtin_inff()) && tok < bad_from ? tok : bad_from;
           }
-        const int other = __shfl_xor(bad_from, 32, 64);
-        bad_from = other < bad_from ? other : bad_from;
-        take_out(R);
+          const int other = __shfl_xor(bad_from, 32, 64);
+          bad_from = other < bad_from ? other : bad_from;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            x[j] = 16 * s + 8 * (j >> 2) + 4 * hi + (j & 3) >= bad_from ? 0.0f : x[j];
+        }
       }
-    }
+      split8<NP>(x, rop[s & 1]);
+    };
+    // T's operands in LDS, later the scores' in their place: of the sixteen columns
+    // s, the row tiles that are not above the diagonal
+    u32x4 tile_op[CT][NP];
+    auto rows_of = [&](int s) { return CT == 1 || s >= 2 ? 1 : 2; };
+    auto read_tiles = [&](int s) {
 #pragma unroll
-    for (int s = 0; s < CS; ++s) {
-      float x[8];
+      for (int t = 0; t < CT; ++t)
+        if (t < rows_of(s)) {
+          const int tile = s >= 2 ? 2 : t;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = R[s / 2][8 * (s & 1) + j];
-      split8<NP>(x, rop[s]);
-    }
-
-    // u = T r, from T's operands in LDS (below O^T from the scores' in their place)
+          for (int p = 0; p < NP; ++p)
+            tile_op[t][p] = *reinterpret_cast<const u32x4*>(
+                tsh + (((tile * 2 + (s & 1)) * NP + p) * 64 + lane) * 16);
+        }
+    };
+    make_r(0);
     if constexpr (!T_AHEAD) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
     }
     f16v U[CT];
-    u32x4 tile_op[2][NP];
-    auto read_tile = [&](int i) {
-#pragma unroll
-      for (int p = 0; p < NP; ++p)
-        tile_op[i & 1][p] = *reinterpret_cast<const u32x4*>(tsh + ((i * NP + p) * 64 + lane) * 16);
-    };
-    read_tile(0);
 #pragma unroll
     for (int t = 0; t < CT; ++t) U[t] = f16v{};
+    step();
 #pragma unroll
-    for (int i = 0; i < TILES * 2; ++i) {
-      const int tt = i / 2 == 0 ? 0 : 1, ts = i / 2 == 2 ? 1 : 0, s = 2 * ts + (i & 1);
-      if (i + 1 < TILES * 2) read_tile(i + 1);
+    for (int s = 0; s < CS; ++s) {
+      read_tiles(s);
+      if (s + 1 < CS) make_r(s + 1);
 #pragma unroll
       for (int p = 0; p < NP; ++p)
 #pragma unroll
         for (int y = 0; y < NP; ++y)
-          if (p + y < NP) U[tt] = mfma(tile_op[i & 1][p], rop[s][y], U[tt]);
+#pragma unroll
+          for (int t = 0; t < CT; ++t)
+            if (p + y < NP && t < rows_of(s))
+              U[s >= 2 ? 1 : t] = mfma(tile_op[t][p], rop[s & 1][y], U[s >= 2 ? 1 : t]);
       step();
     }
 
     if constexpr (OUT) {
       if (CT > 1) __syncthreads();           // T is read
-      if (any_bad) take_out(U);
+      if (any_bad) {
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            U[t][r] = 32 * t + 8 * (r >> 2) + 4 * hi + (r & 3) >= bad_from ? 0.0f : U[t][r];
+      }
       // Scores K Q^T of 32 keys (rows) x 32 queries (columns): eight registers
       // on end are an operand of U^T P^T as they lie.  One tile: every wave for
       // itself; three: a tile a wave, exchanged in LDS.
@@ -741,27 +742,29 @@ void delta_walk_kernel(DeltaArgs a) {
               *reinterpret_cast<u32x4*>(tsh + (((wave * 2 + s) * NP + p) * 64 + lane) * 16) = pop[s][p];
         }
       }
-#pragma unroll
-      for (int s = 0; s < CS; ++s) {
+      // O^T += U^T P^T
+      auto make_u = [&](int s) {
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = U[s / 2][8 * (s & 1) + j];
-        split8<NP>(x, rop[s]);
-      }
-      // O^T += U^T P^T
-      if constexpr (CT > 1) {
-        __syncthreads();
-        read_tile(0);
-      }
+        split8<NP>(x, rop[s & 1]);
+      };
+      make_u(0);
+      if constexpr (CT > 1) __syncthreads();
+      step();
 #pragma unroll
-      for (int i = 0; i < TILES * 2; ++i) {
-        const int qt = i / 2 == 0 ? 0 : 1, kt = i / 2 == 2 ? 1 : 0, s = 2 * kt + (i & 1);
-        if (CT > 1 && i + 1 < TILES * 2) read_tile(i + 1);
+      for (int s = 0; s < CS; ++s) {
+        if (CT > 1) read_tiles(s);
+        if (s + 1 < CS) make_u(s + 1);
 #pragma unroll
         for (int x = 0; x < NP; ++x)
 #pragma unroll
           for (int p = 0; p < NP; ++p)
-            if (p + x < NP) O[qt] = mfma(rop[s][x], CT == 1 ? pop[i & 1][p] : tile_op[i & 1][p], O[qt]);
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+              if (p + x < NP && t < rows_of(s))
+                O[s >= 2 ? 1 : t] = mfma(rop[s & 1][x], CT == 1 ? pop[s & 1][p] : tile_op[t][p],
+                                         O[s >= 2 ? 1 : t]);
         step();
       }
       if (any_bad) {
