@@ -76,10 +76,11 @@ __device__ __forceinline__ u32x4 load16(const T* p) {
   __builtin_memcpy(&r, p, 16);
   return r;
 }
-// The first n (0 to all) of the numbers there, zeros behind.
+// The first n of the numbers there, zeros behind.
 template <typename T>
 __device__ __forceinline__ u32x4 load_some(const T* p, int n) {
   constexpr int PER = 16 / sizeof(T);
+  if (n >= PER) return load16(p);
   Vec<T, PER> v;
 #pragma unroll
   for (int i = 0; i < PER; ++i) v.v[i] = i < n ? p[i] : from_f<T>(0.0f);
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(64 * NW) void linear_few_kernel(LinearArgs a) {
   const int n0 = blockIdx.x * 16;
   const int steps = (a.inner + STEP - 1) / STEP, each = (steps + NW - 1) / NW;
   const int first = wave * each, whole = a.inner / STEP;
-  int last = first + each < steps ? first + each : steps;
+  const int last = first + each < steps ? first + each : steps;
   const T *wp[OPS], *xp[MT];
 #pragma unroll
   for (int o = 0; o < OPS; ++o)
@@ -248,31 +249,32 @@ __global__ __launch_bounds__(64 * NW) void linear_few_kernel(LinearArgs a) {
   for (int o = 0; o < OPS; ++o)
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[o][t] = f4v{};
-  int s = first;
   const int full = last < whole ? last : whole;
-  for (; s + U <= full; s += U) {
+  for (int s = first; s < full; s += U) {    // (conditions on s: the same in every lane)
     u32x4 wv[U][OPS], xv[U][MT];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < U; ++u)
+      if (s + u < full) {
 #pragma unroll
-      for (int o = 0; o < OPS; ++o) wv[u][o] = load16(wp[o] + (int64_t)(s + u) * STEP);
+        for (int o = 0; o < OPS; ++o) wv[u][o] = load16(wp[o] + (int64_t)(s + u) * STEP);
 #pragma unroll
-      for (int t = 0; t < MT; ++t) xv[u][t] = load16(xp[t] + (int64_t)(s + u) * STEP);
-    }
+        for (int t = 0; t < MT; ++t) xv[u][t] = load16(xp[t] + (int64_t)(s + u) * STEP);
+      }
 #pragma unroll
     for (int u = 0; u < U; ++u)
+      if (s + u < full)
 #pragma unroll
-      for (int o = 0; o < OPS; ++o)
+        for (int o = 0; o < OPS; ++o)
 #pragma unroll
-        for (int t = 0; t < MT; ++t) acc[o][t] = mfma16<T>(wv[u][o], xv[u][t], acc[o][t]);
+          for (int t = 0; t < MT; ++t) acc[o][t] = mfma16<T>(wv[u][o], xv[u][t], acc[o][t]);
   }
-  for (; s < last; ++s) {                    // the inner dimension's end: zeros behind it
-    const int left = a.inner - s * STEP - quarter * PER;
+  if (first <= whole && last > whole) {       // the inner dimension's end: zeros behind it
+    const int left = a.inner - whole * STEP - quarter * PER;
     u32x4 wv[OPS], xv[MT];
 #pragma unroll
-    for (int o = 0; o < OPS; ++o) wv[o] = load_some(wp[o] + (int64_t)s * STEP, left);
+    for (int o = 0; o < OPS; ++o) wv[o] = load_some(wp[o] + (int64_t)whole * STEP, left);
 #pragma unroll
-    for (int t = 0; t < MT; ++t) xv[t] = load_some(xp[t] + (int64_t)s * STEP, left);
+    for (int t = 0; t < MT; ++t) xv[t] = load_some(xp[t] + (int64_t)whole * STEP, left);
 #pragma unroll
     for (int o = 0; o < OPS; ++o)
 #pragma unroll
@@ -433,11 +435,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile_kernel(LinearArgs
 
   // Results: 32 rows at a time turned through LDS, each wave for itself, so that
   // eight columns on end of a row are a lane's and a row's lanes lie on end.  The
-  // residual's first rows are loaded here, the others AHEAD turns before they are
-  // added: with one workgroup a CU nothing else would cover their way.
+  // residual's first rows are loaded here, the others a turn before they are added:
+  // with one workgroup a CU nothing else would cover their way.
   float* const turn = reinterpret_cast<float*>(lds + wave * TURN);
-  constexpr int LANES = TN * 4, PARTS = 32 * LANES / 64, TURNS = TM * PARTS;   // LANES of a row
-  constexpr int AHEAD = TURNS < 16 / (int)sizeof(T) ? TURNS : 16 / (int)sizeof(T);
+  constexpr int LANES = TN * 4, PARTS = 32 * LANES / 64;      // LANES of a row
   const int nc = lane % LANES * 8, n = n0 + wn * (BN / WN) + nc;
   const int64_t mt = m0 + wm * (BM / WM) + lane / LANES;
   const bool wide = wide_columns<T>(a);
@@ -447,10 +448,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile_kernel(LinearArgs
     return *reinterpret_cast<const Vec<T, 8>*>((const T*)a.residual + (m < a.rows ? m : a.rows - 1) * a.rr +
                                                (n < a.cols ? n : 0));
   };
-  Vec<T, 8> ahead[AHEAD];
+  Vec<T, 8> ahead[PARTS];
   if (early) {
 #pragma unroll
-    for (int d = 0; d < AHEAD; ++d) ahead[d] = residual_at(d);
+    for (int q = 0; q < PARTS; ++q) ahead[q] = residual_at(q);
   }
   float b[OPS][8];
 #pragma unroll
@@ -496,41 +497,43 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile_kernel(LinearArgs
   }
   meet();                               // LDS is free for the results
 #pragma unroll 1
-  for (int t = 0; t < TURNS; ++t) {
-    if (t % PARTS == 0) {
+  for (int j = 0; j < TM; ++j) {
 #pragma unroll
-      for (int j = 0; j < TM; ++j)
-        if (t == j * PARTS) {
+    for (int c = 0; c < TM; ++c)
+      if (j == c) {
 #pragma unroll
-          for (int i = 0; i < OPS * TN; ++i)
+        for (int i = 0; i < OPS * TN; ++i)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              Vec<float, 4> y;
+          for (int g = 0; g < 4; ++g) {
+            Vec<float, 4> y;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) y.v[e] = acc[i][j][4 * g + e];
-              *reinterpret_cast<Vec<float, 4>*>(turn + col * PITCH + 32 * i + 8 * g + 4 * hi) = y;
-            }
-        }
-    }
-    const int r = t % PARTS * (64 / LANES) + lane / LANES;
-    const int64_t m = mt + t * (64 / LANES);
-    float y[OPS][8];
-#pragma unroll
-    for (int o = 0; o < OPS; ++o)
-#pragma unroll
-      for (int e = 0; e < 8; e += 4) {
-        const Vec<float, 4> v =
-            *reinterpret_cast<const Vec<float, 4>*>(turn + r * PITCH + o * TN * 32 + nc + e);
-#pragma unroll
-        for (int f = 0; f < 4; ++f) y[o][e + f] = v.v[f];
+            for (int e = 0; e < 4; ++e) y.v[e] = acc[i][c][4 * g + e];
+            *reinterpret_cast<Vec<float, 4>*>(turn + col * PITCH + 32 * i + 8 * g + 4 * hi) = y;
+          }
       }
-    const Vec<T, 8> now = ahead[0];
-    if (early) {
+    Vec<T, 8> now[PARTS];
 #pragma unroll
-      for (int d = 0; d + 1 < AHEAD; ++d) ahead[d] = ahead[d + 1];
-      if (t + AHEAD < TURNS) ahead[AHEAD - 1] = residual_at(t + AHEAD);
+    for (int q = 0; q < PARTS; ++q) now[q] = ahead[q];
+    if (early && j + 1 < TM) {
+#pragma unroll
+      for (int q = 0; q < PARTS; ++q) ahead[q] = residual_at((j + 1) * PARTS + q);
     }
-    if (m < a.rows && n < a.cols) finish8<T, OPS>(a, m, n, split, y, b, now, early, wide);
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) {
+      const int r = q * (64 / LANES) + lane / LANES;
+      const int64_t m = mt + (j * PARTS + q) * (64 / LANES);
+      float y[OPS][8];
+#pragma unroll
+      for (int o = 0; o < OPS; ++o)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+          const Vec<float, 4> v =
+              *reinterpret_cast<const Vec<float, 4>*>(turn + r * PITCH + o * TN * 32 + nc + e);
+#pragma unroll
+          for (int f = 0; f < 4; ++f) y[o][e + f] = v.v[f];
+        }
+      if (m < a.rows && n < a.cols) finish8<T, OPS>(a, m, n, split, y, b, now[q], early, wide);
+    }
   }
 }
 
