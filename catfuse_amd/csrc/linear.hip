@@ -30,7 +30,6 @@ struct LinearArgs {
 };
 
 typedef float f4v __attribute__((ext_vector_type(4)));
-typedef float f16v __attribute__((ext_vector_type(16)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -39,22 +38,7 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 // `b`: its columns): 8 numbers of 16 bits, or 4 of 32 taken one at a time (the
 // same ones of both operands, in whatever order).
 template <typename T>
-__device__ __forceinline__ f16v mfma32(u32x4 a, u32x4 b, f16v c) {
-  if constexpr (sizeof(T) == 4) {
-    const f4v x = __builtin_bit_cast(f4v, a), y = __builtin_bit_cast(f4v, b);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
-    return c;
-  } else if constexpr (__is_same(T, bf16_t)) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a),
-                                                   __builtin_bit_cast(bf8, b), c, 0, 0, 0);
-  } else {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a),
-                                                  __builtin_bit_cast(h8, b), c, 0, 0, 0);
-  }
-}
-template <typename T>
-__device__ __forceinline__ f4v mfma16(u32x4 a, u32x4 b, f4v c) {
+__device__ __forceinline__ f4v mfma(u32x4 a, u32x4 b, f4v c) {
   if constexpr (sizeof(T) == 4) {
     const f4v x = __builtin_bit_cast(f4v, a), y = __builtin_bit_cast(f4v, b);
 #pragma unroll
@@ -266,7 +250,7 @@ __global__ __launch_bounds__(64 * NW) void linear_few_kernel(LinearArgs a) {
 #pragma unroll
         for (int o = 0; o < OPS; ++o)
 #pragma unroll
-          for (int t = 0; t < MT; ++t) acc[o][t] = mfma16<T>(wv[u][o], xv[u][t], acc[o][t]);
+          for (int t = 0; t < MT; ++t) acc[o][t] = mfma<T>(wv[u][o], xv[u][t], acc[o][t]);
   }
   if (first <= whole && last > whole) {       // the inner dimension's end: zeros behind it
     const int left = a.inner - whole * STEP - quarter * PER;
@@ -278,7 +262,7 @@ __global__ __launch_bounds__(64 * NW) void linear_few_kernel(LinearArgs a) {
 #pragma unroll
     for (int o = 0; o < OPS; ++o)
 #pragma unroll
-      for (int t = 0; t < MT; ++t) acc[o][t] = mfma16<T>(wv[o], xv[t], acc[o][t]);
+      for (int t = 0; t < MT; ++t) acc[o][t] = mfma<T>(wv[o], xv[t], acc[o][t]);
   }
 #pragma unroll
   for (int o = 0; o < OPS; ++o)
@@ -312,17 +296,23 @@ __global__ __launch_bounds__(64 * NW) void linear_few_kernel(LinearArgs a) {
   }
 }
 
+template <int N> struct Count { static constexpr int value = N; };
+
 // Many rows.  A workgroup takes BM rows of x and BN columns, in steps of 128
 // bytes of the inner dimension (whole lines: half as many a step, four stages,
-// took 642 us where this takes 570, 16384 x 4096 x 4096 bf16), two stages of LDS.
-// Waves WM x WN, each BM / WM rows and BN / WN columns of each product: results as
-// accumulators of 32 columns (their rows) by 32 rows of x (their columns).
+// took 642 us where 570 were taken otherwise, 16384 x 4096 x 4096 bf16), two stages
+// of LDS.  Waves WM x WN, each BM / WM rows and BN / WN columns of each product:
+// results as accumulators of 16 columns (their rows) by 16 rows of x (their
+// columns).  Bound by the card's power rather than by its matrix cores' cycles
+// (63 % of them at 1.6 GHz): products of 16 x 16 x 32, which move half the sums of
+// those of 32 x 32 x 16, took 1107 us where the latter took 1219 (gated, 8192 x 4096
+// x 11264 bf16), and eight waves of 128 x 64 less than four of 128 x 128 (487).
 //
-// A step has four parts (32 bytes of a row for a lane pair).  A part's operands
-// are read from LDS between the products of the part before; before a step's last
-// products the waves meet, when all its operands are in registers and the next
-// stage's copies have landed: the last products then cover the first reads of
-// that stage and the start of the copies into the stage just read.
+// A step has two parts (64 bytes of a row).  A part's operands are read from LDS
+// between the products of the part before; before a step's last products the waves
+// meet, when all its operands are in registers and the next stage's copies have
+// landed: the last products then cover the first reads of that stage and the start
+// of the copies into the stage just read.
 //
 // LDS rows of 128 bytes, their eight pieces exchanged by row (piece ^ row / 2 % 8):
 // sixteen rows on end then spread over all 64 banks.
@@ -330,17 +320,17 @@ __global__ __launch_bounds__(64 * NW) void linear_few_kernel(LinearArgs a) {
 // VEC: rows in pieces of 16 bytes, aligned and whole, not overlapping, copied
 // straight to LDS; else through registers, element by element at the inner
 // dimension's end.
-template <typename T, int BM, int BN, int WM, int WN, int OPS, bool VEC>
+template <typename T, int BM, int BN, int WM, int WN, int NST, int OPS, bool VEC>
 __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile_kernel(LinearArgs a) {
   constexpr int NW = WM * WN, PER = 16 / sizeof(T), STEP = 8 * PER;
   constexpr int ROWS = BM + OPS * BN, STAGE = ROWS * 128;
-  constexpr int TM = BM / WM / 32, TN = BN / WN / 32, WIDE = OPS * TN * 32;
+  constexpr int TM = BM / WM / 16, TN = BN / WN / 16, WIDE = OPS * TN * 16;
   static_assert(ROWS % (8 * NW) == 0 && BM % 8 == 0 && BN % 8 == 0 && NW % 2 == 0, "whole copies");
   // the epilogue turns 32 rows of a wave's results at a time
   constexpr int PITCH = WIDE + 4, TURN = 32 * PITCH * 4;
-  constexpr int LDS = 2 * STAGE > NW * TURN ? 2 * STAGE : NW * TURN;
+  constexpr int LDS = NST * STAGE > NW * TURN ? NST * STAGE : NW * TURN;
   __shared__ __attribute__((aligned(1024))) char lds[LDS];
-  const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, col = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, quarter = lane >> 4, col = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
 
   // Tiles in bands of eight rows of them, a band column by column; each XCD
@@ -388,7 +378,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile_kernel(LinearArgs
     const int base = 8 * wave + 8 * NW * i, k = (from + step) * STEP + piece * PER;
     const int o = OPS == 2 && base >= BM + BN ? 1 : 0;
     if constexpr (VEC) {
-      copy16(base < BM ? xb : wb[o], k < a.inner ? at[i] : 0x80000000u, (uint32_t)((from + step) * 128),
+      copy16(base < BM ? xb : wb[o], k < a.inner && step < steps ? at[i] : 0x80000000u, (uint32_t)((from + step) * 128),
              lds0 + stage * STAGE + base * 128);
     } else {
       const int r = base + (lane >> 3);
@@ -410,27 +400,29 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile_kernel(LinearArgs
         *reinterpret_cast<u32x4*>(lds + stage * STAGE + (8 * wave + 8 * NW * i) * 128 + lane * 16) = regs[i];
     }
   };
-  auto meet = [&]() {                        // copies have landed, reads are done
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  // The next step's copies have landed (as many as later steps' may be on their
+  // way), reads are done.
+  auto meet = [&](auto later) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(decltype(later)::value * COPIES) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
 
-  f16v acc[OPS * TN][TM];
+  f4v acc[OPS * TN][TM];
 #pragma unroll
   for (int i = 0; i < OPS * TN; ++i)
 #pragma unroll
-    for (int j = 0; j < TM; ++j) acc[i][j] = f16v{};
+    for (int j = 0; j < TM; ++j) acc[i][j] = f4v{};
 
   const char* const xs = lds + (wm * (BM / WM) + col) * 128;
   const char* const ws = lds + (BM + wn * (BN / WN) + col) * 128;
   constexpr int READS = TM + OPS * TN, PRODUCTS = TM * OPS * TN;
   u32x4 xv[2][TM], wv[2][OPS * TN];
   auto read = [&](int stage, int s, int i) {
-    const int off = stage * STAGE + (((2 * s + hi) ^ ((col >> 1) & 7)) << 4);
-    if (i < TM) xv[s & 1][i] = *reinterpret_cast<const u32x4*>(xs + i * 32 * 128 + off);
+    const int off = stage * STAGE + (((4 * s + quarter) ^ (col >> 1)) << 4);
+    if (i < TM) xv[s & 1][i] = *reinterpret_cast<const u32x4*>(xs + i * 16 * 128 + off);
     else wv[s & 1][i - TM] =
-        *reinterpret_cast<const u32x4*>(ws + ((i - TM) / TN * BN + (i - TM) % TN * 32) * 128 + off);
+        *reinterpret_cast<const u32x4*>(ws + ((i - TM) / TN * BN + (i - TM) % TN * 16) * 128 + off);
   };
 
   // Results: 32 rows at a time turned through LDS, each wave for itself, so that
@@ -438,7 +430,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile_kernel(LinearArgs
   // residual's first rows are loaded here, the others a turn before they are added:
   // with one workgroup a CU nothing else would cover their way.
   float* const turn = reinterpret_cast<float*>(lds + wave * TURN);
-  constexpr int LANES = TN * 4, PARTS = 32 * LANES / 64;      // LANES of a row
+  constexpr int LANES = TN * 2, PARTS = 32 * LANES / 64;      // LANES of a row
   const int nc = lane % LANES * 8, n = n0 + wn * (BN / WN) + nc;
   const int64_t mt = m0 + wm * (BM / WM) + lane / LANES;
   const bool wide = wide_columns<T>(a);
@@ -448,6 +440,52 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile_kernel(LinearArgs
     return *reinterpret_cast<const Vec<T, 8>*>((const T*)a.residual + (m < a.rows ? m : a.rows - 1) * a.rr +
                                                (n < a.cols ? n : 0));
   };
+
+  if (steps > 0) {
+    fetch_all(0, 0);
+    deposit(0);
+    if constexpr (NST > 2) {
+#pragma unroll
+      for (int i = 1; i < NST; ++i) fetch_all(i, i);
+      meet(Count<NST - 1>());
+    } else {
+      meet(Count<0>());
+      if (steps > 1) fetch_all(1, 1);
+    }
+#pragma unroll
+    for (int i = 0; i < READS; ++i) read(0, 0, i);
+  }
+  for (int step = 0; step < steps; ++step) {
+    const int stage = step % NST, next = (step + 1) % NST;
+    const bool more = step + 1 < steps, copies = NST > 2 || step + NST < steps;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (s == 1) {
+        if (more) deposit(next);
+        meet(Count<NST - 2>());
+        __builtin_amdgcn_s_setprio(1);
+      }
+      if (s == 0) __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+      for (int p = 0; p < PRODUCTS; ++p) {
+        const int i = p / TM, j = p % TM;
+        acc[i][j] = mfma<T>(wv[s & 1][i], xv[s & 1][j], acc[i][j]);
+        // spread over the products: the next part's reads, and in the last part
+        // the copies of the stage that takes this one's place
+#pragma unroll
+        for (int r = p * READS / PRODUCTS; r < (p + 1) * READS / PRODUCTS; ++r) {
+          if (s == 0) read(stage, 1, r);
+          else if (more) read(next, 0, r);
+        }
+        if (s == 1 && copies)
+#pragma unroll
+          for (int c = p * COPIES / PRODUCTS; c < (p + 1) * COPIES / PRODUCTS; ++c)
+            fetch(stage, step + NST, c);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  meet(Count<0>());                     // LDS is free for the results
   Vec<T, 8> ahead[PARTS];
   if (early) {
 #pragma unroll
@@ -458,63 +496,21 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile_kernel(LinearArgs
   for (int o = 0; o < OPS; ++o)
 #pragma unroll
     for (int e = 0; e < 8; ++e) b[o][e] = bias_of<T>(a, o, n + e < a.cols ? n + e : a.cols - 1);
-
-  if (steps > 0) {
-    fetch_all(0, 0);
-    deposit(0);
-    meet();
-    if (steps > 1) fetch_all(1, 1);
-#pragma unroll
-    for (int i = 0; i < READS; ++i) read(0, 0, i);
-  }
-  for (int step = 0; step < steps; ++step) {
-    const int stage = step & 1, next = stage ^ 1;
-    const bool more = step + 1 < steps, two = step + 2 < steps;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      if (s == 3) {
-        if (more) deposit(next);
-        meet();
-      }
-#pragma unroll
-      for (int p = 0; p < PRODUCTS; ++p) {
-        const int i = p / TM, j = p % TM;
-        acc[i][j] = mfma32<T>(wv[s & 1][i], xv[s & 1][j], acc[i][j]);
-        // spread over the products: the next part's reads, and in the last part
-        // the copies of the stage that takes this one's place
-#pragma unroll
-        for (int r = p * READS / PRODUCTS; r < (p + 1) * READS / PRODUCTS; ++r) {
-          if (s < 3) read(stage, s + 1, r);
-          else if (more) read(next, 0, r);
-        }
-        if (s == 3 && two)
-#pragma unroll
-          for (int c = p * COPIES / PRODUCTS; c < (p + 1) * COPIES / PRODUCTS; ++c)
-            fetch(stage, step + 2, c);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-  }
-  meet();                               // LDS is free for the results
 #pragma unroll 1
-  for (int j = 0; j < TM; ++j) {
+  for (int j = 0; j < TM / 2; ++j) {
 #pragma unroll
     for (int c = 0; c < TM; ++c)
-      if (j == c) {
+      if (j == c / 2) {
 #pragma unroll
-        for (int i = 0; i < OPS * TN; ++i)
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            Vec<float, 4> y;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y.v[e] = acc[i][c][4 * g + e];
-            *reinterpret_cast<Vec<float, 4>*>(turn + col * PITCH + 32 * i + 8 * g + 4 * hi) = y;
-          }
+        for (int i = 0; i < OPS * TN; ++i) {
+          const Vec<float, 4> y = {acc[i][c][0], acc[i][c][1], acc[i][c][2], acc[i][c][3]};
+          *reinterpret_cast<Vec<float, 4>*>(turn + (16 * (c & 1) + col) * PITCH + 16 * i + 4 * quarter) = y;
+        }
       }
     Vec<T, 8> now[PARTS];
 #pragma unroll
     for (int q = 0; q < PARTS; ++q) now[q] = ahead[q];
-    if (early && j + 1 < TM) {
+    if (early && j + 1 < TM / 2) {
 #pragma unroll
       for (int q = 0; q < PARTS; ++q) ahead[q] = residual_at((j + 1) * PARTS + q);
     }
@@ -528,7 +524,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile_kernel(LinearArgs
 #pragma unroll
         for (int e = 0; e < 8; e += 4) {
           const Vec<float, 4> v =
-              *reinterpret_cast<const Vec<float, 4>*>(turn + r * PITCH + o * TN * 32 + nc + e);
+              *reinterpret_cast<const Vec<float, 4>*>(turn + r * PITCH + o * TN * 16 + nc + e);
 #pragma unroll
           for (int f = 0; f < 4; ++f) y[o][e + f] = v.v[f];
         }
@@ -567,6 +563,21 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a) {
 }
 
 // How a product is taken.
+// Which kernel, in what pieces.  The times are of bf16.
+//   rows <= 32, and <= 8 or few columns: few rows (7 gated rows of 4096 x 11264 42.0
+//     us, tiles 43.4; 32 of 512 x 1000 4.3 and 6.0).  Else tiles read w no slower and
+//     x less often (32 gated rows of 4096 x 11264: 45 us, few rows 59; 32 of 4096 x
+//     4096 13.1 and 14.2).
+//   256: most work a byte read from L2, one workgroup a CU.  From 5/8 of a tile a CU
+//     on (160 tiles, 2560 x 4096 x 4096: 87 us, 128 112; 128 tiles 82, 128 67).  Not for
+//     32-bit numbers, whose matrix instructions bound every tile alike.
+//   128, two stages and two workgroups a CU: more than a tile a CU (384 tiles, 1500 x
+//     4096 x 4096: 56 us, four stages 67).
+//   128, four stages: more than half a tile a CU (256 tiles, 1024 x 4096 x 4096: 37 us,
+//     two stages 44, 64 54; 192 tiles 34 and 64 46; 128 tiles 32 and 64 28).
+//   64: four stages, two workgroups a CU.  Of long rows that give less than a tile a CU
+//     the inner dimension is split, 16 steps and more a split (64 x 4096 x 4096: 19.6
+//     us whole, 14.1 in four; 256 x 2048 x 2048 would be 13.7 in two, and takes 12.0).
 struct Plan { int few, size, splits, split_steps; };   // few: waves of the few-rows kernel, or 0
 
 constexpr int FEW_ROWS = 32;
@@ -574,26 +585,27 @@ constexpr int CUS = 256;
 
 inline Plan plan_of(const CfLinearArgs& x, bool gated, bool vec) {
   Plan p = {0, 0, 1, 0};
-  const int64_t step = x.dtype == SEQ_F32 ? 32 : 64, steps = (x.inner + step - 1) / step;
-  if (x.rows <= FEW_ROWS) {
+  const bool f32 = x.dtype == SEQ_F32;
+  const int64_t step = f32 ? 32 : 64, steps = (x.inner + step - 1) / step;
+  const int half = gated ? 2 : 1;
+  auto tiles = [&](int64_t bm, int64_t bn) {
+    return ((x.rows + bm - 1) / bm) * ((x.cols + bn / half - 1) / (bn / half));
+  };
+  if (x.rows <= FEW_ROWS && (!vec || x.rows <= 8 || x.rows * tiles(64, 64) < 8 * CUS)) {
     p.few = (x.cols + 15) / 16 >= 2 * CUS ? 4 : 8;
     return p;
   }
-  auto tiles = [&](int64_t bm, int64_t bn) {
-    return ((x.rows + bm - 1) / bm) * ((x.cols + bn - 1) / bn);
-  };
-  const int half = gated ? 2 : 1;
-  p.size = vec && tiles(256, 256 / half) >= CUS ? 256 : tiles(128, 128 / half) >= CUS ? 128 : 64;
-  const int64_t n = tiles(p.size, p.size / half);
-  if (n < CUS && steps >= 16) {
+  p.size = vec && !f32 && 8 * tiles(256, 256) >= 5 * CUS ? 256 : 2 * tiles(128, 128) > CUS ? 128 : 64;
+  p.split_steps = (int)steps;
+  const int64_t n = tiles(64, 64), least = f32 ? 8 : 16;   // (a step of 32 bits takes twice as long)
+  if (p.size == 64 && n < CUS && steps >= 3 * least) {
     int64_t splits = CUS / n;
-    if (splits > steps / 8) splits = steps / 8;
+    if (splits > steps / least) splits = steps / least;
     if (splits > 1) {
       p.split_steps = (int)((steps + splits - 1) / splits);
       p.splits = (int)((steps + p.split_steps - 1) / p.split_steps);
     }
   }
-  if (p.splits <= 1) p.splits = 1, p.split_steps = (int)steps;
   return p;
 }
 
@@ -614,13 +626,13 @@ hipError_t launch_few(const LinearArgs& a, int waves, hipStream_t st) {
   return hipGetLastError();
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int OPS, bool VEC>
+template <typename T, int BM, int BN, int WM, int WN, int NST, int OPS, bool VEC>
 hipError_t launch_tiles(LinearArgs a, hipStream_t st) {
   const int64_t rt = (a.rows + BM - 1) / BM, ct = (a.cols + BN - 1) / BN;
   if (rt * ct > 0xffffffffll / (64 * WM * WN) / a.splits) return hipErrorInvalidValue;
   a.row_tiles = (int)rt;
   a.col_tiles = (int)ct;
-  hipLaunchKernelGGL((linear_tile_kernel<T, BM, BN, WM, WN, OPS, VEC>),
+  hipLaunchKernelGGL((linear_tile_kernel<T, BM, BN, WM, WN, NST, OPS, VEC>),
                      dim3((unsigned)(rt * ct), (unsigned)a.splits), dim3(64 * WM * WN), 0, st, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.parts == nullptr) return e;
@@ -632,10 +644,15 @@ hipError_t launch_tiles(LinearArgs a, hipStream_t st) {
 template <typename T, int OPS, bool VEC>
 hipError_t launch_sizes(const LinearArgs& a, const Plan& p, hipStream_t st) {
   constexpr int N = OPS == 2 ? 2 : 1;
-  if constexpr (VEC)
-    if (p.size == 256) return launch_tiles<T, 256, 256 / N, 2, 4, OPS, true>(a, st);
-  if (p.size == 128) return launch_tiles<T, 128, 128 / N, 2, 2, OPS, VEC>(a, st);
-  return launch_tiles<T, 64, 64 / N, 2, 2 / N, OPS, VEC>(a, st);
+  if constexpr (VEC && sizeof(T) == 2)
+    if (p.size == 256) return launch_tiles<T, 256, 256 / N, 2, 4, 2, OPS, true>(a, st);
+  if (p.size == 128) {
+    if constexpr (VEC)
+      if (((a.rows + 127) / 128) * ((a.cols + 128 / N - 1) / (128 / N)) <= CUS)
+        return launch_tiles<T, 128, 128 / N, 2, 4, 4, OPS, true>(a, st);
+    return launch_tiles<T, 128, 128 / N, 2, 4, 2, OPS, VEC>(a, st);
+  }
+  return launch_tiles<T, 64, 64 / N, 2, 2, VEC ? 4 : 2, OPS, VEC>(a, st);
 }
 
 template <typename T, int OPS>
@@ -650,9 +667,9 @@ hipError_t launch_ops(const LinearArgs& a, const Plan& p, bool vec, hipStream_t 
 }
 
 // Whether x and w have rows of whole aligned 16-byte pieces that do not overlap,
-// 256 of them within 2^31 bytes.  (The plan of a workspace's size takes addresses
-// for aligned: the plans differ in splits only where there are few tiles, which
-// the tile of 256 never is for.)
+// 256 of them within 2^31 bytes.  (The plan of a workspace's size takes rows for
+// such ones.  For others it asks for as much or more: only tiles of 64 are split,
+// by their number, and more than half a tile of 128 a CU is more than a tile of 64.)
 inline bool whole_pieces(const CfLinearArgs& x) {
   const int size = x.dtype == SEQ_F32 ? 4 : 2, per = 16 / size;
   auto vec = [&](const void* base, int64_t stride) {

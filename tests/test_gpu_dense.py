@@ -106,6 +106,18 @@ def test_large(cuda, dtype, M, K, N, gated):
     _check(_run(x, ws, bs, "silu", r), x, ws, bs, "silu", r)
 
 
+# more than half a tile of 128 x 128 a CU, with fewer steps than stages and with more,
+# whole and not; few rows of many columns; long rows split in steps, the last shorter
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("M,K,N", [(1030, 64, 2100), (1100, 136, 2304), (1024, 320, 2048), (17000, 200, 24),
+                                   (40, 72, 17000), (600, 201, 6000), (10, 264, 16500), (32, 1032, 6200),
+                                   (24, 1029, 6200), (64, 4096, 200), (100, 4200, 160), (40, 1607, 200)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_tiles(cuda, dtype, M, K, N, gated):
+    x, ws, bs, r = _make(cuda, M, K, N, dtype, M, gated, dtype, residual=not gated)
+    _check(_run(x, ws, bs, "gelu", r), x, ws, bs, "gelu", r)
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("M", [5, 200])
 def test_activations(cuda, act, M):
