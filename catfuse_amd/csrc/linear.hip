@@ -79,34 +79,40 @@ __device__ __forceinline__ float exp_f(float x) {
   // (an infinite or vanished power stays one)
   return __builtin_fabsf(y) < 126.0f ? __builtin_fmaf(e, low * 0.693147182f, e) : e;
 }
-__device__ __forceinline__ float sigmoid_times(float z, float t) {   // z / (1 + e^-t)
-  return z * __builtin_amdgcn_rcpf(1.0f + exp_f(-t));
+// z / (1 + e^-t).  For outputs of 16 bits the power of two alone will do: off by
+// |t| u, which e^-t or 1 beside it makes less than u.
+template <typename T>
+__device__ __forceinline__ float sigmoid_times(float z, float t) {
+  const float e = sizeof(T) == 4 ? exp_f(-t) : __builtin_amdgcn_exp2f(t * -1.44269502f);
+  return z * __builtin_amdgcn_rcpf(1.0f + e);
 }
-// 1 + erf(x / sqrt(2)) by Abramowitz and Stegun's formula 7.1.26, to 1.5e-7.
-__device__ __forceinline__ float one_plus_erf(float x) {
-  const float y = __builtin_fabsf(x) * 0.707106781f, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, y, 1.0f));
-  float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-  p = __builtin_fmaf(p, t, 1.421413741f);
-  p = __builtin_fmaf(p, t, -0.284496736f);
-  p = __builtin_fmaf(p, t, 0.254829592f) * t;
-  const float tail = p * __builtin_amdgcn_exp2f(y * y * -1.44269504f);    // 1 - erf(y)
-  return x < 0.0f ? tail : 2.0f - tail;
+// x (1 + erf(x / sqrt(2))) / 2 = max(x, 0) - |x| (1 - erf(|x| / sqrt(2))) / 2, the
+// latter by Abramowitz and Stegun's formula 7.1.26, to 1.5e-7 of |x| / 2.
+__device__ __forceinline__ float gelu(float x) {
+  const float y = __builtin_fabsf(x), t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.231641888f, y, 1.0f));
+  float p = __builtin_fmaf(0.530702715f, t, -0.726576014f);
+  p = __builtin_fmaf(p, t, 0.710706871f);
+  p = __builtin_fmaf(p, t, -0.142248368f);
+  p = __builtin_fmaf(p, t, 0.127414796f) * t;
+  const float tail = p * __builtin_amdgcn_exp2f(x * x * -0.721347520f);
+  // (beyond 20 the tail is none, and infinity takes none of it)
+  return __builtin_fmaf(-__builtin_fminf(y, 20.0f), tail, __builtin_fmaxf(x, 0.0f));
 }
-template <int N>
+template <typename T, int N>
 __device__ __forceinline__ void activate(float* z, int kind) {
   if (kind == CF_ACT_RELU) {
 #pragma unroll
     for (int j = 0; j < N; ++j) z[j] = z[j] < 0.0f ? 0.0f : z[j];
   } else if (kind == CF_ACT_SILU) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) z[j] = sigmoid_times(z[j], z[j]);
+    for (int j = 0; j < N; ++j) z[j] = sigmoid_times<T>(z[j], z[j]);
   } else if (kind == CF_ACT_GELU) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) z[j] = 0.5f * z[j] * one_plus_erf(z[j]);
+    for (int j = 0; j < N; ++j) z[j] = gelu(z[j]);
   } else if (kind == CF_ACT_GELU_TANH) {     // 1 + tanh(t) = 2 / (1 + e^(-2 t))
 #pragma unroll
     for (int j = 0; j < N; ++j)
-      z[j] = sigmoid_times(z[j], 1.59576912f * __builtin_fmaf(0.044715f * z[j] * z[j], z[j], z[j]));
+      z[j] = sigmoid_times<T>(z[j], z[j] * __builtin_fmaf(0.0713548163f * z[j], z[j], 1.59576912f));
   }
 }
 
@@ -149,11 +155,13 @@ __device__ __forceinline__ void finish(const LinearArgs& a, int64_t m, int n, co
   }
 #pragma unroll
   for (int j = 0; j < COUNT; ++j) y[j] = s[0][j] + b[0][j];
-  activate<COUNT>(y, a.activation);
+  activate<T, COUNT>(y, a.activation);
+  if constexpr (OPS == 2) {
 #pragma unroll
-  for (int j = 0; j < COUNT; ++j) {
-    if constexpr (OPS == 2) y[j] *= s[1][j] + b[1][j];
-    else y[j] += r[j];
+    for (int j = 0; j < COUNT; ++j) y[j] *= s[1][j] + b[1][j];
+  } else if (a.residual != nullptr) {
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) y[j] += r[j];
   }
   if (wide) {
 #pragma unroll
@@ -568,9 +576,13 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a) {
 //     us, tiles 43.4; 32 of 512 x 1000 4.3 and 6.0).  Else tiles read w no slower and
 //     x less often (32 gated rows of 4096 x 11264: 45 us, few rows 59; 32 of 4096 x
 //     4096 13.1 and 14.2).
-//   256: most work a byte read from L2, one workgroup a CU.  From 5/8 of a tile a CU
-//     on (160 tiles, 2560 x 4096 x 4096: 87 us, 128 112; 128 tiles 82, 128 67).  Not for
-//     32-bit numbers, whose matrix instructions bound every tile alike.
+//   256: most work a byte read from L2, one workgroup a CU.  Taken if its rounds of
+//     the card are no longer than those of 128, four of whose tiles (at two a CU) take
+//     as long as one of it, or 1.2 times as long where the inner dimension is long and
+//     the start and the epilogue, which nothing covers here, count little (25088 x
+//     4096 x 1536, 588 tiles: 293 us, 128 327; 25088 x 384 x 1536 54 and 50; 304 tiles,
+//     4864 x 4096 x 4096: 182 and 167; 160, 2560 x 4096 x 4096: 87 and 112).  Not for 32-bit
+//     numbers, whose matrix instructions bound every tile alike.
 //   128, two stages and two workgroups a CU: more than a tile a CU (384 tiles, 1500 x
 //     4096 x 4096: 56 us, four stages 67).
 //   128, four stages: more than half a tile a CU (256 tiles, 1024 x 4096 x 4096: 37 us,
@@ -595,7 +607,9 @@ inline Plan plan_of(const CfLinearArgs& x, bool gated, bool vec) {
     p.few = (x.cols + 15) / 16 >= 2 * CUS ? 4 : 8;
     return p;
   }
-  p.size = vec && !f32 && 8 * tiles(256, 256) >= 5 * CUS ? 256 : 2 * tiles(128, 128) > CUS ? 128 : 64;
+  const int64_t rounds256 = (tiles(256, 256) + CUS - 1) / CUS, rounds128 = (tiles(128, 128) + 2 * CUS - 1) / (2 * CUS);
+  const bool most = vec && !f32 && 10 * rounds256 <= (steps < 16 ? 5 : 6) * rounds128;
+  p.size = most ? 256 : 2 * tiles(128, 128) > CUS ? 128 : 64;
   p.split_steps = (int)steps;
   const int64_t n = tiles(64, 64), least = f32 ? 8 : 16;   // (a step of 32 bits takes twice as long)
   if (p.size == 64 && n < CUS && steps >= 3 * least) {
