@@ -12,6 +12,7 @@ reference.
 """
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
@@ -66,13 +67,35 @@ def _kinds(q, beta, log_decay):
 
 def _segment(seqs: int, tokens: int, packed: bool, heads: int, dk: int, dv: int) -> int:
     """Tokens a segment; 0: whole sequences."""
+    # The walks along a segment get shorter with it, the walk over the segments'
+    # states longer: least near a constant times the root of the length, 3.5 for wide
+    # keys and 3 for narrow ones (us; one sequence of 1024 tokens and 8 heads of 128
+    # channels: 64 tokens a segment 107, 128 68, 192 74, whole 135; 4096 tokens: 192 140,
+    # 320 118, 448 133, whole 523; 16384 of 64 channels: 192 180, 448 165, 704 179).
+    # No shorter than it takes to have all segments at work at once (16384 tokens, 32
+    # heads: 576 748, 2048 694), by half as many for equal sequences of 65 to 128
+    # channels (four of 4096 tokens and 16 heads: 512 445, 1088 362; but packed 20000,
+    # 10000 and 30000, which end some early: 3776 2153, 8192 2446).  An odd number of
+    # chunks: an even one has all segments read the same channels of memory at a time
+    # (4096 tokens, 8 heads: 256 147, 320 118; 65536 and 4 heads: 1024 602, 1088 479),
+    # which counts once they are many and as long as they drift little.  Whole sequences
+    # if they give workgroups enough (eight of 4096, 32 heads: whole 775, 2112 988; four
+    # of 2048: 328 and 341) or are short (160 tokens, 8 heads: whole 34, 64 37; 196 both
+    # 41; 300 whole 49, 64 44; of 256 channels 74 and 92).
     width = 32 if dk <= 32 else 64 if dk <= 64 else 128
     columns = heads * -(-dv // width)          # workgroups of one segment
     at_once = 2048 if dk <= 32 else 1024 if dk <= 64 else 512 if dk <= 128 else 256
-    if tokens <= 8 * CHUNK or seqs * columns * 4 > at_once:
-        return 0
     total = tokens if packed else seqs * tokens
-    segment = max(4, -(-total * columns // (at_once * CHUNK))) * CHUNK
+    short = (3 if dk <= 128 else 8) * CHUNK
+    if total <= short * seqs or seqs * columns * 4 > at_once:
+        return 0
+    if not packed and 64 < dk <= 128:
+        at_once //= 2
+    chunks = math.ceil(math.sqrt(tokens) * (3.0 if dk <= 64 else 3.5) / CHUNK)
+    chunks = max(chunks, -(-total * columns // (at_once * CHUNK)))
+    if chunks < 32 and (chunks > 2 or total * columns >= chunks * at_once * CHUNK):
+        chunks |= 1
+    segment = chunks * CHUNK
     segments = tokens // segment + seqs if packed else seqs * -(-tokens // segment)
     return segment if segment < tokens and segments <= MAX_SEGMENTS else 0
 
