@@ -75,7 +75,7 @@ struct Unit { u32x4 w[sizeof(T) / 2]; };
 // This thread's units of a chunk's image: piece tid % (D / 8) of the rows
 // tid / (D / 8) + i NT / (D / 8).  Rows from n on and channels from d on are
 // zeros: out of the buffer's range (VEC: 16-byte loads, from aligned rows of
-// whole 16-byte pieces that do not overlap) or not read.
+// whole 16-byte pieces that do not overlap) or masked.
 template <typename T, int U, int D, int NT, bool VEC>
 __device__ __forceinline__ void load_units(Unit<T>* u, const T* base, int n, int64_t stride, int d) {
   constexpr int PER = 16 / sizeof(T), ROWS = NT / (D / 8);
@@ -92,28 +92,40 @@ __device__ __forceinline__ void load_units(Unit<T>* u, const T* base, int n, int
         u[i].w[p] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at + (uint32_t)(i * ROWS * st), 0, 0);
     }
   } else {
-    // element by element, from a base brought to 16 bytes
-    const uintptr_t p = (uintptr_t)base, skip = p & 15;
+    // By words from a base brought to one, whatever a row's alignment: a row of 16
+    // bits that begins inside a word is put together from five of them.  (The last
+    // word may hold two bytes more than the rows do; each word of a load has its own
+    // range check.)  Walks over 16 bits took 216 and 100 us so, and 272 and 128 with a load
+    // for each element.
+    const uintptr_t p = (uintptr_t)base, skip = p & 3;
     const int st = (int)stride * (int)sizeof(T);
-    const __amdgpu_buffer_rsrc_t rsrc =
-        rows_rsrc((const void*)(p - skip), (uint32_t)((n - 1) * st + d * (int)sizeof(T) + (int)skip));
+    const __amdgpu_buffer_rsrc_t rsrc = rows_rsrc(
+        (const void*)(p - skip), (uint32_t)((n - 1) * st + d * (int)sizeof(T) + (int)skip + 3) & ~3u);
+    constexpr int WORDS = 2 * sizeof(T);
+    uint32_t keep[WORDS];                          // channels from d on are none
+#pragma unroll
+    for (int j = 0; j < WORDS; ++j) {
+      if constexpr (sizeof(T) == 4) keep[j] = c0 + j < d ? ~0u : 0u;
+      else keep[j] = c0 + 2 * j + 1 < d ? ~0u : c0 + 2 * j < d ? 0xffffu : 0u;
+    }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int r = row + i * ROWS;
-      const uint32_t at = (uint32_t)(r * st + c0 * (int)sizeof(T) + (int)skip);
-      Vec<T, 8> x;
+      const uint32_t at = r < n && c0 < d ? (uint32_t)(r * st + c0 * (int)sizeof(T) + (int)skip) : OOB;
+      if constexpr (sizeof(T) == 2) {
+        const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at & ~3u, 0, 0);
+        const uint32_t last = __builtin_amdgcn_raw_buffer_load_b32(rsrc, (at & ~3u) + 16, 0, 0);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t off = r < n && c0 + j < d ? at + (uint32_t)(j * sizeof(T)) : OOB;
-        if constexpr (sizeof(T) == 2) {
-          const uint16_t e = __builtin_amdgcn_raw_buffer_load_b16(rsrc, off, 0, 0);
-          x.v[j] = __builtin_bit_cast(T, e);
-        } else {
-          const uint32_t e = __builtin_amdgcn_raw_buffer_load_b32(rsrc, off, 0, 0);
-          x.v[j] = __builtin_bit_cast(T, e);
+        for (int j = 0; j < 4; ++j)
+          u[i].w[0][j] = __builtin_amdgcn_alignbyte(j < 3 ? w[j + 1] : last, w[j], at & 2) & keep[j];
+      } else {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(rsrc, at + 16 * q, 0, 0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) u[i].w[q][j] = w[j] & keep[4 * q + j];
         }
       }
-      u[i] = __builtin_bit_cast(Unit<T>, x);
     }
   }
 }
