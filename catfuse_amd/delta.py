@@ -81,18 +81,24 @@ def _segment(seqs: int, tokens: int, packed: bool, heads: int, dk: int, dv: int)
     # which counts once they are many and as long as they drift little.  Whole sequences
     # if they give workgroups enough (eight of 4096, 32 heads: whole 775, 2112 988; four
     # of 2048: 328 and 341) or are short (160 tokens, 8 heads: whole 34, 64 37; 196 both
-    # 41; 300 whole 49, 64 44; of 256 channels 74 and 92).
+    # 41; 300 whole 49, 64 44; of 256 channels 74 and 92).  Packed ones, whose lengths are
+    # not known here, then are cut where they are longer than most: a little over the
+    # mean (16 heads of 128: sixteen of 50 to 3000 tokens whole 423, cut 281; 24 of 20 to
+    # 2000 whole 405 to 553, cut 457 to 478; sixteen of 1000 whole 217, cut 232), until
+    # they fill the card by themselves.
     width = 32 if dk <= 32 else 64 if dk <= 64 else 128
     columns = heads * -(-dv // width)          # workgroups of one segment
     at_once = 2048 if dk <= 32 else 1024 if dk <= 64 else 512 if dk <= 128 else 256
     total = tokens if packed else seqs * tokens
     short = (3 if dk <= 128 else 8) * CHUNK
-    if total <= short * seqs or seqs * columns * 4 > at_once:
+    if total <= short * seqs or seqs * columns * (1 if packed else 4) > at_once:
         return 0
     if not packed and 64 < dk <= 128:
         at_once //= 2
     chunks = math.ceil(math.sqrt(tokens) * (3.0 if dk <= 64 else 3.5) / CHUNK)
     chunks = max(chunks, -(-total * columns // (at_once * CHUNK)))
+    if seqs * columns * 4 > at_once:               # packed: what is longer than most
+        chunks = max(chunks, -(-total * 21 // (seqs * CHUNK * 20)))
     if chunks < 32 and (chunks > 2 or total * columns >= chunks * at_once * CHUNK):
         chunks |= 1
     segment = chunks * CHUNK
