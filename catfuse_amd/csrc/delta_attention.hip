@@ -195,6 +195,8 @@ __global__ __launch_bounds__(1024) void delta_begins_kernel(DeltaArgs a) {
 // column in registers, then joined in pairs by fp32 matrix instructions:
 //   (A 0; B D)^-1 = (A^-1 0; -D^-1 B A^-1 D^-1).
 // Rows of L from the first one that is not finite on are left out, and of T NaN.
+// Bound by the substitution's chain of dependent steps and by T's bytes (300 a token
+// and head of C = 64, 2.2 TB/s): 65536 tokens x 32 heads of 128 bf16 channels 290 us.
 template <int C> constexpr int solved_size() { return (C / 32) * (C / 32 + 1) / 2 * 6144; }   // bytes
 
 typedef float f4v __attribute__((ext_vector_type(4)));
@@ -402,6 +404,13 @@ __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
 // next products as they lie.  So are eight registers of r and u, tokens
 // 16 s + 4 (lane / 32) + 0 .. 3 and the same plus 8, the order in which T, the
 // scores and K's turned operand have them.
+//
+// Bound by the issue of matrix and vector operations by turns, and by the card's
+// power: 65536 tokens x 32 heads of 128 bf16 channels in 16 segments, outputs 960 us
+// and states 960 (matrix cores 47 and 53 %, vector issue 43 and 53 %, LDS 18 % of the
+// cycles, the clock at 1.8 GHz).  Two workgroups of four waves a CU; chunks of 64 halve
+// the products with the state's parts against 32, for which only bf16 heads of 65 to
+// 128 channels have the registers.
 template <typename T, int DKP, int NW, int C, bool OUT, bool VEC>
 __global__ __launch_bounds__(64 * NW, DKP <= 128 ? 2 : 1)
 void delta_walk_kernel(DeltaArgs a) {
@@ -935,8 +944,9 @@ void delta_walk_kernel(DeltaArgs a) {
 // A workgroup carries 32 columns of a head along a sequence, wave t their rows
 // 32 t .. + 31 in an accumulator (in the walk's order of rows).  Each step puts S
 // into LDS as operands, all rows for all waves; M's rows and N of the next step are
-// loaded meanwhile.  16 segments of 32 heads of 128 x 128: 24 us; with the products
-// of single numbers in lanes, M read by every 8 columns, 620.
+// loaded meanwhile.  Bound by the way of M and the barrier of each step: 16 segments
+// of 32 heads of 128 x 128 take 80 us, 5 a step; with the products of single numbers
+// in lanes, M read by every 8 columns, 620.
 template <int DKP, bool VEC>
 __global__ __launch_bounds__(2 * DKP) void delta_join_kernel(DeltaArgs a) {
   constexpr int KT = DKP / 32, KS = DKP / 16, NP = 3;

@@ -39,7 +39,8 @@ __device__ __forceinline__ int64_t step_slot(const DeltaStepArgs& a, int i) {
 // A workgroup takes CL * VEC columns of one row's and head's state; thread =
 // VEC columns of NR rows, held in registers: k S and q S are both sums over
 // the old state, and q S_new = w q S + (q . k) u, so that one pass reads it
-// and one writes it.
+// and one writes it.  Bound by HBM: 256 rows of 32 heads of 128 x 128 in 218 us, 4.9
+// TB/s, the rate of a large copy; one row of 12 heads of 32 x 32 by its latency, 5.
 template <typename T, int VEC, int CL, int NR>
 __global__ __launch_bounds__(256) void delta_step_kernel(DeltaStepArgs a) {
   constexpr int RG = 256 / CL, COLS = CL * VEC;

@@ -97,7 +97,7 @@ def _segment(seqs: int, tokens: int, packed: bool, heads: int, dk: int, dv: int)
         at_once //= 2
     chunks = math.ceil(math.sqrt(tokens) * (3.0 if dk <= 64 else 3.5) / CHUNK)
     chunks = max(chunks, -(-total * columns // (at_once * CHUNK)))
-    if seqs * columns * 4 > at_once:               # packed: what is longer than most
+    if packed and seqs * columns * 4 > at_once:    # what is longer than most
         chunks = max(chunks, -(-total * 21 // (seqs * CHUNK * 20)))
     if chunks < 32 and (chunks > 2 or total * columns >= chunks * at_once * CHUNK):
         chunks |= 1
@@ -147,8 +147,8 @@ def delta_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: tor
     from token to token.  A token that holds an infinity or NaN does not reach the
     tokens before it; what it does reach may be NaN where the formula gives an
     infinity.
-    The workspace, from torch's allocator, is about 200 bytes a token and head
-    (bf16 heads of 65 to 128 channels; others 140), and for long sequences of a small
+    The workspace, from torch's allocator, is 300 bytes a token and head (bf16
+    heads of 65 to 128 channels; others 204), and for long sequences of a small
     batch, which are walked in segments side by side, [dk, dv + dk] fp32 a segment
     and head."""
     scale = None if scale is None else float(scale)
