@@ -60,6 +60,25 @@ __device__ __forceinline__ u32x4 load16(const T* p) {
   __builtin_memcpy(&r, p, 16);
   return r;
 }
+// The same, read by words: of 16 bits where they may begin inside one, the five they
+// lie in (the fifth only where it holds some of them).
+struct Words { u32x4 w; uint32_t rest, shift; };
+template <typename T>
+__device__ __forceinline__ Words words_at(const T* p) {
+  const char* const a = (const char*)((uintptr_t)p & ~(uintptr_t)3);
+  Words r;
+  r.shift = (uint32_t)((uintptr_t)p & 2);
+  r.w = load16(reinterpret_cast<const uint32_t*>(a));
+  r.rest = *reinterpret_cast<const uint32_t*>(a + (r.shift ? 16 : 12));
+  return r;
+}
+__device__ __forceinline__ u32x4 whole_of(const Words& r) {
+  u32x4 x;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = __builtin_amdgcn_alignbyte(j < 3 ? r.w[j + 1] : r.rest, r.w[j], r.shift);
+  return x;
+}
+__device__ __forceinline__ u32x4 whole_of(const u32x4& x) { return x; }
 // The first n of the numbers there, zeros behind.
 template <typename T>
 __device__ __forceinline__ u32x4 load_some(const T* p, int n) {
@@ -216,10 +235,13 @@ __device__ __forceinline__ bool wide_columns(const LinearArgs& a) {
 // Few rows of x: bound by the bytes of w, each read once.  A workgroup takes 16
 // columns (rows of w) and all rows of x, NW waves a part of the inner dimension
 // each, joined in LDS.  A lane of a product takes 16 bytes of w's row lane % 16,
-// piece lane / 16 of four; U products' loads are in flight.
-template <typename T, int MT, int NW, int OPS>
+// piece lane / 16 of four; U products' loads are in flight.  ODD: rows of 16 bits
+// that begin inside a word, read as the five words they lie in (6 gated rows of 2233
+// x 4821: 19 us; as 16 bytes from their own address 31, of 2232 14).
+// 1 row of 4096 x 4096 and its residual: 8.9 us, 3.8 TB/s.
+template <typename T, int MT, int NW, int OPS, bool ODD>
 __global__ __launch_bounds__(64 * NW) void linear_few_kernel(LinearArgs a) {
-  constexpr int PER = 16 / sizeof(T), STEP = 4 * PER, U = MT * OPS <= 2 ? 8 : 4;
+  constexpr int PER = 16 / sizeof(T), STEP = 4 * PER, U = MT * OPS <= 2 && !ODD ? 8 : 4;
   __shared__ float part[NW][OPS * MT][4][64];
   const int tid = threadIdx.x, lane = tid & 63, row = lane & 15, quarter = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -242,15 +264,20 @@ __global__ __launch_bounds__(64 * NW) void linear_few_kernel(LinearArgs a) {
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[o][t] = f4v{};
   const int full = last < whole ? last : whole;
+  auto take = [](const T* p) {
+    if constexpr (ODD) return words_at(p);
+    else return load16(p);
+  };
+  using Piece = decltype(take(nullptr));
   for (int s = first; s < full; s += U) {    // (conditions on s: the same in every lane)
-    u32x4 wv[U][OPS], xv[U][MT];
+    Piece wv[U][OPS], xv[U][MT];
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (s + u < full) {
 #pragma unroll
-        for (int o = 0; o < OPS; ++o) wv[u][o] = load16(wp[o] + (int64_t)(s + u) * STEP);
+        for (int o = 0; o < OPS; ++o) wv[u][o] = take(wp[o] + (int64_t)(s + u) * STEP);
 #pragma unroll
-        for (int t = 0; t < MT; ++t) xv[u][t] = load16(xp[t] + (int64_t)(s + u) * STEP);
+        for (int t = 0; t < MT; ++t) xv[u][t] = take(xp[t] + (int64_t)(s + u) * STEP);
       }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -258,7 +285,7 @@ __global__ __launch_bounds__(64 * NW) void linear_few_kernel(LinearArgs a) {
 #pragma unroll
         for (int o = 0; o < OPS; ++o)
 #pragma unroll
-          for (int t = 0; t < MT; ++t) acc[o][t] = mfma<T>(wv[u][o], xv[u][t], acc[o][t]);
+          for (int t = 0; t < MT; ++t) acc[o][t] = mfma<T>(whole_of(wv[u][o]), whole_of(xv[u][t]), acc[o][t]);
   }
   if (first <= whole && last > whole) {       // the inner dimension's end: zeros behind it
     const int left = a.inner - whole * STEP - quarter * PER;
@@ -541,6 +568,25 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile_kernel(LinearArgs
   }
 }
 
+// Rows on 128 bytes with zeros behind their last numbers, for tiles that are read in
+// whole pieces: 16 bytes a thread.  Bound by the bytes, read and written once.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_rows_kernel(const T* from, T* to, int64_t rows, int inner,
+                                                          int64_t stride, int to_stride) {
+  constexpr int PER = 16 / sizeof(T);
+  const int units = (inner + PER - 1) / PER;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * units) return;
+  const int64_t row = i / units;
+  const int k = (int)(i % units) * PER;
+  const T* const p = from + row * stride + k;
+  u32x4 x;
+  if (k + PER > inner) x = load_some(p, inner - k);
+  else if constexpr (sizeof(T) == 2) x = whole_of(words_at(p));
+  else x = load16(p);
+  *reinterpret_cast<u32x4*>(to + row * to_stride + k) = x;
+}
+
 // The sums of the splits, in their order, and the epilogue: four columns a thread.
 template <typename T, int OPS>
 __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a) {
@@ -590,22 +636,64 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a) {
 //   64: four stages, two workgroups a CU.  Of long rows that give less than a tile a CU
 //     the inner dimension is split, 16 steps and more a split (64 x 4096 x 4096: 19.6
 //     us whole, 14.1 in four; 256 x 2048 x 2048 would be 13.7 in two, and takes 12.0).
-struct Plan { int few, size, splits, split_steps; };   // few: waves of the few-rows kernel, or 0
+// Rows of 16 bits that are not in whole pieces of 16 bytes are first laid out so in the
+// workspace (pack) if that takes less than it saves: a read and a write of all rows at
+// 4.5 TB/s and 4 us for the launches, against 0.75 of the product's time or 0.55 us a
+// step, whichever is more (9506 x 1121 x 8192: 183 us, read as they lie 318; 300 x 4097 x
+// 4096 42 and 70; 64 x 1121 x 8192, 18773 x 1137 x 137: not).  Those of 32 bits lose too
+// little (2673 x 3321 x 536: 145, whole 110).
+struct Plan {
+  int few, size, splits, split_steps;      // few: waves of the few-rows kernel, or 0
+  bool pack[3];                            // x, w, w2
+};
 
 constexpr int FEW_ROWS = 32;
 constexpr int CUS = 256;
 
-inline Plan plan_of(const CfLinearArgs& x, bool gated, bool vec) {
-  Plan p = {0, 0, 1, 0};
+// Whether rows are whole pieces of 16 bytes, aligned from the first on if it is,
+// and do not overlap.
+inline bool whole_rows(const CfLinearArgs& x, int64_t stride) {
+  const int per = x.dtype == SEQ_F32 ? 4 : 8;
+  return x.inner % per == 0 && stride % per == 0 && stride >= x.inner;
+}
+
+// How x and w are read: in whole pieces of 16 bytes, 256 rows of them within 2^31
+// bytes.  `addresses`: look at those, too.
+inline bool whole_pieces(const CfLinearArgs& x, const Plan& p, bool addresses) {
+  const int size = x.dtype == SEQ_F32 ? 4 : 2;
+  auto whole = [&](const void* base, int64_t stride, bool packed) {
+    return packed || (whole_rows(x, stride) && stride * size * 256 < 0x7fffffffll &&
+                      (!addresses || (uintptr_t)base % 16 == 0));
+  };
+  return whole(x.x, x.x_row, p.pack[0]) && whole(x.w, x.w_row, p.pack[1]) &&
+         (!x.w2 || whole(x.w2, x.w2_row, p.pack[2]));
+}
+
+// The plan does not look at addresses, so that a workspace can be asked for without
+// them.
+inline Plan plan_of(const CfLinearArgs& x, bool gated) {
+  Plan p = {0, 0, 1, 0, {false, false, false}};
   const bool f32 = x.dtype == SEQ_F32;
   const int64_t step = f32 ? 32 : 64, steps = (x.inner + step - 1) / step;
   const int half = gated ? 2 : 1;
   auto tiles = [&](int64_t bm, int64_t bn) {
     return ((x.rows + bm - 1) / bm) * ((x.cols + bn / half - 1) / (bn / half));
   };
+  bool vec = whole_pieces(x, p, false);
   if (x.rows <= FEW_ROWS && (!vec || x.rows <= 8 || x.rows * tiles(64, 64) < 8 * CUS)) {
     p.few = (x.cols + 15) / 16 >= 2 * CUS ? 4 : 8;
     return p;
+  }
+  if (!vec && !f32) {
+    const double columns = (double)half * x.cols, bytes = 4.0 * (x.rows + columns) * x.inner;
+    const double product = 2.0 * x.rows * columns * x.inner / 1.15e9;      // us
+    const double saved = 0.75 * product > 0.55 * steps ? 0.75 * product : 0.55 * steps;
+    if (saved > bytes / 4.5e6 + 4.0) {
+      p.pack[0] = !whole_rows(x, x.x_row);
+      p.pack[1] = !whole_rows(x, x.w_row);
+      p.pack[2] = gated && !whole_rows(x, x.w2_row);
+      vec = whole_pieces(x, p, false);
+    }
   }
   const int64_t rounds256 = (tiles(256, 256) + CUS - 1) / CUS, rounds128 = (tiles(128, 128) + 2 * CUS - 1) / (2 * CUS);
   const bool most = vec && !f32 && 10 * rounds256 <= (steps < 16 ? 5 : 6) * rounds128;
@@ -623,21 +711,40 @@ inline Plan plan_of(const CfLinearArgs& x, bool gated, bool vec) {
   return p;
 }
 
+inline int64_t packed_row(const CfLinearArgs& x) {         // of 16 bits: whole lines
+  return (x.inner + 63) / 64 * 64;
+}
+
+inline int64_t parts_bytes(const CfLinearArgs& x, const Plan& p, bool gated) {
+  return p.few || p.splits < 2 ? 0 : (4 * (gated ? 2 : 1) * p.splits * x.rows * x.cols + 255) / 256 * 256;
+}
+
 inline int64_t workspace_of(const CfLinearArgs& x, const Plan& p, bool gated) {
-  return p.few || p.splits < 2 ? 0 : 4 * (gated ? 2 : 1) * p.splits * x.rows * x.cols;
+  const int64_t rows = (p.pack[0] ? x.rows : 0) + (p.pack[1] ? x.cols : 0) + (p.pack[2] ? x.cols : 0);
+  return parts_bytes(x, p, gated) + 2 * rows * packed_row(x);
+}
+
+template <typename T, int OPS, bool ODD>
+hipError_t launch_rows(const LinearArgs& a, int waves, hipStream_t st) {
+  const dim3 grid((unsigned)((a.cols + 15) / 16));
+  if (a.rows <= 16) {
+    if (waves == 4) hipLaunchKernelGGL((linear_few_kernel<T, 1, 4, OPS, ODD>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((linear_few_kernel<T, 1, 8, OPS, ODD>), grid, dim3(512), 0, st, a);
+  } else {
+    if (waves == 4) hipLaunchKernelGGL((linear_few_kernel<T, 2, 4, OPS, ODD>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((linear_few_kernel<T, 2, 8, OPS, ODD>), grid, dim3(512), 0, st, a);
+  }
+  return hipGetLastError();
 }
 
 template <typename T, int OPS>
 hipError_t launch_few(const LinearArgs& a, int waves, hipStream_t st) {
-  const dim3 grid((unsigned)((a.cols + 15) / 16));
-  if (a.rows <= 16) {
-    if (waves == 4) hipLaunchKernelGGL((linear_few_kernel<T, 1, 4, OPS>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((linear_few_kernel<T, 1, 8, OPS>), grid, dim3(512), 0, st, a);
-  } else {
-    if (waves == 4) hipLaunchKernelGGL((linear_few_kernel<T, 2, 4, OPS>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((linear_few_kernel<T, 2, 8, OPS>), grid, dim3(512), 0, st, a);
+  if constexpr (sizeof(T) == 2) {
+    auto odd = [](const void* base, int64_t stride) { return (uintptr_t)base % 4 != 0 || stride % 2 != 0; };
+    if ((a.rows > 1 ? odd(a.x, a.xr) : odd(a.x, 0)) || odd(a.w[0], a.wr[0]) || (OPS == 2 && odd(a.w[1], a.wr[1])))
+      return launch_rows<T, OPS, true>(a, waves, st);
   }
-  return hipGetLastError();
+  return launch_rows<T, OPS, false>(a, waves, st);
 }
 
 template <typename T, int BM, int BN, int WM, int WN, int NST, int OPS, bool VEC>
@@ -675,22 +782,31 @@ hipError_t launch_linear(const LinearArgs& a, const Plan& p, bool vec, hipStream
   return vec ? launch_sizes<T, OPS, true>(a, p, st) : launch_sizes<T, OPS, false>(a, p, st);
 }
 
+// The rows that the plan says into the workspace, from `at` on; a reads them there.
+inline hipError_t pack_rows(const CfLinearArgs& x, const Plan& p, int64_t at, LinearArgs& a, hipStream_t st) {
+  const int64_t stride = packed_row(x), units = (x.inner + 7) / 8;
+  auto pack = [&](const void*& base, int64_t& row, int64_t rows) {
+    _Float16* const to = (_Float16*)((char*)x.workspace + at);
+    const int64_t blocks = (rows * units + 255) / 256;
+    if (blocks > 0xffffffffll / 256) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((linear_rows_kernel<_Float16>), dim3((unsigned)blocks), dim3(256), 0, st,
+                       (const _Float16*)base, to, rows, (int)x.inner, row, (int)stride);
+    at += 2 * rows * stride;
+    base = to;
+    row = stride;
+    return hipGetLastError();
+  };
+  hipError_t e = hipSuccess;
+  if (p.pack[0]) e = pack(a.x, a.xr, x.rows);
+  if (e == hipSuccess && p.pack[1]) e = pack(a.w[0], a.wr[0], x.cols);
+  if (e == hipSuccess && p.pack[2]) e = pack(a.w[1], a.wr[1], x.cols);
+  if (e == hipSuccess) a.inner = (int)(8 * units);
+  return e;
+}
+
 template <typename T>
 hipError_t launch_ops(const LinearArgs& a, const Plan& p, bool vec, hipStream_t st) {
   return a.w[1] ? launch_linear<T, 2>(a, p, vec, st) : launch_linear<T, 1>(a, p, vec, st);
-}
-
-// Whether x and w have rows of whole aligned 16-byte pieces that do not overlap,
-// 256 of them within 2^31 bytes.  (The plan of a workspace's size takes rows for
-// such ones.  For others it asks for as much or more: only tiles of 64 are split,
-// by their number, and more than half a tile of 128 a CU is more than a tile of 64.)
-inline bool whole_pieces(const CfLinearArgs& x) {
-  const int size = x.dtype == SEQ_F32 ? 4 : 2, per = 16 / size;
-  auto vec = [&](const void* base, int64_t stride) {
-    return (uintptr_t)base % 16 == 0 && stride % per == 0 && stride >= x.inner &&
-           stride * size * 256 < 0x7fffffffll;
-  };
-  return x.inner % per == 0 && vec(x.x, x.x_row) && vec(x.w, x.w_row) && (!x.w2 || vec(x.w2, x.w2_row));
 }
 
 inline bool sizes_make_sense(const CfLinearArgs& x) {
@@ -703,7 +819,7 @@ inline bool sizes_make_sense(const CfLinearArgs& x) {
 CF_API int64_t cf_linear_workspace(const CfLinearArgs* p) {
   if (!p || !sizes_make_sense(*p)) return -1;
   const bool gated = p->w2 != nullptr;
-  return workspace_of(*p, plan_of(*p, gated, true), gated);
+  return workspace_of(*p, plan_of(*p, gated), gated);
 }
 
 CF_API int cf_linear(const CfLinearArgs* p) {
@@ -716,8 +832,7 @@ CF_API int cf_linear(const CfLinearArgs* p) {
   const bool gated = x.w2 != nullptr;
   if (!x.out || (x.inner > 0 && (!x.x || !x.w)) || (gated && x.residual))
     return (int)hipErrorInvalidValue;
-  const bool v = whole_pieces(x);
-  const Plan plan = plan_of(x, gated, v);
+  Plan plan = plan_of(x, gated);
   const int64_t need = workspace_of(x, plan, gated);
   if (need > 0 && (!x.workspace || (uintptr_t)x.workspace % 16 != 0 || x.workspace_bytes < need))
     return (int)hipErrorInvalidValue;
@@ -727,15 +842,23 @@ CF_API int cf_linear(const CfLinearArgs* p) {
   a.bias[0] = x.bias; a.bias[1] = x.bias2;
   a.residual = x.residual;
   a.out = x.out;
-  a.parts = need > 0 ? (float*)x.workspace : nullptr;
+  a.parts = plan.splits > 1 ? (float*)x.workspace : nullptr;
   a.bias_f32 = x.bias_f32 != 0;
   a.activation = (int)x.activation;
   a.rows = x.rows; a.inner = (int)x.inner; a.cols = (int)x.cols;
   a.xr = x.x_row; a.wr[0] = x.w_row; a.wr[1] = x.w2_row; a.rr = x.residual_row; a.orow = x.out_row;
   a.splits = plan.splits; a.split_steps = plan.split_steps;
+  const bool v = whole_pieces(x, plan, true);
+  if (!v && plan.size == 256) plan.size = 128;              // (an address that is no multiple of 16)
   a.row_tiles = a.col_tiles = 0;
   hipStream_t st = (hipStream_t)x.stream;
   hipError_t e;
+  if (plan.pack[0] || plan.pack[1] || plan.pack[2]) {       // 16-bit numbers, whatever they are
+    if (v) {
+      e = pack_rows(x, plan, parts_bytes(x, plan, gated), a, st);
+      if (e != hipSuccess) return (int)e;
+    }
+  }
   if (x.dtype == SEQ_F32) e = launch_ops<float>(a, plan, v, st);
   else if (x.dtype == SEQ_F16) e = launch_ops<_Float16>(a, plan, v, st);
   else e = launch_ops<bf16_t>(a, plan, v, st);

@@ -160,7 +160,9 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
 
     Sums and the epilogue are fp32, each output is rounded once.  Products of a
     small result and a long inner dimension are split along it, with a workspace
-    of the splits' sums (fp32) from torch's allocator."""
+    of the splits' sums (fp32) from torch's allocator; large products of 16-bit
+    rows that are not whole pieces of 16 bytes (an inner dimension or a stride that
+    8 does not divide) take one of as many bytes as those rows have, laid out so."""
     return _product("linear", x, (w,), (bias,), activation, residual, out)
 
 

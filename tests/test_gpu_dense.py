@@ -118,6 +118,57 @@ def test_tiles(cuda, dtype, M, K, N, gated):
     _check(_run(x, ws, bs, "gelu", r), x, ws, bs, "gelu", r)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("M,K,N", [(1100, 1101, 900), (50, 4101, 120), (300, 4100, 500), (1100, 2050, 2000)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_rows_off_pieces(cuda, dtype, M, K, N, gated):
+    """Rows that no 16 bytes divide, between others that are not finite."""
+    x, ws, bs, r = _make(cuda, M, K, N, dtype, 7, gated, dtype, residual=not gated)
+    def among(t):
+        wide = torch.full((t.shape[0] + 2, t.shape[1] + 6), math.nan, dtype=dtype, device=cuda)
+        wide[1:-1, 3:-3] = t
+        return wide[1:-1, 3:-3]
+    want = _run(x, ws, bs, "silu", r)
+    _check(want, x, ws, bs, "silu", r)
+    _check(_run(among(x), tuple(map(among, ws)), bs, "silu", r), x, ws, bs, "silu", r)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("M,N", [(1100, 900), (300, 2000)])
+def test_one_operand_off_pieces(cuda, dtype, M, N):
+    """x, w or the second w alone: the product of whole rows, to the bit where its
+    tiles are the same ones."""
+    K = 4096
+    x, ws, bs, _ = _make(cuda, M, K, N, dtype, 8, True, F32)
+    want = _run(x, ws, bs, "silu")
+    _check(want, x, ws, bs, "silu")
+    def off(t):
+        wide = torch.full((t.shape[0], K + 5), math.inf, dtype=dtype, device=cuda)
+        wide[:, 2:K + 2] = t
+        return wide[:, 2:K + 2]
+    assert torch.equal(_run(off(x), ws, bs, "silu"), want)
+    assert torch.equal(_run(x, (off(ws[0]), ws[1]), bs, "silu"), want)
+    assert torch.equal(_run(x, (ws[0], off(ws[1])), bs, "silu"), want)
+    # whole rows from an address that is not: read as they lie
+    flat = torch.empty(M * K + 1, dtype=dtype, device=cuda)
+    y = flat[1:].view(M, K)
+    y.copy_(x)
+    _check(_run(y, ws, bs, "silu"), x, ws, bs, "silu")
+    _check(_run(y, (off(ws[0]), ws[1]), bs, "silu"), x, ws, bs, "silu")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("M", [1, 2, 16, 30])
+@pytest.mark.parametrize("K", [1, 31, 33, 127, 1001])
+def test_few_rows_inside_words(cuda, dtype, M, K):
+    x, ws, bs, r = _make(cuda, M, K, 50, dtype, 9, False, dtype, residual=True)
+    flat = torch.full((50 * K + 3,), math.nan, dtype=dtype, device=cuda)
+    w = flat[1:50 * K + 1].view(50, K)
+    w.copy_(ws[0])
+    _check(_run(x, (w,), bs, None, r), x, ws, bs, None, r)
+    _check(_run(x, ws, bs, None, r), x, ws, bs, None, r)
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("M", [5, 200])
 def test_activations(cuda, act, M):
