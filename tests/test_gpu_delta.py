@@ -455,6 +455,40 @@ def test_step_strides(cuda):
     assert bool(((odd - want_s).abs() <= 1e-5 * (1 + want_s.abs())).all())
 
 
+@pytest.mark.parametrize("more", [0, 70])
+def test_packed_offsets_either_way(cuda, more):
+    """Sequences few enough to be found without a launch, and the same ones with
+    empty ones between them: the same rows and states, cut into segments or not,
+    offsets that fall or lie outside among them."""
+    for lens in ([5, 0, 64, 130], [900, 0, 1, 2500, 70, 0]):
+        N = sum(lens)
+        x = [t.to(cuda) for t in _inputs((N,), (2, 2, 2), 64, 64, BF16, 31)]
+        cu = [0]
+        for n in lens:
+            cu.append(cu[-1] + n)
+        odd = cu[:2] + [cu[1] - 3] + cu[2:-1] + [N + 1000]
+        spread = cu[:2] + [cu[1]] * more + cu[2:] + [N] * more
+        def run(o):
+            return kernels.delta_attention(*x, cu_seqlens=torch.tensor(o, device=cuda))
+        want, states = run(cu)
+        got, left = run(odd)
+        assert torch.equal(got, want)
+        assert torch.equal(left[[0] + list(range(2, len(lens) + 1))], states) and not bool(left[1].any())
+        got, left = run(spread)
+        a = [b.double().cpu() for b in x]
+        for i, n in enumerate(lens):
+            rows = slice(cu[i], cu[i] + n)
+            w, ws, bound, m = _definition(*(t[rows] for t in a), 64 ** -0.5, None) if n else (None,) * 4
+            at = i if i < 1 else i + more
+            if n == 0:
+                assert not bool(left[at].any())
+                continue
+            depth = 72 * _solve_norm(a[1][rows], a[3][rows], a[4][rows], 2)
+            for o, s in ((want, states[i]), (got, left[at])):
+                _close(o[rows], w, BF16, depth * U32 * bound)
+                _close(s, ws, F32, (depth * U32 * m)[:, None, :])
+
+
 def test_pieces_join(cuda):
     """A prompt in pieces through the states, and the rest of it token by token:
     the whole prompt's output."""
