@@ -669,6 +669,10 @@ inline bool whole_pieces(const CfLinearArgs& x, const Plan& p, bool addresses) {
          (!x.w2 || whole(x.w2, x.w2_row, p.pack[2]));
 }
 
+inline int64_t packed_row(const CfLinearArgs& x) {         // of 16 bits: whole lines
+  return (x.inner + 63) / 64 * 64;
+}
+
 // The plan does not look at addresses, so that a workspace can be asked for without
 // them.
 inline Plan plan_of(const CfLinearArgs& x, bool gated) {
@@ -684,7 +688,9 @@ inline Plan plan_of(const CfLinearArgs& x, bool gated) {
     p.few = (x.cols + 15) / 16 >= 2 * CUS ? 4 : 8;
     return p;
   }
-  if (!vec && !f32) {
+  // (laid out rows have to be near each other, too, and one launch's work)
+  const int64_t longest = x.rows > x.cols ? x.rows : x.cols;
+  if (!vec && !f32 && 2 * 256 * packed_row(x) < 0x7fffffffll && longest * packed_row(x) < 1ll << 34) {
     const double columns = (double)half * x.cols, bytes = 4.0 * (x.rows + columns) * x.inner;
     const double product = 2.0 * x.rows * columns * x.inner / 1.15e9;      // us
     const double saved = 0.75 * product > 0.55 * steps ? 0.75 * product : 0.55 * steps;
@@ -709,10 +715,6 @@ inline Plan plan_of(const CfLinearArgs& x, bool gated) {
     }
   }
   return p;
-}
-
-inline int64_t packed_row(const CfLinearArgs& x) {         // of 16 bits: whole lines
-  return (x.inner + 63) / 64 * 64;
 }
 
 inline int64_t parts_bytes(const CfLinearArgs& x, const Plan& p, bool gated) {

@@ -287,6 +287,15 @@ def test_more_than_32_bits(cuda):
     _check(kernels.linear(rows, w), rows.contiguous(), (w,), (None,), None)
 
 
+def test_rows_too_long_to_lie_near(cuda):
+    """256 rows reach over 2^31 bytes, and no 16 bytes divide one."""
+    M, K, N = 40, 4_200_001, 24
+    g = torch.Generator(device=cuda).manual_seed(3)
+    x = torch.randn(M, K, generator=g, device=cuda).to(BF16)
+    w = torch.randn(N, K, generator=g, device=cuda).to(BF16)
+    _check(kernels.linear(x, w), x, (w,), (None,), None)
+
+
 def test_a_block_of_a_serving_batch(cuda):
     """The projections around the delta rule's attention and its feed-forward
     block, as a serving program runs them: prompts, then single tokens; captured as
