@@ -107,15 +107,18 @@ def _plan(x, ws, biases, activation, residual, out):
     return dev, shape, ws_bytes, tail(ws_bytes)
 
 
-def _product(what, x, ws, biases, activation, residual, out):
+def _product(what, x, w, w2, bias, bias2, activation, residual, out):
     try:
-        key = (_product, _looks(x)) + tuple(_looks(t) for t in ws + biases) + \
-            (activation, _looks(residual), _looks(out), torch.is_grad_enabled())
+        key = (what, activation, torch.is_grad_enabled(), _looks(x), _looks(w), _looks(w2),
+               _looks(bias), _looks(bias2), _looks(residual), _looks(out))
         plan = _PLANS.get(key)
     except (AttributeError, TypeError):      # not tensors: the checks say which
         key = plan = None
     if plan is None:
-        plan = _plan(x, ws, biases, activation, residual, out)
+        if what == "linear":
+            plan = _plan(x, (w,), (bias,), activation, residual, out)
+        else:
+            plan = _plan(x, (w, w2), (bias, bias2), activation, residual, out)
         if key is not None:
             _keep(key, plan)
     dev, shape, ws_bytes, tail = plan
@@ -123,7 +126,7 @@ def _product(what, x, ws, biases, activation, residual, out):
     if given:
         in_place = residual is not None and out.data_ptr() == residual.data_ptr() and \
             out.stride() == residual.stride()
-        _apart(out, (x,) + ws + biases + (() if in_place else (residual,)))
+        _apart(out, (x, w, w2, bias, bias2) + (() if in_place else (residual,)))
     else:
         out = torch.empty(shape, dtype=x.dtype, device=dev)
     _require_gpu(x, "x")
@@ -131,16 +134,16 @@ def _product(what, x, ws, biases, activation, residual, out):
         return out
     work = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     ev = _t0()
-    args = _hip.LINEAR_ARGS[0].pack(_at(x), _at(ws[0]), _at(ws[1]) if len(ws) > 1 else 0,
-                                    _at(biases[0]), _at(biases[1]) if len(ws) > 1 else 0,
-                                    _at(residual), _at(out), _at(work), _hip.stream(dev)) + tail
+    args = _hip.LINEAR_ARGS[0].pack(_at(x), _at(w), _at(w2), _at(bias), _at(bias2), _at(residual),
+                                    _at(out), _at(work), _hip.stream(dev)) + tail
     _call(_hip.lib().cf_linear, "cf_linear", dev, args)
     if given:
         _changed(out)
     if ev is not None:
         rows, K, N = out.numel() // shape[-1], x.shape[-1], shape[-1]
-        _t1(what, ev, flops=2 * len(ws) * rows * K * N,
-            nbytes=x.element_size() * (rows * K + len(ws) * N * K + rows * N *
+        n = 1 if w2 is None else 2
+        _t1(what, ev, flops=2 * n * rows * K * N,
+            nbytes=x.element_size() * (rows * K + n * N * K + rows * N *
                                        (1 + (residual is not None))))
     return out
 
@@ -163,7 +166,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     of the splits' sums (fp32) from torch's allocator; large products of 16-bit
     rows that are not whole pieces of 16 bytes (an inner dimension or a stride that
     8 does not divide) take one of as many bytes as those rows have, laid out so."""
-    return _product("linear", x, (w,), (bias,), activation, residual, out)
+    return _product("linear", x, w, None, bias, None, activation, residual, out)
 
 
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *,
@@ -174,7 +177,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, *,
     half of a gated feed-forward block in one pass over x (`linear` with the
     residual is the other half).  Arguments as of `linear`; both biases of one
     type."""
-    return _product("gated_linear", x, (w_gate, w_up), (bias_gate, bias_up), activation, None, out)
+    return _product("gated_linear", x, w_gate, w_up, bias_gate, bias_up, activation, None, out)
 
 
 __all__ = ["linear", "gated_linear"]

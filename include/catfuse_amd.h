@@ -955,9 +955,11 @@ int cf_rotary(const CfRotaryArgs* args);
  * Rows are *_row elements apart (0 and overlaps allowed for inputs), elements of
  * a row on end; bias and bias2 [cols] fp32 (bias_f32) or of dtype.  out may be
  * the residual itself (the same rows) and must not overlap the inputs otherwise.
- * Small products are split along the inner dimension: the workspace (16-byte
+ * Small products are split along the inner dimension, 16-bit rows that are not
+ * whole pieces of 16 bytes may be laid out again first: the workspace (16-byte
  * aligned) has at least the bytes that cf_linear_workspace gives for the same
- * block (0: none is needed, -1: the sizes make no sense). */
+ * block, whose addresses it does not look at but for w2 being null or not (0: none
+ * is needed, -1: the sizes make no sense). */
 #define CF_LINEAR_MAX_ROWS 1000000000
 #define CF_LINEAR_MAX_WIDTH 16000000
 #define CF_ACT_NONE 0
