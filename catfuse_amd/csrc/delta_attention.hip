@@ -1001,11 +1001,14 @@ template <int DKP, bool VEC>
 __global__ __launch_bounds__(2 * DKP) void delta_join_kernel(DeltaArgs a) {
   constexpr int KT = DKP / 32, KS = DKP / 16, NP = 3;
   __shared__ __attribute__((aligned(16))) char ssh[2][KS * NP * 1024];
+  // a head's workgroups on one XCD (workgroup number mod 8), whose L2 they read M from
+  const int h = blockIdx.z * 8 + (blockIdx.x & 7);
+  if (h >= a.heads) return;
   const int64_t w = blockIdx.y;
   const Place pl = find_place(a, w, a.segment);
   if (pl.seq < 0 || pl.part != 0 || pl.parts < 2) return;
   const int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, col = lane & 31;
-  const int t = __builtin_amdgcn_readfirstlane(tid >> 6), h = blockIdx.z, c0 = blockIdx.x * 32;
+  const int t = __builtin_amdgcn_readfirstlane(tid >> 6), c0 = (blockIdx.x >> 3) * 32;
   // rows of an operand in the order in which an accumulator's are the state's
   const int row = 32 * t + 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
   const uint32_t s_at = c0 + col < a.dv ? 4u * (uint32_t)((32 * t + 8 * hi) * a.dv + c0 + col) : OOB;
@@ -1134,7 +1137,7 @@ hipError_t launch_chunks(DeltaArgs a, hipStream_t st) {
     hipError_t e = launch(delta_walk_kernel<T, DKP, NW, C, false, VEC>,
                           a.value_slices + (a.dk + 32 * NW - 1) / (32 * NW));
     if (e != hipSuccess) return e;
-    const dim3 grid((unsigned)((a.dv + 31) / 32), (unsigned)a.segments, (unsigned)a.heads);
+    const dim3 grid((unsigned)(8 * ((a.dv + 31) / 32)), (unsigned)a.segments, (unsigned)((a.heads + 7) / 8));
     if (a.dk % 4 == 0) hipLaunchKernelGGL((delta_join_kernel<DKP, true>), grid, dim3(2 * DKP), 0, st, a);
     else hipLaunchKernelGGL((delta_join_kernel<DKP, false>), grid, dim3(2 * DKP), 0, st, a);
     e = hipGetLastError();
