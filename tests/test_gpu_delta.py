@@ -166,6 +166,27 @@ def test_long(cuda, dtype, d, N):
     _check(cuda, _inputs((1, N), (2, 1, 2), d, d, dtype, N), state=state)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("dk,dv", [(20, 24), (30, 31), (61, 33), (72, 64), (101, 99), (129, 65),
+                                   (160, 147), (250, 30)])
+def test_long_heads(cuda, dtype, dk, dv):
+    """Segments joined for heads that fill no tile, rows off 16 bytes, three heads."""
+    state = torch.randn(1, 3, dk, dv, generator=torch.Generator().manual_seed(dk))
+    x = _inputs((1, 1000), (3, 1, 3), dk, dv, dtype, dv)
+    first, _ = _check(cuda, x, state=state)
+    # the same bits from rows with other strides and addresses, others not finite around them
+    def among(t):
+        wide = torch.full((t.shape[0], t.shape[1] + 1, t.shape[2] + 1, t.shape[3] + 3), math.nan, dtype=t.dtype)
+        wide[:, 1:, 1:, 1:-2] = t
+        return wide.to(cuda)[:, 1:, 1:, 1:-2]
+    y = [among(t) for t in x[:3]] + [t.to(cuda) for t in x[3:]]
+    out = kernels.delta_attention(*y, state=state.to(cuda), return_state=False)
+    if dk % 8 or dv % 8:
+        assert torch.equal(out, first)
+    else:
+        assert bool(((out - first).abs() <= torch.finfo(dtype).eps * (first.abs() + 1)).all())
+
+
 def test_long_packed(cuda):
     lens = [1, 2100, 0, 700, 64, 3]
     cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32)
