@@ -568,23 +568,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void linear_tile_kernel(LinearArgs
   }
 }
 
-// Rows on 128 bytes with zeros behind their last numbers, for tiles that are read in
-// whole pieces: 16 bytes a thread.  Bound by the bytes, read and written once.
-template <typename T>
-__global__ __launch_bounds__(256) void linear_rows_kernel(const T* from, T* to, int64_t rows, int inner,
-                                                          int64_t stride, int to_stride) {
-  constexpr int PER = 16 / sizeof(T);
-  const int units = (inner + PER - 1) / PER;
+// Rows of 16-bit numbers, whatever they are, on 128 bytes with zeros behind their last
+// ones, for tiles that are read in whole pieces: 16 bytes a thread.  Bound by the
+// bytes, read and written once at 4 TB/s.
+__global__ __launch_bounds__(256) void linear_rows_kernel(const _Float16* from, _Float16* to, int64_t rows,
+                                                          int inner, int64_t stride, int to_stride) {
+  const int units = (inner + 7) / 8;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows * units) return;
   const int64_t row = i / units;
-  const int k = (int)(i % units) * PER;
-  const T* const p = from + row * stride + k;
-  u32x4 x;
-  if (k + PER > inner) x = load_some(p, inner - k);
-  else if constexpr (sizeof(T) == 2) x = whole_of(words_at(p));
-  else x = load16(p);
-  *reinterpret_cast<u32x4*>(to + row * to_stride + k) = x;
+  const int k = (int)(i % units) * 8;
+  const _Float16* const p = from + row * stride + k;
+  *reinterpret_cast<u32x4*>(to + row * to_stride + k) =
+      k + 8 > inner ? load_some(p, inner - k) : whole_of(words_at(p));
 }
 
 // The sums of the splits, in their order, and the epilogue: four columns a thread.
@@ -616,7 +612,6 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a) {
   finish<T, OPS, 4>(a, m, n, y, b, {}, false, wide_columns<T>(a));
 }
 
-// How a product is taken.
 // Which kernel, in what pieces.  The times are of bf16.
 //   rows <= 32, and <= 8 or few columns: few rows (7 gated rows of 4096 x 11264 42.0
 //     us, tiles 43.4; 32 of 512 x 1000 4.3 and 6.0).  Else tiles read w no slower and
@@ -791,7 +786,7 @@ inline hipError_t pack_rows(const CfLinearArgs& x, const Plan& p, int64_t at, Li
     _Float16* const to = (_Float16*)((char*)x.workspace + at);
     const int64_t blocks = (rows * units + 255) / 256;
     if (blocks > 0xffffffffll / 256) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((linear_rows_kernel<_Float16>), dim3((unsigned)blocks), dim3(256), 0, st,
+    hipLaunchKernelGGL(linear_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, st,
                        (const _Float16*)base, to, rows, (int)x.inner, row, (int)stride);
     at += 2 * rows * stride;
     base = to;
@@ -855,11 +850,9 @@ CF_API int cf_linear(const CfLinearArgs* p) {
   a.row_tiles = a.col_tiles = 0;
   hipStream_t st = (hipStream_t)x.stream;
   hipError_t e;
-  if (plan.pack[0] || plan.pack[1] || plan.pack[2]) {       // 16-bit numbers, whatever they are
-    if (v) {
-      e = pack_rows(x, plan, parts_bytes(x, plan, gated), a, st);
-      if (e != hipSuccess) return (int)e;
-    }
+  if (v && (plan.pack[0] || plan.pack[1] || plan.pack[2])) {
+    e = pack_rows(x, plan, parts_bytes(x, plan, gated), a, st);
+    if (e != hipSuccess) return (int)e;
   }
   if (x.dtype == SEQ_F32) e = launch_ops<float>(a, plan, v, st);
   else if (x.dtype == SEQ_F16) e = launch_ops<_Float16>(a, plan, v, st);
