@@ -164,18 +164,18 @@ hipError_t launch_step_r(const DeltaStepArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)((units + CL - 1) / CL), (unsigned)a.heads, (unsigned)a.rows);
   if (rows <= 4) hipLaunchKernelGGL((delta_step_kernel<T, VEC, CL, 4>), grid, dim3(256), 0, st, a);
   else if (rows <= 8) hipLaunchKernelGGL((delta_step_kernel<T, VEC, CL, 8>), grid, dim3(256), 0, st, a);
-  else if (rows <= 16 || CL < 32)
-    hipLaunchKernelGGL((delta_step_kernel<T, VEC, CL, CL < 32 ? 8 : 16>), grid, dim3(256), 0, st, a);
-  else
-    hipLaunchKernelGGL((delta_step_kernel<T, VEC, CL, CL < 32 ? 8 : 32>), grid, dim3(256), 0, st, a);
+  else if constexpr (CL == 32) hipLaunchKernelGGL((delta_step_kernel<T, VEC, CL, 16>), grid, dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
 template <typename T, int VEC>
 hipError_t launch_step_v(const DeltaStepArgs& a, hipStream_t st) {
   const int units = (a.dv + VEC - 1) / VEC;
-  // 32 columns a workgroup where wider ones would leave most of the card idle
-  if (units <= 8 || (int64_t)a.rows * a.heads * ((units + 31) / 32) < 512)
+  // 8 vectors of columns a workgroup (rows of dk / 32 a thread) where 32 would leave
+  // most of the card idle (us; heads of 128: 256 workgroups of 32 11.7, of 8 10.0; 384
+  // 13.1 and 14.5; 2048 62 and 63) or hold more than 16 rows a thread in registers
+  // (heads of 256 x 256: 4096 282 and 228; 512 42 and 35)
+  if (units <= 8 || a.dk > 128 || (int64_t)a.rows * a.heads * ((units + 31) / 32) < 320)
     return launch_step_r<T, VEC, 8>(a, st);
   return launch_step_r<T, VEC, 32>(a, st);
 }
