@@ -233,15 +233,16 @@ __device__ __forceinline__ bool wide_columns(const LinearArgs& a) {
 }
 
 // Few rows of x: bound by the bytes of w, each read once.  A workgroup takes 16
-// columns (rows of w) and all rows of x, NW waves a part of the inner dimension
-// each, joined in LDS.  A lane of a product takes 16 bytes of w's row lane % 16,
-// piece lane / 16 of four; U products' loads are in flight.  ODD: rows of 16 bits
-// that begin inside a word, read as the five words they lie in (6 gated rows of 2233
-// x 4821: 19 us; as 16 bytes from their own address 31, of 2232 14).
-// 1 row of 4096 x 4096 and its residual: 8.9 us, 3.8 TB/s.
-template <typename T, int MT, int NW, int OPS, bool ODD>
-__global__ __launch_bounds__(64 * NW) void linear_few_kernel(LinearArgs a) {
-  constexpr int PER = 16 / sizeof(T), STEP = 4 * PER, U = MT * OPS <= 2 && !ODD ? 8 : 4;
+// columns (rows of w) and all rows of x, eight waves a part of the inner dimension
+// each, joined in LDS (four took as long within 2 %, however many columns).  A lane of
+// a product takes 16 bytes of w's row lane % 16, piece lane / 16 of four; U products'
+// loads are in flight.  1 row of 4096 x 4096 and its residual: 8.9 us, 3.8 TB/s.
+// ODD: rows of 16 bits that begin inside a word, read as the five words they lie in
+// (6 gated rows of 2233 x 4821: 19 us; as 16 bytes from their own address 31, of 2232
+// 14).
+template <typename T, int MT, int OPS, bool ODD>
+__global__ __launch_bounds__(512) void linear_few_kernel(LinearArgs a) {
+  constexpr int NW = 8, PER = 16 / sizeof(T), STEP = 4 * PER, U = MT * OPS <= 2 && !ODD ? 8 : 4;
   __shared__ float part[NW][OPS * MT][4][64];
   const int tid = threadIdx.x, lane = tid & 63, row = lane & 15, quarter = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -638,7 +639,8 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a) {
 // 4096 42 and 70; 64 x 1121 x 8192, 18773 x 1137 x 137: not).  Those of 32 bits lose too
 // little (2673 x 3321 x 536: 145, whole 110).
 struct Plan {
-  int few, size, splits, split_steps;      // few: waves of the few-rows kernel, or 0
+  bool few;                                // the few-rows kernel
+  int size, splits, split_steps;
   bool pack[3];                            // x, w, w2
 };
 
@@ -671,7 +673,7 @@ inline int64_t packed_row(const CfLinearArgs& x) {         // of 16 bits: whole 
 // The plan does not look at addresses, so that a workspace can be asked for without
 // them.
 inline Plan plan_of(const CfLinearArgs& x, bool gated) {
-  Plan p = {0, 0, 1, 0, {false, false, false}};
+  Plan p = {false, 0, 1, 0, {false, false, false}};
   const bool f32 = x.dtype == SEQ_F32;
   const int64_t step = f32 ? 32 : 64, steps = (x.inner + step - 1) / step;
   const int half = gated ? 2 : 1;
@@ -680,7 +682,7 @@ inline Plan plan_of(const CfLinearArgs& x, bool gated) {
   };
   bool vec = whole_pieces(x, p, false);
   if (x.rows <= FEW_ROWS && (!vec || x.rows <= 8 || x.rows * tiles(64, 64) < 8 * CUS)) {
-    p.few = (x.cols + 15) / 16 >= 2 * CUS ? 4 : 8;
+    p.few = true;
     return p;
   }
   // (laid out rows have to be near each other, too, and one launch's work)
@@ -722,26 +724,21 @@ inline int64_t workspace_of(const CfLinearArgs& x, const Plan& p, bool gated) {
 }
 
 template <typename T, int OPS, bool ODD>
-hipError_t launch_rows(const LinearArgs& a, int waves, hipStream_t st) {
+hipError_t launch_rows(const LinearArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)((a.cols + 15) / 16));
-  if (a.rows <= 16) {
-    if (waves == 4) hipLaunchKernelGGL((linear_few_kernel<T, 1, 4, OPS, ODD>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((linear_few_kernel<T, 1, 8, OPS, ODD>), grid, dim3(512), 0, st, a);
-  } else {
-    if (waves == 4) hipLaunchKernelGGL((linear_few_kernel<T, 2, 4, OPS, ODD>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((linear_few_kernel<T, 2, 8, OPS, ODD>), grid, dim3(512), 0, st, a);
-  }
+  if (a.rows <= 16) hipLaunchKernelGGL((linear_few_kernel<T, 1, OPS, ODD>), grid, dim3(512), 0, st, a);
+  else hipLaunchKernelGGL((linear_few_kernel<T, 2, OPS, ODD>), grid, dim3(512), 0, st, a);
   return hipGetLastError();
 }
 
 template <typename T, int OPS>
-hipError_t launch_few(const LinearArgs& a, int waves, hipStream_t st) {
+hipError_t launch_few(const LinearArgs& a, hipStream_t st) {
   if constexpr (sizeof(T) == 2) {
     auto odd = [](const void* base, int64_t stride) { return (uintptr_t)base % 4 != 0 || stride % 2 != 0; };
-    if ((a.rows > 1 ? odd(a.x, a.xr) : odd(a.x, 0)) || odd(a.w[0], a.wr[0]) || (OPS == 2 && odd(a.w[1], a.wr[1])))
-      return launch_rows<T, OPS, true>(a, waves, st);
+    if (odd(a.x, a.rows > 1 ? a.xr : 0) || odd(a.w[0], a.wr[0]) || (OPS == 2 && odd(a.w[1], a.wr[1])))
+      return launch_rows<T, OPS, true>(a, st);
   }
-  return launch_rows<T, OPS, false>(a, waves, st);
+  return launch_rows<T, OPS, false>(a, st);
 }
 
 template <typename T, int BM, int BN, int WM, int WN, int NST, int OPS, bool VEC>
@@ -775,7 +772,7 @@ hipError_t launch_sizes(const LinearArgs& a, const Plan& p, hipStream_t st) {
 
 template <typename T, int OPS>
 hipError_t launch_linear(const LinearArgs& a, const Plan& p, bool vec, hipStream_t st) {
-  if (p.few) return launch_few<T, OPS>(a, p.few, st);
+  if (p.few) return launch_few<T, OPS>(a, st);
   return vec ? launch_sizes<T, OPS, true>(a, p, st) : launch_sizes<T, OPS, false>(a, p, st);
 }
 
