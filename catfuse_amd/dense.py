@@ -134,7 +134,9 @@ def _product(what, x, w, w2, bias, bias2, activation, residual, out):
         return out
     work = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     ev = _t0()
-    args = _hip.LINEAR_ARGS[0].pack(_at(x), _at(w), _at(w2), _at(bias), _at(bias2), _at(residual),
+    # (a second w of no elements has no address, and is there all the same: any one does)
+    second = 0 if w2 is None else _at(w2) or _at(out)
+    args = _hip.LINEAR_ARGS[0].pack(_at(x), _at(w), second, _at(bias), _at(bias2), _at(residual),
                                     _at(out), _at(work), _hip.stream(dev)) + tail
     _call(_hip.lib().cf_linear, "cf_linear", dev, args)
     if given:

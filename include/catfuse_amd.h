@@ -959,7 +959,8 @@ int cf_rotary(const CfRotaryArgs* args);
  * whole pieces of 16 bytes may be laid out again first: the workspace (16-byte
  * aligned) has at least the bytes that cf_linear_workspace gives for the same
  * block, whose addresses it does not look at but for w2 being null or not (0: none
- * is needed, -1: the sizes make no sense). */
+ * is needed, -1: the sizes make no sense).  inner may be 0 (empty sums): x and w are
+ * then not read and may be null, and w2, not read either, still says which of the two. */
 #define CF_LINEAR_MAX_ROWS 1000000000
 #define CF_LINEAR_MAX_WIDTH 16000000
 #define CF_ACT_NONE 0

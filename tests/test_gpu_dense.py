@@ -267,6 +267,20 @@ def test_empty(cuda):
         assert torch.equal(out, (b + 1).expand(M, 7))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("M", [3, 40, 300])
+def test_gated_without_an_inner_dimension(cuda, dtype, M):
+    """Empty sums on both sides: the activated bias times the other."""
+    def z(*s):
+        return torch.zeros(s, dtype=dtype, device=cuda)
+    bg, bu = torch.linspace(-2, 2, 40, device=cuda), torch.linspace(3, -1, 40, device=cuda)
+    for act in ACTS:
+        got = kernels.gated_linear(z(M, 0), z(40, 0), z(40, 0), bias_gate=bg, bias_up=bu, activation=act)
+        _check(got, z(M, 0), (z(40, 0), z(40, 0)), (bg, bu), act)
+        assert not bool(kernels.gated_linear(z(M, 0), z(40, 0), z(40, 0), bias_gate=bg,
+                                             activation=act).any())
+
+
 def test_more_than_32_bits(cuda):
     """An x and an output of more than 2^31 elements, rows more than 2^31 apart."""
     K, N = 64, 96
