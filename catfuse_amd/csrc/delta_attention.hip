@@ -244,7 +244,9 @@ __global__ __launch_bounds__(1024) void delta_begins_kernel(DeltaArgs a) {
 // The products k_t . k_s on the matrix cores; blocks of 16 inverted column by
 // column in registers, then joined in pairs by fp32 matrix instructions:
 //   (A 0; B D)^-1 = (A^-1 0; -D^-1 B A^-1 D^-1).
-// Rows of L from the first one that is not finite on are left out, and of T NaN.
+// Rows of L from the first one that is not finite on are left out, and of T NaN; so are
+// those of T from the first row of a B A^-1 on that is not: a product with the zeros
+// of D^-1 would make NaN of the rows before it.
 // Bound by the substitution's chain of dependent steps and by T's bytes (300 a token
 // and head of C = 64, 2.2 TB/s): 65536 tokens x 32 heads of 128 bf16 channels 290 us.
 template <int C> constexpr int solved_size() { return (C / 32) * (C / 32 + 1) / 2 * 6144; }   // bytes
@@ -376,6 +378,16 @@ __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
   }
   __syncthreads();
   const int c16 = lane & 15, q16 = lane >> 4;
+  auto keep_finite = [&](f4v& m, int row) {  // rows row .. + 3 of a B A^-1
+    const float z = __builtin_fmaf(m[0], 0.0f, m[1] * 0.0f) + __builtin_fmaf(m[2], 0.0f, m[3] * 0.0f);
+    if (__ballot(z != z) == 0) return;
+#pragma unroll
+    for (int j = 3; j >= 0; --j)
+      if (!(__builtin_fabsf(m[j]) < __builtin_inff())) {
+        atomicMin(&bad_sh, row + j);
+        m[j] = 0.0f;
+      }
+  };
   // pairs of 16: B A^-1 (its accumulators are the next product's operand as they
   // lie, if that takes its inner indices 4 q16 + j), then -D^-1 times it
   if (wave < C / 32) {
@@ -387,6 +399,7 @@ __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
       m = __builtin_amdgcn_mfma_f32_16x16x4f32(low[(b0 + 16 + c16) * P + b0 + k],
                                                inv[(b0 + k) * P + b0 + c16], m, 0, 0, 0);
     }
+    keep_finite(m, b0 + 16 + 4 * q16);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       y = __builtin_amdgcn_mfma_f32_16x16x4f32(inv[(b0 + 16 + c16) * P + b0 + 16 + 4 * q16 + j], m[j], y,
@@ -408,6 +421,8 @@ __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
                                                     0, 0, 0);
     }
 #pragma unroll
+    for (int e = 0; e < 2; ++e) keep_finite(m[e], 32 + 16 * e + 4 * q16);
+#pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -418,6 +433,7 @@ __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
     __syncthreads();
   }
 
+  const int nan_from = bad_sh;
   char* const to = a.solved + pair * solved_size<C>();
   for (int u = tid; u < TILES * 128; u += NT) {
     const int tile = u >> 7, half = (u >> 6) & 1, l = u & 63;
@@ -429,7 +445,7 @@ __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
       const Vec<float, 4> y = *reinterpret_cast<const Vec<float, 4>*>(inv + t * P + s0 + 8 * e);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float z = t >= bad_from ? __builtin_nanf("") : y.v[j];
+        const float z = t >= nan_from ? __builtin_nanf("") : y.v[j];
         x[4 * e + j] = s0 + 8 * e + j <= t ? z : 0.0f;
       }
     }
@@ -799,8 +815,24 @@ void delta_walk_kernel(DeltaArgs a) {
     }
 
     if constexpr (OUT) {
+      // (a correction beyond fp32, of values that are not, is one of them)
+      float z = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int t = 0; t < CT; ++t) z = __builtin_fmaf(U[t][r], 0.0f, z);
+      any_bad = any_bad || __ballot(z != z) != 0;
       if (CT > 1) __syncthreads();           // T is read
       if (any_bad) {
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int tok = 32 * t + 8 * (r >> 2) + 4 * hi + (r & 3);
+            bad_from = !(__builtin_fabsf(U[t][r]) < __builtin_inff()) && tok < bad_from ? tok : bad_from;
+          }
+        const int other = __shfl_xor(bad_from, 32, 64);
+        bad_from = other < bad_from ? other : bad_from;
 #pragma unroll
         for (int t = 0; t < CT; ++t)
 #pragma unroll

@@ -865,8 +865,8 @@ int cf_decay_attention_step(const CfDecayStepArgs* args);
  * of dtype; log_decay is 0 or less as a rule, -inf keeps only the token itself.
  * States, cu_seqlens, zero_rest, strides and limits as in
  * CfDecayAttentionArgs; the strides of beta and log_decay are free.  A token that
- * is not finite does not reach the tokens before it; what it does reach may be
- * NaN where the formula gives an infinity.
+ * is not finite, or whose u_t is not, does not reach the tokens before it; what it
+ * does reach may be NaN where the formula gives an infinity.
  * segment (0, or a multiple of CF_DECAY_CHUNK): sequences are split into
  * segments of so many tokens that run side by side; unused where it is not below
  * tokens; at most 65535 segments in all.  The workspace (256-byte aligned) has

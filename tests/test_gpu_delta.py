@@ -346,6 +346,38 @@ def test_keeps_later_values_from_earlier_tokens(cuda, dtype, d, bad, which):
         assert not bool(out[0, 70:, 1].isfinite().any()) and not bool(s[0, 1].isfinite().any())
 
 
+@pytest.mark.parametrize("dtype,d", [(F32, 32), (F32, 128), (BF16, 64), (BF16, 128), (BF16, 256)])
+@pytest.mark.parametrize("what", ["keys", "chain", "long chain", "values"])
+def test_overflow_does_not_reach_earlier_tokens(cuda, dtype, d, what):
+    """Finite numbers whose correction is beyond fp32: a product of two keys, of
+    corrections one after another, or the difference of two values of one key."""
+    x = dict(zip(("q", "k", "v", "beta", "log_decay"),
+                 (t.to(cuda) for t in _inputs((1, 150), (2, 2, 2), d, d, dtype, 3))))
+    at = {"keys": (70, 75), "chain": (66, 72, 84), "long chain": (66, 84, 104), "values": (70, 75)}[what]
+    end = at[-1]
+    x["q"] *= 0.01
+    x["k"][..., 5] = 0.0
+    x["log_decay"].zero_()
+    x["beta"][0, list(at)] = 1.0
+    x["v"][0, at[0], 1] = 20.0
+    if what == "values":
+        x["k"][0, list(at), 1] = 0.0
+        x["k"][0, list(at), 1, 5] = 1.0
+        x["v"][0, at[0], 1, 7] = 2e38
+        x["v"][0, end, 1, 7] = -3e38
+    else:
+        x["k"][0, list(at), 1, 5] = 3e19 if what == "keys" else 1e10
+    want, _ = kernels.delta_attention(*(t[:, :end].contiguous() for t in x.values()))
+    out, s = kernels.delta_attention(*x.values())
+    assert bool(want.isfinite().all())
+    assert torch.equal(out[:, :end], want)
+    assert bool(out[0, :, 0].isfinite().all()) and bool(s[0, 0].isfinite().all())
+    columns = [7] if what == "values" else list(range(d))
+    assert not bool(out[0, end:, 1][:, columns].isfinite().any())
+    rest = [c for c in range(d) if c not in columns]
+    assert bool(out[0, :, 1, rest].isfinite().all()) and bool(s[0, 1][:, rest].isfinite().all())
+
+
 def test_state_that_is_not_finite(cuda):
     """An infinity in a column of the state: the other columns keep their bits."""
     x = [t.to(cuda) for t in _inputs((1, 100), (2, 2, 2), 64, 64, BF16, 3)]
