@@ -23,7 +23,8 @@
 //
 // Precision as in decay_attention.hip: numbers that are not bf16 ones enter a
 // product as parts of eight bits, products of parts below 2^-24 of the whole
-// left out; T by fp32 forward substitution and products of its blocks.
+// left out; sums of log decays in 64 bits, the powers that numbers enter and leave
+// the state with to 2^-22; T by fp32 forward substitution and products of its blocks.
 //
 // No counterpart in the reference.
 #include "cf_chunk.h"
@@ -236,6 +237,14 @@ __global__ __launch_bounds__(1024) void delta_begins_kernel(DeltaArgs a) {
   }
 }
 
+// 2^x to about an ulp, whatever x is: rounded to fp32 alone, x of 16 to 24 would be
+// 6.6e-7 of the power off, and every number that goes into the state or comes out of
+// it has such a factor.  (A power beyond fp32, or below it, is one.)
+__device__ __forceinline__ float power_of_two(double x) {
+  const float y = (float)x, e = __builtin_amdgcn_exp2f(y);
+  return __builtin_fabsf(y) < 126.0f ? __builtin_fmaf(e, (float)(x - (double)y) * 0.693147182f, e) : e;
+}
+
 // T of one chunk and head.  In the workspace T lies as the walk's operands: for
 // each tile of 32 x 32 that is not above the diagonal ((0,0) (1,0) (1,1)), each half
 // of its columns and each of three parts the eight numbers of each lane: row
@@ -244,6 +253,9 @@ __global__ __launch_bounds__(1024) void delta_begins_kernel(DeltaArgs a) {
 // The products k_t . k_s on the matrix cores; blocks of 16 inverted column by
 // column in registers, then joined in pairs by fp32 matrix instructions:
 //   (A 0; B D)^-1 = (A^-1 0; -D^-1 B A^-1 D^-1).
+// L's powers, and the scores' in the walk, are of single floats: rounding x moves 2^x
+// by up to |x| 2^-24 ln 2 of itself, and as x is below zero by 0.4 x 2^-24 of a weight
+// of one at most.
 // Rows of L from the first one that is not finite on are left out, and of T NaN; so are
 // those of T from the first row of a B A^-1 on that is not: a product with the zeros
 // of D^-1 would make NaN of the rows before it.
@@ -643,12 +655,12 @@ void delta_walk_kernel(DeltaArgs a) {
     if (wave == 0) {                         // lane: token lane % C; no lane is masked off
       const double x = fall + gone, end = __shfl(x, C - 1, 64);
       const bool fold = __ballot(!(__builtin_fabs(x) <= 24.0)) == 0;
-      const float e = __builtin_amdgcn_exp2f((float)x), high = (float)fall;
+      const float e = power_of_two(x), high = (float)fall;
       fall_sh[lane % C] = {high, (float)(fall - (double)high)};
       beta_sh[lane % C] = beta;
       since_sh[lane % C] = beta * e;
       query_sh[lane % C] = a.scale * e;
-      end_sh[lane % C] = __builtin_amdgcn_exp2f((float)(fold ? -x : end - x));
+      end_sh[lane % C] = power_of_two(fold ? -x : end - x);
       gone = fold ? end : 0.0;
       auto two = [&](float* to, double f) {
         to[0] = (float)f;

@@ -141,12 +141,13 @@ def delta_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: tor
 
     Returns (out [.., H, dv], state after the last token), or out alone without
     return_state.  Sums and states are fp32, products exact to 2^-24 of their
-    factors for every type.  With keys of a length of at most 1 and beta in 0 .. 1
+    factors for every type, powers of the decays to 2^-22 (from token to token within
+    a chunk, to 2^-22 of one).  With keys of a length of at most 1 and beta in 0 .. 1
     (or keys of length 1 and beta in 0 .. 2) a step does not make errors grow; keys
-    that are longer (|k|^2 beta > 2) let the state itself and its errors grow
-    from token to token.  A token that holds an infinity or NaN, or whose u_t is
-    beyond fp32, does not reach the tokens before it; what it does reach may be NaN
-    where the formula gives an infinity.
+    that are longer (|k|^2 beta > 2) let the state itself and its errors grow from
+    token to token.  A token that holds an infinity or NaN, or whose u_t is beyond
+    fp32, does not reach the tokens before it; what it does reach may be NaN where
+    the formula gives an infinity.
     The workspace, from torch's allocator, is 300 bytes a token and head (bf16
     heads of 65 to 128 channels; others 204), and for long sequences of a small
     batch, which are walked in segments side by side, [dk, dv + dk] fp32 a segment

@@ -213,6 +213,46 @@ def test_decays_and_betas(cuda, dtype):
         _check(cuda, (q, k, v, (2 * beta).to(dtype), f.to(dtype)), state=state)
 
 
+def test_powers_of_the_decays(cuda):
+    """A state that only fades, asked channel by channel, and values written last,
+    one key each: each number is one product with exp of a sum of log decays.
+
+    Roundings in units of u = 2^-24 of it: the power of two 2 (an ulp), what its
+    argument's rounding is put back with 1, the scale 1, the product with the state or
+    with u 1; the state's fading 2 in each of at most 5 chunks before (a product with a
+    sum of two floats), 2 more for 2^G' behind the last.  Products with a number of a
+    single part, others zeros, lose none: 15 for outputs, 14 for a state that fades, 6
+    for what the last chunk wrote."""
+    N, H = 190, 8
+    g = torch.Generator().manual_seed(11)
+    rate = torch.tensor([0.01, 0.05, 0.07, 0.085, 0.1, 0.11, 0.2, 0.4])
+    f = -rate * (0.5 + torch.rand(1, N, H, generator=g))
+    f[0, 100:130, 0] = -1.3                  # a fall of 56 powers of two within a chunk
+    fall = f[0].double().cumsum(0)
+    for dtype, d in ((F32, 16), (F32, 128), (F16, 64), (BF16, 16), (BF16, 128)):
+        state = torch.randn(1, H, d, d, generator=g)
+        t = torch.arange(N)
+        q = torch.zeros(1, N, H, d)
+        q[0, t, :, t % d] = 1.0
+        zero, v = torch.zeros_like(q), torch.randn(1, N, H, d, generator=g).to(dtype)
+        q = q.to(dtype)
+        out, left = kernels.delta_attention(*(x.to(cuda) for x in (q, zero.to(dtype), v, 0 * f, f)),
+                                            scale=1.0, state=state.to(cuda))
+        want = torch.exp(fall)[:, :, None] * state[0].double()[:, t % d].transpose(0, 1)
+        _close(out[0], want, dtype, 15 * U32 * want.abs())
+        want = torch.exp(fall[-1])[:, None, None] * state[0].double()
+        _close(left[0], want, F32, 14 * U32 * want.abs())
+        # sixteen of the last tokens write
+        k, beta = zero.clone(), torch.zeros_like(f)
+        wrote = torch.arange(N - 20, N - 4)
+        k[0, wrote, :, wrote - wrote[0]] = 1.0
+        beta[0, wrote] = 1.0
+        _, left = kernels.delta_attention(*(x.to(cuda) for x in (q, k.to(dtype), v, beta, f)))
+        want = torch.exp(fall[-1] - fall[wrote])[:, :, None] * v[0, wrote].double()
+        _close(left[0, :, :16].transpose(0, 1), want, F32, 6 * U32 * want.abs())
+        assert not bool(left[0, :, 16:].any())
+
+
 def test_one_key(cuda):
     """Every token has the same key: the state holds the last value alone."""
     for dtype in (F32, F16, BF16):
