@@ -98,24 +98,47 @@ __device__ __forceinline__ float exp_f(float x) {
   // (an infinite or vanished power stays one)
   return __builtin_fabsf(y) < 126.0f ? __builtin_fmaf(e, low * 0.693147182f, e) : e;
 }
-// z / (1 + e^-t).  For outputs of 16 bits the power of two alone will do: off by
-// |t| u, which e^-t or 1 beside it makes less than u.
+// z / (1 + e^-t).  For outputs of 16 bits the power of two alone will do: rounding its
+// argument moves it, and so the result, by |t| 2^-24 of itself, 5e-6 where fp32 ends;
+// the output is then rounded by 2.4e-4 of itself (fp16) or more.
 template <typename T>
 __device__ __forceinline__ float sigmoid_times(float z, float t) {
   const float e = sizeof(T) == 4 ? exp_f(-t) : __builtin_amdgcn_exp2f(t * -1.44269502f);
   return z * __builtin_amdgcn_rcpf(1.0f + e);
 }
-// x (1 + erf(x / sqrt(2))) / 2 = max(x, 0) - |x| (1 - erf(|x| / sqrt(2))) / 2, the
-// latter by Abramowitz and Stegun's formula 7.1.26, to 1.5e-7 of |x| / 2.
+// x (1 + erf(x / sqrt(2))) / 2 = max(x, 0) - |x| Q(|x|), Q(y) = (1 - erf(y / sqrt(2))) / 2.
+template <typename T>
 __device__ __forceinline__ float gelu(float x) {
-  const float y = __builtin_fabsf(x), t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.231641888f, y, 1.0f));
+  const float a = __builtin_fabsf(x);
+  if constexpr (sizeof(T) == 4) {
+    // Q(y) e^(y^2 / 2) as a polynomial in 1 / (1 + 0.345 y), fitted here to 2.4e-8 of
+    // itself from 0 to 14.5 (least squares, weights by the errors until they are even);
+    // what rounding y^2 loses is put into the power.  To 16 x 2^-24 of the result,
+    // however small (5 measured); 4000 x 384 x 1536 takes 59.0 us with it, 55.6 with
+    // the formula below.  Beyond 20 Q is none (a NaN stays).
+    const float y = a > 20.0f ? 20.0f : a, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.345f, y, 1.0f));
+    float p = __builtin_fmaf(-0.0281517822f, t, 0.14423351f);
+    p = __builtin_fmaf(p, t, -0.269153401f);
+    p = __builtin_fmaf(p, t, 0.185054465f);
+    p = __builtin_fmaf(p, t, -0.0362378173f);
+    p = __builtin_fmaf(p, t, 0.111267676f);
+    p = __builtin_fmaf(p, t, 0.117362f);
+    p = __builtin_fmaf(p, t, 0.138005239f);
+    p = __builtin_fmaf(p, t, 0.137620113f) * t;
+    const float s = y * y, low = __builtin_fmaf(y, y, -s);
+    const float e = exp_f(-0.5f * s);
+    return __builtin_fmaf(-y, p * __builtin_fmaf(e, -0.5f * low, e), __builtin_fmaxf(x, 0.0f));
+  }
+  // For 16 bits Q by Abramowitz and Stegun's formula 7.1.26, to 2.6e-7 of one: 1e-4 of
+  // the result at -3, 1e-3 at -4, which is what rounding 1 + erf to fp32 leaves there.
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.231641888f, a, 1.0f));
   float p = __builtin_fmaf(0.530702715f, t, -0.726576014f);
   p = __builtin_fmaf(p, t, 0.710706871f);
   p = __builtin_fmaf(p, t, -0.142248368f);
   p = __builtin_fmaf(p, t, 0.127414796f) * t;
   const float tail = p * __builtin_amdgcn_exp2f(x * x * -0.721347520f);
   // (beyond 20 the tail is none, and infinity takes none of it)
-  return __builtin_fmaf(-__builtin_fminf(y, 20.0f), tail, __builtin_fmaxf(x, 0.0f));
+  return __builtin_fmaf(-__builtin_fminf(a, 20.0f), tail, __builtin_fmaxf(x, 0.0f));
 }
 template <typename T, int N>
 __device__ __forceinline__ void activate(float* z, int kind) {
@@ -127,7 +150,7 @@ __device__ __forceinline__ void activate(float* z, int kind) {
     for (int j = 0; j < N; ++j) z[j] = sigmoid_times<T>(z[j], z[j]);
   } else if (kind == CF_ACT_GELU) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) z[j] = gelu(z[j]);
+    for (int j = 0; j < N; ++j) z[j] = gelu<T>(z[j]);
   } else if (kind == CF_ACT_GELU_TANH) {     // 1 + tanh(t) = 2 / (1 + e^(-2 t))
 #pragma unroll
     for (int j = 0; j < N; ++j)

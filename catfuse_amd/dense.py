@@ -159,7 +159,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     of one type; the last dimension contiguous, rows evenly apart (any distance,
     0 too).  bias [cols], fp32 or of x's type.
     activation: None, "relu", "silu" (z / (1 + e^-z)), "gelu" (by the error
-    function) or "gelu_tanh" (its approximation by tanh).
+    function: to 2^-20 of its value, for outputs of 16 bits to 2.6e-7 of |z|) or
+    "gelu_tanh" (its approximation by tanh).
     out: a tensor for the output, apart from the inputs; it may be the residual
     itself, which is then added to in place.
 

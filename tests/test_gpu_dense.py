@@ -184,6 +184,24 @@ def test_activations(cuda, act, M):
         assert bool((y[1] == math.inf).all()) and bool(y[[0, 2, 3]].isfinite().all())
 
 
+@pytest.mark.parametrize("M", [20, 400])
+def test_gelu_of_small_values(cuda, M):
+    """fp32: relative to the result, also where it is nearly all cancelled.  Units of
+    u = 2^-24: the reciprocal 2 (an ulp) and its argument 1, of which the tail has at
+    most 1.3 times as much; the polynomial 3 (in a model of it, its fit among them);
+    the power 4, products 3, the sum 1: 16."""
+    x = torch.linspace(-12.5, 6, 40 * M, device=cuda).view(M, 40)[:, :1].contiguous()
+    w = torch.ones(1, 1, device=cuda)
+    for z in (x, x * 0.2, x.abs() * -1e-20):
+        want = z.double() * torch.special.erfc(z.double() * -0.5 ** 0.5) / 2   # (1 + erf cancels)
+        got = kernels.linear(z, w, activation="gelu").double()
+        off = ((got - want).abs() / want.abs().clamp(min=2.0 ** -126)).max().item()
+        assert off <= 16 * U32
+    bad = torch.tensor([[math.nan], [math.inf], [-math.inf], [0.0]], device=cuda)
+    y = kernels.linear(bad, w, activation="gelu")[:, 0]
+    assert bool(y[0].isnan()) and y[1:].tolist() == [math.inf, 0.0, 0.0]
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("M", [1, 20, 150])
 def test_strides(cuda, dtype, M):
