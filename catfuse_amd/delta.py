@@ -20,7 +20,7 @@ from torch.autograd.graph import increment_version as _changed
 
 from catfuse_amd import _hip
 from catfuse_amd.runtime import _t0, _t1
-from catfuse_amd.sequence import (_DTYPES, _PLANS, _at, _call, _keep, _looks, _require,
+from catfuse_amd.sequence import (_DTYPES, _at, _call, _keep, _looks, _planned, _require,
                                   _require_apart, _require_gpu, _require_index, _require_output,
                                   _require_rows, _span, CHUNK, MAX_HEADS, MAX_KEY_DIM, MAX_SEQUENCES,
                                   MAX_TOKEN_STRIDE, MAX_TOKENS, MAX_VALUE_DIM)
@@ -157,7 +157,7 @@ def delta_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: tor
         key = (delta_attention, _looks(q), _looks(k), _looks(v), _looks(beta), _looks(log_decay),
                _looks(state), _looks(cu_seqlens), _looks(out), scale, return_state,
                torch.is_grad_enabled())
-        plan = _PLANS.get(key)
+        plan = _planned(key)
     except (AttributeError, TypeError):      # not tensors: the checks say which
         key = plan = None
     if plan is None:
@@ -268,7 +268,7 @@ def delta_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta
         key = (delta_attention_step, _looks(q), _looks(k), _looks(v), _looks(beta),
                _looks(log_decay), _looks(state), _looks(slots), _looks(out), scale,
                torch.is_grad_enabled())
-        plan = _PLANS.get(key)
+        plan = _planned(key)
     except (AttributeError, TypeError):      # not tensors: the checks say which
         key = plan = None
     if plan is None:

@@ -20,7 +20,7 @@ from torch.autograd.graph import increment_version as _changed
 
 from catfuse_amd import _hip
 from catfuse_amd.runtime import _t0, _t1
-from catfuse_amd.sequence import (_DTYPES, _PLANS, _at, _call, _keep, _looks, _require,
+from catfuse_amd.sequence import (_DTYPES, _at, _call, _keep, _looks, _planned, _require,
                                   _require_apart, _require_gpu, _require_output, _require_rows)
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}   # CF_ACT_*
@@ -111,7 +111,7 @@ def _product(what, x, w, w2, bias, bias2, activation, residual, out):
     try:
         key = (what, activation, torch.is_grad_enabled(), _looks(x), _looks(w), _looks(w2),
                _looks(bias), _looks(bias2), _looks(residual), _looks(out))
-        plan = _PLANS.get(key)
+        plan = _planned(key)
     except (AttributeError, TypeError):      # not tensors: the checks say which
         key = plan = None
     if plan is None:

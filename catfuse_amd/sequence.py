@@ -8,10 +8,11 @@ and what its heads go through before: the norm of each head and the rotation
 by the token's position on one to three axes (`qk_norm_rotary`, `rotary`).
 
 Inference only, like the rest of the package: an input that requires a
-gradient is refused while gradients are recorded.  Everything runs on the
-current stream of the inputs' device and neither waits for the GPU nor reads
-values back, so calls can be captured into a HIP graph; what is wrong with
-values in device memory (offsets, slots) is handled on the device, as each
+gradient is refused while gradients are recorded, and one with a forward-mode
+tangent always.  Everything runs on the current stream of the inputs' device
+and neither waits for the GPU nor reads values back, so calls can be captured
+into a HIP graph; what is wrong with values in device memory (offsets, slots)
+is handled on the device, as each
 function says.  No counterpart in the reference.
 """
 from __future__ import annotations
@@ -19,6 +20,7 @@ from __future__ import annotations
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad as _forward
 # Tensors that a kernel writes count as changed, as after an in-place operation
 # of torch: the package's copies of a fused output and autograd's saved tensors
 # go by that count.
@@ -56,6 +58,18 @@ def _looks(t):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.device, t.requires_grad)
 
 
+def _tangent(t) -> bool:
+    """Whether forward-mode differentiation goes through a tensor (which no_grad
+    does not stop); outside of its levels it goes through none."""
+    return _forward._current_level >= 0 and _forward.unpack_dual(t).tangent is not None
+
+
+def _planned(key):
+    """The plan kept for a key; none at a level of forward mode, where the checks
+    look for tangents."""
+    return _PLANS.get(key) if _forward._current_level < 0 else None
+
+
 def _keep(key, plan):
     if len(_PLANS) >= 512:
         _PLANS.clear()
@@ -72,7 +86,7 @@ def _at(t) -> int:
 # ---------------------------------------------------------------------------
 
 def _require(t, name: str, dtype, dev=None) -> None:
-    """A tensor of one of the dtypes, on `dev`, without a gradient."""
+    """A tensor of one of the dtypes, on `dev`, without a gradient or tangent."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dtype not in dtype:
@@ -82,6 +96,9 @@ def _require(t, name: str, dtype, dev=None) -> None:
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires a gradient: this operator is for inference (call it "
                            "under torch.no_grad() or detach the input)")
+    if _tangent(t):
+        raise RuntimeError(f"{name} carries a forward-mode tangent: this operator is for inference "
+                           "(unpack its primal value)")
 
 
 def _require_gpu(t, name: str) -> None:
@@ -261,7 +278,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     try:
         key = (decay_attention, _looks(q), _looks(k), _looks(v), _looks(log_decay), _looks(state),
                _looks(cu_seqlens), _looks(out), scale, return_state, torch.is_grad_enabled())
-        plan = _PLANS.get(key)
+        plan = _planned(key)
     except (AttributeError, TypeError):      # not tensors: the checks say which
         key = plan = None
     if plan is None:
@@ -365,7 +382,7 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     try:
         key = (decay_attention_step, _looks(q), _looks(k), _looks(v), _looks(log_decay),
                _looks(state), _looks(slots), _looks(out), scale, torch.is_grad_enabled())
-        plan = _PLANS.get(key)
+        plan = _planned(key)
     except (AttributeError, TypeError):      # not tensors: the checks say which
         key = plan = None
     if plan is None:
@@ -497,7 +514,7 @@ def _rotate(x, k, positions, freqs, sections, interleaved, inverse, norm, eps, w
         key = (_rotate, _looks(x), _looks(k), _looks(positions), _looks(freqs), sections,
                interleaved, inverse, norm, eps, _looks(weights[0]), _looks(weights[1]),
                _looks(outs[0]), _looks(outs[1]), torch.is_grad_enabled())
-        plan = _PLANS.get(key)
+        plan = _planned(key)
     except (AttributeError, TypeError):      # not tensors: the checks say which
         key = plan = None
     if plan is None:

@@ -284,3 +284,43 @@ def test_token_dimensions_reduce_to_two_strides():
     assert s((1, 7, 1), [(5, 3, 9)]) == (1, 7, [(0, 3)])
     with pytest.raises(ValueError, match="two strides"):
         s((2, 3, 4), [(1, 100, 7)])
+
+
+def _calls():
+    """One call of each operator that takes real values, by its inputs' names."""
+    q, k, v = torch.zeros(1, 3, 4, 8), torch.zeros(1, 3, 2, 8), torch.zeros(1, 3, 2, 6)
+    beta, f, state = torch.zeros(1, 3, 4), torch.zeros(1, 3, 4), torch.zeros(1, 4, 8, 6)
+    pos, freqs, w = torch.arange(3), kernels.rotary_freqs(4), torch.zeros(6, 8)
+    return [
+        (kernels.decay_attention, dict(q=q, k=k, v=v, log_decay=torch.zeros(4), state=state)),
+        (kernels.decay_attention_step, dict(q=q[0], k=k[0], v=v[0], log_decay=torch.zeros(4),
+                                            state=torch.zeros(3, 4, 8, 6))),
+        (kernels.rotary, dict(x=q[0], positions=pos, freqs=freqs)),
+        (kernels.qk_norm_rotary, dict(q=q[0], k=k[0], positions=pos, freqs=freqs,
+                                      q_weight=torch.ones(8))),
+        (kernels.delta_attention, dict(q=q, k=k, v=v, beta=beta, log_decay=f, state=state)),
+        (kernels.delta_attention_step, dict(q=q[0], k=k[0], v=v[0], beta=beta[0], log_decay=f[0],
+                                            state=torch.zeros(3, 4, 8, 6))),
+        (kernels.linear, dict(x=q, w=w, bias=torch.zeros(6), residual=torch.zeros(1, 3, 4, 6))),
+        (kernels.gated_linear, dict(x=q, w_gate=w, w_up=w + 1, bias_gate=torch.zeros(6)))]
+
+
+@pytest.mark.parametrize("i", range(8))
+def test_tangents_are_refused(i):
+    """By every input of every operator, also after a call of the same shapes that
+    passed the checks, and where no gradients are recorded."""
+    from torch.autograd import forward_ad
+    call, inputs = _calls()[i]
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        call(**inputs)
+    with forward_ad.dual_level(), torch.no_grad():
+        for name, t in inputs.items():
+            if t.is_floating_point():
+                dual = forward_ad.make_dual(t.clone(), torch.ones_like(t))
+                with pytest.raises(RuntimeError, match="tangent"):
+                    call(**dict(inputs, **{name: dual}))
+                plain = forward_ad.unpack_dual(dual).primal
+                with pytest.raises(RuntimeError, match="GPU tensor"):
+                    call(**dict(inputs, **{name: plain}))
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        call(**inputs)
