@@ -1209,8 +1209,20 @@ hipError_t launch_delta(const DeltaArgs& a, hipStream_t st) {
 
 }  // namespace
 
+// A block's sizes, whatever its addresses and strides.
+static bool sizes_make_sense(const CfDeltaAttentionArgs& x) {
+  if (x.seqs < 0 || x.seqs > CF_DECAY_MAX_SEQS || x.tokens < 0 || x.tokens > CF_DECAY_MAX_TOKENS ||
+      !delta_heads_fit(x.heads, x.q_heads, x.k_heads, x.v_heads) || x.dk < 1 || x.dk > CF_DECAY_MAX_DK ||
+      x.dv < 1 || x.dv > CF_DECAY_MAX_DV || x.dtype < 0 || x.dtype > 2 || x.segment < 0 ||
+      x.segment % CF_DECAY_CHUNK != 0)
+    return false;
+  // the join's grid
+  return x.segment == 0 || x.segment >= x.tokens ||
+         (x.cu_seqlens ? x.tokens / x.segment + x.seqs : x.seqs * units_of(x.tokens, x.segment)) <= 65535;
+}
+
 CF_API int64_t cf_delta_workspace(const CfDeltaAttentionArgs* p) {
-  if (!p || p->heads < 1 || p->seqs < 0 || p->tokens < 0 || p->segment < 0) return -1;
+  if (!p || !sizes_make_sense(*p)) return -1;
   const CfDeltaAttentionArgs& x = *p;
   const int64_t C = chunk_of(x.dtype, x.dk);
   const int64_t solved = (C / 32) * (C / 32 + 1) / 2 * 6144;
@@ -1228,11 +1240,7 @@ CF_API int64_t cf_delta_workspace(const CfDeltaAttentionArgs* p) {
 CF_API int cf_delta_attention(const CfDeltaAttentionArgs* p) {
   if (!p) return (int)hipErrorInvalidValue;
   const CfDeltaAttentionArgs& x = *p;
-  if (x.seqs < 0 || x.tokens < 0 || !delta_heads_fit(x.heads, x.q_heads, x.k_heads, x.v_heads) ||
-      x.dk < 1 || x.dk > CF_DECAY_MAX_DK || x.dv < 1 || x.dv > CF_DECAY_MAX_DV || x.dtype < 0 ||
-      x.dtype > 2 || x.seqs > CF_DECAY_MAX_SEQS || x.tokens > CF_DECAY_MAX_TOKENS || x.segment < 0 ||
-      x.segment % CF_DECAY_CHUNK != 0 || x.workspace_bytes < 0)
-    return (int)hipErrorInvalidValue;
+  if (!sizes_make_sense(x) || x.workspace_bytes < 0) return (int)hipErrorInvalidValue;
   for (int64_t s : {x.q_token, x.k_token, x.v_token, x.out_token})
     if (s < 0 || s > CF_DECAY_MAX_TOKEN_STRIDE) return (int)hipErrorInvalidValue;
   if (x.seqs == 0) return 0;
@@ -1261,7 +1269,6 @@ CF_API int cf_delta_attention(const CfDeltaAttentionArgs* p) {
   a.segment = x.segment > 0 && x.segment < x.tokens ? x.segment : 0;
   a.segments = a.segment == 0 ? x.seqs
                : a.cu ? x.tokens / a.segment + x.seqs : x.seqs * units_of(x.tokens, a.segment);
-  if (a.segment > 0 && a.segments > 65535) return (int)hipErrorInvalidValue;   // the join's grid
   char* at = (char*)x.workspace;
   a.begins = (int64_t*)at;
   a.before = a.begins + x.seqs + 1;

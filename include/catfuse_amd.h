@@ -870,8 +870,9 @@ int cf_decay_attention_step(const CfDecayStepArgs* args);
  * segment (0, or a multiple of CF_DECAY_CHUNK): sequences are split into
  * segments of so many tokens that run side by side; unused where it is not below
  * tokens; at most 65535 segments in all.  The workspace (256-byte aligned) has
- * at least the bytes that cf_delta_workspace gives for the same block (-1: the
- * block makes no sense); every call needs one, and it is free again when the
+ * at least the bytes that cf_delta_workspace gives for the same block (-1: its
+ * sizes make no sense; of the addresses it looks at cu_seqlens being null or not, and
+ * at no strides); every call needs one, and it is free again when the
  * call's work on the stream is done. */
 typedef struct CfDeltaAttentionArgs {
   const void* q;

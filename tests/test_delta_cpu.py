@@ -212,3 +212,19 @@ def test_step_refuses_overlaps():
     with pytest.raises(ValueError, match="out overlaps"):
         _step(state=state, out=state.flatten()[:72].view(3, 4, 6))
     assert math.prod(state.shape) == 960
+
+
+def test_workspace_refuses():
+    """The sizes that a call refuses, and none of its strides."""
+    L, fine = _hip.lib(), dict(segment=0, workspace=256, workspace_bytes=1 << 40)
+    assert L.cf_delta_workspace(None) == -1
+    for bad in (dict(seqs=-1), dict(seqs=65536), dict(tokens=-1), dict(tokens=2 * 10 ** 9 + 1),
+                dict(heads=0), dict(heads=-2), dict(heads=4097), dict(q_heads=2), dict(k_heads=0),
+                dict(heads=3, v_heads=2), dict(dk=0), dict(dk=257), dict(dv=0), dict(dv=1025),
+                dict(dv=2000), dict(dtype=3), dict(dtype=9), dict(dtype=-1), dict(segment=100),
+                dict(segment=-64), dict(segment=64, tokens=64 * 65536),
+                dict(segment=64, tokens=64 * 65536, cu_seqlens=0)):
+        block = _attention(**dict(fine, **bad))
+        assert L.cf_delta_workspace(block) == -1, bad
+        assert L.cf_delta_attention(block) == INVALID, bad
+    assert L.cf_delta_workspace(_attention(**dict(fine, q_token=-1, out_head=-5, scale=0.0))) > 0
