@@ -228,3 +228,14 @@ def test_workspace_refuses():
         assert L.cf_delta_workspace(block) == -1, bad
         assert L.cf_delta_attention(block) == INVALID, bad
     assert L.cf_delta_workspace(_attention(**dict(fine, q_token=-1, out_head=-5, scale=0.0))) > 0
+
+
+@pytest.mark.parametrize("seqs", [16, 31, 63, 64, 1000])
+def test_workspace_of_packed_rows(seqs):
+    """The rows that packed sequences begin at and the segments before them, two
+    64-bit numbers for each and one end."""
+    f = dict(dtype=0, dk=32, dv=32, seqs=seqs, cu_seqlens=256, segment=0)
+    begins = (16 * (seqs + 1) + 255) // 256 * 256
+    assert _hip.lib().cf_delta_workspace(_attention(tokens=0, **f)) == begins
+    chunks = (5000 // 32 + seqs) * (6144 + 12 * 32)
+    assert _hip.lib().cf_delta_workspace(_attention(tokens=5000, **f)) == begins + chunks
