@@ -149,9 +149,11 @@ def delta_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: tor
     fp32, does not reach the tokens before it; what it does reach may be NaN where
     the formula gives an infinity.
     The workspace, from torch's allocator, is 300 bytes a token and head (bf16
-    heads of 65 to 128 channels; others 204), and for long sequences of a small
-    batch, which are walked in segments side by side, [dk, dv + dk] fp32 a segment
-    and head."""
+    heads of 65 to 128 channels, whose sequences count as whole multiples of 64
+    tokens; others 204 and 32), and for long sequences of a small batch, which are
+    walked in segments side by side, [dk, dv + dk] fp32 a segment and head.  Many
+    short sequences are computed in groups, so that the former is at most three
+    times what the tokens themselves take, and 1 GiB."""
     scale = None if scale is None else float(scale)
     try:
         key = (delta_attention, _looks(q), _looks(k), _looks(v), _looks(beta), _looks(log_decay),

@@ -239,3 +239,26 @@ def test_workspace_of_packed_rows(seqs):
     assert _hip.lib().cf_delta_workspace(_attention(tokens=0, **f)) == begins
     chunks = (5000 // 32 + seqs) * (6144 + 12 * 32)
     assert _hip.lib().cf_delta_workspace(_attention(tokens=5000, **f)) == begins + chunks
+
+
+@pytest.mark.parametrize("dtype,dk,a_token", [(2, 128, 300), (2, 64, 204), (0, 128, 204), (1, 256, 204)])
+@pytest.mark.parametrize("heads", [1, 32, 4096])
+def test_workspace_of_short_sequences(dtype, dk, a_token, heads):
+    """At most three times what the tokens take and 1 GiB (or one sequence's), by
+    however many sequences; what the tokens take and a chunk for each sequence
+    where they have half a chunk on average."""
+    C = 64 if a_token == 300 else 32
+    def need(**f):
+        return _hip.lib().cf_delta_workspace(_attention(dtype=dtype, dk=dk, dv=dk, heads=heads,
+                                                        segment=0, **f))
+    for seqs in (1, 100, 256, 4096, 65535):
+        for mean in (0, 1, 3, C // 2 - 1, C // 2, C, 1000):
+            for cu in (0, 256):
+                tokens = mean * (seqs if cu else 1) + (5 if cu else 0)
+                begins = (16 * (seqs + 1) + 255) // 256 * 256 if cu else 0
+                total = tokens if cu else tokens * seqs
+                got = need(seqs=seqs, tokens=tokens, cu_seqlens=cu) - begins
+                one = a_token * C * heads
+                assert 0 <= got <= 3 * a_token * heads * total + max(1 << 30, one) + one
+                if mean >= C // 2:
+                    assert got == (tokens // C + seqs if cu else seqs * -(-tokens // C)) * one

@@ -318,6 +318,50 @@ def test_many_sequences(cuda, B, N, H):
         _close(left[b], s, F32, (depth * U32 * n)[:, None, :])
 
 
+@pytest.mark.parametrize("dtype,d", [(F32, 16), (BF16, 16), (BF16, 72)])
+@pytest.mark.parametrize("packed", [False, True])
+def test_workspace_of_many_short_sequences(cuda, dtype, d, packed):
+    """Tens of thousands of prompts of no, one or a few tokens: each as its definition,
+    in a workspace that is bound by the tokens."""
+    g = torch.Generator().manual_seed(5)
+    B, H, dv = 30000 if d < 32 else 12000, 8, 8
+    if packed:
+        lens = torch.randint(0, 3, (B,), generator=g)
+        lens[7], lens[B // 2], lens[-1] = 90, 200, 65
+        at = torch.cat([torch.zeros(1, dtype=torch.int64), lens.cumsum(0)]) + 3
+        lead, given = (int(at[-1]) + 5,), at.clone()
+        given[B // 3] = 0                    # counts as its predecessor
+        at[B // 3] = at[B // 3 - 1]
+    else:
+        lead, given = (B, 2), None
+    q, k, v, beta, f = _inputs(lead, (H, 1, H), d, dv, dtype, 3, H=H)
+    state = torch.randn(B, H, d, dv, generator=g)
+    x = [t.to(cuda) for t in (q, k, v, beta, f)]
+    state_in = state.to(cuda)
+    more = dict(state=state_in, cu_seqlens=None if given is None else given.to(cuda))
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    out, left = kernels.delta_attention(*x, **more)
+    torch.cuda.synchronize()
+    took = torch.cuda.max_memory_allocated() - held
+    tokens = math.prod(lead)
+    a_token = 300 if dtype == BF16 and d > 64 else 204
+    took -= out.numel() * out.element_size() + left.numel() * 4 + 32 * (B + 1) + 4096
+    assert took <= (1 << 30) + 3 * a_token * tokens * H
+    if packed:
+        assert not bool(out[:3].any()) and not bool(out[-5:].any())
+    picks = [0, 1, 7, 8, B // 3 - 1, B // 3, B // 3 + 1, B // 2, B - 2, B - 1]
+    picks += torch.randint(0, B, (40,), generator=g).tolist()
+    for b in picks:
+        i, j = (int(at[b]), int(at[b + 1])) if packed else (0, 2)
+        a = [(t[i:j] if packed else t[b]).double() for t in (q, k, v, beta, f)]
+        want, s, bound, n = _definition(*a, d ** -0.5, state[b].double())
+        depth = 72 * _solve_norm(a[1], a[3], a[4], H)
+        _close(out[i:j] if packed else out[b], want, dtype, depth * U32 * bound)
+        _close(left[b], s, F32, (depth * U32 * n)[:, None, :])
+
+
 def test_strides(cuda):
     """Heads of one fused projection, transposed and expanded ones, betas among
     other columns, an output among other columns, misaligned rows: the values of
