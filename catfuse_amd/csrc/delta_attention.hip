@@ -105,12 +105,17 @@ constexpr int64_t LANE_SEQS = 63, LANE_CHUNKS = 8192;
 // Place w in a numbering of units: with gaps (above), without, or without the
 // sequences' last ones; w becomes the number with gaps.
 enum Numbers { GAPS, DENSE, INNER };
-__device__ __forceinline__ Place place_in_lanes(const DeltaArgs& a, int64_t& w, int unit, Numbers numbers) {
+__device__ __forceinline__ Place place_in_lanes(const DeltaArgs& a, int64_t& w, int unit, Numbers numbers,
+                                                int64_t* ends = nullptr) {
   const int lane = threadIdx.x & 63, seqs = (int)a.seqs;
   int begin = lane <= seqs ? (int)seq_offset(a.cu, a.cu_wide, lane, a.tokens) : 0;
   for (int d = 1; d < 64; d *= 2) {          // none below its predecessor
     const int o = __shfl_up(begin, d, 64);
     if (lane >= d && o > begin) begin = o;
+  }
+  if (ends != nullptr) {
+    ends[0] = __builtin_amdgcn_readlane(begin, 0);
+    ends[1] = __builtin_amdgcn_readlane(begin, seqs);
   }
   const int len = __shfl_down(begin, 1, 64) - begin;
   const int units = (int)(((unsigned)len + (unsigned)unit - 1u) / (unsigned)unit), own = len > 0 ? units : 1;
@@ -142,9 +147,11 @@ __device__ __forceinline__ Place place_in_lanes(const DeltaArgs& a, int64_t& w, 
   return s;
 }
 
-__device__ __forceinline__ Place find_place(const DeltaArgs& a, int64_t w, int64_t unit) {
+// ends: of packed sequences, the first one's first row and the row behind the last.
+__device__ __forceinline__ Place find_place(const DeltaArgs& a, int64_t w, int64_t unit,
+                                            int64_t* ends = nullptr) {
   if (a.cu != nullptr && a.begins == nullptr)
-    return place_in_lanes(a, w, (int)(unit < INT32_MAX ? unit : INT32_MAX), GAPS);
+    return place_in_lanes(a, w, (int)(unit < INT32_MAX ? unit : INT32_MAX), GAPS, ends);
   Place s;
   s.row0 = 0;
   if (a.cu == nullptr) {
@@ -159,6 +166,10 @@ __device__ __forceinline__ Place find_place(const DeltaArgs& a, int64_t w, int64
   s.seq = -1;
   s.part = s.parts = s.begin = s.len = s.row0 = 0;
   const int64_t row0 = a.group ? a.begins[0] : 0;
+  if (ends != nullptr) {
+    ends[0] = a.begins[0];
+    ends[1] = a.begins[a.seqs];
+  }
   const int64_t lo = last_at_most(a.seqs, w, [&](int64_t i) { return i + (a.begins[i] - row0) / unit; });
   if (lo < 0) return s;
   const int64_t begin = uniform(a.begins[lo]), len = uniform(a.begins[lo + 1]) - begin;
@@ -271,6 +282,23 @@ template <int C> constexpr int solved_size() { return (C / 32) * (C / 32 + 1) / 
 
 typedef float f4v __attribute__((ext_vector_type(4)));
 
+//
+// Rows of no sequence are set to zeros here, a part by every workgroup: 1000 tokens of
+// 16 heads of 128 bf16 channels in 65536 rows take 150 us (118 into a given output), by
+// the walks' first and last workgroups alone 1260.
+template <typename T, int NT, bool VEC>
+__device__ __forceinline__ void clear_rest(const DeltaArgs& a, int64_t w, int h, const int64_t* ends) {
+  constexpr int PER = VEC ? 16 / (int)sizeof(T) : 1;
+  const int64_t front = a.zero_rest & 1 ? ends[0] : 0, rest = front + (a.zero_rest & 2 ? a.tokens - ends[1] : 0);
+  if (w >= rest) return;
+  const int units = a.dv / PER;              // of a row
+  const int64_t count = ((rest - w + a.chunks - 1) / a.chunks) * units;
+  for (int64_t i = threadIdx.x; i < count; i += NT) {
+    const int64_t r = w + i / units * a.chunks, t = r < front ? r : ends[1] + (r - front);
+    *reinterpret_cast<Vec<T, PER>*>((T*)a.out + t * a.ot + h * a.oh + i % units * PER) = Vec<T, PER>{};
+  }
+}
+
 template <typename T, int DKP, int C, int NT, bool VEC>
 __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
   constexpr int NL = parts_of<T>(), NP = 3, KS = DKP / 16, CT = C / 32, TILES = CT * (CT + 1) / 2;
@@ -289,7 +317,9 @@ __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
   const int64_t pair = a.first + blockIdx.x;
   const int64_t w = uniform(pair / a.heads);
   const int h = (int)(pair - w * a.heads);
-  const Place pl = find_place(a, w, C);
+  int64_t ends[2] = {0, a.tokens};
+  const Place pl = find_place(a, w, C, ends);
+  if (a.cu != nullptr && a.zero_rest) clear_rest<T, NT, VEC>(a, w, h, ends);
   if (pl.seq < 0 || pl.len == 0) return;
   const int64_t row0 = a.cu != nullptr ? 0 : pl.seq, begin = pl.begin + pl.part * C;
   const int n = (int)(pl.len - pl.part * C < C ? pl.len - pl.part * C : C);
@@ -1027,15 +1057,6 @@ void delta_walk_kernel(DeltaArgs a) {
       for (int r = 0; r < 16; ++r)
         __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, (float)S[t][r]), rs,
                                               s_off(t, r), 0, 0);
-  }
-  if (OUT && a.cu != nullptr && a.zero_rest) {   // rows of no sequence
-    T* const all = (T*)a.out + h * a.oh + c0;
-    auto clear = [&](int64_t from, int64_t to) {
-      for (int64_t t = from + tid / DVW; t < to; t += NT / DVW)
-        if (tid % DVW < dvs) all[t * a.ot + tid % DVW] = from_f<T>(0.0f);
-    };
-    if ((a.zero_rest & 1) && pl.seq == 0 && pl.part == 0) clear(0, pl.begin);
-    if ((a.zero_rest & 2) && pl.seq == a.seqs - 1 && last) clear(pl.begin + pl.len, a.tokens);
   }
 }
 

@@ -296,6 +296,28 @@ def test_rest_rows(cuda):
     assert torch.equal(o[0], out[20:]) and torch.equal(s[0], left[2])
 
 
+@pytest.mark.parametrize("dtype,H,d", [(BF16, 3, 64), (F16, 2, 13), (F32, 5, 32), (BF16, 2, 100)])
+@pytest.mark.parametrize("cu", [[0, 100, 130], [20000, 20007], [3, 3], [5, 5] + [9] * 80 + [40, 30000],
+                                [30000, 30000], [-4, 50000]])
+def test_mostly_rest_rows(cuda, dtype, H, d, cu):
+    """Few tokens in many rows: all others zero in a new output, on whatever memory,
+    and none touched in one given."""
+    N = 30000
+    q, k, v, beta, f = (t.to(cuda) for t in _inputs((N,), (H, 1, H), d, d, dtype, 4, H=H))
+    offsets = torch.tensor(cu, device=cuda)
+    used = torch.full((N, H, d), 7.0, dtype=dtype, device=cuda)
+    del used                                 # (its memory may be the output's)
+    out = kernels.delta_attention(q, k, v, beta, f, cu_seqlens=offsets, return_state=False)
+    first, end = max(cu[0], 0), min(max(cu), N)
+    assert not bool(out[:first].any()) and not bool(out[end:].any())
+    given = torch.full((N, H, d), 7.0, dtype=dtype, device=cuda)
+    kernels.delta_attention(q, k, v, beta, f, cu_seqlens=offsets, return_state=False, out=given)
+    assert torch.equal(given[first:end], out[first:end])
+    assert bool((given[:first] == 7).all()) and bool((given[end:] == 7).all())
+    if end > first:
+        assert bool(out[first:end].any(2).any(1).all())
+
+
 @pytest.mark.parametrize("B,N,H", [(3000, 9000, 2), (1025, 9000, 1), (130, 70000, 2)])
 def test_many_sequences(cuda, B, N, H):
     """More sequences than one scan or one search takes, many empty, some offsets
