@@ -765,16 +765,25 @@ hipError_t launch_few(const LinearArgs& a, hipStream_t st) {
 }
 
 template <typename T, int BM, int BN, int WM, int WN, int NST, int OPS, bool VEC>
-hipError_t launch_tiles(LinearArgs a, hipStream_t st) {
-  const int64_t rt = (a.rows + BM - 1) / BM, ct = (a.cols + BN - 1) / BN;
-  if (rt * ct > 0xffffffffll / (64 * WM * WN) / a.splits) return hipErrorInvalidValue;
-  a.row_tiles = (int)rt;
-  a.col_tiles = (int)ct;
-  hipLaunchKernelGGL((linear_tile_kernel<T, BM, BN, WM, WN, NST, OPS, VEC>),
-                     dim3((unsigned)(rt * ct), (unsigned)a.splits), dim3(64 * WM * WN), 0, st, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.parts == nullptr) return e;
-  const int64_t n = a.rows * ((a.cols + 3) / 4);
+hipError_t launch_tiles(const LinearArgs& a, hipStream_t st) {
+  const int64_t ct = (a.cols + BN - 1) / BN;
+  // a launch has fewer than 2^32 threads: more tiles take several, of whole bands
+  const int64_t most = 0xffffffffll / (64 * WM * WN) / ct / 8 * 8 * BM;
+  for (int64_t m = 0; m < a.rows; m += most) {
+    LinearArgs b = a;
+    b.x = (const T*)a.x + m * a.xr;
+    b.out = (T*)a.out + m * a.orow;
+    if (a.residual) b.residual = (const T*)a.residual + m * a.rr;
+    b.rows = a.rows - m < most ? a.rows - m : most;
+    b.row_tiles = (int)((b.rows + BM - 1) / BM);
+    b.col_tiles = (int)ct;
+    hipLaunchKernelGGL((linear_tile_kernel<T, BM, BN, WM, WN, NST, OPS, VEC>),
+                       dim3((unsigned)(b.row_tiles * ct), (unsigned)a.splits), dim3(64 * WM * WN), 0, st, b);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  if (a.parts == nullptr) return hipSuccess;
+  const int64_t n = a.rows * ((a.cols + 3) / 4);   // (splits have fewer tiles than the card CUs)
   hipLaunchKernelGGL((linear_join_kernel<T, OPS>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
   return hipGetLastError();
 }

@@ -319,6 +319,24 @@ def test_more_than_32_bits(cuda):
     _check(kernels.linear(rows, w), rows.contiguous(), (w,), (None,), None)
 
 
+def test_more_tiles_than_a_launch_takes(cuda):
+    """Rows of one number and columns that just begin a second tile: 8.4 million tiles
+    of 512 threads and more."""
+    M, N = 540_000_001, 65
+    x = torch.zeros(M, 1, dtype=BF16, device=cuda)
+    pick = torch.tensor([0, 1, 129, M // 3, M // 2, 536_870_911, 536_870_912, M - 130, M - 1], device=cuda)
+    x[pick, 0] = torch.arange(1, len(pick) + 1, device=cuda).to(BF16)
+    g = torch.Generator(device=cuda).manual_seed(1)
+    w, w2 = (torch.randn(N, 1, generator=g, device=cuda).to(BF16) for _ in range(2))
+    out = kernels.gated_linear(x, w, w2)
+    _check(out[pick], x[pick], (w, w2), (None, None), "silu")
+    some = torch.arange(0, M, 10007, device=cuda)
+    some = some[~torch.isin(some, pick)]
+    assert not bool(out[some].any())
+    del out, x, some
+    torch.cuda.empty_cache()
+
+
 def test_rows_too_long_to_lie_near(cuda):
     """256 rows reach over 2^31 bytes, and no 16 bytes divide one."""
     M, K, N = 40, 4_200_001, 24
