@@ -96,7 +96,7 @@ __device__ __forceinline__ float exp_f(float x) {
   const float low = __builtin_fmaf(x, 1.44269502f, -y) + x * 1.92596299e-8f;
   const float e = __builtin_amdgcn_exp2f(y);
   // (an infinite or vanished power stays one)
-  return __builtin_fabsf(y) < 126.0f ? __builtin_fmaf(e, low * 0.693147182f, e) : e;
+  return __builtin_fabsf(y) < 127.9f ? __builtin_fmaf(e, low * 0.693147182f, e) : e;
 }
 // z / (1 + e^-t).  For outputs of 16 bits the power of two alone will do: rounding its
 // argument moves it, and so the result, by |t| 2^-24 of itself, 5e-6 where fp32 ends;
@@ -104,7 +104,10 @@ __device__ __forceinline__ float exp_f(float x) {
 template <typename T>
 __device__ __forceinline__ float sigmoid_times(float z, float t) {
   const float e = sizeof(T) == 4 ? exp_f(-t) : __builtin_amdgcn_exp2f(t * -1.44269502f);
-  return z * __builtin_amdgcn_rcpf(1.0f + e);
+  if (__is_same(T, _Float16)) return z * __builtin_amdgcn_rcpf(1.0f + e);
+  // (the reciprocal of what is beyond 2^126 would be lost, z times it not: t to -88)
+  const float s = e > 0x1p64f ? 0x1p-64f : 1.0f;
+  return (z * s) * __builtin_amdgcn_rcpf(__builtin_fmaf(e, s, s));
 }
 // x (1 + erf(x / sqrt(2))) / 2 = max(x, 0) - |x| Q(|x|), Q(y) = (1 - erf(y / sqrt(2))) / 2.
 template <typename T>

@@ -202,6 +202,28 @@ def test_gelu_of_small_values(cuda, M):
     assert bool(y[0].isnan()) and y[1:].tolist() == [math.inf, 0.0, 0.0]
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M", [20, 400])
+def test_sigmoids_of_small_values(cuda, dtype, M):
+    """silu and gelu_tanh relative to the result, down to the smallest normal numbers.
+    Units of u = 2^-24: the power 4, the sum 1, the reciprocal 2, products 2: 9; t of
+    gelu_tanh is off by 3 u of itself, and the power by |t| times that.  For bf16 the
+    power's argument is rounded, |t| u, and the output to half a unit."""
+    w = torch.ones(1, 1, dtype=dtype, device=cuda)
+    for act, low in (("silu", -88.5), ("gelu_tanh", -9.5)):
+        z = torch.linspace(low, 3, 40 * M, device=cuda).view(M, 40)[:, :1].to(dtype)
+        x = z.double()
+        t = x if act == "silu" else 2 * math.sqrt(2 / math.pi) * (x + 0.044715 * x ** 3)
+        want = x / (1 + torch.exp(-t))
+        got = kernels.linear(z.contiguous(), w, activation=act).double()
+        tol = (9 + 4 * t.abs() * ((act != "silu") + (dtype != F32))) * U32 * want.abs()
+        i = torch.finfo(dtype)
+        tol = tol + (i.eps / 2 * want.abs() if dtype != F32 else 0)
+        ok = want.abs() >= i.smallest_normal
+        assert int(ok.sum()) > 0.9 * M
+        assert bool(((got - want).abs() <= tol)[ok].all())
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("M", [1, 20, 150])
 def test_strides(cuda, dtype, M):
