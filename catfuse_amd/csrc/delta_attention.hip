@@ -277,7 +277,7 @@ __device__ __forceinline__ float power_of_two(double x) {
 // those of T from the first row of a B A^-1 on that is not: a product with the zeros
 // of D^-1 would make NaN of the rows before it.
 // Bound by the substitution's chain of dependent steps and by T's bytes (300 a token
-// and head of C = 64, 2.2 TB/s): 65536 tokens x 32 heads of 128 bf16 channels 290 us.
+// and head of C = 64, 2.0 TB/s): 65536 tokens x 32 heads of 128 bf16 channels 310 us.
 template <int C> constexpr int solved_size() { return (C / 32) * (C / 32 + 1) / 2 * 6144; }   // bytes
 
 typedef float f4v __attribute__((ext_vector_type(4)));
@@ -520,8 +520,8 @@ __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
 // scores and K's turned operand have them.
 //
 // Bound by the issue of matrix and vector operations by turns, and by the card's
-// power: 65536 tokens x 32 heads of 128 bf16 channels in 16 segments, outputs 960 us
-// and states 960 (matrix cores 47 and 53 %, vector issue 43 and 53 %, LDS 18 % of the
+// power: 65536 tokens x 32 heads of 128 bf16 channels in 16 segments, outputs 990 us
+// and states 1010 (matrix cores 47 and 53 %, vector issue 44 and 54 %, LDS 18 % of the
 // cycles, the clock at 1.8 GHz).  Two workgroups of four waves a CU; chunks of 64 halve
 // the products with the state's parts against 32, for which only bf16 heads of 65 to
 // 128 channels have the registers.

@@ -640,30 +640,30 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearArgs a) {
 }
 
 // Which kernel, in what pieces.  The times are of bf16.
-//   rows <= 32, and <= 8 or few columns: few rows (7 gated rows of 4096 x 11264 42.0
-//     us, tiles 43.4; 32 of 512 x 1000 4.3 and 6.0).  Else tiles read w no slower and
-//     x less often (32 gated rows of 4096 x 11264: 45 us, few rows 59; 32 of 4096 x
-//     4096 13.1 and 14.2).
+//   rows <= 32, and <= 8 or few columns: few rows (1 gated row of 4096 x 11264 37.0 us,
+//     tiles 39.4, 8 rows 42.2 and 39.9; 8 rows of 4096 x 4096 9.8 and 19.7, 32 of 512 x
+//     1000 4.6 and 5.9).  Else tiles read w no slower and x less often (32 gated rows
+//     of 4096 x 11264: 39 us, few rows 59; 32 of 4096 x 4096 13.4 and 14.7).
 //   256: most work a byte read from L2, one workgroup a CU.  Taken if its rounds of
 //     the card are no longer than those of 128, four of whose tiles (at two a CU) take
 //     as long as one of it, or 1.2 times as long where the inner dimension is long and
 //     the start and the epilogue, which nothing covers here, count little (25088 x
-//     4096 x 1536, 588 tiles: 293 us, 128 327; 25088 x 384 x 1536 54 and 50; 304 tiles,
-//     4864 x 4096 x 4096: 182 and 167; 160, 2560 x 4096 x 4096: 87 and 112).  Not for 32-bit
+//     4096 x 1536, 588 tiles: 289 us, 128 324; 25088 x 384 x 1536 55 and 51; 304 tiles,
+//     4864 x 4096 x 4096: 177 and 167; 160, 2560 x 4096 x 4096: 88 and 104).  Not for 32-bit
 //     numbers, whose matrix instructions bound every tile alike.
 //   128, two stages and two workgroups a CU: more than a tile a CU (384 tiles, 1500 x
-//     4096 x 4096: 56 us, four stages 67).
+//     4096 x 4096: 57 to 60 us, four stages 67).
 //   128, four stages: more than half a tile a CU (256 tiles, 1024 x 4096 x 4096: 37 us,
-//     two stages 44, 64 54; 192 tiles 34 and 64 46; 128 tiles 32 and 64 28).
+//     two stages 44, 64 53; 192 tiles 33 and 64 45; 128 tiles 32 and 64 29).
 //   64: four stages, two workgroups a CU.  Of long rows that give less than a tile a CU
-//     the inner dimension is split, 16 steps and more a split (64 x 4096 x 4096: 19.6
-//     us whole, 14.1 in four; 256 x 2048 x 2048 would be 13.7 in two, and takes 12.0).
+//     the inner dimension is split, 16 steps and more a split (64 x 4096 x 4096: 19.8
+//     us whole, 14.5 in four; 256 x 2048 x 2048 would be 13.8 in two, and takes 12.1).
 // Rows of 16 bits that are not in whole pieces of 16 bytes are first laid out so in the
 // workspace (pack) if that takes less than it saves: a read and a write of all rows at
 // 4.5 TB/s and 4 us for the launches, against 0.75 of the product's time or 0.55 us a
-// step, whichever is more (9506 x 1121 x 8192: 183 us, read as they lie 318; 300 x 4097 x
+// step, whichever is more (9506 x 1121 x 8192: 193 us, read as they lie 310; 300 x 4097 x
 // 4096 42 and 70; 64 x 1121 x 8192, 18773 x 1137 x 137: not).  Those of 32 bits lose too
-// little (2673 x 3321 x 536: 145, whole 110).
+// little (2673 x 3321 x 536: 150, 2672 x 3320 x 536 109).
 struct Plan {
   bool few;                                // the few-rows kernel
   int size, splits, split_steps;

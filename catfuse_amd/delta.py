@@ -70,22 +70,24 @@ def _segment(seqs: int, tokens: int, packed: bool, heads: int, dk: int, dv: int)
     # The walks along a segment get shorter with it, the walk over the segments'
     # states longer: least near a constant times the root of the length, 3.5 for wide
     # keys and 3 for narrow ones (us; one sequence of 1024 tokens and 8 heads of 128
-    # channels: 64 tokens a segment 107, 128 68, 192 74, whole 135; 4096 tokens: 192 140,
-    # 320 118, 448 133, whole 523; 16384 of 64 channels: 192 180, 448 165, 704 179).
+    # channels: 64 tokens a segment 76, 128 65, 192 69, whole 138; 4096 tokens: 192 128,
+    # 320 120, 448 136, whole 529; 16384 of 64 channels: 192 179, 448 167, 704 181).
     # No shorter than it takes to have all segments at work at once (16384 tokens, 32
-    # heads: 576 748, 2048 694), by half as many for equal sequences of 65 to 128
-    # channels (four of 4096 tokens and 16 heads: 512 445, 1088 362; but packed 20000,
-    # 10000 and 30000, which end some early: 3776 2153, 8192 2446).  An odd number of
-    # chunks: an even one has all segments read the same channels of memory at a time
-    # (4096 tokens, 8 heads: 256 147, 320 118; 65536 and 4 heads: 1024 602, 1088 479),
-    # which counts once they are many and as long as they drift little.  Whole sequences
-    # if they give workgroups enough (eight of 4096, 32 heads: whole 775, 2112 988; four
-    # of 2048: 328 and 341) or are short (160 tokens, 8 heads: whole 34, 64 37; 196 both
-    # 41; 300 whole 49, 64 44; of 256 channels 74 and 92).  Packed ones, whose lengths are
-    # not known here, then are cut where they are longer than most: a little over the
-    # mean (16 heads of 128: sixteen of 50 to 3000 tokens whole 423, cut 281; 24 of 20 to
-    # 2000 whole 405 to 553, cut 457 to 478; sixteen of 1000 whole 217, cut 232), until
-    # they fill the card by themselves.
+    # heads: 576 750, 2048 698), by half as many for equal sequences of 65 to 128
+    # channels (two of 8192 tokens and 16 heads: 576 393, 1088 373; four of 4096: 367 and
+    # 372; but packed 20000, 10000 and 30000, which end some early: 3776 2197, 8192
+    # 2434).  An odd number of chunks: with an even one all segments may read the same
+    # channels of memory at a time (4096 tokens, 16 heads: 256 168, 320 140; 8192: 512
+    # 244, 576 220; 5000 of 4 heads of 256 channels: 256 311, 320 265; where they do not,
+    # the even number is better by 2 to 10 %: 5000 of 8 heads of 32: 71 and 76), which
+    # counts once they are many and as long as they drift little.  Whole sequences if
+    # they give workgroups enough (eight of 4096, 32 heads: whole 784, 2112 979; four of
+    # 2048: 329 and 341) or are short (160 tokens, 8 heads: whole 36, 64 37; 196 43 and
+    # 39; 300 51 and 43; of 256 channels 76 and 87).  Packed ones, whose lengths are not
+    # known here, then are cut where they are longer than most: a little over the mean
+    # (16 heads of 128: sixteen of 50 to 3000 tokens whole 419, cut 273; 24 of 20 to 2000
+    # whole 405 to 553, cut 457 to 478; sixteen of 1000 whole 203, cut 219), until they
+    # fill the card by themselves.
     width = 32 if dk <= 32 else 64 if dk <= 64 else 128
     columns = heads * -(-dv // width)          # workgroups of one segment
     at_once = 2048 if dk <= 32 else 1024 if dk <= 64 else 512 if dk <= 128 else 256
@@ -145,9 +147,10 @@ def delta_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: tor
     a chunk, to 2^-22 of one).  With keys of a length of at most 1 and beta in 0 .. 1
     (or keys of length 1 and beta in 0 .. 2) a step does not make errors grow; keys
     that are longer (|k|^2 beta > 2) let the state itself and its errors grow from
-    token to token.  A token that holds an infinity or NaN, or whose u_t is beyond
-    fp32, does not reach the tokens before it; what it does reach may be NaN where
-    the formula gives an infinity.
+    token to token, and where |k|^2 beta itself is beyond fp32 the results may be NaN.
+    Numbers of a state and u_t are computed so between 2^-100 and 2^100.  A token that
+    holds an infinity or NaN, or whose u_t is beyond fp32, does not reach the tokens
+    before it; what it does reach may be NaN where the formula gives an infinity.
     The workspace, from torch's allocator, is 300 bytes a token and head (bf16
     heads of 65 to 128 channels, whose sequences count as whole multiples of 64
     tokens; others 204 and 32), and for long sequences of a small batch, which are
