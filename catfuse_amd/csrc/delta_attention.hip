@@ -426,9 +426,12 @@ __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
   }
   __syncthreads();
   const int c16 = lane & 15, q16 = lane >> 4;
-  auto keep_finite = [&](f4v& m, int row) {  // rows row .. + 3 of a B A^-1
+  // a B A^-1, rows row .. + 3: whether all of it is finite; those numbers that are not out
+  auto finite = [&](const f4v& m) {
     const float z = __builtin_fmaf(m[0], 0.0f, m[1] * 0.0f) + __builtin_fmaf(m[2], 0.0f, m[3] * 0.0f);
-    if (__ballot(z != z) == 0) return;
+    return __ballot(z != z) == 0;
+  };
+  auto keep_finite = [&](f4v& m, int row) {
 #pragma unroll
     for (int j = 3; j >= 0; --j)
       if (!(__builtin_fabsf(m[j]) < __builtin_inff())) {
@@ -440,18 +443,25 @@ __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
   // lie, if that takes its inner indices 4 q16 + j), then -D^-1 times it
   if (wave < C / 32) {
     const int b0 = 32 * wave;
-    f4v m = {}, y = {};
+    f4v m = {}, y;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int k = 4 * j + q16;
       m = __builtin_amdgcn_mfma_f32_16x16x4f32(low[(b0 + 16 + c16) * P + b0 + k],
                                                inv[(b0 + k) * P + b0 + c16], m, 0, 0, 0);
     }
-    keep_finite(m, b0 + 16 + 4 * q16);
+    auto times_m = [&]() {
+      y = f4v{};
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      y = __builtin_amdgcn_mfma_f32_16x16x4f32(inv[(b0 + 16 + c16) * P + b0 + 16 + 4 * q16 + j], m[j], y,
-                                               0, 0, 0);
+      for (int j = 0; j < 4; ++j)
+        y = __builtin_amdgcn_mfma_f32_16x16x4f32(inv[(b0 + 16 + c16) * P + b0 + 16 + 4 * q16 + j], m[j], y,
+                                                 0, 0, 0);
+    };
+    times_m();
+    if (!finite(m)) {
+      keep_finite(m, b0 + 16 + 4 * q16);
+      times_m();
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) inv[(b0 + 16 + 4 * q16 + j) * P + b0 + c16] = -y[j];
   }
@@ -459,7 +469,7 @@ __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
   if constexpr (C > 32) {
     // the pair of 32: wave = 16 rows (i) and 16 columns (j) of its lower left block
     const int i0 = 32 + 16 * (wave & 1), j0 = 16 * (wave >> 1);
-    f4v m[2] = {{}, {}}, y = {};
+    f4v m[2] = {{}, {}}, y;
 #pragma unroll
     for (int k0 = 0; k0 < 32; k0 += 4) {
       const float x = inv[(k0 + q16) * P + j0 + c16];
@@ -468,14 +478,21 @@ __global__ __launch_bounds__(NT) void delta_solve_kernel(DeltaArgs a) {
         m[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(low[(32 + 16 * e + c16) * P + k0 + q16], x, m[e],
                                                     0, 0, 0);
     }
+    auto times_m = [&]() {
+      y = f4v{};
 #pragma unroll
-    for (int e = 0; e < 2; ++e) keep_finite(m[e], 32 + 16 * e + 4 * q16);
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+        for (int j = 0; j < 4; ++j)
+          y = __builtin_amdgcn_mfma_f32_16x16x4f32(inv[(i0 + c16) * P + 32 + 16 * e + 4 * q16 + j], m[e][j],
+                                                   y, 0, 0, 0);
+    };
+    times_m();
+    if (!finite(m[0]) || !finite(m[1])) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        y = __builtin_amdgcn_mfma_f32_16x16x4f32(inv[(i0 + c16) * P + 32 + 16 * e + 4 * q16 + j], m[e][j],
-                                                 y, 0, 0, 0);
+      for (int e = 0; e < 2; ++e) keep_finite(m[e], 32 + 16 * e + 4 * q16);
+      times_m();
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) inv[(i0 + 4 * q16 + j) * P + j0 + c16] = -y[j];
     __syncthreads();
@@ -863,30 +880,7 @@ void delta_walk_kernel(DeltaArgs a) {
     }
 
     if constexpr (OUT) {
-      // (a correction beyond fp32, of values that are not, is one of them)
-      float z = 0.0f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-#pragma unroll
-        for (int t = 0; t < CT; ++t) z = __builtin_fmaf(U[t][r], 0.0f, z);
-      any_bad = any_bad || __ballot(z != z) != 0;
       if (CT > 1) __syncthreads();           // T is read
-      if (any_bad) {
-#pragma unroll
-        for (int t = 0; t < CT; ++t)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int tok = 32 * t + 8 * (r >> 2) + 4 * hi + (r & 3);
-            bad_from = !(__builtin_fabsf(U[t][r]) < __builtin_inff()) && tok < bad_from ? tok : bad_from;
-          }
-        const int other = __shfl_xor(bad_from, 32, 64);
-        bad_from = other < bad_from ? other : bad_from;
-#pragma unroll
-        for (int t = 0; t < CT; ++t)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            U[t][r] = 32 * t + 8 * (r >> 2) + 4 * hi + (r & 3) >= bad_from ? 0.0f : U[t][r];
-      }
       // Scores K Q^T of 32 keys (rows) x 32 queries (columns): eight registers
       // on end are an operand of U^T P^T as they lie.  One tile: every wave for
       // itself; three: a tile a wave, exchanged in LDS.
@@ -932,6 +926,30 @@ void delta_walk_kernel(DeltaArgs a) {
             for (int p = 0; p < NP; ++p)
               *reinterpret_cast<u32x4*>(tsh + (((wave * 2 + s) * NP + p) * 64 + lane) * 16) = pop[s][p];
         }
+      }
+      // A correction beyond fp32, of values that are not, is one of those.  (Looked for
+      // here, behind the scores, where its products have long been done.)
+      float z = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int t = 0; t < CT; ++t) z = __builtin_fmaf(U[t][r], 0.0f, z);
+      any_bad = any_bad || __ballot(z != z) != 0;
+      if (any_bad) {
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int tok = 32 * t + 8 * (r >> 2) + 4 * hi + (r & 3);
+            bad_from = !(__builtin_fabsf(U[t][r]) < __builtin_inff()) && tok < bad_from ? tok : bad_from;
+          }
+        const int other = __shfl_xor(bad_from, 32, 64);
+        bad_from = other < bad_from ? other : bad_from;
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            U[t][r] = 32 * t + 8 * (r >> 2) + 4 * hi + (r & 3) >= bad_from ? 0.0f : U[t][r];
       }
       // O^T += U^T P^T
       auto make_u = [&](int s) {
